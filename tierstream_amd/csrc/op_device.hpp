@@ -1,0 +1,172 @@
+// Device parts the model operators share: the two 16-bit types with their matrix instruction, activations, 4-bit blocks,
+// and the 64 x 64 tile that takes any stride and alignment.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "op_launch.hpp"
+
+namespace tsa {
+namespace op {
+
+typedef uint16_t u16;
+typedef uint16_t bits4 __attribute__((ext_vector_type(4)));
+typedef uint16_t bits8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// v_mfma_f32_16x16x32: lane l holds row (a) or column (b) l % 16 at k = 8 (l / 16) + 0..7, and of the result column
+// l % 16 at rows 4 (l / 16) + 0..3. Products of 16-bit values are exact in 32 bits; sums are kept in 32.
+struct Bf16 {
+  typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ f32x4 mfma(bits8 a, bits8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float up(u16 v) { return __builtin_bit_cast(float, uint32_t(v) << 16); }
+  static __device__ __forceinline__ u16 down(float v) { return __builtin_bit_cast(u16, (__bf16)v); }
+};
+struct F16 {
+  typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ f32x4 mfma(bits8 a, bits8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float up(u16 v) { return float(__builtin_bit_cast(_Float16, v)); }
+  static __device__ __forceinline__ u16 down(float v) { return __builtin_bit_cast(u16, (_Float16)v); }
+};
+
+__device__ __forceinline__ float sigmoid(float v) { return 1.0f / (1.0f + expf(-v)); }
+
+// act(v). The tanh form is v / (1 + exp(-2 z)), the same function as v (1 + tanh z) / 2 without the difference of
+// nearly equal numbers at large negative z.
+__device__ __forceinline__ float activate(uint32_t act, float v) {
+  switch (act) {
+    case TSA_ACT_SILU: return v * sigmoid(v);
+    case TSA_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678f));
+    case TSA_ACT_GELU_TANH: return v * sigmoid(1.5957691f * (v + 0.044715f * v * v * v));
+    case TSA_ACT_RELU: return v > 0.0f ? v : (v == v ? 0.0f : v);
+    default: return v;
+  }
+}
+// act'(v)
+__device__ __forceinline__ float slope(uint32_t act, float v) {
+  switch (act) {
+    case TSA_ACT_SILU: {
+      const float s = sigmoid(v);
+      return s * (1.0f + v * (1.0f - s));
+    }
+    case TSA_ACT_GELU:
+      return 0.5f * (1.0f + erff(v * 0.70710678f)) + v * expf(-0.5f * v * v) * 0.39894228f;
+    case TSA_ACT_GELU_TANH: {
+      const float s = sigmoid(1.5957691f * (v + 0.044715f * v * v * v));
+      return s + v * s * (1.0f - s) * 1.5957691f * (1.0f + 0.134145f * v * v);
+    }
+    case TSA_ACT_RELU: return v > 0.0f ? 1.0f : 0.0f;
+    default: return 1.0f;
+  }
+}
+
+__device__ __forceinline__ float load_as_float(const void* p, uint64_t i, uint32_t type) {
+  if (type == TSA_F32) return static_cast<const float*>(p)[i];
+  const u16 v = static_cast<const u16*>(p)[i];
+  return type == TSA_BF16 ? Bf16::up(v) : F16::up(v);
+}
+__device__ __forceinline__ void store_float(void* p, uint64_t i, uint32_t type, float v) {
+  if (type == TSA_F32) static_cast<float*>(p)[i] = v;
+  else static_cast<u16*>(p)[i] = type == TSA_BF16 ? Bf16::down(v) : F16::down(v);
+}
+
+// ---- the 64 x 64 tile for any stride ----------------------------------------------------------------------------------
+// A matrix operand: element (r, k) at base + r rs + k ks, rows through `map` if there is one; zero outside rows x n.
+struct Operand {
+  const u16* base = nullptr;
+  uint64_t rs = 0, ks = 1;
+  uint32_t rows = 0, n = 0;
+  const uint32_t* map = nullptr;
+  __device__ __forceinline__ bits8 load8(uint32_t r, uint32_t k) const {
+    bits8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (r >= rows) return v;
+    const u16* p = base + uint64_t(map ? map[r] : r) * rs;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i)
+      if (k + i < n) v[i] = p[uint64_t(k + i) * ks];
+    return v;
+  }
+};
+
+// Rows of 4-bit blocks: the values 8 at a time without their scale (whole numbers -8..7, exact in either type).
+template <class T>
+struct Q4Operand {
+  const unsigned char* base = nullptr;
+  uint64_t row_bytes = 0;
+  uint32_t rows = 0, n = 0;
+  __device__ __forceinline__ bits8 load8(uint32_t r, uint32_t k) const {
+    bits8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (r >= rows || k >= n) return v;
+    const unsigned char* p = base + r * row_bytes + uint64_t(k / 32) * kQ4Bytes + 2 + (k & 15u);
+    const uint32_t shift = k & 16u ? 4 : 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) v[i] = T::down(float(int((p[i] >> shift) & 15u) - 8));
+    return v;
+  }
+  __device__ __forceinline__ float scale(uint32_t r, uint32_t k) const {
+    if (r >= rows || k >= n) return 0.0f;
+    const unsigned char* p = base + r * row_bytes + uint64_t(k / 32) * kQ4Bytes;
+    return F16::up(u16(p[0] | p[1] << 8));
+  }
+};
+
+struct TileMemory {
+  u16 a[64][40], b[64][40];  // 32 values a row, 8 of padding
+  float scale[64];
+};
+
+// acc[i][j] += the products of rows a0.. of `a` and rows b0.. of `b` over all k, by 256 threads: wave w covers a's rows
+// 32 (w & 1).. and b's 32 (w >> 1)..; lane l's values are a-rows 16 i + 4 (l / 16) + 0..3, b-row 16 j + l % 16 of them.
+template <class T, bool kQ4, class A, class B>
+__device__ __forceinline__ void tile64(const A& a, uint32_t a0, const B& b, uint32_t b0, uint32_t n, TileMemory& m,
+                                       f32x4 (&acc)[2][2]) {
+  const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6;
+  const uint32_t ar = (wave & 1u) * 32 + (lane & 15u), br = (wave >> 1) * 32 + (lane & 15u), kq = (lane >> 4) * 8;
+  for (uint32_t k = 0; k < n; k += 32) {
+    const bits8 va = a.load8(a0 + t / 4, k + (t & 3u) * 8), vb = b.load8(b0 + t / 4, k + (t & 3u) * 8);
+    __syncthreads();  // the last step's reads are done
+    *reinterpret_cast<bits8*>(&m.a[t / 4][(t & 3u) * 8]) = va;
+    *reinterpret_cast<bits8*>(&m.b[t / 4][(t & 3u) * 8]) = vb;
+    if constexpr (kQ4)
+      if (t < 64) m.scale[t] = a.scale(a0 + t, k);
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+      const bits8 fa = *reinterpret_cast<const bits8*>(&m.a[ar + 16 * i][kq]);
+#pragma unroll
+      for (uint32_t j = 0; j < 2; ++j) {
+        const bits8 fb = *reinterpret_cast<const bits8*>(&m.b[br + 16 * j][kq]);
+        if constexpr (kQ4) {  // 32 values are one block: its sum in whole steps, then the scale in 32 bits
+          const f32x4 c = T::mfma(fa, fb, f32x4{0, 0, 0, 0});
+          const float* s = &m.scale[(wave & 1u) * 32 + 16 * i + (lane >> 4) * 4];
+#pragma unroll
+          for (uint32_t r = 0; r < 4; ++r) acc[i][j][r] += s[r] * c[r];
+        } else {
+          acc[i][j] = T::mfma(fa, fb, acc[i][j]);
+        }
+      }
+    }
+  }
+}
+
+// f(a-row, b-row, value) for every value of a wave's part of the tile.
+template <class F>
+__device__ __forceinline__ void each64(const f32x4 (&acc)[2][2], F&& f) {
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (uint32_t i = 0; i < 2; ++i)
+#pragma unroll
+    for (uint32_t j = 0; j < 2; ++j)
+#pragma unroll
+      for (uint32_t r = 0; r < 4; ++r)
+        f((wave & 1u) * 32 + 16 * i + (lane >> 4) * 4 + r, (wave >> 1) * 32 + 16 * j + (lane & 15u), acc[i][j][r]);
+}
+
+}  // namespace op
+}  // namespace tsa

@@ -1,0 +1,461 @@
+// Gated feed-forward blocks of the chosen experts, and their gradients.
+//
+// The pairs (row, j) are grouped by expert first (plan_kernel, one workgroup). Then
+//   forward:   h = act(gate x) * (up x) of every pair; y' = down h; y_t = residual_t + sum_j w_tj y'_tj.
+//   backward:  b = down^T dy; d w = <h, b>; the two halves dg = w b up act'(gate), du = w b act(gate), and w h of every
+//              pair; dx' = gate^T dg + up^T du, added over a row's pairs; d gate = dg^T x, d up = du^T x and
+//              d down = dy^T (w h) over an expert's pairs.
+// h, dg, du and w h are rounded once to the operands' 16 bits, as the matrix instructions take them; y' and dx' stay in
+// 32 bits until the row's sum, and w is applied there or before the rounding. No sum depends on an order that changes.
+#include "op_device.hpp"
+
+namespace tsa {
+namespace op {
+namespace {
+
+constexpr uint32_t kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
+
+__device__ __forceinline__ void part_pointers(const ExpertMap& m, uint32_t e, const char* (&p)[3]) {
+  if (m.form == 2) {
+    const int32_t s = ss_dg_slot(&m.view, m.gated, int32_t(e));
+    for (int i = 0; i < 3; ++i)
+      p[i] = static_cast<const char*>(m.view.parts[i].base) + uint64_t(uint32_t(s)) * m.view.parts[i].stride;
+  } else if (m.form == 1) {
+    for (int i = 0; i < 3; ++i) p[i] = reinterpret_cast<const char*>(m.table[e]) + m.stride[i];
+  } else {
+    for (int i = 0; i < 3; ++i) p[i] = m.part[i] + e * m.stride[i];
+  }
+}
+
+// The expert of a pair, or ~0: an id out of range, or a table entry of 0.
+__device__ __forceinline__ uint32_t expert_of(const ExpertMap& m, const int32_t* ids, uint32_t pair) {
+  const uint32_t e = ids ? uint32_t(ids[pair]) : 0;
+  if (e >= m.n || (m.form == 1 && m.table[e] == 0)) return ~0u;
+  return e;
+}
+
+// Sum of v over the threads before this one, and over all of them (kPlanThreads threads).
+__device__ __forceinline__ uint32_t scan(uint32_t v, uint32_t* buf, uint32_t* total) {
+  const uint32_t t = threadIdx.x;
+  buf[t] = v;
+  __syncthreads();
+  for (uint32_t s = 1; s < kPlanThreads; s <<= 1) {
+    const uint32_t o = t >= s ? buf[t - s] : 0;
+    __syncthreads();
+    buf[t] += o;
+    __syncthreads();
+  }
+  const uint32_t r = buf[t] - v;
+  *total = buf[kPlanThreads - 1];
+  __syncthreads();
+  return r;
+}
+
+// Groups the pairs by expert, stably: each wave counts its stretch of pairs per expert, the counts are summed over
+// experts and waves, then each wave places its stretch 64 pairs at a time, a pair behind those of its expert in lower
+// lanes. `rows_per_tile` sorted positions of one expert make a tile.
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(ExpertMap m, const int32_t* ids, Plan p, uint32_t rows_per_tile) {
+  extern __shared__ uint32_t lds[];
+  uint32_t* buf = lds;                    // [kPlanThreads]
+  uint32_t* count = lds + kPlanThreads;   // [kPlanWaves][n]
+  const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6, n = m.n;
+  for (uint32_t i = t; i < kPlanWaves * n; i += kPlanThreads) count[i] = 0;
+  __syncthreads();
+  const uint32_t stretch = ((p.pairs + kPlanThreads - 1) / kPlanThreads) * 64;
+  const uint64_t from = uint64_t(wave) * stretch;
+  for (uint32_t i = 0; i < stretch; i += 64) {
+    const uint64_t pair = from + i + lane;
+    if (pair >= p.pairs) break;
+    const uint32_t e = expert_of(m, ids, uint32_t(pair));
+    if (e != ~0u) atomicAdd(&count[wave * n + e], 1u);
+  }
+  __syncthreads();
+  uint32_t mine = 0;
+  if (t < n)
+    for (uint32_t w = 0; w < kPlanWaves; ++w) mine += count[w * n + t];
+  uint32_t all, tiles;
+  const uint32_t first = scan(mine, buf, &all);
+  const uint32_t n_tiles = (mine + rows_per_tile - 1) / rows_per_tile;
+  const uint32_t tile0 = scan(n_tiles, buf, &tiles);
+  if (t < n) {
+    p.first[t] = first;
+    uint32_t at = first;
+    for (uint32_t w = 0; w < kPlanWaves; ++w) {
+      const uint32_t c = count[w * n + t];
+      count[w * n + t] = at;
+      at += c;
+    }
+    if (mine) {
+      const char* q[3];
+      part_pointers(m, t, q);
+      for (int i = 0; i < 3; ++i) p.part[3 * t + i] = q[i];
+    }
+    for (uint32_t i = 0; i < n_tiles; ++i) {
+      p.tile[2 * (tile0 + i)] = t;
+      p.tile[2 * (tile0 + i) + 1] = first + i * rows_per_tile;
+    }
+  }
+  if (t == 0) {
+    p.first[n] = all;
+    *p.n_tiles = tiles;
+  }
+  __syncthreads();
+  for (uint32_t i = 0; i < stretch; i += 64) {
+    const uint64_t pair = from + i + lane;
+    if (from + i >= p.pairs) break;
+    const bool on = pair < p.pairs;
+    const uint32_t e = on ? expert_of(m, ids, uint32_t(pair)) : ~0u;
+    uint64_t same = __ballot(e != ~0u);
+    for (uint32_t b = 0; b < 9; ++b) {  // (n <= 512)
+      const uint64_t set = __ballot((e >> b) & 1u);
+      same &= (e >> b) & 1u ? set : ~set;
+    }
+    uint32_t at = 0;
+    if (e != ~0u) {
+      at = __hip_atomic_load(&count[wave * n + e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) +
+           uint32_t(__popcll(same & ((1ull << lane) - 1)));
+      p.pair[at] = uint32_t(pair);
+      p.row[at] = uint32_t(pair) / p.top_k;
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (e != ~0u && (same >> lane) == 1)  // the last lane of its expert
+      __hip_atomic_store(&count[wave * n + e], at + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    __builtin_amdgcn_wave_barrier();
+    if (on) p.at[pair] = e != ~0u ? int32_t(at) : -1;
+  }
+}
+
+// One tile's expert and rows (rows_per_tile of the plan); false behind the last tile.
+struct TileRows {
+  uint32_t e, first, rows;
+  const uint32_t* map;
+};
+__device__ __forceinline__ bool tile_rows(const Plan& p, uint32_t tile, uint32_t rows_per_tile, TileRows& t) {
+  if (tile >= *p.n_tiles) return false;
+  t.e = p.tile[2 * tile];
+  t.first = p.tile[2 * tile + 1];
+  const uint32_t end = p.first[t.e + 1];
+  t.rows = end - t.first < rows_per_tile ? end - t.first : rows_per_tile;
+  t.map = p.row + t.first;
+  return true;
+}
+
+// ---- any stride and alignment: 64 x 64 tiles ------------------------------------------------------------------------
+template <class T, bool kQ4, class B>
+__device__ __forceinline__ void weight_tile(const char* w, uint64_t rows, uint32_t n, uint32_t r0, const B& x, TileMemory& m,
+                                            f32x4 (&acc)[2][2]) {
+  if constexpr (kQ4) {
+    const Q4Operand<T> a{reinterpret_cast<const unsigned char*>(w), uint64_t(n / kQ4Block) * kQ4Bytes, uint32_t(rows), n};
+    tile64<T, true>(a, r0, x, 0, n, m, acc);
+  } else {
+    const Operand a{reinterpret_cast<const u16*>(w), n, 1, uint32_t(rows), n, nullptr};
+    tile64<T, false>(a, r0, x, 0, n, m, acc);
+  }
+}
+
+template <class T, bool kQ4>
+__global__ __launch_bounds__(256) void gate_up_any_kernel(Plan p, const u16* x, uint64_t x_stride, uint32_t d, uint32_t f,
+                                                          uint32_t act, u16* h) {
+  __shared__ TileMemory m;
+  const uint32_t tf = (f + 63) / 64;
+  const uint32_t f0 = blockIdx.x % tf * 64;
+  TileRows t;
+  if (!tile_rows(p, blockIdx.x / tf, 64, t)) return;
+  const Operand xs{x, x_stride, 1, t.rows, d, t.map};
+  f32x4 g[2][2] = {}, u[2][2] = {};
+  weight_tile<T, kQ4>(p.part[3 * t.e], f, d, f0, xs, m, g);
+  weight_tile<T, kQ4>(p.part[3 * t.e + 1], f, d, f0, xs, m, u);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) g[i][j][r] = activate(act, g[i][j][r]) * u[i][j][r];
+  each64(g, [&](uint32_t i, uint32_t j, float v) {
+    if (f0 + i < f && j < t.rows) h[uint64_t(t.first + j) * f + f0 + i] = T::down(v);
+  });
+}
+
+template <class T, bool kQ4>
+__global__ __launch_bounds__(256) void down_any_kernel(Plan p, const u16* h, uint32_t d, uint32_t f, float* out) {
+  __shared__ TileMemory m;
+  const uint32_t td = (d + 63) / 64;
+  const uint32_t d0 = blockIdx.x % td * 64;
+  TileRows t;
+  if (!tile_rows(p, blockIdx.x / td, 64, t)) return;
+  const Operand hs{h + uint64_t(t.first) * f, f, 1, t.rows, f, nullptr};
+  f32x4 acc[2][2] = {};
+  weight_tile<T, kQ4>(p.part[3 * t.e + 2], d, f, d0, hs, m, acc);
+  each64(acc, [&](uint32_t i, uint32_t j, float v) {
+    if (d0 + i < d && j < t.rows) out[uint64_t(t.first + j) * d + d0 + i] = v;
+  });
+}
+
+// out_t = residual_t + sum_j w_tj v_{at(t, j)}, in the order of j
+template <class T>
+__global__ __launch_bounds__(256) void combine_kernel(Plan p, uint32_t rows, uint32_t d, const float* v, const float* weights,
+                                                      const u16* residual, uint64_t residual_stride, u16* out,
+                                                      uint64_t out_stride) {
+  const uint64_t total = uint64_t(rows) * d;
+  for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += uint64_t(gridDim.x) * 256) {
+    const uint32_t row = uint32_t(i / d), c = uint32_t(i % d);
+    float s = residual ? T::up(residual[row * residual_stride + c]) : 0.0f;
+    for (uint32_t j = 0; j < p.top_k; ++j) {
+      const uint64_t pair = uint64_t(row) * p.top_k + j;
+      const int32_t at = p.at[pair];
+      if (at >= 0) s += (weights ? weights[pair] : 1.0f) * v[uint64_t(uint32_t(at)) * d + c];
+    }
+    out[row * out_stride + c] = T::down(s);
+  }
+}
+
+// Of every pair: dg | du as one row of 2 f values, w h, and this tile's share of d w (d_share[f tile][sorted position]).
+template <class T>
+__global__ __launch_bounds__(256) void hidden_grad_any_kernel(Plan p, const u16* x, uint64_t x_stride, const u16* dy,
+                                                              uint64_t dy_stride, const float* weights, uint32_t d, uint32_t f,
+                                                              uint32_t act, u16* dgu, u16* wh, float* d_share) {
+  __shared__ TileMemory m;
+  __shared__ float share[64][2];
+  const uint32_t tf = (f + 63) / 64;
+  const uint32_t ft = blockIdx.x % tf, f0 = ft * 64;
+  TileRows t;
+  if (!tile_rows(p, blockIdx.x / tf, 64, t)) return;
+  const Operand xs{x, x_stride, 1, t.rows, d, t.map}, dys{dy, dy_stride, 1, t.rows, d, t.map};
+  f32x4 g[2][2] = {}, u[2][2] = {}, b[2][2] = {};
+  weight_tile<T, false>(p.part[3 * t.e], f, d, f0, xs, m, g);
+  weight_tile<T, false>(p.part[3 * t.e + 1], f, d, f0, xs, m, u);
+  const Operand down{reinterpret_cast<const u16*>(p.part[3 * t.e + 2]), 1, f, f, d, nullptr};  // (f, d): its columns as rows
+  tile64<T, false>(down, f0, dys, 0, d, m, b);
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const uint32_t r = (wave >> 1) * 32 + 16 * j + (lane & 15u);
+    const uint32_t pos = t.first + r;
+    const float w = r < t.rows && weights ? weights[p.pair[pos]] : 1.0f;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t c = f0 + (wave & 1u) * 32 + 16 * i + (lane >> 4) * 4 + q;
+        const float a = activate(act, g[i][j][q]), back = b[i][j][q];
+        if (c >= f || r >= t.rows) continue;
+        sum += a * u[i][j][q] * back;
+        dgu[uint64_t(pos) * 2 * f + c] = T::down(w * back * u[i][j][q] * slope(act, g[i][j][q]));
+        dgu[uint64_t(pos) * 2 * f + f + c] = T::down(w * back * a);
+        wh[uint64_t(pos) * f + c] = T::down(w * a * u[i][j][q]);
+      }
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (lane < 16) share[r][wave & 1u] = sum;
+  }
+  __syncthreads();
+  if (threadIdx.x < t.rows) d_share[uint64_t(ft) * p.pairs + t.first + threadIdx.x] = share[threadIdx.x][0] + share[threadIdx.x][1];
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void input_grad_any_kernel(Plan p, const u16* dgu, uint32_t d, uint32_t f, float* out) {
+  __shared__ TileMemory m;
+  const uint32_t td = (d + 63) / 64;
+  const uint32_t d0 = blockIdx.x % td * 64;
+  TileRows t;
+  if (!tile_rows(p, blockIdx.x / td, 64, t)) return;
+  f32x4 acc[2][2] = {};
+  for (int half = 0; half < 2; ++half) {
+    const Operand w{reinterpret_cast<const u16*>(p.part[3 * t.e + half]), 1, d, d, f, nullptr};
+    const Operand v{dgu + uint64_t(t.first) * 2 * f + half * f, uint64_t(2) * f, 1, t.rows, f, nullptr};
+    tile64<T, false>(w, d0, v, 0, f, m, acc);
+  }
+  each64(acc, [&](uint32_t i, uint32_t j, float v) {
+    if (d0 + i < d && j < t.rows) out[uint64_t(t.first + j) * d + d0 + i] = v;
+  });
+}
+
+// out[e][b][a] = sum over expert e's pairs of left[pair][a] right[pair][b] (0 for an expert without pairs): left through
+// the rows' map where left_map, right where right_map.
+template <class T>
+__global__ __launch_bounds__(256) void weight_grad_any_kernel(Plan p, const u16* left, uint64_t left_stride, bool left_map,
+                                                              uint32_t n_left, const u16* right, uint64_t right_stride,
+                                                              bool right_map, uint32_t n_right, u16* out) {
+  __shared__ TileMemory m;
+  const uint32_t ta = (n_left + 63) / 64, tb = (n_right + 63) / 64;
+  const uint32_t per = ta * tb;
+  for (uint64_t tile = blockIdx.x; tile < uint64_t(p.n) * per; tile += gridDim.x) {
+    const uint32_t e = uint32_t(tile / per), a0 = uint32_t(tile % per) % ta * 64, b0 = uint32_t(tile % per) / ta * 64;
+    const uint32_t first = p.first[e], n = p.first[e + 1] - first;
+    // (k runs over the pairs: element (r, k) at k stride + r)
+    struct Rows {
+      const u16* base;
+      uint64_t stride;
+      const uint32_t* map;
+      uint32_t rows, n;
+      __device__ __forceinline__ bits8 load8(uint32_t r, uint32_t k) const {
+        bits8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (r >= rows) return v;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i)
+          if (k + i < n) v[i] = base[uint64_t(map ? map[k + i] : k + i) * stride + r];
+        return v;
+      }
+    };
+    const Rows l{left_map ? left : left + first * left_stride, left_stride, left_map ? p.row + first : nullptr, n_left, n};
+    const Rows r{right_map ? right : right + first * right_stride, right_stride, right_map ? p.row + first : nullptr, n_right, n};
+    f32x4 acc[2][2] = {};
+    tile64<T, false>(l, a0, r, b0, n, m, acc);
+    each64(acc, [&](uint32_t i, uint32_t j, float v) {
+      if (a0 + i < n_left && b0 + j < n_right) out[(uint64_t(e) * n_right + b0 + j) * n_left + a0 + i] = T::down(v);
+    });
+    __syncthreads();
+  }
+}
+
+__global__ __launch_bounds__(256) void weights_grad_kernel(Plan p, uint32_t shares, const float* d_share, float* dweights) {
+  for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < p.pairs; i += uint64_t(gridDim.x) * 256) {
+    const int32_t at = p.at[i];
+    float s = 0.0f;
+    if (at >= 0)
+      for (uint32_t k = 0; k < shares; ++k) s += d_share[uint64_t(k) * p.pairs + uint32_t(at)];
+    dweights[i] = s;
+  }
+}
+
+// ---- the workspace --------------------------------------------------------------------------------------------------
+struct Room {
+  uint64_t bytes = 0;
+  char* base;
+  explicit Room(void* p) : base(static_cast<char*>(p)) {}
+  template <class V>
+  V* take(uint64_t n) {
+    V* p = reinterpret_cast<V*>(base + bytes);
+    bytes += up_to(n * sizeof(V), 256);
+    return p;
+  }
+};
+
+uint32_t most_tiles(uint32_t pairs, uint32_t n, uint32_t rows_per_tile) {
+  return pairs / rows_per_tile + (n < pairs ? n : pairs);
+}
+
+Plan take_plan(Room& r, uint32_t n, uint32_t pairs, uint32_t top_k, uint32_t rows_per_tile) {
+  Plan p;
+  p.part = r.take<const char*>(uint64_t(3) * n);
+  p.first = r.take<uint32_t>(n + 1);
+  p.pair = r.take<uint32_t>(pairs);
+  p.row = r.take<uint32_t>(pairs);
+  p.at = r.take<int32_t>(pairs);
+  p.tile = r.take<uint32_t>(uint64_t(2) * most_tiles(pairs, n, rows_per_tile));
+  p.n_tiles = r.take<uint32_t>(1);
+  p.pairs = pairs;
+  p.top_k = top_k;
+  p.n = n;
+  return p;
+}
+
+struct Forward {
+  Plan plan;
+  u16* h;
+  float* out;
+};
+Forward take_forward(Room& r, uint32_t n, uint32_t d, uint32_t f, uint32_t rows, uint32_t top_k) {
+  Forward w;
+  w.plan = take_plan(r, n, rows * top_k, top_k, 64);
+  w.h = r.take<u16>(uint64_t(rows) * top_k * f);
+  w.out = r.take<float>(uint64_t(rows) * top_k * d);
+  return w;
+}
+struct Backward {
+  Plan plan;
+  u16 *dgu, *wh;
+  float *share, *out;
+};
+Backward take_backward(Room& r, uint32_t n, uint32_t d, uint32_t f, uint32_t rows, uint32_t top_k) {
+  const uint64_t pairs = uint64_t(rows) * top_k;
+  Backward w;
+  w.plan = take_plan(r, n, uint32_t(pairs), top_k, 64);
+  w.dgu = r.take<u16>(pairs * 2 * f);
+  w.wh = r.take<u16>(pairs * f);
+  w.share = r.take<float>(pairs * ((f + 63) / 64));
+  w.out = r.take<float>(pairs * d);
+  return w;
+}
+
+uint32_t blocks(uint64_t n) { return uint32_t(n < (1u << 20) ? n : (1u << 20)); }
+
+int launch_plan(const ExpertMap& e, const int32_t* ids, const Plan& p, uint32_t rows_per_tile, hipStream_t s) {
+  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kPlanThreads), 4 * (kPlanThreads + kPlanWaves * e.n), s, e, ids, p,
+                     rows_per_tile);
+  return int(hipGetLastError());
+}
+
+template <class T, bool kQ4>
+int forward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& a, void* ws, hipStream_t s) {
+  Room room(ws);
+  const Forward w = take_forward(room, e.n, d, f, a.rows, a.top_k);
+  if (int err = launch_plan(e, a.ids, w.plan, 64, s)) return err;
+  const uint32_t tiles = most_tiles(w.plan.pairs, e.n, 64);
+  hipLaunchKernelGGL((gate_up_any_kernel<T, kQ4>), dim3(tiles * ((f + 63) / 64)), dim3(256), 0, s, w.plan,
+                     static_cast<const u16*>(a.x), a.x_stride, d, f, a.act, w.h);
+  hipLaunchKernelGGL((down_any_kernel<T, kQ4>), dim3(tiles * ((d + 63) / 64)), dim3(256), 0, s, w.plan, w.h, d, f, w.out);
+  hipLaunchKernelGGL((combine_kernel<T>), dim3(blocks((uint64_t(a.rows) * d + 255) / 256)), dim3(256), 0, s, w.plan, a.rows, d,
+                     w.out, a.weights, static_cast<const u16*>(a.residual), a.residual_stride, static_cast<u16*>(a.y),
+                     a.y_stride);
+  return int(hipGetLastError());
+}
+
+template <class T>
+int backward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_grad_args& a, void* ws, hipStream_t s) {
+  Room room(ws);
+  const Backward w = take_backward(room, e.n, d, f, a.rows, a.top_k);
+  if (int err = launch_plan(e, a.ids, w.plan, 64, s)) return err;
+  const uint32_t tiles = most_tiles(w.plan.pairs, e.n, 64), tf = (f + 63) / 64, td = (d + 63) / 64;
+  const u16 *x = static_cast<const u16*>(a.x), *dy = static_cast<const u16*>(a.dy);
+  if (tiles)
+    hipLaunchKernelGGL((hidden_grad_any_kernel<T>), dim3(tiles * tf), dim3(256), 0, s, w.plan, x, a.x_stride, dy, a.dy_stride,
+                       a.weights, d, f, a.act, w.dgu, w.wh, w.share);
+  if (a.dx && tiles) {
+    hipLaunchKernelGGL((input_grad_any_kernel<T>), dim3(tiles * td), dim3(256), 0, s, w.plan, w.dgu, d, f, w.out);
+    hipLaunchKernelGGL((combine_kernel<T>), dim3(blocks((uint64_t(a.rows) * d + 255) / 256)), dim3(256), 0, s, w.plan, a.rows,
+                       d, w.out, static_cast<const float*>(nullptr), static_cast<const u16*>(nullptr), uint64_t(0),
+                       static_cast<u16*>(a.dx), a.dx_stride);
+  }
+  if (a.dweights && tiles)
+    hipLaunchKernelGGL(weights_grad_kernel, dim3(blocks((w.plan.pairs + 255) / 256)), dim3(256), 0, s, w.plan, tf, w.share,
+                       a.dweights);
+  if (a.dgate) {
+    const uint32_t g = blocks(uint64_t(e.n) * tf * td);
+    for (int half = 0; half < 2; ++half)
+      hipLaunchKernelGGL((weight_grad_any_kernel<T>), dim3(g), dim3(256), 0, s, w.plan, x, a.x_stride, true, d,
+                         w.dgu + half * uint64_t(f), uint64_t(2) * f, false, f, static_cast<u16*>(half ? a.dup : a.dgate));
+    hipLaunchKernelGGL((weight_grad_any_kernel<T>), dim3(g), dim3(256), 0, s, w.plan, w.wh, uint64_t(f), false, f, dy,
+                       a.dy_stride, true, d, static_cast<u16*>(a.ddown));
+  }
+  return int(hipGetLastError());
+}
+
+}  // namespace
+}  // namespace op
+
+uint64_t ffn_workspace(uint32_t n, uint32_t d, uint32_t f, uint32_t, uint32_t rows, uint32_t top_k) {
+  op::Room room(nullptr);
+  op::take_forward(room, n, d, f, rows, top_k);
+  return room.bytes;
+}
+int launch_ffn(const ExpertMap& e, uint32_t d, uint32_t f, uint32_t w_type, const tsa_ffn_args& a, void* ws,
+               hipStream_t stream) {
+  if (a.rows == 0) return 0;
+  const bool q4 = w_type == TSA_Q4;
+  if (a.type == TSA_BF16)
+    return q4 ? op::forward<op::Bf16, true>(e, d, f, a, ws, stream) : op::forward<op::Bf16, false>(e, d, f, a, ws, stream);
+  return q4 ? op::forward<op::F16, true>(e, d, f, a, ws, stream) : op::forward<op::F16, false>(e, d, f, a, ws, stream);
+}
+
+uint64_t ffn_backward_workspace(uint32_t n, uint32_t d, uint32_t f, uint32_t rows, uint32_t top_k) {
+  op::Room room(nullptr);
+  op::take_backward(room, n, d, f, rows, top_k);
+  return room.bytes;
+}
+int launch_ffn_backward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_grad_args& a, void* ws, hipStream_t stream) {
+  return a.type == TSA_BF16 ? op::backward<op::Bf16>(e, d, f, a, ws, stream) : op::backward<op::F16>(e, d, f, a, ws, stream);
+}
+
+}  // namespace tsa
