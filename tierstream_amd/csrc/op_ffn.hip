@@ -7,7 +7,7 @@
 //              d down = dy^T (w h) over an expert's pairs.
 // h, dg, du and w h are rounded once to the operands' 16 bits, as the matrix instructions take them; y' and dx' stay in
 // 32 bits until the row's sum, and w is applied there or before the rounding. No sum depends on an order that changes.
-#include "op_device.hpp"
+#include "op_stream.hpp"
 
 namespace tsa {
 namespace op {
@@ -191,6 +191,150 @@ __global__ __launch_bounds__(256) void down_any_kernel(Plan p, const u16* h, uin
   });
 }
 
+// ---- few rows: the weights' bytes -------------------------------------------------------------------------------------
+// The part pointers of an expert in LDS, by thread 0 of the workgroup; false (to every thread) if there is none.
+__device__ __forceinline__ bool resolve(const ExpertMap& m, uint32_t e, const char* (&p)[3]) {
+  if (e == ~0u) return false;
+  part_pointers(m, e, p);
+  return true;
+}
+
+// One row of x: pair j is blockIdx.y, h_j = w_j act(gate x) (up x) for 16 columns a workgroup.
+template <class T, class W, bool kTail>
+__global__ __launch_bounds__(64 * most_waves(1)) void gate_up_one_kernel(ExpertMap m, const int32_t* ids, const float* weights,
+                                                                         const u16* x, uint32_t d, uint32_t f, uint32_t act,
+                                                                         u16* h) {
+  extern __shared__ f32x4 part[];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const char* p[3];
+  if (!resolve(m, expert_of(m, ids, blockIdx.y), p)) return;
+  const uint32_t c0 = blockIdx.x * 16 + (lane & 15u), col = c0 < f ? c0 : f - 1;
+  f32x4 acc[2][1] = {};
+  stream_chunks<W, 2, 1, kTail>((d + kChunk - 1) / kChunk, wave, waves, [&](uint32_t c, W (&w)[2], const u16* (&row)[1]) {
+    w[0] = W(p[0], d, col, d);
+    w[1] = W(p[1], d, col, d);
+    row[0] = x;
+    return c * kChunk;
+  }, acc);
+  const f32x4 v[2] = {acc[0][0], acc[1][0]};
+  join_waves<2>(part, v, wave, waves, [&](auto&& sum) {
+    if (wave != 0) return;
+    const float g = sum(0)[0], u = sum(1)[0];
+    if (lane < 16 && c0 < f) h[uint64_t(blockIdx.y) * f + c0] = T::down((weights ? weights[blockIdx.y] : 1.0f) * activate(act, g) * u);
+  });
+}
+
+// y = residual + sum_j down_j h_j: one row over the chunks of all its experts.
+template <class T, class W, bool kTail>
+__global__ __launch_bounds__(64 * most_waves(1)) void down_one_kernel(ExpertMap m, const int32_t* ids, uint32_t top_k,
+                                                                      const u16* h, uint32_t d, uint32_t f,
+                                                                      const u16* residual, u16* y) {
+  extern __shared__ f32x4 part[];
+  __shared__ const char* down[TSA_ROUTE_MAX_TOP_K];
+  __shared__ uint32_t from[TSA_ROUTE_MAX_TOP_K], n_live;
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  if (wave == 0) {
+    const char* p[3];
+    const bool on = lane < top_k && resolve(m, expert_of(m, ids, lane), p);
+    const uint64_t live = __ballot(on);
+    if (on) {
+      const uint32_t i = uint32_t(__popcll(live & ((1ull << lane) - 1)));
+      down[i] = p[2];
+      from[i] = lane;
+    }
+    if (lane == 0) n_live = uint32_t(__popcll(live));
+  }
+  __syncthreads();
+  const uint32_t c0 = blockIdx.x * 16 + (lane & 15u), col = c0 < d ? c0 : d - 1, per = (f + kChunk - 1) / kChunk;
+  f32x4 acc[1][1] = {};
+  stream_chunks<W, 1, 1, kTail>(n_live * per, wave, waves, [&](uint32_t c, W (&w)[1], const u16* (&row)[1]) {
+    const uint32_t j = c / per;
+    w[0] = W(down[j], f, col, f);
+    row[0] = h + uint64_t(from[j]) * f;
+    return (c - j * per) * kChunk;
+  }, acc);
+  const f32x4 v[1] = {acc[0][0]};
+  join_waves<1>(part, v, wave, waves, [&](auto&& sum) {
+    if (wave != 0) return;
+    const float s = sum(0)[0] + (residual && c0 < d ? T::up(residual[c0]) : 0.0f);
+    if (lane < 16 && c0 < d) y[c0] = T::down(s);
+  });
+}
+
+// A tile of at most 16 CT pairs of one expert, 16 columns of gate and up a workgroup.
+template <class T, class W, int CT, bool kTail>
+__global__ __launch_bounds__(64 * most_waves(CT)) void gate_up_few_kernel(Plan p, const u16* x, uint64_t x_stride, uint32_t d,
+                                                                          uint32_t f, uint32_t act, u16* h) {
+  extern __shared__ f32x4 part[];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  TileRows t;
+  if (!tile_rows(p, blockIdx.y, 16 * CT, t)) return;
+  const char *gate = p.part[3 * t.e], *up = p.part[3 * t.e + 1];
+  const uint32_t c0 = blockIdx.x * 16 + (lane & 15u), col = c0 < f ? c0 : f - 1;
+  const u16* rows[CT];
+#pragma unroll
+  for (int i = 0; i < CT; ++i) {
+    const uint32_t r = 16 * i + (lane & 15u);
+    rows[i] = r < t.rows ? x + t.map[r] * x_stride : nullptr;
+  }
+  f32x4 acc[2][CT] = {};
+  stream_chunks<W, 2, CT, kTail>((d + kChunk - 1) / kChunk, wave, waves, [&](uint32_t c, W (&w)[2], const u16* (&row)[CT]) {
+    w[0] = W(gate, d, col, d);
+    w[1] = W(up, d, col, d);
+#pragma unroll
+    for (int i = 0; i < CT; ++i) row[i] = rows[i];
+    return c * kChunk;
+  }, acc);
+  f32x4 v[2 * CT];
+#pragma unroll
+  for (int i = 0; i < 2 * CT; ++i) v[i] = acc[i / CT][i % CT];
+  join_waves<2 * CT>(part, v, wave, waves, [&](auto&& sum) {
+    for (uint32_t i = wave; i < CT; i += waves) {
+      const f32x4 g = sum(i), u = sum(CT + i);
+#pragma unroll
+      for (uint32_t q = 0; q < 4; ++q) {
+        const uint32_t r = 16 * i + (lane >> 4) * 4 + q;
+        if (r < t.rows && c0 < f) h[uint64_t(t.first + r) * f + c0] = T::down(activate(act, g[q]) * u[q]);
+      }
+    }
+  });
+}
+
+template <class T, class W, int CT, bool kTail>
+__global__ __launch_bounds__(64 * most_waves(CT)) void down_few_kernel(Plan p, const u16* h, uint32_t d, uint32_t f, float* out) {
+  extern __shared__ f32x4 part[];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  TileRows t;
+  if (!tile_rows(p, blockIdx.y, 16 * CT, t)) return;
+  const char* down = p.part[3 * t.e + 2];
+  const uint32_t c0 = blockIdx.x * 32 + (lane & 15u);
+  f32x4 acc[2][CT] = {};
+  stream_chunks<W, 2, CT, kTail>((f + kChunk - 1) / kChunk, wave, waves, [&](uint32_t c, W (&w)[2], const u16* (&row)[CT]) {
+    w[0] = W(down, f, c0 < d ? c0 : d - 1, f);
+    w[1] = W(down, f, c0 + 16 < d ? c0 + 16 : d - 1, f);
+#pragma unroll
+    for (uint32_t i = 0; i < CT; ++i) {
+      const uint32_t r = 16 * i + (lane & 15u);
+      row[i] = r < t.rows ? h + uint64_t(t.first + r) * f : nullptr;
+    }
+    return c * kChunk;
+  }, acc);
+  f32x4 v[2 * CT];
+#pragma unroll
+  for (int i = 0; i < 2 * CT; ++i) v[i] = acc[i / CT][i % CT];
+  join_waves<2 * CT>(part, v, wave, waves, [&](auto&& sum) {
+    for (uint32_t i = wave; i < 2 * CT; i += waves) {
+      const f32x4 s = sum(i);
+      const uint32_t c = c0 + 16 * (i / CT);
+#pragma unroll
+      for (uint32_t q = 0; q < 4; ++q) {
+        const uint32_t r = 16 * (i % CT) + (lane >> 4) * 4 + q;
+        if (r < t.rows && c < d) out[uint64_t(t.first + r) * d + c] = s[q];
+      }
+    }
+  });
+}
+
 // out_t = residual_t + sum_j w_tj v_{at(t, j)}, in the order of j
 template <class T>
 __global__ __launch_bounds__(256) void combine_kernel(Plan p, uint32_t rows, uint32_t d, const float* v, const float* weights,
@@ -358,7 +502,7 @@ struct Forward {
 };
 Forward take_forward(Room& r, uint32_t n, uint32_t d, uint32_t f, uint32_t rows, uint32_t top_k) {
   Forward w;
-  w.plan = take_plan(r, n, rows * top_k, top_k, 64);
+  w.plan = take_plan(r, n, rows * top_k, top_k, 16);  // (the smallest tiles any path takes)
   w.h = r.take<u16>(uint64_t(rows) * top_k * f);
   w.out = r.take<float>(uint64_t(rows) * top_k * d);
   return w;
@@ -387,8 +531,66 @@ int launch_plan(const ExpertMap& e, const int32_t* ids, const Plan& p, uint32_t 
   return int(hipGetLastError());
 }
 
+bool aligned16(const void* p, uint64_t stride_bytes) { return (reinterpret_cast<uintptr_t>(p) | stride_bytes) % 16 == 0; }
+
+// Whether every weight row, x row and row of h starts 16-byte aligned and holds whole groups of 8 values. The addresses of
+// a table's units are the device's: its units are 256-byte aligned, as the library lays them out.
+bool wide_rows(const ExpertMap& e, uint32_t d, uint32_t f, bool q4, const void* x, uint64_t x_stride) {
+  if (d % 8 || f % 8 || !aligned16(x, 2 * x_stride)) return false;
+  if (q4) return true;
+  for (int p = 0; p < 3; ++p) {
+    if (e.form == 0 && !aligned16(e.part[p], e.stride[p])) return false;
+    if (e.form == 1 && e.stride[p] % 16) return false;
+    if (e.form == 2 && !aligned16(e.view.parts[p].base, e.view.parts[p].stride)) return false;
+  }
+  return true;
+}
+
+template <class T, class W, bool kTail>
+int forward_one(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& a, void* ws, hipStream_t s) {
+  u16* h = static_cast<u16*>(ws);
+  const uint32_t tf = (f + 15) / 16, td = (d + 15) / 16;
+  const uint32_t w1 = stream_waves(uint64_t(tf) * a.top_k, chunks_of(d), 16);
+  hipLaunchKernelGGL((gate_up_one_kernel<T, W, kTail>), dim3(tf, a.top_k), dim3(64 * w1), w1 * 2048, s, e, a.ids, a.weights,
+                     static_cast<const u16*>(a.x), d, f, a.act, h);
+  const uint32_t w2 = stream_waves(td, uint64_t(chunks_of(f)) * a.top_k, 16);
+  hipLaunchKernelGGL((down_one_kernel<T, W, kTail>), dim3(td), dim3(64 * w2), w2 * 1024, s, e, a.ids, a.top_k, h, d, f,
+                     static_cast<const u16*>(a.residual), static_cast<u16*>(a.y));
+  return int(hipGetLastError());
+}
+
+template <class T, class W, int CT, bool kTail>
+int forward_few(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& a, const Forward& w, hipStream_t s) {
+  if (int err = launch_plan(e, a.ids, w.plan, 16 * CT, s)) return err;
+  const uint32_t tiles = most_tiles(w.plan.pairs, e.n, 16 * CT), tf = (f + 15) / 16, td = (d + 31) / 32;
+  const uint32_t w1 = stream_waves(uint64_t(tf) * tiles, chunks_of(d), most_waves(CT));
+  hipLaunchKernelGGL((gate_up_few_kernel<T, W, CT, kTail>), dim3(tf, tiles), dim3(64 * w1), w1 * CT * 2048, s, w.plan,
+                     static_cast<const u16*>(a.x), a.x_stride, d, f, a.act, w.h);
+  const uint32_t w2 = stream_waves(uint64_t(td) * tiles, chunks_of(f), most_waves(CT));
+  hipLaunchKernelGGL((down_few_kernel<T, W, CT, kTail>), dim3(td, tiles), dim3(64 * w2), w2 * CT * 2048, s, w.plan, w.h, d, f,
+                     w.out);
+  hipLaunchKernelGGL((combine_kernel<T>), dim3(blocks((uint64_t(a.rows) * d + 255) / 256)), dim3(256), 0, s, w.plan, a.rows, d,
+                     w.out, a.weights, static_cast<const u16*>(a.residual), a.residual_stride, static_cast<u16*>(a.y),
+                     a.y_stride);
+  return int(hipGetLastError());
+}
+
+template <class T, class W, bool kTail>
+int forward_stream(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& a, void* ws, hipStream_t s) {
+  if (a.rows == 1) return forward_one<T, W, kTail>(e, d, f, a, ws, s);
+  Room room(ws);
+  const Forward w = take_forward(room, e.n, d, f, a.rows, a.top_k);
+  const uint32_t each = w.plan.pairs / e.n;  // pairs of an expert if all are asked for alike
+  if (each <= 8) return forward_few<T, W, 1, kTail>(e, d, f, a, w, s);
+  if (each <= 24) return forward_few<T, W, 2, kTail>(e, d, f, a, w, s);
+  return forward_few<T, W, 4, kTail>(e, d, f, a, w, s);
+}
+
 template <class T, bool kQ4>
 int forward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& a, void* ws, hipStream_t s) {
+  typedef std::conditional_t<kQ4, RowsQ4<T>, Rows16<T>> W;
+  if (wide_rows(e, d, f, kQ4, a.x, a.x_stride) && uint64_t(a.rows) * a.top_k <= uint64_t(64) * e.n)
+    return d % kChunk || f % kChunk ? forward_stream<T, W, true>(e, d, f, a, ws, s) : forward_stream<T, W, false>(e, d, f, a, ws, s);
   Room room(ws);
   const Forward w = take_forward(room, e.n, d, f, a.rows, a.top_k);
   if (int err = launch_plan(e, a.ids, w.plan, 64, s)) return err;

@@ -1,5 +1,5 @@
 // y = act(x W^T + bias) + residual.
-#include "op_device.hpp"
+#include "op_stream.hpp"
 
 namespace tsa {
 namespace op {
@@ -34,6 +34,61 @@ __global__ __launch_bounds__(256) void linear_any_kernel(tsa_linear_args a) {
   }
 }
 
+// Few rows: a workgroup takes 16 R weight rows and 16 CT rows of x.
+template <class T, class W, int R, int CT, bool kTail>
+__global__ __launch_bounds__(64 * most_waves(CT)) void linear_few_kernel(tsa_linear_args a) {
+  extern __shared__ f32x4 part[];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const uint32_t n0 = blockIdx.x * 16 * R, r0 = blockIdx.y * 16 * CT;
+  f32x4 acc[R][CT] = {};
+  stream_chunks<W, R, CT, kTail>((a.n_in + kChunk - 1) / kChunk, wave, waves, [&](uint32_t c, W (&w)[R], const u16* (&x)[CT]) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const uint32_t n = n0 + 16 * r + (lane & 15u);
+      w[r] = W(a.w, a.w_stride, n < a.n_out ? n : a.n_out - 1, a.n_in);
+    }
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+      const uint32_t row = a.rows == 1 ? 0 : r0 + 16 * t + (lane & 15u);
+      x[t] = row < a.rows ? static_cast<const u16*>(a.x) + row * a.x_stride : nullptr;
+    }
+    return c * kChunk;
+  }, acc);
+  f32x4 v[R * CT];
+#pragma unroll
+  for (int i = 0; i < R * CT; ++i) v[i] = acc[i / CT][i % CT];
+  join_waves<R * CT>(part, v, wave, waves, [&](auto&& sum) {
+    for (uint32_t i = wave; i < R * CT; i += waves) {
+      const f32x4 s = sum(i);
+      const uint32_t n = n0 + 16 * (i / CT) + (lane & 15u), row = r0 + 16 * (i % CT) + (lane >> 4) * 4;
+      if (n >= a.n_out) continue;
+#pragma unroll
+      for (uint32_t q = 0; q < 4; ++q)
+        if (row + q < a.rows) finish_linear(a, row + q, n, s[q]);
+    }
+  });
+}
+
+template <class T, class W, int R, int CT>
+int launch_few(const tsa_linear_args& a, hipStream_t stream) {
+  const uint32_t tn = (a.n_out + 16 * R - 1) / (16 * R), tr = (a.rows + 16 * CT - 1) / (16 * CT);
+  const uint32_t waves = stream_waves(uint64_t(tn) * tr, chunks_of(a.n_in), most_waves(CT));
+  if (a.n_in % kChunk)
+    hipLaunchKernelGGL((linear_few_kernel<T, W, R, CT, true>), dim3(tn, tr), dim3(64 * waves), waves * R * CT * 1024, stream, a);
+  else
+    hipLaunchKernelGGL((linear_few_kernel<T, W, R, CT, false>), dim3(tn, tr), dim3(64 * waves), waves * R * CT * 1024, stream, a);
+  return int(hipGetLastError());
+}
+
+template <class T, class W>
+int launch_few(const tsa_linear_args& a, hipStream_t stream) {
+  if (a.rows <= 16) return a.n_out >= 16384 ? launch_few<T, W, 2, 1>(a, stream) : launch_few<T, W, 1, 1>(a, stream);
+  if (a.rows <= 32) return launch_few<T, W, 2, 2>(a, stream);
+  return launch_few<T, W, 2, 4>(a, stream);
+}
+
+bool aligned16(const void* p, uint64_t stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0; }
+
 }  // namespace
 }  // namespace op
 
@@ -41,6 +96,14 @@ uint64_t linear_workspace(const tsa_linear_args&) { return 0; }
 
 int launch_linear(const tsa_linear_args& a, void*, hipStream_t stream) {
   if (a.rows == 0 || a.n_out == 0) return 0;
+  const bool wide = a.n_in % 8 == 0 && op::aligned16(a.x, a.x_stride) && (a.w_type == TSA_Q4 || op::aligned16(a.w, a.w_stride));
+  if (wide && a.rows <= 64) {
+    if (a.x_type == TSA_BF16)
+      return a.w_type == TSA_Q4 ? op::launch_few<op::Bf16, op::RowsQ4<op::Bf16>>(a, stream)
+                                : op::launch_few<op::Bf16, op::Rows16<op::Bf16>>(a, stream);
+    return a.w_type == TSA_Q4 ? op::launch_few<op::F16, op::RowsQ4<op::F16>>(a, stream)
+                              : op::launch_few<op::F16, op::Rows16<op::F16>>(a, stream);
+  }
   const uint64_t tiles = (uint64_t(a.n_out) + 63) / 64 * ((uint64_t(a.rows) + 63) / 64);
   const dim3 grid(uint32_t(tiles < (1u << 20) ? tiles : (1u << 20)));
 #define CALL(T, Q) hipLaunchKernelGGL((op::linear_any_kernel<op::T, Q>), grid, dim3(256), 0, stream, a)

@@ -1,0 +1,222 @@
+// Products of weights with few rows of x (at most 64): bound by the bytes of the weights, which cross memory once and go
+// straight to registers in the layout the matrix instruction takes, without LDS.
+//
+// The result column of v_mfma_f32_16x16x32 (operand b) is a weight row, the result row (operand a) a row of x: lane l holds
+// weight row l % 16 at 8 values of each 32, and of the result the x rows 4 (l / 16) + 0..3. The order of the 32 values
+// inside a step is free as long as both operands use the same, so a 4-bit lane takes the 4 bytes 4 (l / 16).. of a block
+// in one load: values 4 (l / 16) + 0..3 from their low halves, 16 more from their high ones.
+//
+// The waves of a workgroup take turns along the row in chunks of 128 values, each with the next chunk's loads in flight
+// while it multiplies this one's, and add up through LDS. x is read from the caches.
+#pragma once
+
+#include "op_device.hpp"
+
+namespace tsa {
+namespace op {
+
+constexpr uint32_t kChunk = 128;  // values of a weight row per chunk: 4 steps
+
+typedef __attribute__((address_space(1))) const bits8 gbits8_t;
+typedef __attribute__((address_space(1))) const bits4 gbits4_t;
+
+__device__ __forceinline__ bits8 load_bits8(const u16* p) {
+  return *reinterpret_cast<gbits8_t*>(reinterpret_cast<uintptr_t>(p));
+}
+
+// Weights are read once: past the caches.
+__device__ __forceinline__ bits8 load_stream(const u16* p) {
+  return __builtin_nontemporal_load(reinterpret_cast<gbits8_t*>(reinterpret_cast<uintptr_t>(p)));
+}
+
+// 16-bit weight rows: base at row 0, `stride` values apart, rows and pointers 16-byte aligned, n a multiple of 8.
+template <class T>
+struct Rows16 {
+  struct Chunk {
+    bits8 v[4];
+  };
+  const u16* p;  // this lane's row at its first value
+  uint32_t n;
+  Rows16() = default;
+  __device__ __forceinline__ Rows16(const void* base, uint64_t stride, uint32_t row, uint32_t n_) : n(n_) {
+    p = static_cast<const u16*>(base) + row * stride + (threadIdx.x & 48u) / 2;
+  }
+  // The chunk at k; kTail: the row may end inside it (zeros from there on).
+  template <bool kTail>
+  __device__ __forceinline__ void load(Chunk& c, uint32_t k) const {
+    const uint32_t q = (threadIdx.x & 48u) / 2;
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+      c.v[s] = !kTail || k + 32 * s + q < n ? load_stream(p + k + 32 * s) : bits8{0, 0, 0, 0, 0, 0, 0, 0};
+  }
+  // Values of x for the step at k, from its row.
+  template <bool kTail>
+  static __device__ __forceinline__ bits8 x_at(const u16* row, uint32_t k, uint32_t n) {
+    const uint32_t at = k + (threadIdx.x & 48u) / 2;
+    return !kTail || at < n ? load_bits8(row + at) : bits8{0, 0, 0, 0, 0, 0, 0, 0};
+  }
+  template <int R, int CT>
+  static __device__ __forceinline__ void multiply(const Chunk (&c)[R], int s, const bits8 (&x)[CT], f32x4 (&acc)[R][CT]) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int t = 0; t < CT; ++t) acc[r][t] = T::mfma(x[t], c[r].v[s], acc[r][t]);
+  }
+};
+
+// 4-bit halves as 16-bit floating values, offset so that it takes a byte permutation: bf16 holds 16 + q as 0x4180 + 8 q,
+// half precision 1024 + q as 0x6400 + q. The offset's part of the sum is taken off with a product of x and the constant
+// (exact: -24 and -1032 have a short form in either type): bf16 keeps 24 instead of 136 so that it cancels few bits.
+template <class T>
+struct HalfBytes;
+template <>
+struct HalfBytes<Bf16> {
+  static constexpr u16 kMinus = 0xC1C0;  // -24
+  static __device__ __forceinline__ bits8 unpack(uint32_t v) {
+    const uint32_t lo = ((v << 3) & 0x78787878u) | 0x80808080u, hi = ((v >> 1) & 0x78787878u) | 0x80808080u;
+    const u32x4 r = {__builtin_amdgcn_perm(0x41414141u, lo, 0x04010400u), __builtin_amdgcn_perm(0x41414141u, lo, 0x04030402u),
+                     __builtin_amdgcn_perm(0x41414141u, hi, 0x04010400u), __builtin_amdgcn_perm(0x41414141u, hi, 0x04030402u)};
+    return __builtin_bit_cast(bits8, r);
+  }
+};
+template <>
+struct HalfBytes<F16> {
+  static constexpr u16 kMinus = 0xCE00;  // -24
+  // 16 + q as 0x4C00 + 64 q: the byte pair (0x4C + q / 4, 64 (q % 4)) by shifting the half byte over the pair
+  static __device__ __forceinline__ bits8 unpack(uint32_t v) {
+    const uint32_t lo = v & 0x0F0F0F0Fu, hi = (v >> 4) & 0x0F0F0F0Fu;
+    const u32x4 r = {(__builtin_amdgcn_perm(0, lo, 0x0C010C00u) << 6) | 0x4C004C00u,
+                     (__builtin_amdgcn_perm(0, lo, 0x0C030C02u) << 6) | 0x4C004C00u,
+                     (__builtin_amdgcn_perm(0, hi, 0x0C010C00u) << 6) | 0x4C004C00u,
+                     (__builtin_amdgcn_perm(0, hi, 0x0C030C02u) << 6) | 0x4C004C00u};
+    return __builtin_bit_cast(bits8, r);
+  }
+};
+
+// Rows of 4-bit blocks back to back (n / 32 blocks each), 4-byte aligned at the base. A step is one block: its products
+// are summed in whole steps of the scale, which is applied to the sum in 32 bits.
+template <class T>
+struct RowsQ4 {
+  struct Chunk {
+    uint32_t v[4];
+    u16 scale[4];
+  };
+  const unsigned char* p;  // this lane's row, first block
+  uint32_t n;
+  RowsQ4() = default;
+  __device__ __forceinline__ RowsQ4(const void* base, uint64_t, uint32_t row, uint32_t n_) : n(n_) {
+    p = static_cast<const unsigned char*>(base) + uint64_t(row) * (n_ / kQ4Block * kQ4Bytes);
+  }
+  struct __attribute__((packed, aligned(2))) Word {
+    uint32_t v;
+  };
+  typedef __attribute__((address_space(1))) const Word gword_t;
+  typedef __attribute__((address_space(1))) const u16 ghalf_t;
+  __device__ __forceinline__ void load_block(Chunk& c, int s, uint32_t k) const {
+    const uintptr_t b = reinterpret_cast<uintptr_t>(p) + (k / kQ4Block) * kQ4Bytes;
+    c.scale[s] = *reinterpret_cast<ghalf_t*>(b);
+    c.v[s] = reinterpret_cast<gword_t*>(b + 2 + (threadIdx.x & 48u) / 4)->v;
+  }
+  template <bool kTail>
+  __device__ __forceinline__ void load(Chunk& c, uint32_t k) const {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      if (kTail) c.scale[s] = 0, c.v[s] = 0;
+      if (!kTail || k + 32 * s < n) load_block(c, s, k + 32 * s);
+    }
+  }
+  template <bool kTail>
+  static __device__ __forceinline__ bits8 x_at(const u16* row, uint32_t k, uint32_t n) {
+    if (kTail && k >= n) return bits8{0, 0, 0, 0, 0, 0, 0, 0};
+    const uintptr_t at = reinterpret_cast<uintptr_t>(row + k + (threadIdx.x & 48u) / 4);
+    const bits4 lo = *reinterpret_cast<gbits4_t*>(at), hi = *reinterpret_cast<gbits4_t*>(at + 32);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  template <int R, int CT>
+  static __device__ __forceinline__ void multiply(const Chunk (&c)[R], int s, const bits8 (&x)[CT], f32x4 (&acc)[R][CT]) {
+    constexpr u16 m = HalfBytes<T>::kMinus;
+    bits8 w[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) w[r] = HalfBytes<T>::unpack(c[r].v[s]);
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+      const f32x4 off = T::mfma(x[t], bits8{m, m, m, m, m, m, m, m}, f32x4{0, 0, 0, 0});
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const f32x4 sum = T::mfma(x[t], w[r], off);
+        const float scale = F16::up(c[r].scale[s]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[r][t][i] += scale * sum[i];
+      }
+    }
+  }
+};
+
+// acc[r][t] += chunks wave, wave + waves, .. below n_chunks. at(c, w, row) gives chunk c's weight rows w[r], this lane's x
+// row of each tile (operand a: lane l gives row l % 16; with one row in all, every lane gives it; null for none) and
+// returns its first value k. The next chunk's x is loaded with its weights: loads return in order, so one issued later
+// would wait for all of them.
+template <class W, int R, int CT, bool kTail, class At>
+__device__ __forceinline__ void stream_chunks(uint32_t n_chunks, uint32_t wave, uint32_t waves, At&& at, f32x4 (&acc)[R][CT]) {
+  struct Step {
+    typename W::Chunk c[R];
+    bits8 x[4][CT];
+  };
+  auto load = [&](Step& b, uint32_t c) {
+    W w[R];
+    const u16* row[CT];
+    const uint32_t k = at(c, w, row);
+#pragma unroll
+    for (int r = 0; r < R; ++r) w[r].template load<kTail>(b.c[r], k);
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int t = 0; t < CT; ++t)
+        b.x[s][t] = row[t] ? W::template x_at<kTail>(row[t], k + 32 * s, w[0].n) : bits8{0, 0, 0, 0, 0, 0, 0, 0};
+  };
+  auto multiply = [&](const Step& b) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) W::template multiply<R, CT>(b.c, s, b.x[s], acc);
+  };
+  uint32_t c = wave;
+  if (c >= n_chunks) return;
+  Step now;
+  load(now, c);
+  for (; c + waves < n_chunks; c += waves) {
+    Step next;
+    load(next, c + waves);
+    multiply(now);
+    now = next;
+  }
+  multiply(now);
+}
+
+// The waves' sums added in their order: part[wave][i][lane], i over the wave's V vectors; thread (wave, lane) calls
+// f(i, lane, sum) for i = wave, wave + waves, ... of `use` vectors.
+template <int V, class F>
+__device__ __forceinline__ void join_waves(f32x4* part, const f32x4 (&v)[V], uint32_t wave, uint32_t waves, F&& f) {
+  const uint32_t lane = threadIdx.x & 63u;
+#pragma unroll
+  for (int i = 0; i < V; ++i) part[(wave * V + i) * 64 + lane] = v[i];
+  __syncthreads();
+  f([&](uint32_t i) {
+    f32x4 s = part[i * 64 + lane];
+    for (uint32_t w = 1; w < waves; ++w) s += part[(w * V + i) * 64 + lane];
+    return s;
+  });
+}
+
+// The registers of CT tiles of x bound the waves of a workgroup.
+constexpr uint32_t most_waves(int CT) { return CT == 1 ? 16 : CT == 2 ? 8 : 4; }
+
+// Waves per workgroup: enough that the launch has about 8 a CU (256 CUs), at least 2 chunks each, a power of two.
+inline uint32_t stream_waves(uint64_t workgroups, uint64_t chunks, uint32_t most) {
+  uint32_t w = 4;
+  while (w < most && workgroups * w < 2048) w *= 2;
+  while (w > 1 && w * 2 > chunks) w /= 2;
+  return w;
+}
+inline uint32_t chunks_of(uint32_t n) { return (n + kChunk - 1) / kChunk; }
+
+}  // namespace op
+}  // namespace tsa
