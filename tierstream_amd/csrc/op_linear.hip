@@ -1,5 +1,6 @@
 // y = act(x W^T + bias) + residual.
 #include "op_stream.hpp"
+#include "op_tile.hpp"
 
 namespace tsa {
 namespace op {
@@ -10,6 +11,42 @@ __device__ __forceinline__ void finish_linear(const tsa_linear_args& a, uint32_t
   v = activate(a.act, v);
   if (a.residual) v += load_as_float(a.residual, uint64_t(row) * a.residual_stride + n, a.y_type);
   store_float(a.y, uint64_t(row) * a.y_stride + n, a.y_type, v);
+}
+
+// Four values next to each other, in one access where the rows start so that it is aligned.
+__device__ __forceinline__ void finish_linear4(const tsa_linear_args& a, uint32_t row, uint32_t n, f32x4 v) {
+  const uint64_t size = a.y_type == TSA_F32 ? 4 : 2;
+  const uint64_t odd = (reinterpret_cast<uintptr_t>(a.y) | a.y_stride * size | reinterpret_cast<uintptr_t>(a.residual) |
+                        a.residual_stride * size) & (4 * size - 1);
+  if (odd || n + 4 > a.n_out || (reinterpret_cast<uintptr_t>(a.bias) & 7u)) {
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+      if (n + i < a.n_out) finish_linear(a, row, n + i, v[i]);
+    return;
+  }
+  const auto up = [&](u16 b) { return a.x_type == TSA_BF16 ? Bf16::up(b) : F16::up(b); };
+  if (a.bias) {
+    const bits4 b = *reinterpret_cast<const bits4*>(static_cast<const u16*>(a.bias) + n);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += up(b[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = activate(a.act, v[i]);
+  const uint64_t at = uint64_t(row) * a.y_stride + n, from = uint64_t(row) * a.residual_stride + n;
+  if (a.y_type == TSA_F32) {
+    if (a.residual) v += *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.residual) + from);
+    *reinterpret_cast<f32x4*>(static_cast<float*>(a.y) + at) = v;
+    return;
+  }
+  if (a.residual) {
+    const bits4 r = *reinterpret_cast<const bits4*>(static_cast<const u16*>(a.residual) + from);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += up(r[i]);
+  }
+  bits4 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = a.y_type == TSA_BF16 ? Bf16::down(v[i]) : F16::down(v[i]);
+  *reinterpret_cast<bits4*>(static_cast<u16*>(a.y) + at) = o;
 }
 
 template <class T, bool kQ4>
@@ -82,9 +119,38 @@ int launch_few(const tsa_linear_args& a, hipStream_t stream) {
 
 template <class T, class W>
 int launch_few(const tsa_linear_args& a, hipStream_t stream) {
-  if (a.rows <= 16) return a.n_out >= 16384 ? launch_few<T, W, 2, 1>(a, stream) : launch_few<T, W, 1, 1>(a, stream);
+  if (a.rows <= 16) return launch_few<T, W, 1, 1>(a, stream);
   if (a.rows <= 32) return launch_few<T, W, 2, 2>(a, stream);
   return launch_few<T, W, 2, 4>(a, stream);
+}
+
+// Many rows: tiles of 256 weight rows and 32 MJ rows of x.
+template <class T, int MJ, int NB>
+__global__ __launch_bounds__(kTileThreads) void linear_tile_kernel(tsa_linear_args a) {
+  extern __shared__ f32x4 memory[];
+  const uint32_t wave = threadIdx.x >> 6;
+  const TileAt t = tile_at(blockIdx.x, (a.n_out + 255) / 256, (a.rows + 32 * MJ - 1) / (32 * MJ));
+  const uint32_t n0 = t.a * 256, r0 = t.b * 32 * MJ;
+  TileRowsSource<8> w(a.n_in, wave & 1u, [&](uint32_t r) {
+    const uint32_t n = n0 + r;
+    return static_cast<const u16*>(a.w) + (n < a.n_out ? n : a.n_out - 1) * a.w_stride;
+  });
+  TileRowsSource<MJ> x(a.n_in, wave >> 1, [&](uint32_t r) {
+    const uint32_t row = r0 + r;
+    return static_cast<const u16*>(a.x) + (row < a.rows ? row : a.rows - 1) * a.x_stride;
+  });
+  f32x4 acc[8][MJ] = {};
+  tile_product<T, 8, MJ, NB>(w, x, a.n_in, lds_offset(memory), acc);
+  each_row4(memory, acc, [&](uint32_t row, uint32_t n, f32x4 v) {
+    if (r0 + row < a.rows && n0 + n < a.n_out) finish_linear4(a, r0 + row, n0 + n, v);
+  });
+}
+
+template <class T, int MJ, int NB>
+int launch_tile(const tsa_linear_args& a, hipStream_t stream) {
+  const uint32_t tiles = (a.n_out + 255) / 256 * ((a.rows + 32 * MJ - 1) / (32 * MJ));
+  hipLaunchKernelGGL((linear_tile_kernel<T, MJ, NB>), dim3(tiles), dim3(kTileThreads), tile_lds(8, MJ, NB), stream, a);
+  return int(hipGetLastError());
 }
 
 bool aligned16(const void* p, uint64_t stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0; }
@@ -103,6 +169,10 @@ int launch_linear(const tsa_linear_args& a, void*, hipStream_t stream) {
                                 : op::launch_few<op::Bf16, op::Rows16<op::Bf16>>(a, stream);
     return a.w_type == TSA_Q4 ? op::launch_few<op::F16, op::RowsQ4<op::F16>>(a, stream)
                               : op::launch_few<op::F16, op::Rows16<op::F16>>(a, stream);
+  }
+  if (wide && a.w_type != TSA_Q4 && a.rows < (1u << 24) && a.n_out < (1u << 24)) {
+    if (a.x_type == TSA_BF16) return a.rows <= 128 ? op::launch_tile<op::Bf16, 4, 4>(a, stream) : op::launch_tile<op::Bf16, 8, 4>(a, stream);
+    return a.rows <= 128 ? op::launch_tile<op::F16, 4, 4>(a, stream) : op::launch_tile<op::F16, 8, 4>(a, stream);
   }
   const uint64_t tiles = (uint64_t(a.n_out) + 63) / 64 * ((uint64_t(a.rows) + 63) / 64);
   const dim3 grid(uint32_t(tiles < (1u << 20) ? tiles : (1u << 20)));
