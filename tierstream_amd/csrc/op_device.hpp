@@ -23,6 +23,10 @@ struct Bf16 {
   static __device__ __forceinline__ f32x4 mfma(bits8 a, bits8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
   }
+  // c += a b, c in the accumulator registers and staying where it is (for loops whose accumulators fill them).
+  static __device__ __forceinline__ void mfma_in_place(f32x4& c, bits8 a, bits8 b) {
+    asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  }
   static __device__ __forceinline__ float up(u16 v) { return __builtin_bit_cast(float, uint32_t(v) << 16); }
   static __device__ __forceinline__ u16 down(float v) { return __builtin_bit_cast(u16, (__bf16)v); }
 };
@@ -30,6 +34,10 @@ struct F16 {
   typedef _Float16 v8 __attribute__((ext_vector_type(8)));
   static __device__ __forceinline__ f32x4 mfma(bits8 a, bits8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+  // c += a b, c in the accumulator registers and staying where it is (for loops whose accumulators fill them).
+  static __device__ __forceinline__ void mfma_in_place(f32x4& c, bits8 a, bits8 b) {
+    asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
   }
   static __device__ __forceinline__ float up(u16 v) { return float(__builtin_bit_cast(_Float16, v)); }
   static __device__ __forceinline__ u16 down(float v) { return __builtin_bit_cast(u16, (_Float16)v); }
