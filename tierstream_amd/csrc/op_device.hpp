@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "op_launch.hpp"
 
 namespace tsa {
@@ -43,14 +45,28 @@ struct F16 {
   static __device__ __forceinline__ u16 down(float v) { return __builtin_bit_cast(u16, (_Float16)v); }
 };
 
-__device__ __forceinline__ float sigmoid(float v) { return 1.0f / (1.0f + expf(-v)); }
+// 1 / (1 + exp(-v)) with the hardware's exponential and reciprocal: a few units of the last place of 32 bits for |v| below
+// about 8, an absolute error below that beyond.
+__device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.0f + __expf(-v)); }
+
+// Phi(v) = (1 + erf(v / sqrt 2)) / 2 by formula 7.1.26 of Abramowitz and Stegun's Handbook of Mathematical Functions (erf to
+// 1.5e-7), with the exponential that the slope needs too.
+struct Normal {
+  float phi, density;  // density without its factor 1 / sqrt(2 pi)
+};
+__device__ __forceinline__ Normal normal(float v) {
+  const float x = fabsf(v) * 0.70710678f, e = __expf(-x * x);
+  const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * x);
+  const float tail = 0.5f * t * e * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  return {v < 0.0f ? tail : 1.0f - tail, e};
+}
 
 // act(v). The tanh form is v / (1 + exp(-2 z)), the same function as v (1 + tanh z) / 2 without the difference of
 // nearly equal numbers at large negative z.
 __device__ __forceinline__ float activate(uint32_t act, float v) {
   switch (act) {
     case TSA_ACT_SILU: return v * sigmoid(v);
-    case TSA_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678f));
+    case TSA_ACT_GELU: return v * normal(v).phi;
     case TSA_ACT_GELU_TANH: return v * sigmoid(1.5957691f * (v + 0.044715f * v * v * v));
     case TSA_ACT_RELU: return v > 0.0f ? v : (v == v ? 0.0f : v);
     default: return v;
@@ -63,8 +79,10 @@ __device__ __forceinline__ float slope(uint32_t act, float v) {
       const float s = sigmoid(v);
       return s * (1.0f + v * (1.0f - s));
     }
-    case TSA_ACT_GELU:
-      return 0.5f * (1.0f + erff(v * 0.70710678f)) + v * expf(-0.5f * v * v) * 0.39894228f;
+    case TSA_ACT_GELU: {
+      const Normal p = normal(v);
+      return p.phi + v * p.density * 0.39894228f;
+    }
     case TSA_ACT_GELU_TANH: {
       const float s = sigmoid(1.5957691f * (v + 0.044715f * v * v * v));
       return s + v * s * (1.0f - s) * 1.5957691f * (1.0f + 0.134145f * v * v);

@@ -8,6 +8,7 @@
 // h, dg, du and w h are rounded once to the operands' 16 bits, as the matrix instructions take them; y' and dx' stay in
 // 32 bits until the row's sum, and w is applied there or before the rounding. No sum depends on an order that changes.
 #include "op_stream.hpp"
+#include "op_tile.hpp"
 
 namespace tsa {
 namespace op {
@@ -335,6 +336,218 @@ __global__ __launch_bounds__(64 * most_waves(CT)) void down_few_kernel(Plan p, c
   });
 }
 
+// ---- many rows: tiles of 128 pairs of an expert ----------------------------------------------------------------------
+constexpr uint32_t kTileRows = 128;
+
+// The plan's tile and the a-tile of a workgroup, over the tiles there are (known on the device only).
+__device__ __forceinline__ bool tile_of(const Plan& p, uint32_t na, TileRows& t, uint32_t& a) {
+  if (blockIdx.x >= na * *p.n_tiles) return false;
+  const TileAt at = tile_at(blockIdx.x, na, *p.n_tiles);
+  a = at.a;
+  return tile_rows(p, at.b, kTileRows, t);
+}
+
+// 4 values next to each other a lane, to rows of 16 bits or 32.
+template <class V>
+struct RowsOut {
+  struct Fetched {};
+  V* out;
+  uint64_t stride;
+  uint32_t rows, c0, n_cols, c = 0;
+  __device__ __forceinline__ void columns(uint32_t a) { c = c0 + a; }
+  __device__ __forceinline__ Fetched fetch(uint32_t) const { return {}; }
+  template <class T>
+  __device__ __forceinline__ void put(uint32_t r, f32x4 v) const {
+    if (r >= rows || c >= n_cols) return;  // (columns are a multiple of 8: all four or none)
+    if constexpr (sizeof(V) == 4) {
+      *reinterpret_cast<f32x4*>(out + r * stride + c) = v;
+    } else {
+      bits4 o;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = T::down(v[i]);
+      *reinterpret_cast<bits4*>(out + r * stride + c) = o;
+    }
+  }
+};
+template <class T, class V>
+struct TypedOut : RowsOut<V> {
+  __device__ __forceinline__ void finish(uint32_t r, f32x4 v, const typename RowsOut<V>::Fetched&) const {
+    this->template put<T>(r, v);
+  }
+};
+
+// Gate and up rows of the same 128 columns as one operand of 256: each wave gets 64 of both.
+template <class T>
+__device__ __forceinline__ TileRowsSource<8> gate_up_source(const Plan& p, const TileRows& t, uint32_t d, uint32_t f,
+                                                            uint32_t f0) {
+  const u16 *gate = reinterpret_cast<const u16*>(p.part[3 * t.e]), *up = reinterpret_cast<const u16*>(p.part[3 * t.e + 1]);
+  return TileRowsSource<8>(d, threadIdx.x >> 6 & 1u, [&](uint32_t r) {
+    const uint32_t c = f0 + (r >> 7) * 64 + (r & 63u);
+    return (r & 64u ? up : gate) + uint64_t(c < f ? c : f - 1) * d;
+  });
+}
+__device__ __forceinline__ TileRowsSource<4> mapped_rows(const TileRows& t, const u16* x, uint64_t stride, uint32_t n) {
+  return TileRowsSource<4>(n, threadIdx.x >> 7, [&](uint32_t r) { return x + t.map[r < t.rows ? r : t.rows - 1] * stride; });
+}
+__device__ __forceinline__ TileRowsSource<4> sorted_rows(const TileRows& t, const u16* x, uint64_t stride, uint32_t n) {
+  return TileRowsSource<4>(n, threadIdx.x >> 7,
+                           [&](uint32_t r) { return x + uint64_t(t.first + (r < t.rows ? r : t.rows - 1)) * stride; });
+}
+
+template <class T>
+__global__ __launch_bounds__(kTileThreads, 2) void gate_up_tile_kernel(Plan p, const u16* x, uint64_t x_stride, uint32_t d,
+                                                                       uint32_t f, uint32_t act, u16* h) {
+  extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
+  TileRows t;
+  uint32_t at;
+  if (!tile_of(p, (f + 127) / 128, t, at)) return;
+  auto w = gate_up_source<T>(p, t, d, f, at * 128);
+  auto xs = mapped_rows(t, x, x_stride, d);
+  f32x4 acc[8][4] = {};
+  tile_product<T, 8, 4, 3>(w, xs, d, lds_offset(memory), acc);
+  f32x4 v[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[i][j][q] = activate(act, acc[i][j][q]) * acc[i + 4][j][q];
+  TypedOut<T, u16> out{{h + uint64_t(t.first) * f, f, t.rows, at * 128, f}};
+  hand_out<4, 4, 4>(memory, v, out);
+}
+
+template <class T>
+__global__ __launch_bounds__(kTileThreads, 2) void down_tile_kernel(Plan p, const u16* h, uint32_t d, uint32_t f, float* out) {
+  extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
+  TileRows t;
+  uint32_t at;
+  if (!tile_of(p, (d + 255) / 256, t, at)) return;
+  const u16* down = reinterpret_cast<const u16*>(p.part[3 * t.e + 2]);
+  TileRowsSource<8> w(f, threadIdx.x >> 6 & 1u, [&](uint32_t r) {
+    const uint32_t c = at * 256 + r;
+    return down + uint64_t(c < d ? c : d - 1) * f;
+  });
+  auto hs = sorted_rows(t, h, f, f);
+  f32x4 acc[8][4] = {};
+  tile_product<T, 8, 4, 3>(w, hs, f, lds_offset(memory), acc);
+  TypedOut<T, float> o{{out + uint64_t(t.first) * d, d, t.rows, at * 256, d}};
+  hand_out<8, 4, 2>(memory, acc, o);
+}
+
+// As hidden_grad_any_kernel: gate, up and down's products one after the other in their own accumulators, 128 columns of d_ff.
+template <class T>
+__global__ __launch_bounds__(kTileThreads, 1) void hidden_grad_tile_kernel(Plan p, const u16* x, uint64_t x_stride,
+                                                                           const u16* dy, uint64_t dy_stride,
+                                                                           const float* weights, uint32_t d, uint32_t f,
+                                                                           uint32_t act, u16* dgu, u16* wh, float* d_share) {
+  extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
+  __shared__ float share[kTileRows][2];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  TileRows t;
+  uint32_t at;
+  if (!tile_of(p, (f + 127) / 128, t, at)) return;
+  const uint32_t f0 = at * 128;
+  f32x4 gu[8][4] = {}, b[4][4] = {};
+  {
+    auto w = gate_up_source<T>(p, t, d, f, f0);
+    auto xs = mapped_rows(t, x, x_stride, d);
+    tile_product<T, 8, 4, 4>(w, xs, d, lds_offset(memory), gu);
+  }
+  {
+    TileColumnsSource<4, false> w(d, wave & 1u, reinterpret_cast<const u16*>(p.part[3 * t.e + 2]), f, f0, f);
+    auto dys = mapped_rows(t, dy, dy_stride, d);
+    tile_product<T, 4, 4, 4>(w, dys, d, lds_offset(memory), b);
+  }
+  f32x4 dg[4][4], du[4][4], h[4][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t r = (wave >> 1) * 64 + 16 * j + (lane & 15u);
+    const float w = r < t.rows && weights ? weights[p.pair[t.first + r]] : 1.0f;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool in = f0 + (wave & 1u) * 64 + 16 * i + (lane >> 4) * 4 < f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float g = gu[i][j][q], u = gu[i + 4][j][q], a = activate(act, g), back = b[i][j][q];
+        if (in) sum += a * u * back;
+        dg[i][j][q] = w * back * u * slope(act, g);
+        du[i][j][q] = w * back * a;
+        h[i][j][q] = w * a * u;
+      }
+    }
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (lane < 16) share[r][wave & 1u] = sum;
+  }
+  TypedOut<T, u16> out{{dgu + uint64_t(t.first) * 2 * f, uint64_t(2) * f, t.rows, f0, f}};
+  hand_out<4, 4, 4>(memory, dg, out);  // (behind its barrier `share` is whole)
+  if (threadIdx.x < t.rows) d_share[uint64_t(at) * p.pairs + t.first + threadIdx.x] = share[threadIdx.x][0] + share[threadIdx.x][1];
+  out.out += f;
+  hand_out<4, 4, 4>(memory, du, out);
+  out.out = wh + uint64_t(t.first) * f;
+  out.stride = f;
+  hand_out<4, 4, 4>(memory, h, out);
+}
+
+template <class T>
+__global__ __launch_bounds__(kTileThreads, 2) void input_grad_tile_kernel(Plan p, const u16* dgu, uint32_t d, uint32_t f,
+                                                                          float* out) {
+  extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
+  TileRows t;
+  uint32_t at;
+  if (!tile_of(p, (d + 255) / 256, t, at)) return;
+  f32x4 acc[8][4] = {};
+#pragma unroll 1
+  for (uint32_t half = 0; half < 2; ++half) {
+    TileColumnsSource<8, false> w(f, threadIdx.x >> 6 & 1u, reinterpret_cast<const u16*>(p.part[3 * t.e + half]), d, at * 256, d);
+    auto v = sorted_rows(t, dgu + half * f, uint64_t(2) * f, f);
+    tile_product<T, 8, 4, 3>(w, v, f, lds_offset(memory), acc);
+  }
+  TypedOut<T, float> o{{out + uint64_t(t.first) * d, d, t.rows, at * 256, d}};
+  hand_out<8, 4, 2>(memory, acc, o);
+}
+
+// Rows of an expert's pairs by way of a map in LDS.
+constexpr uint32_t kMapRows = 1024;
+
+// As weight_grad_any_kernel, out[e][b][a]: 256 columns a of `left` and 128 columns b of `right` a workgroup, the sum over the
+// expert's pairs. One of the two is read through the rows' map (kMapLeft: left). Columns from n_right on belong to out2 (the
+// gradients of gate and up are one product).
+template <class T, bool kMapLeft>
+__global__ __launch_bounds__(kTileThreads, 2) void weight_grad_tile_kernel(Plan p, const u16* left, uint64_t left_stride,
+                                                                           uint32_t n_left, const u16* right,
+                                                                           uint64_t right_stride, uint32_t n_right,
+                                                                           uint32_t n_outs, u16* out, u16* out2) {
+  extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
+  uint32_t* map = reinterpret_cast<uint32_t*>(memory) + tile_lds(8, 4, 3) / 4;
+  const uint32_t wave = threadIdx.x >> 6;
+  const uint32_t ta = (n_left + 255) / 256, tb = (n_right + 127) / 128, per = ta * tb * n_outs;
+  const uint32_t e = blockIdx.x / per, in = blockIdx.x % per;
+  const uint32_t a0 = in % ta * 256, which = in / ta / tb, b0 = in / ta % tb * 128;
+  const uint32_t first = p.first[e], pairs = p.first[e + 1] - first;
+  right += which * n_right;
+  f32x4 acc[8][4] = {};
+#pragma unroll 1
+  for (uint32_t k = 0; k < pairs; k += kMapRows) {
+    const uint32_t n = pairs - k < kMapRows ? pairs - k : kMapRows;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n; i += kTileThreads) map[i] = p.row[first + k + i];
+    __syncthreads();
+    if constexpr (kMapLeft) {
+      TileColumnsSource<8, true> l(n, wave & 1u, left, left_stride, a0, n_left, map);
+      TileColumnsSource<4, false> r(n, wave >> 1, right + uint64_t(first + k) * right_stride, right_stride, b0, n_right);
+      tile_product<T, 8, 4, 3>(l, r, n, lds_offset(memory), acc);
+    } else {
+      TileColumnsSource<8, false> l(n, wave & 1u, left + uint64_t(first + k) * left_stride, left_stride, a0, n_left);
+      TileColumnsSource<4, true> r(n, wave >> 1, right, right_stride, b0, n_right, map);
+      tile_product<T, 8, 4, 3>(l, r, n, lds_offset(memory), acc);
+    }
+  }
+  TypedOut<T, u16> o{{(which ? out2 : out) + (uint64_t(e) * n_right + b0) * n_left, n_left, n_right - b0, a0, n_left}};
+  hand_out<8, 4, 2>(memory, acc, o);
+}
+
 // out_t = residual_t + sum_j w_tj v_{at(t, j)}, in the order of j
 template <class T>
 __global__ __launch_bounds__(256) void combine_kernel(Plan p, uint32_t rows, uint32_t d, const float* v, const float* weights,
@@ -536,7 +749,7 @@ bool aligned16(const void* p, uint64_t stride_bytes) { return (reinterpret_cast<
 // Whether every weight row, x row and row of h starts 16-byte aligned and holds whole groups of 8 values. The addresses of
 // a table's units are the device's: its units are 256-byte aligned, as the library lays them out.
 bool wide_rows(const ExpertMap& e, uint32_t d, uint32_t f, bool q4, const void* x, uint64_t x_stride) {
-  if (d % 8 || f % 8 || !aligned16(x, 2 * x_stride)) return false;
+  if (d % 8 || f % 8 || !aligned16(x, 2 * x_stride) || x_stride >= 1u << 24) return false;
   if (q4) return true;
   for (int p = 0; p < 3; ++p) {
     if (e.form == 0 && !aligned16(e.part[p], e.stride[p])) return false;
@@ -586,11 +799,29 @@ int forward_stream(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_arg
   return forward_few<T, W, 4, kTail>(e, d, f, a, w, s);
 }
 
+template <class T>
+int forward_tiles(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& a, void* ws, hipStream_t s) {
+  Room room(ws);
+  const Forward w = take_forward(room, e.n, d, f, a.rows, a.top_k);
+  if (int err = launch_plan(e, a.ids, w.plan, kTileRows, s)) return err;
+  const uint32_t tiles = most_tiles(w.plan.pairs, e.n, kTileRows);
+  hipLaunchKernelGGL((gate_up_tile_kernel<T>), dim3(tiles * ((f + 127) / 128)), dim3(kTileThreads), tile_lds(8, 4, 3), s, w.plan,
+                     static_cast<const u16*>(a.x), a.x_stride, d, f, a.act, w.h);
+  hipLaunchKernelGGL((down_tile_kernel<T>), dim3(tiles * ((d + 255) / 256)), dim3(kTileThreads), tile_lds(8, 4, 3), s, w.plan, w.h,
+                     d, f, w.out);
+  hipLaunchKernelGGL((combine_kernel<T>), dim3(blocks((uint64_t(a.rows) * d + 255) / 256)), dim3(256), 0, s, w.plan, a.rows, d,
+                     w.out, a.weights, static_cast<const u16*>(a.residual), a.residual_stride, static_cast<u16*>(a.y),
+                     a.y_stride);
+  return int(hipGetLastError());
+}
+
 template <class T, bool kQ4>
 int forward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& a, void* ws, hipStream_t s) {
   typedef std::conditional_t<kQ4, RowsQ4<T>, Rows16<T>> W;
   if (wide_rows(e, d, f, kQ4, a.x, a.x_stride) && uint64_t(a.rows) * a.top_k <= uint64_t(64) * e.n)
     return d % kChunk || f % kChunk ? forward_stream<T, W, true>(e, d, f, a, ws, s) : forward_stream<T, W, false>(e, d, f, a, ws, s);
+  if constexpr (!kQ4)
+    if (wide_rows(e, d, f, false, a.x, a.x_stride)) return forward_tiles<T>(e, d, f, a, ws, s);
   Room room(ws);
   const Forward w = take_forward(room, e.n, d, f, a.rows, a.top_k);
   if (int err = launch_plan(e, a.ids, w.plan, 64, s)) return err;
@@ -605,7 +836,41 @@ int forward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& a, v
 }
 
 template <class T>
+int backward_tiles(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_grad_args& a, void* ws, hipStream_t s) {
+  Room room(ws);
+  const Backward w = take_backward(room, e.n, d, f, a.rows, a.top_k);
+  if (int err = launch_plan(e, a.ids, w.plan, kTileRows, s)) return err;
+  const uint32_t tiles = most_tiles(w.plan.pairs, e.n, kTileRows), tf = (f + 127) / 128, td = (d + 255) / 256;
+  const u16 *x = static_cast<const u16*>(a.x), *dy = static_cast<const u16*>(a.dy);
+  if (tiles)
+    hipLaunchKernelGGL((hidden_grad_tile_kernel<T>), dim3(tiles * tf), dim3(kTileThreads), tile_lds(8, 4, 4), s, w.plan, x,
+                       a.x_stride, dy, a.dy_stride, a.weights, d, f, a.act, w.dgu, w.wh, w.share);
+  if (a.dx && tiles) {
+    hipLaunchKernelGGL((input_grad_tile_kernel<T>), dim3(tiles * td), dim3(kTileThreads), tile_lds(8, 4, 3), s, w.plan, w.dgu, d, f,
+                       w.out);
+    hipLaunchKernelGGL((combine_kernel<T>), dim3(blocks((uint64_t(a.rows) * d + 255) / 256)), dim3(256), 0, s, w.plan, a.rows,
+                       d, w.out, static_cast<const float*>(nullptr), static_cast<const u16*>(nullptr), uint64_t(0),
+                       static_cast<u16*>(a.dx), a.dx_stride);
+  }
+  if (a.dweights && tiles)
+    hipLaunchKernelGGL(weights_grad_kernel, dim3(blocks((w.plan.pairs + 255) / 256)), dim3(256), 0, s, w.plan, tf, w.share,
+                       a.dweights);
+  if (a.dgate) {
+    constexpr uint32_t kLds = tile_lds(8, 4, 3) + 4 * kMapRows;
+    hipLaunchKernelGGL((weight_grad_tile_kernel<T, true>), dim3(e.n * td * tf * 2), dim3(kTileThreads), kLds, s, w.plan, x,
+                       a.x_stride, d, w.dgu, uint64_t(2) * f, f, 2u, static_cast<u16*>(a.dgate), static_cast<u16*>(a.dup));
+    hipLaunchKernelGGL((weight_grad_tile_kernel<T, false>), dim3(e.n * ((f + 255) / 256) * ((d + 127) / 128)), dim3(kTileThreads),
+                       kLds, s, w.plan, w.wh, uint64_t(f), f, dy, a.dy_stride, d, 1u, static_cast<u16*>(a.ddown),
+                       static_cast<u16*>(nullptr));
+  }
+  return int(hipGetLastError());
+}
+
+template <class T>
 int backward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_grad_args& a, void* ws, hipStream_t s) {
+  if (wide_rows(e, d, f, false, a.x, a.x_stride) && aligned16(a.dy, 2 * a.dy_stride) && a.dy_stride < 1u << 24 && aligned16(a.dgate, 0) && aligned16(a.dup, 0) &&
+      aligned16(a.ddown, 0))
+    return backward_tiles<T>(e, d, f, a, ws, s);
   Room room(ws);
   const Backward w = take_backward(room, e.n, d, f, a.rows, a.top_k);
   if (int err = launch_plan(e, a.ids, w.plan, 64, s)) return err;

@@ -1,0 +1,299 @@
+// Products with many rows: tiles of 32 NI rows of `a` times 32 MJ rows of `b`, by four waves (2 x 2, each 16 NI x 16 MJ), one
+// to a SIMD, whose accumulators take half of its registers. Both operands go through LDS: a wave of 128 x 128 reads 32 KiB
+// there for 64 matrix instructions, half of what LDS gives in that time.
+//
+// A step is 32 values of the sum. Its operands are loaded straight to LDS (global_load_lds_dwordx4, NB buffers in turn) and
+// from there to a second set of registers while the step before is multiplied. Two steps, a cache line of every row, are
+// loaded together: by themselves each took the lines' halves from L2 again (a quarter of the time of a long product).
+// With 4 buffers step t (odd) waits for steps t + 1 and t + 2, loaded two steps earlier, and behind its barrier loads t + 3
+// and t + 4 over t - 1 and t, whose reads every wave has done. With 3, so that two workgroups fit a CU, step t (even)
+// loads t + 2 and t + 3 and step t + 1 waits for them.
+//
+// Operands come in two forms. Rows: the values of the sum lie next to each other; a row's 64 bytes a step are 4 pieces,
+// piece c at place c ^ (row / 4 mod 4), so that 16 lanes reading one piece of 16 rows hit all banks. Columns (the operand
+// is transposed in memory): 32 rows of the tile's columns, read with ds_read_b64_tr_b16, which gives each lane of 16 one
+// column of 4 rows; pairs of pieces are permuted by the row so that the 8 rows of a half wave hit all banks. In both, the
+// permutation is made by the loads' addresses: LDS itself is filled in lane order.
+#pragma once
+
+#include "op_device.hpp"
+
+namespace tsa {
+namespace op {
+
+constexpr uint32_t kTileThreads = 256;
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4_t;
+typedef __attribute__((address_space(3))) const bits8 lds_bits8_t;
+
+static __device__ const u32x4 kZeroPiece = {0, 0, 0, 0};  // what a load past the end of the sum reads
+
+// 64 lanes x 16 bytes to LDS at `at` (the same in every lane) in lane order.
+__device__ __forceinline__ void load_to_lds(const void* g, uint32_t at) {
+  asm volatile(
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %0, off"
+      :
+      : "v"(g), "s"(at)
+      : "memory", "m0");
+}
+__device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_loads_and_meet() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ uint32_t lds_offset(const void* p) {
+  return uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)p));
+}
+
+// An operand of 32 NF rows, in rows: at(r) gives row r's first value (any valid row for r behind the last).
+template <int NF>
+struct TileRowsSource {
+  static constexpr int kLoads = NF / 2;
+  const u16* p[kLoads];
+  uint32_t k, n, mine;
+  uint32_t frag;  // this lane's place of its wave's first fragment
+
+  template <class At>
+  __device__ __forceinline__ TileRowsSource(uint32_t n_, uint32_t half, At&& at) : n(n_) {
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    mine = __builtin_amdgcn_readfirstlane(wave) * kLoads * 1024;
+    k = ((lane & 3u) ^ (lane >> 4)) * 8;
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) p[j] = at((wave * kLoads + j) * 16 + lane / 4) + k;
+    frag = (half * NF * 16 + (lane & 15u)) * 64 + (((lane >> 4) ^ ((lane >> 2) & 3u)) * 16);
+  }
+  // Load j of the next two steps (kCheck: the sum may end inside them); then, after all of them, on to the two behind.
+  template <bool kCheck>
+  __device__ __forceinline__ void issue(int j, uint32_t lds0, uint32_t lds1) {
+    if (kCheck) {
+      load_to_lds(k < n ? static_cast<const void*>(p[j]) : &kZeroPiece, lds0 + mine + j * 1024);
+      load_to_lds(k + 32 < n ? static_cast<const void*>(p[j] + 32) : &kZeroPiece, lds1 + mine + j * 1024);
+    } else {
+      load_to_lds(p[j], lds0 + mine + j * 1024);
+      load_to_lds(p[j] + 32, lds1 + mine + j * 1024);
+    }
+    p[j] += 64;
+  }
+  __device__ __forceinline__ void advance() { k += 64; }
+  __device__ __forceinline__ bits8 read(uint32_t lds, int i) const {
+    return *reinterpret_cast<lds_bits8_t*>(lds + frag + i * 1024);
+  }
+};
+
+__device__ __forceinline__ uint64_t uniform(uint64_t v) {
+  return uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(uint32_t(v >> 32)))) << 32 |
+         uint32_t(__builtin_amdgcn_readfirstlane(uint32_t(v)));
+}
+// 64 lanes x 16 bytes from one base (the same in every lane) and a 32-bit offset each.
+__device__ __forceinline__ void load_offset_to_lds(uint64_t base, uint32_t offset, uint32_t at) {
+  asm volatile(
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %0, %1"
+      :
+      : "v"(offset), "s"(base), "s"(at)
+      : "memory", "m0");
+}
+
+// In columns: 32 NF columns from `first` on (n_cols in all, a multiple of 8), row k of the sum at at + k stride, or with a
+// map (in LDS) at at + map[k] stride. stride is below 2^24. Buffers are 512-byte aligned: a fragment's place is its wave's
+// first one's with the fragment's number in three bits that the permutation turns.
+template <int NF, bool kMap>
+struct TileColumnsSource {
+  static constexpr int kLoads = NF / 2;
+  static constexpr uint32_t kPieces = 4 * NF;  // 16-byte pieces of a row
+  uint64_t base;
+  uint32_t offset[kLoads];  // bytes: of the lane's column, and without a map of its row
+  uint32_t stride, k, n, mine, frag;
+  const uint32_t* map;
+
+  static __device__ __forceinline__ uint32_t turn(uint32_t kk) { return (((kk & 3u) | ((kk >> 3) & 1u) << 2) << 1) & (kPieces - 1); }
+  __device__ __forceinline__ TileColumnsSource(uint32_t n_, uint32_t half, const u16* at, uint64_t stride_, uint32_t first,
+                                               uint32_t n_cols, const uint32_t* map_ = nullptr)
+      : base(uniform(reinterpret_cast<uint64_t>(at))), stride(uint32_t(stride_) * 2), k(0), n(n_), map(map_) {
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    mine = __builtin_amdgcn_readfirstlane(wave) * kLoads * 1024;
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const uint32_t i = (wave * kLoads + j) * 64 + lane;
+      const uint32_t c = first + ((i % kPieces) ^ turn(i / kPieces)) * 8;
+      offset[j] = (c < n_cols ? c : n_cols - 8) * 2 + (kMap ? 0 : i / kPieces * stride);
+    }
+    const uint32_t kk = (lane >> 4) * 8 + ((lane & 15u) >> 2);
+    frag = kk * (kPieces * 16) + ((half * NF * 2 + ((lane & 3u) >> 1)) ^ turn(kk)) * 16 + (lane & 1u) * 8;
+  }
+  __device__ __forceinline__ uint32_t row_of(int j) const {  // of the lane's piece, in its step
+    return (mine + j * 1024 + (threadIdx.x & 63u) * 16) / (kPieces * 16);
+  }
+  // Load j of the next two steps, as TileRowsSource's.
+  template <bool kCheck>
+  __device__ __forceinline__ void issue(int j, uint32_t lds0, uint32_t lds1) {
+#pragma unroll
+    for (uint32_t s = 0; s < 2; ++s) {
+      const uint32_t to = (s ? lds1 : lds0) + mine + j * 1024;
+      if constexpr (kMap || kCheck) {
+        const uint32_t row = k + 32 * s + row_of(j);
+        const bool in = !kCheck || row < n;
+        uint64_t g = base + offset[j];
+        if constexpr (kMap) g += uint64_t(map[in ? row : 0]) * stride;
+        else g += uint64_t(32 * s) * stride;
+        load_to_lds(in ? reinterpret_cast<const void*>(g) : &kZeroPiece, to);
+      } else {
+        load_offset_to_lds(base + uint64_t(32 * s) * stride, offset[j], to);
+      }
+    }
+  }
+  __device__ __forceinline__ void advance() {
+    k += 64;
+    if (!kMap) base += uint64_t(64) * stride;
+  }
+  __device__ __forceinline__ bits8 read(uint32_t lds, int i) const {
+    const uint32_t at = (lds + frag) ^ (32u * i);
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4_t*>(at));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4_t*>(at + 4 * kPieces * 16));
+    return __builtin_bit_cast(bits8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+};
+
+constexpr uint32_t tile_lds(int NI, int MJ, int NB) { return uint32_t(NI + MJ) * 2048u * uint32_t(NB); }
+
+// Every accumulator through an empty statement: what is written before it is not read, and what is read after it not
+// written, on the other side. The compiler counts no wait states behind assembly, so they stand beside it.
+template <int NI, int MJ>
+__device__ __forceinline__ void settle(f32x4 (&acc)[NI][MJ]) {
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < MJ; ++j) asm volatile("" : "+a"(acc[i][j]));
+}
+
+// acc[i][j] += a's rows 16 i.. of this wave's half times b's rows 16 j.. of its half, over the sources' n values. Lane l
+// holds a-rows 4 (l / 16) + 0..3 and b-row l % 16 of each.
+template <class T, int NI, int MJ, int NB, class A, class B>
+__device__ __forceinline__ void tile_product(A& a, B& b, uint32_t n, uint32_t lds, f32x4 (&acc)[NI][MJ]) {
+  static_assert(NB == 3 || NB == 4, "buffers");
+  constexpr int kLoads = (NI + MJ) / 2;  // of a step, each thread
+  constexpr uint32_t kA = NI * 2048, kBuffer = (NI + MJ) * 2048;
+  const auto issue = [&](auto check, int j, uint32_t at0, uint32_t at1) {  // load j of two steps, of both operands
+    if (j < A::kLoads) a.template issue<decltype(check)::value>(j, at0, at1);
+    else b.template issue<decltype(check)::value>(j - A::kLoads, at0 + kA, at1 + kA);
+  };
+  const auto issue_all = [&](uint32_t at0, uint32_t at1) {
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) issue(std::true_type{}, j, at0, at1);
+    a.advance();
+    b.advance();
+  };
+  __syncthreads();  // the last product's reads are done
+  issue_all(lds, lds + kBuffer);
+  if (NB == 4) issue_all(lds + 2 * kBuffer, lds + 3 * kBuffer);
+  wait_loads_and_meet<NB == 4 ? 2 * kLoads : 0>();
+  bits8 fa[2][NI], fb[2][MJ];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) fa[0][i] = a.read(lds, i);
+#pragma unroll
+  for (int j = 0; j < MJ; ++j) fb[0][j] = b.read(lds + kA, j);
+  settle(acc);
+  asm volatile("s_nop 7");
+  uint32_t at = 0;  // this step's buffer
+  const auto behind = [&](uint32_t steps) { return lds + (at + steps >= NB ? at + steps - NB : at + steps) * kBuffer; };
+  // A step, product by product: a read of the next step's operands every kPer, the loads in between. Left to itself the
+  // compiler puts the reads behind the last product, where nothing hides them.
+  const auto step = [&](auto now_, auto loads, auto check) {
+    constexpr int now = decltype(now_)::value, kFrags = NI + MJ, kPer = NI * MJ / kFrags;
+    const uint32_t from = behind(1);
+    const uint32_t to0 = NB == 4 ? behind(3) : behind(2), to1 = lds + at * kBuffer;
+#pragma unroll
+    for (int x = 0; x < NI * MJ; ++x) {
+      if (x % kPer == 0 && x / kPer < kFrags) {
+        const int r = x / kPer;
+        if (r < MJ) fb[now ^ 1][r] = b.read(from + kA, r);
+        else fa[now ^ 1][r - MJ] = a.read(from, r - MJ);
+        if (decltype(loads)::value && r % 2 == 0 && r / 2 < kLoads) issue(check, r / 2, to0, to1);
+      }
+      T::mfma_in_place(acc[x / MJ][x % MJ], fa[now][x / MJ], fb[now][x % MJ]);
+      if (x % kPer == kPer - 1) __builtin_amdgcn_sched_barrier(0);
+    }
+    if (decltype(loads)::value) {
+      a.advance();
+      b.advance();
+    }
+    at = at + 1 == NB ? 0 : at + 1;
+  };
+  const auto two_steps = [&](auto check) {
+    using Zero = std::integral_constant<int, 0>;
+    using One = std::integral_constant<int, 1>;
+    if (NB == 4) {
+      step(Zero{}, std::false_type{}, check);
+      wait_loads_and_meet<0>();
+      step(One{}, std::true_type{}, check);
+    } else {
+      meet();
+      step(Zero{}, std::true_type{}, check);
+      wait_loads_and_meet<0>();
+      step(One{}, std::false_type{}, check);
+    }
+  };
+  constexpr uint32_t kAhead = NB == 4 ? 6 : 4;  // the last step that two steps from t on load, + 1
+  uint32_t t = 0;
+  for (; (t + kAhead) * 32 <= n; t += 2) two_steps(std::false_type{});
+  for (; t * 32 < n; t += 2) two_steps(std::true_type{});  // (steps past the end multiply zeros)
+  // The loads past the end have landed, and the last results are written before anything reads them (18 wait states).
+  asm volatile("s_waitcnt vmcnt(0)\n\ts_nop 15\n\ts_nop 3" ::: "memory");
+  settle(acc);
+}
+
+// Hands a wave's part of a tile to `out`, 4 values of a-rows next to each other at a time, rows counted in the tile: by way
+// of LDS (the wave's own JP fragments of b at a time), so that lanes next to each other have values next to each other.
+// out.columns(a-row): this lane's 4 a-rows, once; out.fetch(b-row) gives what finish() of that row needs from memory, for 8
+// rows before the first finish(b-row, values, fetched): one after the other, each would be a memory latency.
+template <int NI, int MJ, int JP, class Out>
+__device__ __forceinline__ void hand_out(void* memory, const f32x4 (&acc)[NI][MJ], Out& out) {
+  constexpr uint32_t kLanes = NI * 4, kRows = 64 / kLanes;  // lanes a row, rows at once
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  f32x4* mine = static_cast<f32x4*>(memory) + wave * (JP * 16 * kLanes);
+  out.columns((wave & 1u) * 16 * NI + (lane % kLanes) * 4);
+  __syncthreads();  // the product's reads are done
+#pragma unroll
+  for (int j0 = 0; j0 < MJ; j0 += JP) {
+#pragma unroll
+    for (int j = 0; j < JP; ++j)
+#pragma unroll
+      for (int i = 0; i < NI; ++i)  // (piece p of row r at p ^ r mod 16: both ways hit all banks)
+        mine[(16 * j + (lane & 15u)) * kLanes + ((4 * i + (lane >> 4)) ^ ((lane & 15u) % kLanes))] = acc[i][j0 + j];
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+    for (uint32_t r0 = lane / kLanes; r0 < 16 * JP; r0 += 8 * kRows) {
+      const uint32_t base = (wave >> 1) * 16 * MJ + 16 * j0 + r0;
+      typename Out::Fetched got[8];
+#pragma unroll
+      for (uint32_t x = 0; x < 8; ++x) got[x] = out.fetch(base + x * kRows);
+#pragma unroll
+      for (uint32_t x = 0; x < 8; ++x) {
+        const uint32_t r = r0 + x * kRows;
+        out.finish(base + x * kRows, mine[r * kLanes + ((lane % kLanes) ^ ((r & 15u) % kLanes))], got[x]);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// Which tile a workgroup takes: neighbouring workgroups go to the 8 XCDs in turn, each with a cache of its own, so each
+// XCD gets a stretch of tiles, and a stretch walks 8 b-tiles by 8, a-tile after a-tile: what runs at once shares operands.
+struct TileAt {
+  uint32_t a, b;
+};
+__device__ __forceinline__ TileAt tile_at(uint32_t block, uint32_t na, uint32_t nb) {
+  const uint32_t total = na * nb, per = total / 8, rest = total % 8, xcd = block % 8;
+  const uint32_t id = xcd * per + (xcd < rest ? xcd : rest) + block / 8;
+  const uint32_t group = id / (8 * na), first = group * 8, in = id - group * 8 * na;
+  const uint32_t wide = nb - first < 8 ? nb - first : 8;
+  return {in / wide, first + in % wide};
+}
+
+}  // namespace op
+}  // namespace tsa
