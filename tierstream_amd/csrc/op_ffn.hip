@@ -434,12 +434,29 @@ __global__ __launch_bounds__(kTileThreads, 2) void down_tile_kernel(Plan p, cons
   hand_out<8, 4, 2>(memory, acc, o);
 }
 
-// As hidden_grad_any_kernel: gate, up and down's products one after the other in their own accumulators, 128 columns of d_ff.
+// back = down^T dy of every pair, 256 columns of d_ff: in 32 bits, for the kernel behind it. (One kernel for all three
+// products needs 192 accumulators a lane, so one workgroup a CU: 496 us in a training step of 128 experts.)
 template <class T>
-__global__ __launch_bounds__(kTileThreads, 1) void hidden_grad_tile_kernel(Plan p, const u16* x, uint64_t x_stride,
-                                                                           const u16* dy, uint64_t dy_stride,
-                                                                           const float* weights, uint32_t d, uint32_t f,
-                                                                           uint32_t act, u16* dgu, u16* wh, float* d_share) {
+__global__ __launch_bounds__(kTileThreads, 2) void back_tile_kernel(Plan p, const u16* dy, uint64_t dy_stride, uint32_t d,
+                                                                    uint32_t f, float* back) {
+  extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
+  TileRows t;
+  uint32_t at;
+  if (!tile_of(p, (f + 255) / 256, t, at)) return;
+  TileColumnsSource<8, false> w(d, threadIdx.x >> 6 & 1u, reinterpret_cast<const u16*>(p.part[3 * t.e + 2]), f, at * 256, f);
+  auto dys = mapped_rows(t, dy, dy_stride, d);
+  f32x4 acc[8][4] = {};
+  tile_product<T, 8, 4, 3>(w, dys, d, lds_offset(memory), acc);
+  TypedOut<T, float> o{{back + uint64_t(t.first) * f, f, t.rows, at * 256, f}};
+  hand_out<8, 4, 2>(memory, acc, o);
+}
+
+// As hidden_grad_any_kernel from gate's and up's products and `back`, 128 columns of d_ff.
+template <class T>
+__global__ __launch_bounds__(kTileThreads, 2) void hidden_grad_tile_kernel(Plan p, const u16* x, uint64_t x_stride,
+                                                                           const float* back, const float* weights, uint32_t d,
+                                                                           uint32_t f, uint32_t act, u16* dgu, u16* wh,
+                                                                           float* d_share) {
   extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
   __shared__ float share[kTileRows][2];
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
@@ -447,47 +464,46 @@ __global__ __launch_bounds__(kTileThreads, 1) void hidden_grad_tile_kernel(Plan 
   uint32_t at;
   if (!tile_of(p, (f + 127) / 128, t, at)) return;
   const uint32_t f0 = at * 128;
-  f32x4 gu[8][4] = {}, b[4][4] = {};
-  {
-    auto w = gate_up_source<T>(p, t, d, f, f0);
-    auto xs = mapped_rows(t, x, x_stride, d);
-    tile_product<T, 8, 4, 4>(w, xs, d, lds_offset(memory), gu);
-  }
-  {
-    TileColumnsSource<4, false> w(d, wave & 1u, reinterpret_cast<const u16*>(p.part[3 * t.e + 2]), f, f0, f);
-    auto dys = mapped_rows(t, dy, dy_stride, d);
-    tile_product<T, 4, 4, 4>(w, dys, d, lds_offset(memory), b);
-  }
-  f32x4 dg[4][4], du[4][4], h[4][4];
+  f32x4 gu[8][4] = {};
+  auto ws = gate_up_source<T>(p, t, d, f, f0);
+  auto xs = mapped_rows(t, x, x_stride, d);
+  tile_product<T, 8, 4, 3>(ws, xs, d, lds_offset(memory), gu);
+  f32x4 h[4][4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t r = (wave >> 1) * 64 + 16 * j + (lane & 15u);
-    const float w = r < t.rows && weights ? weights[p.pair[t.first + r]] : 1.0f;
+    const uint32_t r = (wave >> 1) * 64 + 16 * j + (lane & 15u), pos = t.first + (r < t.rows ? r : t.rows - 1);
+    const float w = weights ? weights[p.pair[pos]] : 1.0f;
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const bool in = f0 + (wave & 1u) * 64 + 16 * i + (lane >> 4) * 4 < f;
+      const uint32_t c = f0 + (wave & 1u) * 64 + 16 * i + (lane >> 4) * 4;
+      const f32x4 b = c < f ? *reinterpret_cast<const f32x4*>(back + uint64_t(pos) * f + c) : f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const float g = gu[i][j][q], u = gu[i + 4][j][q], a = activate(act, g), back = b[i][j][q];
-        if (in) sum += a * u * back;
-        dg[i][j][q] = w * back * u * slope(act, g);
-        du[i][j][q] = w * back * a;
+        const float g = gu[i][j][q], u = gu[i + 4][j][q], a = activate(act, g);
+        sum += a * u * b[q];
         h[i][j][q] = w * a * u;
+        gu[i][j][q] = w * b[q] * u * slope(act, g);  // dg, du in the products' places
+        gu[i + 4][j][q] = w * b[q] * a;
       }
     }
     sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
-    if (lane < 16) share[r][wave & 1u] = sum;
+    if (lane < 16) share[(wave >> 1) * 64 + 16 * j + lane][wave & 1u] = sum;
   }
-  TypedOut<T, u16> out{{dgu + uint64_t(t.first) * 2 * f, uint64_t(2) * f, t.rows, f0, f}};
-  hand_out<4, 4, 4>(memory, dg, out);  // (behind its barrier `share` is whole)
+  TypedOut<T, u16> out{{wh + uint64_t(t.first) * f, f, t.rows, f0, f}};
+  hand_out<4, 4, 4>(memory, h, out);  // (behind its barrier `share` is whole)
   if (threadIdx.x < t.rows) d_share[uint64_t(at) * p.pairs + t.first + threadIdx.x] = share[threadIdx.x][0] + share[threadIdx.x][1];
-  out.out += f;
-  hand_out<4, 4, 4>(memory, du, out);
-  out.out = wh + uint64_t(t.first) * f;
-  out.stride = f;
-  hand_out<4, 4, 4>(memory, h, out);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) h[i][j] = gu[i + 4 * half][j];
+    out.out = dgu + uint64_t(t.first) * 2 * f + half * f;
+    out.stride = uint64_t(2) * f;
+    hand_out<4, 4, 4>(memory, h, out);
+  }
 }
 
 template <class T>
@@ -498,18 +514,16 @@ __global__ __launch_bounds__(kTileThreads, 2) void input_grad_tile_kernel(Plan p
   uint32_t at;
   if (!tile_of(p, (d + 255) / 256, t, at)) return;
   f32x4 acc[8][4] = {};
-#pragma unroll 1
-  for (uint32_t half = 0; half < 2; ++half) {
+  const auto add = [&](uint32_t half) {
     TileColumnsSource<8, false> w(f, threadIdx.x >> 6 & 1u, reinterpret_cast<const u16*>(p.part[3 * t.e + half]), d, at * 256, d);
     auto v = sorted_rows(t, dgu + half * f, uint64_t(2) * f, f);
     tile_product<T, 8, 4, 3>(w, v, f, lds_offset(memory), acc);
-  }
+  };
+  add(0);
+  add(1);
   TypedOut<T, float> o{{out + uint64_t(t.first) * d, d, t.rows, at * 256, d}};
   hand_out<8, 4, 2>(memory, acc, o);
 }
-
-// Rows of an expert's pairs by way of a map in LDS.
-constexpr uint32_t kMapRows = 1024;
 
 // As weight_grad_any_kernel, out[e][b][a]: 256 columns a of `left` and 128 columns b of `right` a workgroup, the sum over the
 // expert's pairs. One of the two is read through the rows' map (kMapLeft: left). Columns from n_right on belong to out2 (the
@@ -528,41 +542,82 @@ __global__ __launch_bounds__(kTileThreads, 2) void weight_grad_tile_kernel(Plan 
   const uint32_t first = p.first[e], pairs = p.first[e + 1] - first;
   right += which * n_right;
   f32x4 acc[8][4] = {};
-#pragma unroll 1
-  for (uint32_t k = 0; k < pairs; k += kMapRows) {
-    const uint32_t n = pairs - k < kMapRows ? pairs - k : kMapRows;
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n; i += kTileThreads) map[i] = p.row[first + k + i];
+  const auto fill = [&](uint32_t from) {  // half of the ring
+    for (uint32_t i = from + threadIdx.x; i < from + kMapRing / 2 && i < pairs; i += kTileThreads)
+      map[i % kMapRing] = p.row[first + i];
+  };
+  const auto refill = [&](uint32_t k) {
+    if (k && k % (kMapRing / 2) == 0 && k + kMapRing / 2 < pairs) fill(k + kMapRing / 2);
+  };
+  if (pairs) {  // (an expert without pairs gets zeros)
+    fill(0);
+    fill(kMapRing / 2);
     __syncthreads();
     if constexpr (kMapLeft) {
-      TileColumnsSource<8, true> l(n, wave & 1u, left, left_stride, a0, n_left, map);
-      TileColumnsSource<4, false> r(n, wave >> 1, right + uint64_t(first + k) * right_stride, right_stride, b0, n_right);
-      tile_product<T, 8, 4, 3>(l, r, n, lds_offset(memory), acc);
+      TileColumnsSource<8, true> l(pairs, wave & 1u, left, left_stride, a0, n_left, map);
+      TileColumnsSource<4, false> r(pairs, wave >> 1, right + uint64_t(first) * right_stride, right_stride, b0, n_right);
+      tile_product<T, 8, 4, 3>(l, r, pairs, lds_offset(memory), acc, refill);
     } else {
-      TileColumnsSource<8, false> l(n, wave & 1u, left + uint64_t(first + k) * left_stride, left_stride, a0, n_left);
-      TileColumnsSource<4, true> r(n, wave >> 1, right, right_stride, b0, n_right, map);
-      tile_product<T, 8, 4, 3>(l, r, n, lds_offset(memory), acc);
+      TileColumnsSource<8, false> l(pairs, wave & 1u, left + uint64_t(first) * left_stride, left_stride, a0, n_left);
+      TileColumnsSource<4, true> r(pairs, wave >> 1, right, right_stride, b0, n_right, map);
+      tile_product<T, 8, 4, 3>(l, r, pairs, lds_offset(memory), acc, refill);
     }
   }
   TypedOut<T, u16> o{{(which ? out2 : out) + (uint64_t(e) * n_right + b0) * n_left, n_left, n_right - b0, a0, n_left}};
   hand_out<8, 4, 2>(memory, acc, o);
 }
 
-// out_t = residual_t + sum_j w_tj v_{at(t, j)}, in the order of j
-template <class T>
+// out_t = residual_t + sum_j w_tj v_{at(t, j)}, in the order of j; kWide columns a thread (a multiple of 4: one access each).
+template <class T, int kWide>
 __global__ __launch_bounds__(256) void combine_kernel(Plan p, uint32_t rows, uint32_t d, const float* v, const float* weights,
                                                       const u16* residual, uint64_t residual_stride, u16* out,
                                                       uint64_t out_stride) {
-  const uint64_t total = uint64_t(rows) * d;
+  const uint32_t per = d / kWide;
+  const uint64_t total = uint64_t(rows) * per;
   for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += uint64_t(gridDim.x) * 256) {
-    const uint32_t row = uint32_t(i / d), c = uint32_t(i % d);
-    float s = residual ? T::up(residual[row * residual_stride + c]) : 0.0f;
-    for (uint32_t j = 0; j < p.top_k; ++j) {
-      const uint64_t pair = uint64_t(row) * p.top_k + j;
-      const int32_t at = p.at[pair];
-      if (at >= 0) s += (weights ? weights[pair] : 1.0f) * v[uint64_t(uint32_t(at)) * d + c];
+    const uint32_t row = uint32_t(i / per), c = uint32_t(i % per) * kWide;
+    float s[kWide];
+    if constexpr (kWide == 4) {
+      const bits4 r = residual ? *reinterpret_cast<const bits4*>(residual + row * residual_stride + c) : bits4{0, 0, 0, 0};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) s[q] = T::up(r[q]);
+    } else {
+      s[0] = residual ? T::up(residual[row * residual_stride + c]) : 0.0f;
     }
-    out[row * out_stride + c] = T::down(s);
+    for (uint32_t j0 = 0; j0 < p.top_k; j0 += 4) {  // four at once: one after the other each is a memory latency
+      int32_t at[4];
+      float w[4], x[4][kWide];
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        const uint64_t pair = uint64_t(row) * p.top_k + j0 + j;
+        at[j] = j0 + j < p.top_k ? p.at[pair] : -1;
+        w[j] = j0 + j < p.top_k && weights ? weights[pair] : 1.0f;
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        const float* from = v + uint64_t(uint32_t(at[j] < 0 ? 0 : at[j])) * d + c;
+        if constexpr (kWide == 4) {
+          const f32x4 y = at[j] >= 0 ? *reinterpret_cast<const f32x4*>(from) : f32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) x[j][q] = y[q];
+        } else {
+          x[j][0] = at[j] >= 0 ? *from : 0.0f;
+        }
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j)
+        if (at[j] >= 0)
+#pragma unroll
+          for (int q = 0; q < kWide; ++q) s[q] += w[j] * x[j][q];
+    }
+    if constexpr (kWide == 4) {
+      bits4 o;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) o[q] = T::down(s[q]);
+      *reinterpret_cast<bits4*>(out + row * out_stride + c) = o;
+    } else {
+      out[row * out_stride + c] = T::down(s[0]);
+    }
   }
 }
 
@@ -723,7 +778,7 @@ Forward take_forward(Room& r, uint32_t n, uint32_t d, uint32_t f, uint32_t rows,
 struct Backward {
   Plan plan;
   u16 *dgu, *wh;
-  float *share, *out;
+  float *share, *out, *back;  // (back and out share their place: out is written behind back's last reader)
 };
 Backward take_backward(Room& r, uint32_t n, uint32_t d, uint32_t f, uint32_t rows, uint32_t top_k) {
   const uint64_t pairs = uint64_t(rows) * top_k;
@@ -732,7 +787,7 @@ Backward take_backward(Room& r, uint32_t n, uint32_t d, uint32_t f, uint32_t row
   w.dgu = r.take<u16>(pairs * 2 * f);
   w.wh = r.take<u16>(pairs * f);
   w.share = r.take<float>(pairs * ((f + 63) / 64));
-  w.out = r.take<float>(pairs * d);
+  w.out = w.back = r.take<float>(pairs * (d > f ? d : f));
   return w;
 }
 
@@ -741,6 +796,21 @@ uint32_t blocks(uint64_t n) { return uint32_t(n < (1u << 20) ? n : (1u << 20)); 
 int launch_plan(const ExpertMap& e, const int32_t* ids, const Plan& p, uint32_t rows_per_tile, hipStream_t s) {
   hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kPlanThreads), 4 * (kPlanThreads + kPlanWaves * e.n), s, e, ids, p,
                      rows_per_tile);
+  return int(hipGetLastError());
+}
+
+template <class T>
+int launch_combine(const Plan& p, uint32_t rows, uint32_t d, const float* v, const float* weights, const void* residual,
+                   uint64_t residual_stride, void* out, uint64_t out_stride, hipStream_t s) {
+  const u16* r = static_cast<const u16*>(residual);
+  u16* o = static_cast<u16*>(out);
+  const uint64_t odd = reinterpret_cast<uintptr_t>(residual) | 2 * residual_stride | reinterpret_cast<uintptr_t>(out) | 2 * out_stride;
+  if (d % 4 == 0 && odd % 8 == 0)
+    hipLaunchKernelGGL((combine_kernel<T, 4>), dim3(blocks((uint64_t(rows) * d / 4 + 255) / 256)), dim3(256), 0, s, p, rows, d, v,
+                       weights, r, residual_stride, o, out_stride);
+  else
+    hipLaunchKernelGGL((combine_kernel<T, 1>), dim3(blocks((uint64_t(rows) * d + 255) / 256)), dim3(256), 0, s, p, rows, d, v,
+                       weights, r, residual_stride, o, out_stride);
   return int(hipGetLastError());
 }
 
@@ -782,10 +852,7 @@ int forward_few(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& 
   const uint32_t w2 = stream_waves(uint64_t(td) * tiles, chunks_of(f), most_waves(CT));
   hipLaunchKernelGGL((down_few_kernel<T, W, CT, kTail>), dim3(td, tiles), dim3(64 * w2), w2 * CT * 2048, s, w.plan, w.h, d, f,
                      w.out);
-  hipLaunchKernelGGL((combine_kernel<T>), dim3(blocks((uint64_t(a.rows) * d + 255) / 256)), dim3(256), 0, s, w.plan, a.rows, d,
-                     w.out, a.weights, static_cast<const u16*>(a.residual), a.residual_stride, static_cast<u16*>(a.y),
-                     a.y_stride);
-  return int(hipGetLastError());
+  return launch_combine<T>(w.plan, a.rows, d, w.out, a.weights, a.residual, a.residual_stride, a.y, a.y_stride, s);
 }
 
 template <class T, class W, bool kTail>
@@ -809,10 +876,7 @@ int forward_tiles(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args
                      static_cast<const u16*>(a.x), a.x_stride, d, f, a.act, w.h);
   hipLaunchKernelGGL((down_tile_kernel<T>), dim3(tiles * ((d + 255) / 256)), dim3(kTileThreads), tile_lds(8, 4, 3), s, w.plan, w.h,
                      d, f, w.out);
-  hipLaunchKernelGGL((combine_kernel<T>), dim3(blocks((uint64_t(a.rows) * d + 255) / 256)), dim3(256), 0, s, w.plan, a.rows, d,
-                     w.out, a.weights, static_cast<const u16*>(a.residual), a.residual_stride, static_cast<u16*>(a.y),
-                     a.y_stride);
-  return int(hipGetLastError());
+  return launch_combine<T>(w.plan, a.rows, d, w.out, a.weights, a.residual, a.residual_stride, a.y, a.y_stride, s);
 }
 
 template <class T, bool kQ4>
@@ -829,10 +893,7 @@ int forward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& a, v
   hipLaunchKernelGGL((gate_up_any_kernel<T, kQ4>), dim3(tiles * ((f + 63) / 64)), dim3(256), 0, s, w.plan,
                      static_cast<const u16*>(a.x), a.x_stride, d, f, a.act, w.h);
   hipLaunchKernelGGL((down_any_kernel<T, kQ4>), dim3(tiles * ((d + 63) / 64)), dim3(256), 0, s, w.plan, w.h, d, f, w.out);
-  hipLaunchKernelGGL((combine_kernel<T>), dim3(blocks((uint64_t(a.rows) * d + 255) / 256)), dim3(256), 0, s, w.plan, a.rows, d,
-                     w.out, a.weights, static_cast<const u16*>(a.residual), a.residual_stride, static_cast<u16*>(a.y),
-                     a.y_stride);
-  return int(hipGetLastError());
+  return launch_combine<T>(w.plan, a.rows, d, w.out, a.weights, a.residual, a.residual_stride, a.y, a.y_stride, s);
 }
 
 template <class T>
@@ -842,21 +903,22 @@ int backward_tiles(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_gra
   if (int err = launch_plan(e, a.ids, w.plan, kTileRows, s)) return err;
   const uint32_t tiles = most_tiles(w.plan.pairs, e.n, kTileRows), tf = (f + 127) / 128, td = (d + 255) / 256;
   const u16 *x = static_cast<const u16*>(a.x), *dy = static_cast<const u16*>(a.dy);
-  if (tiles)
-    hipLaunchKernelGGL((hidden_grad_tile_kernel<T>), dim3(tiles * tf), dim3(kTileThreads), tile_lds(8, 4, 4), s, w.plan, x,
-                       a.x_stride, dy, a.dy_stride, a.weights, d, f, a.act, w.dgu, w.wh, w.share);
+  if (tiles) {
+    hipLaunchKernelGGL((back_tile_kernel<T>), dim3(tiles * ((f + 255) / 256)), dim3(kTileThreads), tile_lds(8, 4, 3), s, w.plan, dy,
+                       a.dy_stride, d, f, w.back);
+    hipLaunchKernelGGL((hidden_grad_tile_kernel<T>), dim3(tiles * tf), dim3(kTileThreads), tile_lds(8, 4, 3), s, w.plan, x,
+                       a.x_stride, w.back, a.weights, d, f, a.act, w.dgu, w.wh, w.share);
+  }
   if (a.dx && tiles) {
     hipLaunchKernelGGL((input_grad_tile_kernel<T>), dim3(tiles * td), dim3(kTileThreads), tile_lds(8, 4, 3), s, w.plan, w.dgu, d, f,
                        w.out);
-    hipLaunchKernelGGL((combine_kernel<T>), dim3(blocks((uint64_t(a.rows) * d + 255) / 256)), dim3(256), 0, s, w.plan, a.rows,
-                       d, w.out, static_cast<const float*>(nullptr), static_cast<const u16*>(nullptr), uint64_t(0),
-                       static_cast<u16*>(a.dx), a.dx_stride);
+    if (int err = launch_combine<T>(w.plan, a.rows, d, w.out, nullptr, nullptr, 0, a.dx, a.dx_stride, s)) return err;
   }
   if (a.dweights && tiles)
     hipLaunchKernelGGL(weights_grad_kernel, dim3(blocks((w.plan.pairs + 255) / 256)), dim3(256), 0, s, w.plan, tf, w.share,
                        a.dweights);
   if (a.dgate) {
-    constexpr uint32_t kLds = tile_lds(8, 4, 3) + 4 * kMapRows;
+    constexpr uint32_t kLds = tile_lds(8, 4, 3) + 4 * kMapRing;
     hipLaunchKernelGGL((weight_grad_tile_kernel<T, true>), dim3(e.n * td * tf * 2), dim3(kTileThreads), kLds, s, w.plan, x,
                        a.x_stride, d, w.dgu, uint64_t(2) * f, f, 2u, static_cast<u16*>(a.dgate), static_cast<u16*>(a.dup));
     hipLaunchKernelGGL((weight_grad_tile_kernel<T, false>), dim3(e.n * ((f + 255) / 256) * ((d + 127) / 128)), dim3(kTileThreads),
@@ -881,9 +943,7 @@ int backward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_grad_args
                        a.weights, d, f, a.act, w.dgu, w.wh, w.share);
   if (a.dx && tiles) {
     hipLaunchKernelGGL((input_grad_any_kernel<T>), dim3(tiles * td), dim3(256), 0, s, w.plan, w.dgu, d, f, w.out);
-    hipLaunchKernelGGL((combine_kernel<T>), dim3(blocks((uint64_t(a.rows) * d + 255) / 256)), dim3(256), 0, s, w.plan, a.rows,
-                       d, w.out, static_cast<const float*>(nullptr), static_cast<const u16*>(nullptr), uint64_t(0),
-                       static_cast<u16*>(a.dx), a.dx_stride);
+    if (int err = launch_combine<T>(w.plan, a.rows, d, w.out, nullptr, nullptr, 0, a.dx, a.dx_stride, s)) return err;
   }
   if (a.dweights && tiles)
     hipLaunchKernelGGL(weights_grad_kernel, dim3(blocks((w.plan.pairs + 255) / 256)), dim3(256), 0, s, w.plan, tf, w.share,

@@ -99,6 +99,9 @@ __device__ __forceinline__ void load_offset_to_lds(uint64_t base, uint32_t offse
       : "memory", "m0");
 }
 
+// A map in LDS is a ring of kMapRing entries, refilled half by half while the sum goes on.
+constexpr uint32_t kMapRing = 2048;
+
 // In columns: 32 NF columns from `first` on (n_cols in all, a multiple of 8), row k of the sum at at + k stride, or with a
 // map (in LDS) at at + map[k] stride. stride is below 2^24. Buffers are 512-byte aligned: a fragment's place is its wave's
 // first one's with the fragment's number in three bits that the permutation turns.
@@ -139,7 +142,7 @@ struct TileColumnsSource {
         const uint32_t row = k + 32 * s + row_of(j);
         const bool in = !kCheck || row < n;
         uint64_t g = base + offset[j];
-        if constexpr (kMap) g += uint64_t(map[in ? row : 0]) * stride;
+        if constexpr (kMap) g += uint64_t(map[in ? row % kMapRing : 0]) * stride;
         else g += uint64_t(32 * s) * stride;
         load_to_lds(in ? reinterpret_cast<const void*>(g) : &kZeroPiece, to);
       } else {
@@ -173,8 +176,13 @@ __device__ __forceinline__ void settle(f32x4 (&acc)[NI][MJ]) {
 
 // acc[i][j] += a's rows 16 i.. of this wave's half times b's rows 16 j.. of its half, over the sources' n values. Lane l
 // holds a-rows 4 (l / 16) + 0..3 and b-row l % 16 of each.
-template <class T, int NI, int MJ, int NB, class A, class B>
-__device__ __forceinline__ void tile_product(A& a, B& b, uint32_t n, uint32_t lds, f32x4 (&acc)[NI][MJ]) {
+// every_two(k): behind the barrier of each second step (3 buffers), when every wave has issued the loads of the values below
+// k + 64.
+struct Nothing {
+  __device__ __forceinline__ void operator()(uint32_t) const {}
+};
+template <class T, int NI, int MJ, int NB, class A, class B, class F = Nothing>
+__device__ __forceinline__ void tile_product(A& a, B& b, uint32_t n, uint32_t lds, f32x4 (&acc)[NI][MJ], F&& every_two = F{}) {
   static_assert(NB == 3 || NB == 4, "buffers");
   constexpr int kLoads = (NI + MJ) / 2;  // of a step, each thread
   constexpr uint32_t kA = NI * 2048, kBuffer = (NI + MJ) * 2048;
@@ -224,7 +232,7 @@ __device__ __forceinline__ void tile_product(A& a, B& b, uint32_t n, uint32_t ld
     }
     at = at + 1 == NB ? 0 : at + 1;
   };
-  const auto two_steps = [&](auto check) {
+  const auto two_steps = [&](auto check, uint32_t t) {
     using Zero = std::integral_constant<int, 0>;
     using One = std::integral_constant<int, 1>;
     if (NB == 4) {
@@ -233,6 +241,7 @@ __device__ __forceinline__ void tile_product(A& a, B& b, uint32_t n, uint32_t ld
       step(One{}, std::true_type{}, check);
     } else {
       meet();
+      every_two(t * 32);
       step(Zero{}, std::true_type{}, check);
       wait_loads_and_meet<0>();
       step(One{}, std::false_type{}, check);
@@ -240,8 +249,8 @@ __device__ __forceinline__ void tile_product(A& a, B& b, uint32_t n, uint32_t ld
   };
   constexpr uint32_t kAhead = NB == 4 ? 6 : 4;  // the last step that two steps from t on load, + 1
   uint32_t t = 0;
-  for (; (t + kAhead) * 32 <= n; t += 2) two_steps(std::false_type{});
-  for (; t * 32 < n; t += 2) two_steps(std::true_type{});  // (steps past the end multiply zeros)
+  for (; (t + kAhead) * 32 <= n; t += 2) two_steps(std::false_type{}, t);
+  for (; t * 32 < n; t += 2) two_steps(std::true_type{}, t);  // (steps past the end multiply zeros)
   // The loads past the end have landed, and the last results are written before anything reads them (18 wait states).
   asm volatile("s_waitcnt vmcnt(0)\n\ts_nop 15\n\ts_nop 3" ::: "memory");
   settle(acc);
