@@ -187,7 +187,7 @@ def linear64(x, w, bias, residual, act):
     return y if residual is None else y + residual.double()
 
 
-LINEAR = [(1, 64, 16), (1, 4096, 4096), (2, 200, 33), (7, 72, 257), (16, 512, 96), (17, 1000, 130), (33, 256, 64),
+LINEAR = [(1, 64, 16), (1, 4096, 4096), (1, 1280, 37), (1, 256, 16), (1, 2560, 200), (2, 200, 33), (7, 72, 257), (16, 512, 96), (17, 1000, 130), (33, 256, 64),
           (64, 2048, 520), (65, 96, 128), (129, 320, 384), (300, 640, 256), (515, 1096, 776)]
 
 
@@ -315,7 +315,7 @@ def ffn64(layer, x, ids, weights, residual, act, dy=None):
     return y if dy is None else (dx, dw, grads)
 
 
-FFN = [(1, 1, 1, 64, 64), (1, 8, 2, 256, 512), (1, 4, 3, 96, 160), (2, 8, 2, 512, 128), (5, 16, 4, 128, 96), (32, 40, 8, 256, 192),
+FFN = [(1, 1, 1, 64, 64), (1, 6, 3, 1280, 768), (1, 9, 8, 768, 2304), (1, 3, 2, 256, 1024),(1, 8, 2, 256, 512), (1, 4, 3, 96, 160), (2, 8, 2, 512, 128), (5, 16, 4, 128, 96), (32, 40, 8, 256, 192),
        (37, 8, 2, 320, 256), (64, 2, 2, 128, 416), (200, 3, 2, 160, 288), (300, 5, 3, 512, 256), (700, 2, 1, 256, 320)]
 
 

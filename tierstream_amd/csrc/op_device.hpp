@@ -102,6 +102,23 @@ __device__ __forceinline__ void store_float(void* p, uint64_t i, uint32_t type, 
   else static_cast<u16*>(p)[i] = type == TSA_BF16 ? Bf16::down(v) : F16::down(v);
 }
 
+// ---- loads straight to LDS ----
+static __device__ const u32x4 kZeroPiece = {0, 0, 0, 0};  // what a load past the end of a row or a sum reads
+
+// 64 lanes x 16 bytes to LDS at `at` (the same in every lane) in lane order.
+__device__ __forceinline__ void load_to_lds(const void* g, uint32_t at) {
+  asm volatile(
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %0, off"
+      :
+      : "v"(g), "s"(at)
+      : "memory", "m0");
+}
+__device__ __forceinline__ uint32_t lds_offset(const void* p) {
+  return uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)p));
+}
+
 // ---- the 64 x 64 tile for any stride ----------------------------------------------------------------------------------
 // A matrix operand: element (r, k) at base + r rs + k ks, rows through `map` if there is one; zero outside rows x n.
 struct Operand {

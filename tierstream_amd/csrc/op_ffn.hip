@@ -225,33 +225,42 @@ __global__ __launch_bounds__(64 * most_waves(1)) void gate_up_one_kernel(ExpertM
   });
 }
 
+// The experts of one row that add something: part `which` of each and its j, in the order of j.
+struct LiveExperts {
+  const char* part[TSA_ROUTE_MAX_TOP_K];
+  uint32_t from[TSA_ROUTE_MAX_TOP_K], n;
+};
+__device__ __forceinline__ void find_live(const ExpertMap& m, const int32_t* ids, uint32_t top_k, int which, LiveExperts& live) {
+  const uint32_t lane = threadIdx.x;
+  if (lane < 64) {
+    const char* p[3];
+    const bool on = lane < top_k && resolve(m, expert_of(m, ids, lane), p);
+    const uint64_t has = __ballot(on);
+    if (on) {
+      const uint32_t i = uint32_t(__popcll(has & ((1ull << lane) - 1)));
+      live.part[i] = p[which];
+      live.from[i] = lane;
+    }
+    if (lane == 0) live.n = uint32_t(__popcll(has));
+  }
+  __syncthreads();
+}
+
 // y = residual + sum_j down_j h_j: one row over the chunks of all its experts.
 template <class T, class W, bool kTail>
 __global__ __launch_bounds__(64 * most_waves(1)) void down_one_kernel(ExpertMap m, const int32_t* ids, uint32_t top_k,
                                                                       const u16* h, uint32_t d, uint32_t f,
                                                                       const u16* residual, u16* y) {
   extern __shared__ f32x4 part[];
-  __shared__ const char* down[TSA_ROUTE_MAX_TOP_K];
-  __shared__ uint32_t from[TSA_ROUTE_MAX_TOP_K], n_live;
+  __shared__ LiveExperts live;
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  if (wave == 0) {
-    const char* p[3];
-    const bool on = lane < top_k && resolve(m, expert_of(m, ids, lane), p);
-    const uint64_t live = __ballot(on);
-    if (on) {
-      const uint32_t i = uint32_t(__popcll(live & ((1ull << lane) - 1)));
-      down[i] = p[2];
-      from[i] = lane;
-    }
-    if (lane == 0) n_live = uint32_t(__popcll(live));
-  }
-  __syncthreads();
+  find_live(m, ids, top_k, 2, live);
   const uint32_t c0 = blockIdx.x * 16 + (lane & 15u), col = c0 < d ? c0 : d - 1, per = (f + kChunk - 1) / kChunk;
   f32x4 acc[1][1] = {};
-  stream_chunks<W, 1, 1, kTail>(n_live * per, wave, waves, [&](uint32_t c, W (&w)[1], const u16* (&row)[1]) {
+  stream_chunks<W, 1, 1, kTail>(live.n * per, wave, waves, [&](uint32_t c, W (&w)[1], const u16* (&row)[1]) {
     const uint32_t j = c / per;
-    w[0] = W(down[j], f, col, f);
-    row[0] = h + uint64_t(from[j]) * f;
+    w[0] = W(live.part[j], f, col, f);
+    row[0] = h + uint64_t(live.from[j]) * f;
     return (c - j * per) * kChunk;
   }, acc);
   const f32x4 v[1] = {acc[0][0]};
@@ -259,6 +268,54 @@ __global__ __launch_bounds__(64 * most_waves(1)) void down_one_kernel(ExpertMap 
     if (wave != 0) return;
     const float s = sum(0)[0] + (residual && c0 < d ? T::up(residual[c0]) : 0.0f);
     if (lane < 16 && c0 < d) y[c0] = T::down(s);
+  });
+}
+
+// The same two with 4-bit weights by way of LDS (d and f multiples of 256, 16-byte aligned weights).
+template <class T>
+__global__ __launch_bounds__(64 * kQ4Waves) void gate_up_q4_kernel(ExpertMap m, const int32_t* ids, const float* weights,
+                                                                   const u16* x, uint32_t d, uint32_t f, uint32_t act, u16* h) {
+  extern __shared__ f32x4 memory[];
+  __shared__ float part[kQ4Waves * 2 * 16];
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const char* p[3];
+  if (!resolve(m, expert_of(m, ids, blockIdx.y), p)) return;
+  const uint32_t c0 = blockIdx.x * 16;
+  const uint64_t row = uint64_t(d / kQ4Block) * kQ4Bytes;
+  float acc[2] = {};
+  stream_q4<T, 2>((d + 511) / 512, wave, waves, f - c0 < 16 ? f - c0 : 16, d, lds_offset(memory) + wave * 2 * Q4Stage<2>::kBytes,
+                  [&](uint32_t s, const char* (&base)[2], const u16*& xs) {
+                    base[0] = p[0] + c0 * row;
+                    base[1] = p[1] + c0 * row;
+                    xs = x;
+                    return s * 512;
+                  }, acc);
+  join_q4<2>(part, acc, wave, waves, [&](const float (&s)[2]) {
+    if (c0 + lane < f)
+      h[uint64_t(blockIdx.y) * f + c0 + lane] = T::down((weights ? weights[blockIdx.y] : 1.0f) * activate(act, s[0]) * s[1]);
+  });
+}
+
+template <class T>
+__global__ __launch_bounds__(64 * kQ4Waves) void down_q4_kernel(ExpertMap m, const int32_t* ids, uint32_t top_k, const u16* h,
+                                                                uint32_t d, uint32_t f, const u16* residual, u16* y) {
+  extern __shared__ f32x4 memory[];
+  __shared__ float part[kQ4Waves * 16];
+  __shared__ LiveExperts live;
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  find_live(m, ids, top_k, 2, live);
+  const uint32_t c0 = blockIdx.x * 16, per = (f + 1023) / 1024;
+  const uint64_t row = uint64_t(f / kQ4Block) * kQ4Bytes;
+  float acc[1] = {};
+  stream_q4<T, 1>(live.n * per, wave, waves, d - c0 < 16 ? d - c0 : 16, f, lds_offset(memory) + wave * 2 * Q4Stage<1>::kBytes,
+                  [&](uint32_t s, const char* (&base)[1], const u16*& xs) {
+                    const uint32_t j = s / per;
+                    base[0] = live.part[j] + c0 * row;
+                    xs = h + uint64_t(live.from[j]) * f;
+                    return (s - j * per) * 1024;
+                  }, acc);
+  join_q4<1>(part, acc, wave, waves, [&](const float (&s)[1]) {
+    if (c0 + lane < d) y[c0 + lane] = T::down(s[0] + (residual ? T::up(residual[c0 + lane]) : 0.0f));
   });
 }
 
@@ -818,15 +875,17 @@ bool aligned16(const void* p, uint64_t stride_bytes) { return (reinterpret_cast<
 
 // Whether every weight row, x row and row of h starts 16-byte aligned and holds whole groups of 8 values. The addresses of
 // a table's units are the device's: its units are 256-byte aligned, as the library lays them out.
-bool wide_rows(const ExpertMap& e, uint32_t d, uint32_t f, bool q4, const void* x, uint64_t x_stride) {
-  if (d % 8 || f % 8 || !aligned16(x, 2 * x_stride) || x_stride >= 1u << 24) return false;
-  if (q4) return true;
+bool wide_weights(const ExpertMap& e) {
   for (int p = 0; p < 3; ++p) {
     if (e.form == 0 && !aligned16(e.part[p], e.stride[p])) return false;
     if (e.form == 1 && e.stride[p] % 16) return false;
     if (e.form == 2 && !aligned16(e.view.parts[p].base, e.view.parts[p].stride)) return false;
   }
   return true;
+}
+bool wide_rows(const ExpertMap& e, uint32_t d, uint32_t f, bool q4, const void* x, uint64_t x_stride) {
+  if (d % 8 || f % 8 || !aligned16(x, 2 * x_stride) || x_stride >= 1u << 24) return false;
+  return q4 || wide_weights(e);
 }
 
 template <class T, class W, bool kTail>
@@ -838,6 +897,19 @@ int forward_one(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& 
                      static_cast<const u16*>(a.x), d, f, a.act, h);
   const uint32_t w2 = stream_waves(td, uint64_t(chunks_of(f)) * a.top_k, 16);
   hipLaunchKernelGGL((down_one_kernel<T, W, kTail>), dim3(td), dim3(64 * w2), w2 * 1024, s, e, a.ids, a.top_k, h, d, f,
+                     static_cast<const u16*>(a.residual), static_cast<u16*>(a.y));
+  return int(hipGetLastError());
+}
+
+template <class T>
+int forward_one_q4(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& a, void* ws, hipStream_t s) {
+  u16* h = static_cast<u16*>(ws);
+  const uint32_t tf = (f + 15) / 16, td = (d + 15) / 16;
+  const uint32_t w1 = q4_waves(uint64_t(tf) * a.top_k, (d + 511) / 512);
+  hipLaunchKernelGGL((gate_up_q4_kernel<T>), dim3(tf, a.top_k), dim3(64 * w1), w1 * 2 * Q4Stage<2>::kBytes, s, e, a.ids, a.weights,
+                     static_cast<const u16*>(a.x), d, f, a.act, h);
+  const uint32_t w2 = q4_waves(td, uint64_t((f + 1023) / 1024) * a.top_k);
+  hipLaunchKernelGGL((down_q4_kernel<T>), dim3(td), dim3(64 * w2), w2 * 2 * Q4Stage<1>::kBytes, s, e, a.ids, a.top_k, h, d, f,
                      static_cast<const u16*>(a.residual), static_cast<u16*>(a.y));
   return int(hipGetLastError());
 }
@@ -882,6 +954,8 @@ int forward_tiles(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args
 template <class T, bool kQ4>
 int forward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& a, void* ws, hipStream_t s) {
   typedef std::conditional_t<kQ4, RowsQ4<T>, Rows16<T>> W;
+  if constexpr (kQ4)
+    if (a.rows == 1 && d % 256 == 0 && f % 256 == 0 && aligned16(a.x, 0) && wide_weights(e)) return forward_one_q4<T>(e, d, f, a, ws, s);
   if (wide_rows(e, d, f, kQ4, a.x, a.x_stride) && uint64_t(a.rows) * a.top_k <= uint64_t(64) * e.n)
     return d % kChunk || f % kChunk ? forward_stream<T, W, true>(e, d, f, a, ws, s) : forward_stream<T, W, false>(e, d, f, a, ws, s);
   if constexpr (!kQ4)

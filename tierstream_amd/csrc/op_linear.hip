@@ -128,6 +128,32 @@ __global__ __launch_bounds__(64 * most_waves(CT)) void linear_few_kernel(tsa_lin
   });
 }
 
+// One row, 4-bit weights by way of LDS (n_in a multiple of 256).
+template <class T>
+__global__ __launch_bounds__(64 * kQ4Waves) void linear_q4_kernel(tsa_linear_args a) {
+  extern __shared__ f32x4 memory[];
+  __shared__ float part[kQ4Waves * 16];
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const uint32_t n0 = blockIdx.x * 16;
+  float acc[1] = {};
+  stream_q4<T, 1>((a.n_in + 1023) / 1024, wave, waves, a.n_out - n0 < 16 ? a.n_out - n0 : 16, a.n_in,
+                  lds_offset(memory) + wave * 2 * Q4Stage<1>::kBytes, [&](uint32_t s, const char* (&base)[1], const u16*& x) {
+                    base[0] = static_cast<const char*>(a.w) + uint64_t(n0) * (a.n_in / kQ4Block * kQ4Bytes);
+                    x = static_cast<const u16*>(a.x);
+                    return s * 1024;
+                  }, acc);
+  join_q4<1>(part, acc, wave, waves, [&](const float (&s)[1]) {
+    if (n0 + lane < a.n_out) finish_linear(a, 0, n0 + lane, s[0]);
+  });
+}
+
+template <class T>
+int launch_q4(const tsa_linear_args& a, hipStream_t stream) {
+  const uint32_t tn = (a.n_out + 15) / 16, waves = q4_waves(tn, (a.n_in + 1023) / 1024);
+  hipLaunchKernelGGL((linear_q4_kernel<T>), dim3(tn), dim3(64 * waves), waves * 2 * Q4Stage<1>::kBytes, stream, a);
+  return int(hipGetLastError());
+}
+
 template <class T, class W, int R, int CT>
 int launch_few(const tsa_linear_args& a, hipStream_t stream) {
   const uint32_t tn = (a.n_out + 16 * R - 1) / (16 * R), tr = (a.rows + 16 * CT - 1) / (16 * CT);
@@ -186,6 +212,8 @@ uint64_t linear_workspace(const tsa_linear_args&) { return 0; }
 int launch_linear(const tsa_linear_args& a, void*, hipStream_t stream) {
   if (a.rows == 0 || a.n_out == 0) return 0;
   const bool wide = a.n_in % 8 == 0 && op::aligned16(a.x, a.x_stride) && (a.w_type == TSA_Q4 || op::aligned16(a.w, a.w_stride));
+  if (wide && a.rows == 1 && a.w_type == TSA_Q4 && a.n_in % 256 == 0 && op::aligned16(a.w, 0))
+    return a.x_type == TSA_BF16 ? op::launch_q4<op::Bf16>(a, stream) : op::launch_q4<op::F16>(a, stream);
   if (wide && a.rows <= 64) {
     if (a.x_type == TSA_BF16)
       return a.w_type == TSA_Q4 ? op::launch_few<op::Bf16, op::RowsQ4<op::Bf16>>(a, stream)

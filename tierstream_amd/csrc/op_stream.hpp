@@ -206,6 +206,114 @@ __device__ __forceinline__ void join_waves(f32x4* part, const f32x4 (&v)[V], uin
   });
 }
 
+// ---- one row of x, 4-bit rows through LDS ----
+//
+// A 4-bit lane's own loads are 2 and 4 bytes, 16 lines an instruction: 1.1 TB/s. Here a wave fills LDS of its own in 16-byte
+// pieces (load_to_lds), a stage of 9 KiB at a time with the next one in flight: 1024 / R values of 16 rows of R parts, laid
+// out as [8 blocks][row][144 bytes], and x's values of the stage behind it. Two blocks are 9 words: the first one's half
+// bytes are the words q and q + 1 shifted by 16 bits, the second one's word q + 5 (q = lane / 16), the scales the low half of
+// word 0 and the high half of word 4. A row's 36 words put 16 rows x 4 lanes on all banks. All 16 rows of operand a are the
+// one row of x, so every result row is the same and one accumulator a part is kept.
+template <int R>
+struct Q4Stage {
+  static constexpr uint32_t kValues = 1024 / R, kGroups = 4 / R, kXLoads = 2 / R, kLoads = 9 + kXLoads;
+  static constexpr uint32_t kBytes = kLoads * 1024, kBuffers = 2;
+};
+
+// Adds stages wave, wave + waves, .. below n_stages to acc. at(s, base, x) gives the stage's parts' first row of the tile,
+// the row of x, and returns its first value k; rows: the tile's rows (up to 16), n: values of a row, a multiple of 256.
+// Addresses are 16-byte aligned. lds: this wave's 2 x kBytes.
+template <class T, int R, class At>
+__device__ __forceinline__ void stream_q4(uint32_t n_stages, uint32_t wave, uint32_t waves, uint32_t rows, uint32_t n, uint32_t lds,
+                                          At&& at, float (&acc)[R]) {
+  typedef Q4Stage<R> S;
+  const uint32_t lane = threadIdx.x & 63u, q = lane >> 4, row_bytes = n / kQ4Block * kQ4Bytes;
+  const auto issue = [&](uint32_t s, uint32_t to) {
+    const char* base[R];
+    const u16* x;
+    const uint32_t k = at(s, base, x);
+#pragma unroll
+    for (uint32_t l = 0; l < 9; ++l) {
+      const uint32_t p = l * 64 + lane, piece = p % 9, row = p / 9 % (16 * R), g = p / (9 * 16 * R);
+      const uint32_t r = (row & 15u) < rows ? row & 15u : rows - 1;
+      const uint64_t off = uint64_t(r) * row_bytes + (k + (k + 256 * g < n ? 256 * g : 0)) / 256 * 144 + piece * 16;
+      load_to_lds((R == 1 || row < 16 ? base[0] : base[R - 1]) + off, to + l * 1024);
+    }
+#pragma unroll
+    for (uint32_t l = 0; l < S::kXLoads; ++l) {
+      const uint32_t v = k + l * 512 + lane * 8;
+      load_to_lds(v < n ? static_cast<const void*>(x + v) : &kZeroPiece, to + (9 + l) * 1024);
+    }
+  };
+  typedef __attribute__((address_space(3))) const uint32_t lds_word_t;
+  typedef __attribute__((address_space(3))) const bits4 lds_bits4_t;
+  const auto add = [&](uint32_t from) {
+    for (uint32_t g = 0; g < S::kGroups; ++g)
+#pragma unroll
+      for (uint32_t pair = 0; pair < 4; ++pair) {
+        bits8 x[2];
+        f32x4 off[2];
+        constexpr u16 m = HalfBytes<T>::kMinus;
+#pragma unroll
+        for (uint32_t b = 0; b < 2; ++b) {
+          const uint32_t xa = from + 9216 + (g * 256 + pair * 64 + b * 32 + q * 4) * 2;
+          const bits4 lo = *reinterpret_cast<lds_bits4_t*>(xa), hi = *reinterpret_cast<lds_bits4_t*>(xa + 32);
+          x[b] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+          off[b] = T::mfma(x[b], bits8{m, m, m, m, m, m, m, m}, f32x4{0, 0, 0, 0});
+        }
+#pragma unroll
+        for (uint32_t r = 0; r < R; ++r) {
+          lds_word_t* w = reinterpret_cast<lds_word_t*>(from + ((g * R + r) * 16 + (lane & 15u)) * 144 + pair * 36);
+          const uint32_t w0 = w[q], w1 = w[q + 1], w5 = w[q + 5], s0 = w[0], s1 = w[4];
+          const f32x4 even = T::mfma(x[0], HalfBytes<T>::unpack(__builtin_amdgcn_alignbit(w1, w0, 16)), off[0]);
+          const f32x4 odd = T::mfma(x[1], HalfBytes<T>::unpack(w5), off[1]);
+          acc[r] += F16::up(u16(s0)) * even[0];
+          acc[r] += F16::up(u16(s1 >> 16)) * odd[0];
+        }
+      }
+  };
+  if (wave >= n_stages) return;
+  issue(wave, lds);
+  uint32_t now = 0;
+  for (uint32_t s = wave; s < n_stages; s += waves) {
+    if (s + waves < n_stages) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads of the buffer that is filled now
+      issue(s + waves, lds + (now ^ 1) * S::kBytes);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::kLoads) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    add(lds + now * S::kBytes);
+    now ^= 1;
+  }
+}
+
+constexpr uint32_t kQ4Waves = 4;
+// Waves per workgroup: enough for about 6 a CU, which is what LDS holds.
+inline uint32_t q4_waves(uint64_t workgroups, uint64_t stages) {
+  uint32_t w = 1;
+  while (w < kQ4Waves && workgroups * w < 1536 && 2 * w <= stages) w *= 2;
+  return w;
+}
+
+// The waves' sums added in their order, by wave 0: lanes 0..15 call f(acc of the tile's row lane).
+template <int R, class F>
+__device__ __forceinline__ void join_q4(float* part, const float (&acc)[R], uint32_t wave, uint32_t waves, F&& f) {
+  const uint32_t lane = threadIdx.x & 63u;
+  if (lane < 16)
+#pragma unroll
+    for (int r = 0; r < R; ++r) part[(wave * R + r) * 16 + lane] = acc[r];
+  __syncthreads();
+  if (wave != 0 || lane >= 16) return;
+  float s[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    s[r] = part[r * 16 + lane];
+    for (uint32_t w = 1; w < waves; ++w) s[r] += part[(w * R + r) * 16 + lane];
+  }
+  f(s);
+}
+
 // The registers of CT tiles of x bound the waves of a workgroup.
 constexpr uint32_t most_waves(int CT) { return CT == 1 ? 16 : CT == 2 ? 8 : 4; }
 

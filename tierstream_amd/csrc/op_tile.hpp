@@ -27,26 +27,10 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4_t;
 typedef __attribute__((address_space(3))) const bits8 lds_bits8_t;
 
-static __device__ const u32x4 kZeroPiece = {0, 0, 0, 0};  // what a load past the end of the sum reads
-
-// 64 lanes x 16 bytes to LDS at `at` (the same in every lane) in lane order.
-__device__ __forceinline__ void load_to_lds(const void* g, uint32_t at) {
-  asm volatile(
-      "s_mov_b32 m0, %1\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %0, off"
-      :
-      : "v"(g), "s"(at)
-      : "memory", "m0");
-}
 __device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void wait_loads_and_meet() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
-}
-
-__device__ __forceinline__ uint32_t lds_offset(const void* p) {
-  return uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)p));
 }
 
 // An operand of 32 NF rows, in rows: at(r) gives row r's first value (any valid row for r behind the last).
