@@ -16,11 +16,24 @@ namespace {
 
 constexpr uint32_t kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
 
+// What ss_dg_slot gives for id e (below m.n), with its loads at once instead of one behind the other's test: they stand in
+// front of every product of a decode step.
+__device__ __forceinline__ int32_t slot_of(const ExpertMap& m, uint32_t e) {
+  const ss_dg_device_view& v = m.view;
+  const uint32_t abort = __hip_atomic_load(v.abort, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const uint32_t base = v.unit_base[m.gated], end = v.unit_base[m.gated + 1];
+  const bool in = e < end - base;
+  const int32_t s = in ? __hip_atomic_load(v.slot_of + base + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+  if (abort || !in) return int32_t(v.guard_slot);
+  if (s >= 0) return s;
+  if (v.absent_err) atomicOr(v.absent_err, 1u);  // (null where the view's version has none)
+  return int32_t(v.guard_slot);
+}
+
 __device__ __forceinline__ void part_pointers(const ExpertMap& m, uint32_t e, const char* (&p)[3]) {
   if (m.form == 2) {
-    const int32_t s = ss_dg_slot(&m.view, m.gated, int32_t(e));
-    for (int i = 0; i < 3; ++i)
-      p[i] = static_cast<const char*>(m.view.parts[i].base) + uint64_t(uint32_t(s)) * m.view.parts[i].stride;
+    const uint64_t s = uint32_t(slot_of(m, e));
+    for (int i = 0; i < 3; ++i) p[i] = static_cast<const char*>(m.view.parts[i].base) + s * m.view.parts[i].stride;
   } else if (m.form == 1) {
     for (int i = 0; i < 3; ++i) p[i] = reinterpret_cast<const char*>(m.table[e]) + m.stride[i];
   } else {

@@ -288,12 +288,13 @@ __device__ __forceinline__ void stream_q4(uint32_t n_stages, uint32_t wave, uint
   }
 }
 
-constexpr uint32_t kQ4Waves = 4;
-// Waves per workgroup: enough for about 6 a CU, which is what LDS holds.
+constexpr uint32_t kQ4Waves = 7;  // what LDS holds
+// Waves per workgroup: enough for 4 a CU. Eight 24.8 MB experts, gate and up (1024 workgroups): 32 us with one wave each, 37 with
+// two, 44 with four; down (448 workgroups): 39, 29, 25.5 and 27.6 us with one, two, three and four.
 inline uint32_t q4_waves(uint64_t workgroups, uint64_t stages) {
-  uint32_t w = 1;
-  while (w < kQ4Waves && workgroups * w < 1536 && 2 * w <= stages) w *= 2;
-  return w;
+  uint64_t w = (1024 + workgroups - 1) / workgroups;
+  if (w > kQ4Waves) w = kQ4Waves;
+  return uint32_t(w < stages ? w : stages);
 }
 
 // The waves' sums added in their order, by wave 0: lanes 0..15 call f(acc of the tile's row lane).
