@@ -74,28 +74,48 @@ def _ops() -> C.CDLL:
     return _lib
 
 
+# Calls of a decode step take microseconds on the device: what runs on the host for each is kept short. Names of types are
+# looked up once per type.
+_of_dtype: dict = {}
+
+
 def _type(t) -> int:
-    return _TYPES[str(t.dtype)]
+    d = t.dtype
+    kind = _of_dtype.get(d)
+    if kind is None:
+        kind = _of_dtype[d] = _TYPES[str(d)]
+    return kind
 
 
 def _mat(t, rows: int, cols: int, what: str, kind: int | None = None):
     """(pointer, row stride) of a matrix with contiguous rows."""
-    if t is None:
-        return None, 0
-    if tuple(t.shape) != (rows, cols) or (cols > 1 and t.stride(1) != 1):
+    stride = t.stride()
+    if t.shape != (rows, cols) or (cols > 1 and stride[1] != 1):
         raise ValueError(f"{what}: a [{rows}][{cols}] matrix with contiguous rows, not {tuple(t.shape)}")
     if kind is not None and _type(t) != kind:
         raise ValueError(f"{what}: another type than the operator's ({t.dtype})")
-    return t.data_ptr(), t.stride(0)
+    return t.data_ptr(), stride[0]
+
+
+_dtype_named: dict = {}
 
 
 def _vec(t, shape, dtype: str, what: str):
     """Pointer of a contiguous array."""
     if t is None:
         return None
-    if tuple(t.shape) != tuple(shape) or str(t.dtype) != dtype or not t.is_contiguous():
+    d = t.dtype
+    name = _dtype_named.get(d)
+    if name is None:
+        name = _dtype_named[d] = str(d)
+    if t.shape != shape or name != dtype or not t.is_contiguous():
         raise ValueError(f"{what}: a contiguous {dtype} array of {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
+
+
+def _ok(status: int) -> None:
+    if status:
+        check(status)
 
 
 def _room(workspace):
@@ -105,53 +125,53 @@ def _room(workspace):
 # ---- the choice of experts -------------------------------------------------------------------------------------------
 def _route_args(logits, ids, weights, renorm, scale):
     rows, n = logits.shape
-    k = ids.shape[1]
+    shape = (rows, ids.shape[1])
     p, stride = _mat(logits, rows, n, "logits")
-    return TsaRouteArgs(p, stride, _vec(ids, (rows, k), "torch.int32", "ids"),
-                        _vec(weights, (rows, k), "torch.float32", "weights"), rows, n, k, _type(logits), int(renorm), scale)
+    return TsaRouteArgs(p, stride, _vec(ids, shape, "torch.int32", "ids"), _vec(weights, shape, "torch.float32", "weights"), rows, n,
+                        shape[1], _type(logits), renorm, scale)
 
 
 def route(logits, ids, weights, *, renorm=True, scale=1.0, stream=None) -> None:
     """ids int32 [rows][top_k] and weights float32 [rows][top_k] of each row's largest logits (tsa_route)."""
-    check(_ops().tsa_route(C.byref(_route_args(logits, ids, weights, renorm, scale)), stream))
+    _ok(_ops().tsa_route(_route_args(logits, ids, weights, renorm, scale), stream))
 
 
 def route_backward(logits, ids, dweights, dlogits, *, renorm=True, scale=1.0, stream=None) -> None:
     """dlogits (the logits' type) from dweights (tsa_route_backward)."""
     a = _route_args(logits, ids, None, renorm, scale)
     p, stride = _mat(dlogits, a.rows, a.n_experts, "dlogits", a.type)
-    check(_ops().tsa_route_backward(C.byref(a), _vec(dweights, ids.shape, "torch.float32", "dweights"), p, stride, stream))
+    _ok(_ops().tsa_route_backward(a, _vec(dweights, ids.shape, "torch.float32", "dweights"), p, stride, stream))
 
 
 # ---- products ----------------------------------------------------------------------------------------------------------
 def _linear_args(x, w, y, bias=None, residual=None, act="none"):
     (rows, n_in), n_out = x.shape, w.shape[0]
     kind, w_kind, y_kind = _type(x), _type(w), _type(y)
-    a = TsaLinearArgs(rows=rows, n_in=n_in, n_out=n_out, x_type=kind, w_type=w_kind, y_type=y_kind, act=ACTS[act])
-    a.x, a.x_stride = _mat(x, rows, n_in, "x")
+    xp, xs = _mat(x, rows, n_in, "x")
     if w_kind == Q4:
         if n_in % _Q4_BLOCK or not w.is_contiguous():
             raise ValueError("w: 4-bit weights are whole blocks of 32 values, rows back to back")
-        a.w, a.w_stride = _mat(w, n_out, n_in // _Q4_BLOCK * _Q4_BYTES, "w")[0], n_in
+        wp, ws = _mat(w, n_out, n_in // _Q4_BLOCK * _Q4_BYTES, "w")[0], n_in
     else:
-        a.w, a.w_stride = _mat(w, n_out, n_in, "w")
-    a.y, a.y_stride = _mat(y, rows, n_out, "y")
-    if bias is not None:
-        a.bias = _vec(bias, (n_out,), str(x.dtype), "bias")
-    if residual is not None:
-        a.residual, a.residual_stride = _mat(residual, rows, n_out, "residual", y_kind)
-    return a
+        wp, ws = _mat(w, n_out, n_in, "w")
+    yp, ys = _mat(y, rows, n_out, "y")
+    rp, rs = (None, 0) if residual is None else _mat(residual, rows, n_out, "residual", y_kind)
+    bp = None if bias is None else _vec(bias, (n_out,), str(x.dtype), "bias")
+    return TsaLinearArgs(xp, xs, wp, ws, bp, rp, rs, yp, ys, rows, n_in, n_out, kind, w_kind, y_kind, ACTS[act], 0)
 
 
 def linear_workspace(x, w, y) -> int:
     """Workspace bytes of linear(x, w, y, ...)."""
-    return int(_ops().tsa_linear_workspace(C.byref(_linear_args(x, w, y))))
+    rows, n_in = x.shape
+    a = TsaLinearArgs(None, 0, None, 0, None, None, 0, None, 0, rows, n_in, w.shape[0], _type(x), _type(w), _type(y), 0, 0)
+    return _ops().tsa_linear_workspace(a)
 
 
 def linear(x, w, y, *, bias=None, residual=None, act="none", workspace=None, stream=None) -> None:
     """y = act(x w^T + bias) + residual (tsa_linear). w: [n_out][n_in] of x's type, or uint8 [n_out][n_in / 32 * 18]."""
     a = _linear_args(x, w, y, bias, residual, act)
-    check(_ops().tsa_linear(C.byref(a), *_room(workspace), stream))
+    ws, n = _room(workspace)
+    _ok(_ops().tsa_linear(a, ws, n, stream))
 
 
 # ---- gated feed-forward blocks --------------------------------------------------------------------------------------------
@@ -197,7 +217,7 @@ class Experts:
 
 
 def ffn_workspace(e: Experts, rows: int, top_k: int = 1) -> int:
-    return int(_ops().tsa_ffn_workspace(C.byref(e.s), rows, top_k))
+    return _ops().tsa_ffn_workspace(e.s, rows, top_k)
 
 
 def _pairs(a, e: Experts, x, ids, weights):
@@ -218,11 +238,12 @@ def ffn(e: Experts, x, y, *, ids=None, weights=None, residual=None, act="silu", 
     a.y, a.y_stride = _mat(y, rows, d, "y", a.type)
     if residual is not None:
         a.residual, a.residual_stride = _mat(residual, rows, d, "residual", a.type)
-    check(_ops().tsa_ffn(C.byref(e.s), C.byref(a), *_room(workspace), stream))
+    ws, n = _room(workspace)
+    _ok(_ops().tsa_ffn(e.s, a, ws, n, stream))
 
 
 def ffn_backward_workspace(e: Experts, rows: int, top_k: int = 1) -> int:
-    return int(_ops().tsa_ffn_backward_workspace(C.byref(e.s), rows, top_k))
+    return _ops().tsa_ffn_backward_workspace(e.s, rows, top_k)
 
 
 def ffn_backward(e: Experts, x, dy, dx=None, *, ids=None, weights=None, dweights=None, dgate=None, dup=None, ddown=None,
@@ -238,4 +259,5 @@ def ffn_backward(e: Experts, x, dy, dx=None, *, ids=None, weights=None, dweights
     a.dgate = _vec(dgate, (n, f, d), str(x.dtype), "dgate")
     a.dup = _vec(dup, (n, f, d), str(x.dtype), "dup")
     a.ddown = _vec(ddown, (n, d, f), str(x.dtype), "ddown")
-    check(_ops().tsa_ffn_backward(C.byref(e.s), C.byref(a), *_room(workspace), stream))
+    ws, n = _room(workspace)
+    _ok(_ops().tsa_ffn_backward(e.s, a, ws, n, stream))
