@@ -15,7 +15,7 @@
  * SS_E_INVALID (argument checks, done on the host before any launch), SS_E_BACKEND (a HIP error).
  *
  * Alignment: every matrix at its element's size, workspaces at 16 bytes. Rows that start 16-byte aligned (base and
- * stride) and hold a multiple of 8 values take the wide loads and are several times faster. 4-bit weights: 4 bytes.
+ * stride) and hold a multiple of 8 values are the fastest. 4-bit weights: 4 bytes; 16 is faster.
  */
 #ifndef TIERSTREAM_AMD_TSA_OPS_H
 #define TIERSTREAM_AMD_TSA_OPS_H
@@ -75,7 +75,8 @@ typedef struct tsa_linear_args {
   uint32_t act;
   uint32_t reserved;
 } tsa_linear_args;
-/* Workspace bytes of a call (0: none is used). */
+/* Workspace bytes of a call (0: none is used): where more than 64 rows are to be multiplied and rows of x or w do not start
+ * 16-byte aligned or are no multiple of 8 values, these are packed first. Sizes are below 2^24, rows x n_out below 2^37. */
 SS_API uint64_t tsa_linear_workspace(const tsa_linear_args* a);
 SS_API ss_status tsa_linear(const tsa_linear_args* a, void* workspace, uint64_t workspace_bytes, void* stream);
 

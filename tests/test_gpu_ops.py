@@ -188,7 +188,7 @@ def linear64(x, w, bias, residual, act):
 
 
 LINEAR = [(1, 64, 16), (1, 4096, 4096), (1, 1280, 37), (1, 256, 16), (1, 2560, 200), (2, 200, 33), (7, 72, 257), (16, 512, 96), (17, 1000, 130), (33, 256, 64),
-          (64, 2048, 520), (65, 96, 128), (129, 320, 384), (300, 640, 256), (515, 1096, 776)]
+          (64, 2048, 520), (65, 96, 128), (129, 320, 384), (300, 640, 256), (515, 1096, 776), (200, 32, 16)]
 
 
 @pytest.mark.parametrize("rows,n_in,n_out", LINEAR)
@@ -212,7 +212,7 @@ def test_linear(ops, rows, n_in, n_out, kind, weights):
 
 
 @pytest.mark.parametrize("pad,shift", [(0, 0), (1, 0), (3, 1), (8, 4), (0, 1)])
-@pytest.mark.parametrize("rows,n_in,n_out", [(1, 1, 1), (1, 129, 40), (5, 63, 17), (70, 1001, 65), (140, 264, 300)])
+@pytest.mark.parametrize("rows,n_in,n_out", [(1, 1, 1), (1, 129, 40), (5, 63, 17), (33, 515, 70), (64, 255, 33), (70, 1001, 65), (140, 264, 300)])
 def test_linear_any_alignment(ops, pad, shift, rows, n_in, n_out):
     g = gen(pad * 10 + shift)
     x, w = mat(g, rows, n_in, "bf16", pad, shift), mat(g, n_out, n_in, "bf16", pad, shift, sigma=0.1)

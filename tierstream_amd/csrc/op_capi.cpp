@@ -61,7 +61,8 @@ void check_linear(const char* what, const tsa_linear_args* a) {
   REQUIRE(a->y_type == a->x_type || a->y_type == TSA_F32, SS_E_INVALID, std::string(what) + ": y of x's type or TSA_F32");
   REQUIRE(a->w_type != TSA_Q4 || a->n_in % kQ4Block == 0, SS_E_INVALID, std::string(what) + ": 4-bit rows hold a multiple of 32 values");
   REQUIRE(a->n_in >= 1, SS_E_INVALID, std::string(what) + ": n_in 0");
-  REQUIRE(uint64_t(a->rows) < (1u << 31) && a->n_in < (1u << 31) && a->n_out < (1u << 31), SS_E_INVALID, std::string(what) + ": sizes below 2^31");
+  REQUIRE(a->rows < (1u << 24) && a->n_in < (1u << 24) && a->n_out < (1u << 24) && uint64_t(a->rows) * a->n_out < (uint64_t(1) << 37),
+          SS_E_INVALID, std::string(what) + ": sizes below 2^24, rows x n_out below 2^37");
   check_act(what, a->act, true);
 }
 

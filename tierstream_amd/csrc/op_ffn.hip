@@ -504,6 +504,58 @@ __global__ __launch_bounds__(kTileThreads, 2) void down_tile_kernel(Plan p, cons
   hand_out<8, 4, 2>(memory, acc, o);
 }
 
+// The two with 4-bit weights: 64 columns of gate and up, 128 of down a tile.
+template <class T>
+__global__ __launch_bounds__(kTileThreads, 2) void gate_up_q4_tile_kernel(Plan p, const u16* x, uint64_t x_stride, uint32_t d,
+                                                                          uint32_t f, uint32_t act, u16* h) {
+  extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
+  TileRows t;
+  uint32_t at;
+  if (!tile_of(p, (f + 63) / 64, t, at)) return;
+  const char *gate = p.part[3 * t.e], *up = p.part[3 * t.e + 1];
+  TileQ4Source<T> w(d, threadIdx.x >> 6 & 1u, [&](uint32_t r) {  // of each wave's 64 rows: 32 gate, 32 up
+    const uint32_t c = at * 64 + (r >> 6) * 32 + (r & 31u);
+    return reinterpret_cast<const unsigned char*>(r & 32u ? up : gate) + uint64_t(c < f ? c : f - 1) * (d / kQ4Block * kQ4Bytes);
+  });
+  auto xs = mapped_rows(t, x, x_stride, d);
+  f32x4 acc[8][4] = {};
+  tile_product<T, 8, 4, 3>(w, xs, d, lds_offset(memory), acc);
+  f32x4 v[2][4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x4 g = TileQ4Source<T>::whole(acc[i][j], acc[i + 4][j]), u = TileQ4Source<T>::whole(acc[i + 2][j], acc[i + 6][j]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[i][j][q] = activate(act, g[q]) * u[q];
+    }
+  TypedOut<T, u16> out{{h + uint64_t(t.first) * f, f, t.rows, at * 64, f}};
+  hand_out<2, 4, 4>(memory, v, out);
+}
+
+template <class T>
+__global__ __launch_bounds__(kTileThreads, 2) void down_q4_tile_kernel(Plan p, const u16* h, uint32_t d, uint32_t f, float* out) {
+  extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
+  TileRows t;
+  uint32_t at;
+  if (!tile_of(p, (d + 127) / 128, t, at)) return;
+  const unsigned char* down = reinterpret_cast<const unsigned char*>(p.part[3 * t.e + 2]);
+  TileQ4Source<T> w(f, threadIdx.x >> 6 & 1u, [&](uint32_t r) {
+    const uint32_t c = at * 128 + r;
+    return down + uint64_t(c < d ? c : d - 1) * (f / kQ4Block * kQ4Bytes);
+  });
+  auto hs = sorted_rows(t, h, f, f);
+  f32x4 acc[8][4] = {};
+  tile_product<T, 8, 4, 3>(w, hs, f, lds_offset(memory), acc);
+  f32x4 v[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[i][j] = TileQ4Source<T>::whole(acc[i][j], acc[i + 4][j]);
+  TypedOut<T, float> o{{out + uint64_t(t.first) * d, d, t.rows, at * 128, d}};
+  hand_out<4, 4, 4>(memory, v, o);
+}
+
 // back = down^T dy of every pair, 256 columns of d_ff: in 32 bits, for the kernel behind it. (One kernel for all three
 // products needs 192 accumulators a lane, so one workgroup a CU: 496 us in a training step of 128 experts.)
 template <class T>
@@ -951,16 +1003,22 @@ int forward_stream(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_arg
   return forward_few<T, W, 4, kTail>(e, d, f, a, w, s);
 }
 
-template <class T>
+template <class T, bool kQ4>
 int forward_tiles(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& a, void* ws, hipStream_t s) {
   Room room(ws);
   const Forward w = take_forward(room, e.n, d, f, a.rows, a.top_k);
   if (int err = launch_plan(e, a.ids, w.plan, kTileRows, s)) return err;
   const uint32_t tiles = most_tiles(w.plan.pairs, e.n, kTileRows);
-  hipLaunchKernelGGL((gate_up_tile_kernel<T>), dim3(tiles * ((f + 127) / 128)), dim3(kTileThreads), tile_lds(8, 4, 3), s, w.plan,
-                     static_cast<const u16*>(a.x), a.x_stride, d, f, a.act, w.h);
-  hipLaunchKernelGGL((down_tile_kernel<T>), dim3(tiles * ((d + 255) / 256)), dim3(kTileThreads), tile_lds(8, 4, 3), s, w.plan, w.h,
-                     d, f, w.out);
+  constexpr uint32_t kF = kQ4 ? 64 : 128, kD = kQ4 ? 128 : 256;  // columns a tile
+  const dim3 up(tiles * ((f + kF - 1) / kF)), down(tiles * ((d + kD - 1) / kD));
+  const u16* x = static_cast<const u16*>(a.x);
+  if constexpr (kQ4) {
+    hipLaunchKernelGGL((gate_up_q4_tile_kernel<T>), up, dim3(kTileThreads), tile_lds(8, 4, 3), s, w.plan, x, a.x_stride, d, f, a.act, w.h);
+    hipLaunchKernelGGL((down_q4_tile_kernel<T>), down, dim3(kTileThreads), tile_lds(8, 4, 3), s, w.plan, w.h, d, f, w.out);
+  } else {
+    hipLaunchKernelGGL((gate_up_tile_kernel<T>), up, dim3(kTileThreads), tile_lds(8, 4, 3), s, w.plan, x, a.x_stride, d, f, a.act, w.h);
+    hipLaunchKernelGGL((down_tile_kernel<T>), down, dim3(kTileThreads), tile_lds(8, 4, 3), s, w.plan, w.h, d, f, w.out);
+  }
   return launch_combine<T>(w.plan, a.rows, d, w.out, a.weights, a.residual, a.residual_stride, a.y, a.y_stride, s);
 }
 
@@ -969,10 +1027,9 @@ int forward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& a, v
   typedef std::conditional_t<kQ4, RowsQ4<T>, Rows16<T>> W;
   if constexpr (kQ4)
     if (a.rows == 1 && d % 256 == 0 && f % 256 == 0 && aligned16(a.x, 0) && wide_weights(e)) return forward_one_q4<T>(e, d, f, a, ws, s);
-  if (wide_rows(e, d, f, kQ4, a.x, a.x_stride) && uint64_t(a.rows) * a.top_k <= uint64_t(64) * e.n)
+  if (uint64_t(a.rows) * a.top_k <= uint64_t(64) * e.n)
     return d % kChunk || f % kChunk ? forward_stream<T, W, true>(e, d, f, a, ws, s) : forward_stream<T, W, false>(e, d, f, a, ws, s);
-  if constexpr (!kQ4)
-    if (wide_rows(e, d, f, false, a.x, a.x_stride)) return forward_tiles<T>(e, d, f, a, ws, s);
+  if (wide_rows(e, d, f, kQ4, a.x, a.x_stride)) return forward_tiles<T, kQ4>(e, d, f, a, ws, s);
   Room room(ws);
   const Forward w = take_forward(room, e.n, d, f, a.rows, a.top_k);
   if (int err = launch_plan(e, a.ids, w.plan, 64, s)) return err;

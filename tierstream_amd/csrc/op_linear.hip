@@ -71,28 +71,6 @@ struct LinearOut {
   }
 };
 
-template <class T, bool kQ4>
-__global__ __launch_bounds__(256) void linear_any_kernel(tsa_linear_args a) {
-  __shared__ TileMemory m;
-  const uint32_t tn = (a.n_out + 63) / 64;
-  const uint64_t tiles = uint64_t(tn) * ((uint64_t(a.rows) + 63) / 64);
-  const Operand x{static_cast<const u16*>(a.x), a.x_stride, 1, a.rows, a.n_in, nullptr};
-  for (uint64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const uint32_t n0 = uint32_t(tile % tn) * 64, r0 = uint32_t(tile / tn) * 64;
-    f32x4 acc[2][2] = {};
-    if constexpr (kQ4) {
-      const Q4Operand<T> w{static_cast<const unsigned char*>(a.w), weight_row_bytes(a.n_in, TSA_Q4), a.n_out, a.n_in};
-      tile64<T, true>(w, n0, x, r0, a.n_in, m, acc);
-    } else {
-      const Operand w{static_cast<const u16*>(a.w), a.w_stride, 1, a.n_out, a.n_in, nullptr};
-      tile64<T, false>(w, n0, x, r0, a.n_in, m, acc);
-    }
-    each64(acc, [&](uint32_t i, uint32_t j, float v) {
-      if (n0 + i < a.n_out && r0 + j < a.rows) finish_linear(a, r0 + j, n0 + i, v);
-    });
-  }
-}
-
 // Few rows: a workgroup takes 16 R weight rows and 16 CT rows of x.
 template <class T, class W, int R, int CT, bool kTail>
 __global__ __launch_bounds__(64 * most_waves(CT)) void linear_few_kernel(tsa_linear_args a) {
@@ -202,40 +180,103 @@ int launch_tile(const tsa_linear_args& a, hipStream_t stream) {
   return int(hipGetLastError());
 }
 
+// The same with 4-bit weights, 128 rows of them a tile.
+template <class T>
+__global__ __launch_bounds__(kTileThreads, 2) void linear_q4_tile_kernel(tsa_linear_args a) {
+  extern __shared__ f32x4 memory[];
+  const uint32_t wave = threadIdx.x >> 6;
+  const TileAt t = tile_at(blockIdx.x, (a.n_out + 127) / 128, (a.rows + 127) / 128);
+  const uint32_t n0 = t.a * 128, r0 = t.b * 128;
+  TileQ4Source<T> w(a.n_in, wave & 1u, [&](uint32_t r) {
+    const uint32_t n = n0 + r;
+    return static_cast<const unsigned char*>(a.w) + uint64_t(n < a.n_out ? n : a.n_out - 1) * (a.n_in / kQ4Block * kQ4Bytes);
+  });
+  TileRowsSource<4> x(a.n_in, wave >> 1, [&](uint32_t r) {
+    const uint32_t row = r0 + r;
+    return static_cast<const u16*>(a.x) + (row < a.rows ? row : a.rows - 1) * a.x_stride;
+  });
+  f32x4 acc[8][4] = {};
+  tile_product<T, 8, 4, 3>(w, x, a.n_in, lds_offset(memory), acc);
+  f32x4 v[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[i][j] = TileQ4Source<T>::whole(acc[i][j], acc[i + 4][j]);
+  LinearOut<T> out(a, r0, n0);
+  hand_out<4, 4, 4>(memory, v, out);
+}
+
+template <class T>
+int launch_q4_tile(const tsa_linear_args& a, hipStream_t stream) {
+  const uint32_t tiles = (a.n_out + 127) / 128 * ((a.rows + 127) / 128);
+  hipLaunchKernelGGL((linear_q4_tile_kernel<T>), dim3(tiles), dim3(kTileThreads), tile_lds(8, 4, 3), stream, a);
+  return int(hipGetLastError());
+}
+
+// Rows of `from` to rows of `to_stride` values (a multiple of 8, zeros behind the n there are): what the tiles' loads take.
+__global__ __launch_bounds__(256) void pack_kernel(const u16* from, uint64_t from_stride, uint32_t rows, uint32_t n, u16* to,
+                                                   uint32_t to_stride) {
+  const uint32_t per = to_stride / 8;
+  const uint64_t total = uint64_t(rows) * per;
+  for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += uint64_t(gridDim.x) * 256) {
+    const uint32_t row = uint32_t(i / per), c = uint32_t(i % per) * 8;
+    *reinterpret_cast<bits8*>(to + uint64_t(row) * to_stride + c) = load_end(from + row * from_stride + c, int(n - c));
+  }
+}
+
 bool aligned16(const void* p, uint64_t stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0; }
 
 }  // namespace
 }  // namespace op
 
-uint64_t linear_workspace(const tsa_linear_args&) { return 0; }
+constexpr uint32_t kFewRows = 64;  // up to here the weights are streamed, in tiles beyond
 
-int launch_linear(const tsa_linear_args& a, void*, hipStream_t stream) {
-  if (a.rows == 0 || a.n_out == 0) return 0;
-  const bool wide = a.n_in % 8 == 0 && op::aligned16(a.x, a.x_stride) && (a.w_type == TSA_Q4 || op::aligned16(a.w, a.w_stride));
-  if (wide && a.rows == 1 && a.w_type == TSA_Q4 && a.n_in % 256 == 0 && op::aligned16(a.w, 0))
-    return a.x_type == TSA_BF16 ? op::launch_q4<op::Bf16>(a, stream) : op::launch_q4<op::F16>(a, stream);
-  if (wide && a.rows <= 64) {
-    if (a.x_type == TSA_BF16)
-      return a.w_type == TSA_Q4 ? op::launch_few<op::Bf16, op::RowsQ4<op::Bf16>>(a, stream)
-                                : op::launch_few<op::Bf16, op::Rows16<op::Bf16>>(a, stream);
-    return a.w_type == TSA_Q4 ? op::launch_few<op::F16, op::RowsQ4<op::F16>>(a, stream)
-                              : op::launch_few<op::F16, op::Rows16<op::F16>>(a, stream);
-  }
-  if (wide && a.w_type != TSA_Q4 && a.rows < (1u << 24) && a.n_out < (1u << 24)) {
-    return a.x_type == TSA_BF16 ? op::launch_tile<op::Bf16>(a, stream) : op::launch_tile<op::F16>(a, stream);
-  }
-  const uint64_t tiles = (uint64_t(a.n_out) + 63) / 64 * ((uint64_t(a.rows) + 63) / 64);
-  const dim3 grid(uint32_t(tiles < (1u << 20) ? tiles : (1u << 20)));
-#define CALL(T, Q) hipLaunchKernelGGL((op::linear_any_kernel<op::T, Q>), grid, dim3(256), 0, stream, a)
-  if (a.x_type == TSA_BF16) {
-    if (a.w_type == TSA_Q4) CALL(Bf16, true);
-    else CALL(Bf16, false);
-  } else {
-    if (a.w_type == TSA_Q4) CALL(F16, true);
-    else CALL(F16, false);
-  }
-#undef CALL
+// What a call with more rows packs first: x, the weights, neither or both.
+namespace {
+bool pack_x(const tsa_linear_args& a) { return a.rows > kFewRows && (a.n_in % 8 || !op::aligned16(a.x, a.x_stride)); }
+bool pack_w(const tsa_linear_args& a) {
+  return a.rows > kFewRows && a.w_type != TSA_Q4 && (a.n_in % 8 || !op::aligned16(a.w, a.w_stride));
+}
+int pack(const void* from, uint64_t stride, uint32_t rows, uint32_t n, void* to, hipStream_t stream) {
+  const uint32_t wide = uint32_t(up_to(n, 8));
+  const uint64_t blocks = (uint64_t(rows) * (wide / 8) + 255) / 256;
+  hipLaunchKernelGGL(op::pack_kernel, dim3(uint32_t(blocks < 65536 ? blocks : 65536)), dim3(256), 0, stream,
+                     static_cast<const op::u16*>(from), stride, rows, n, static_cast<op::u16*>(to), wide);
   return int(hipGetLastError());
+}
+}  // namespace
+
+uint64_t linear_workspace(const tsa_linear_args& a) {
+  return up_to(a.n_in, 8) * 2 * ((pack_x(a) ? a.rows : 0) + uint64_t(pack_w(a) ? a.n_out : 0));
+}
+
+int launch_linear(const tsa_linear_args& a0, void* workspace, hipStream_t stream) {
+  tsa_linear_args a = a0;
+  if (a.rows == 0 || a.n_out == 0) return 0;
+  const bool bf16 = a.x_type == TSA_BF16, q4 = a.w_type == TSA_Q4;
+  if (a.rows == 1 && q4 && a.n_in % 256 == 0 && op::aligned16(a.w, 0) && op::aligned16(a.x, 0))
+    return bf16 ? op::launch_q4<op::Bf16>(a, stream) : op::launch_q4<op::F16>(a, stream);
+  if (a.rows <= kFewRows) {
+    if (bf16) return q4 ? op::launch_few<op::Bf16, op::RowsQ4<op::Bf16>>(a, stream) : op::launch_few<op::Bf16, op::Rows16<op::Bf16>>(a, stream);
+    return q4 ? op::launch_few<op::F16, op::RowsQ4<op::F16>>(a, stream) : op::launch_few<op::F16, op::Rows16<op::F16>>(a, stream);
+  }
+  const uint32_t wide = uint32_t(up_to(a.n_in, 8));
+  const bool px = pack_x(a), pw = pack_w(a);
+  op::u16* room = static_cast<op::u16*>(workspace);
+  if (px) {
+    if (int err = pack(a.x, a.x_stride, a.rows, a.n_in, room, stream)) return err;
+    a.x = room;
+    a.x_stride = wide;
+    room += uint64_t(a.rows) * wide;
+  }
+  if (pw) {
+    if (int err = pack(a.w, a.w_stride, a.n_out, a.n_in, room, stream)) return err;
+    a.w = room;
+    a.w_stride = wide;
+  }
+  a.n_in = wide;  // (packed rows end in zeros; unpacked ones are whole)
+  if (q4) return bf16 ? op::launch_q4_tile<op::Bf16>(a, stream) : op::launch_q4_tile<op::F16>(a, stream);
+  return bf16 ? op::launch_tile<op::Bf16>(a, stream) : op::launch_tile<op::F16>(a, stream);
 }
 
 }  // namespace tsa

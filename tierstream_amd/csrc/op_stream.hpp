@@ -17,19 +17,30 @@ namespace op {
 
 constexpr uint32_t kChunk = 128;  // values of a weight row per chunk: 4 steps
 
-typedef __attribute__((address_space(1))) const bits8 gbits8_t;
-typedef __attribute__((address_space(1))) const bits4 gbits4_t;
+// 16-byte accesses at any element's alignment (the hardware takes them at every address).
+typedef bits8 bits8_any __attribute__((aligned(2)));
+typedef bits4 bits4_any __attribute__((aligned(2)));
+typedef __attribute__((address_space(1))) const bits8_any gbits8_t;
+typedef __attribute__((address_space(1))) const bits4_any gbits4_t;
 
 __device__ __forceinline__ bits8 load_bits8(const u16* p) {
   return *reinterpret_cast<gbits8_t*>(reinterpret_cast<uintptr_t>(p));
 }
-
 // Weights are read once: past the caches.
 __device__ __forceinline__ bits8 load_stream(const u16* p) {
   return __builtin_nontemporal_load(reinterpret_cast<gbits8_t*>(reinterpret_cast<uintptr_t>(p)));
 }
+// The first `left` of 8 values (0 or fewer: none), zeros behind them.
+__device__ __forceinline__ bits8 load_end(const u16* p, int left) {
+  bits8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (left >= 8) return load_bits8(p);
+#pragma unroll
+  for (int i = 0; i < 7; ++i)
+    if (i < left) v[i] = p[i];
+  return v;
+}
 
-// 16-bit weight rows: base at row 0, `stride` values apart, rows and pointers 16-byte aligned, n a multiple of 8.
+// 16-bit weight rows: base at row 0, `stride` values apart, at any alignment.
 template <class T>
 struct Rows16 {
   struct Chunk {
@@ -47,13 +58,13 @@ struct Rows16 {
     const uint32_t q = (threadIdx.x & 48u) / 2;
 #pragma unroll
     for (int s = 0; s < 4; ++s)
-      c.v[s] = !kTail || k + 32 * s + q < n ? load_stream(p + k + 32 * s) : bits8{0, 0, 0, 0, 0, 0, 0, 0};
+      c.v[s] = !kTail || k + 32 * s + q + 8 <= n ? load_stream(p + k + 32 * s) : load_end(p + k + 32 * s, int(n) - int(k + 32 * s + q));
   }
   // Values of x for the step at k, from its row.
   template <bool kTail>
   static __device__ __forceinline__ bits8 x_at(const u16* row, uint32_t k, uint32_t n) {
     const uint32_t at = k + (threadIdx.x & 48u) / 2;
-    return !kTail || at < n ? load_bits8(row + at) : bits8{0, 0, 0, 0, 0, 0, 0, 0};
+    return !kTail || at + 8 <= n ? load_bits8(row + at) : load_end(row + at, int(n) - int(at));
   }
   template <int R, int CT>
   static __device__ __forceinline__ void multiply(const Chunk (&c)[R], int s, const bits8 (&x)[CT], f32x4 (&acc)[R][CT]) {

@@ -63,8 +63,80 @@ struct TileRowsSource {
     p[j] += 64;
   }
   __device__ __forceinline__ void advance() { k += 64; }
+  __device__ __forceinline__ void stage(uint32_t, uint32_t) {}
   __device__ __forceinline__ bits8 read(uint32_t lds, int i) const {
     return *reinterpret_cast<lds_bits8_t*>(lds + frag + i * 1024);
+  }
+};
+
+// Rows of 4-bit blocks: 128 weight rows as 256 rows of the tile, 64 of each wave's half the values' leading 16 bits and 64
+// what is left of them. A value (q - 8) s has 15 bits, so both together are exact: bf16 takes the value itself, half
+// precision an eighth of it (no scale overflows) and 2^12 times the rest (none underflows). whole() joins the two sums.
+// A thread takes one block of a row every two steps: from memory to registers two steps ahead, then to LDS in the places
+// where loads put rows.
+template <class T>
+struct TileQ4Source {
+  static constexpr int kLoads = 0;
+  static constexpr bool kHalf = std::is_same_v<T, F16>;
+  const unsigned char* p;
+  uint32_t k, n, put, turn, frag;
+  u32x4 v;
+  u16 scale;
+
+  typedef u32x4 words_any __attribute__((aligned(2)));
+  typedef __attribute__((address_space(1))) const words_any gwords_t;
+  typedef __attribute__((address_space(1))) const u16 ghalf_t;
+  typedef __attribute__((address_space(3))) bits8 lds_put_t;
+
+  template <class At>
+  __device__ __forceinline__ TileQ4Source(uint32_t n_, uint32_t half, At&& at) : n(n_) {
+    const uint32_t lane = threadIdx.x & 63u, r = threadIdx.x / 2, second = threadIdx.x & 1u;
+    p = at(r) + second * kQ4Bytes;
+    k = second * kQ4Block;
+    const uint32_t row = (r / 64) * 128 + r % 64;
+    put = row * 64;
+    turn = (row >> 2) & 3u;
+    frag = (half * 128 + (lane & 15u)) * 64 + (((lane >> 4) ^ ((lane >> 2) & 3u)) * 16);
+    fetch();
+  }
+  __device__ __forceinline__ void fetch() {
+    v = u32x4{0, 0, 0, 0};
+    scale = 0;
+    if (k < n) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+      scale = *reinterpret_cast<ghalf_t*>(at);
+      v = *reinterpret_cast<gwords_t*>(at + 2);
+    }
+    p += 2 * kQ4Bytes;
+    k += 2 * kQ4Block;
+  }
+  template <bool kCheck>
+  __device__ __forceinline__ void issue(int, uint32_t, uint32_t) {}
+  __device__ __forceinline__ void advance() {}
+  // The fetched blocks to the buffers of their two steps, and the next ones from memory.
+  __device__ __forceinline__ void stage(uint32_t lds0, uint32_t lds1) {
+    const uint32_t to = (threadIdx.x & 1u ? lds1 : lds0) + put;
+    const float s = F16::up(scale) * (kHalf ? 0.125f : 1.0f), s8 = -8.0f * s;
+#pragma unroll
+    for (uint32_t c = 0; c < 4; ++c) {  // values 8 c..: bytes 8 (c mod 2).. of the block, low halves first
+      bits8 hi, lo;
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) {
+        const uint32_t byte = 8 * (c & 1u) + i, q = (v[byte / 4] >> (8 * (byte & 3u) + 4 * (c >> 1))) & 15u;
+        const float w = __builtin_fmaf(float(q), s, s8);  // exact
+        hi[i] = T::down(w);
+        lo[i] = T::down((w - T::up(hi[i])) * (kHalf ? 4096.0f : 1.0f));
+      }
+      *reinterpret_cast<lds_put_t*>(to + ((c ^ turn) * 16)) = hi;
+      *reinterpret_cast<lds_put_t*>(to + 64 * 64 + ((c ^ turn) * 16)) = lo;
+    }
+    fetch();
+  }
+  __device__ __forceinline__ bits8 read(uint32_t lds, int i) const {
+    return *reinterpret_cast<lds_bits8_t*>(lds + frag + i * 1024);
+  }
+  static __device__ __forceinline__ f32x4 whole(f32x4 hi, f32x4 lo) {
+    return kHalf ? (hi + lo * (1.0f / 4096)) * 8.0f : hi + lo;
   }
 };
 
@@ -138,6 +210,7 @@ struct TileColumnsSource {
     k += 64;
     if (!kMap) base += uint64_t(64) * stride;
   }
+  __device__ __forceinline__ void stage(uint32_t, uint32_t) {}
   __device__ __forceinline__ bits8 read(uint32_t lds, int i) const {
     const uint32_t at = (lds + frag) ^ (32u * i);
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4_t*>(at));
@@ -168,7 +241,7 @@ struct Nothing {
 template <class T, int NI, int MJ, int NB, class A, class B, class F = Nothing>
 __device__ __forceinline__ void tile_product(A& a, B& b, uint32_t n, uint32_t lds, f32x4 (&acc)[NI][MJ], F&& every_two = F{}) {
   static_assert(NB == 3 || NB == 4, "buffers");
-  constexpr int kLoads = (NI + MJ) / 2;  // of a step, each thread
+  constexpr int kLoads = A::kLoads + B::kLoads;  // of a step, each thread
   constexpr uint32_t kA = NI * 2048, kBuffer = (NI + MJ) * 2048;
   const auto issue = [&](auto check, int j, uint32_t at0, uint32_t at1) {  // load j of two steps, of both operands
     if (j < A::kLoads) a.template issue<decltype(check)::value>(j, at0, at1);
@@ -181,6 +254,7 @@ __device__ __forceinline__ void tile_product(A& a, B& b, uint32_t n, uint32_t ld
     b.advance();
   };
   __syncthreads();  // the last product's reads are done
+  a.stage(lds, lds + kBuffer);
   issue_all(lds, lds + kBuffer);
   if (NB == 4) issue_all(lds + 2 * kBuffer, lds + 3 * kBuffer);
   wait_loads_and_meet<NB == 4 ? 2 * kLoads : 0>();
@@ -226,6 +300,7 @@ __device__ __forceinline__ void tile_product(A& a, B& b, uint32_t n, uint32_t ld
     } else {
       meet();
       every_two(t * 32);
+      a.stage(behind(2), lds + at * kBuffer);
       step(Zero{}, std::true_type{}, check);
       wait_loads_and_meet<0>();
       step(One{}, std::false_type{}, check);

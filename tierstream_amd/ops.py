@@ -163,7 +163,9 @@ def _linear_args(x, w, y, bias=None, residual=None, act="none"):
 def linear_workspace(x, w, y) -> int:
     """Workspace bytes of linear(x, w, y, ...)."""
     rows, n_in = x.shape
-    a = TsaLinearArgs(None, 0, None, 0, None, None, 0, None, 0, rows, n_in, w.shape[0], _type(x), _type(w), _type(y), 0, 0)
+    kind = _type(w)
+    a = TsaLinearArgs(x.data_ptr(), x.stride()[0], w.data_ptr(), n_in if kind == Q4 else w.stride()[0], None, None, 0, None, 0, rows,
+                      n_in, w.shape[0], _type(x), kind, _type(y), 0, 0)
     return _ops().tsa_linear_workspace(a)
 
 
