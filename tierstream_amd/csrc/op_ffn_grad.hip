@@ -1,0 +1,361 @@
+// The gradients of the gated feed-forward blocks.
+//
+// b = down^T dy of every pair; with gate x and up x computed again, d w = <h, b>, dg = w b up act'(gate), du = w b act(gate) and
+// w h; dx' = gate^T dg + up^T du, added over a row's pairs; d gate = dg^T x, d up = du^T x and d down = dy^T (w h) over an expert's
+// pairs. dg, du and w h are rounded once to the operands' 16 bits; b and dx' stay in 32 bits. No sum depends on an order that
+// changes.
+#include "op_pairs.hpp"
+
+namespace tsa {
+namespace op {
+namespace {
+
+// Of every pair: dg | du as one row of 2 f values, w h, and this tile's share of d w (d_share[f tile][sorted position]).
+template <class T>
+__global__ __launch_bounds__(256) void hidden_grad_any_kernel(Plan p, const u16* x, uint64_t x_stride, const u16* dy,
+                                                              uint64_t dy_stride, const float* weights, uint32_t d, uint32_t f,
+                                                              uint32_t act, u16* dgu, u16* wh, float* d_share) {
+  __shared__ TileMemory m;
+  __shared__ float share[64][2];
+  const uint32_t tf = (f + 63) / 64;
+  const uint32_t ft = blockIdx.x % tf, f0 = ft * 64;
+  TileRows t;
+  if (!tile_rows(p, blockIdx.x / tf, 64, t)) return;
+  const Operand xs{x, x_stride, 1, t.rows, d, t.map}, dys{dy, dy_stride, 1, t.rows, d, t.map};
+  f32x4 g[2][2] = {}, u[2][2] = {}, b[2][2] = {};
+  weight_tile<T, false>(p.part[3 * t.e], f, d, f0, xs, m, g);
+  weight_tile<T, false>(p.part[3 * t.e + 1], f, d, f0, xs, m, u);
+  const Operand down{reinterpret_cast<const u16*>(p.part[3 * t.e + 2]), 1, f, f, d, nullptr};  // (f, d): its columns as rows
+  tile64<T, false>(down, f0, dys, 0, d, m, b);
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const uint32_t r = (wave >> 1) * 32 + 16 * j + (lane & 15u);
+    const uint32_t pos = t.first + r;
+    const float w = r < t.rows && weights ? weights[p.pair[pos]] : 1.0f;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t c = f0 + (wave & 1u) * 32 + 16 * i + (lane >> 4) * 4 + q;
+        const float a = activate(act, g[i][j][q]), back = b[i][j][q];
+        if (c >= f || r >= t.rows) continue;
+        sum += a * u[i][j][q] * back;
+        dgu[uint64_t(pos) * 2 * f + c] = T::down(w * back * u[i][j][q] * slope(act, g[i][j][q]));
+        dgu[uint64_t(pos) * 2 * f + f + c] = T::down(w * back * a);
+        wh[uint64_t(pos) * f + c] = T::down(w * a * u[i][j][q]);
+      }
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (lane < 16) share[r][wave & 1u] = sum;
+  }
+  __syncthreads();
+  if (threadIdx.x < t.rows) d_share[uint64_t(ft) * p.pairs + t.first + threadIdx.x] = share[threadIdx.x][0] + share[threadIdx.x][1];
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void input_grad_any_kernel(Plan p, const u16* dgu, uint32_t d, uint32_t f, float* out) {
+  __shared__ TileMemory m;
+  const uint32_t td = (d + 63) / 64;
+  const uint32_t d0 = blockIdx.x % td * 64;
+  TileRows t;
+  if (!tile_rows(p, blockIdx.x / td, 64, t)) return;
+  f32x4 acc[2][2] = {};
+  for (int half = 0; half < 2; ++half) {
+    const Operand w{reinterpret_cast<const u16*>(p.part[3 * t.e + half]), 1, d, d, f, nullptr};
+    const Operand v{dgu + uint64_t(t.first) * 2 * f + half * f, uint64_t(2) * f, 1, t.rows, f, nullptr};
+    tile64<T, false>(w, d0, v, 0, f, m, acc);
+  }
+  each64(acc, [&](uint32_t i, uint32_t j, float v) {
+    if (d0 + i < d && j < t.rows) out[uint64_t(t.first + j) * d + d0 + i] = v;
+  });
+}
+
+// out[e][b][a] = sum over expert e's pairs of left[pair][a] right[pair][b] (0 for an expert without pairs): left through
+// the rows' map where left_map, right where right_map.
+template <class T>
+__global__ __launch_bounds__(256) void weight_grad_any_kernel(Plan p, const u16* left, uint64_t left_stride, bool left_map,
+                                                              uint32_t n_left, const u16* right, uint64_t right_stride,
+                                                              bool right_map, uint32_t n_right, u16* out) {
+  __shared__ TileMemory m;
+  const uint32_t ta = (n_left + 63) / 64, tb = (n_right + 63) / 64;
+  const uint32_t per = ta * tb;
+  for (uint64_t tile = blockIdx.x; tile < uint64_t(p.n) * per; tile += gridDim.x) {
+    const uint32_t e = uint32_t(tile / per), a0 = uint32_t(tile % per) % ta * 64, b0 = uint32_t(tile % per) / ta * 64;
+    const uint32_t first = p.first[e], n = p.first[e + 1] - first;
+    // (k runs over the pairs: element (r, k) at k stride + r)
+    struct Rows {
+      const u16* base;
+      uint64_t stride;
+      const uint32_t* map;
+      uint32_t rows, n;
+      __device__ __forceinline__ bits8 load8(uint32_t r, uint32_t k) const {
+        bits8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (r >= rows) return v;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i)
+          if (k + i < n) v[i] = base[uint64_t(map ? map[k + i] : k + i) * stride + r];
+        return v;
+      }
+    };
+    const Rows l{left_map ? left : left + first * left_stride, left_stride, left_map ? p.row + first : nullptr, n_left, n};
+    const Rows r{right_map ? right : right + first * right_stride, right_stride, right_map ? p.row + first : nullptr, n_right, n};
+    f32x4 acc[2][2] = {};
+    tile64<T, false>(l, a0, r, b0, n, m, acc);
+    each64(acc, [&](uint32_t i, uint32_t j, float v) {
+      if (a0 + i < n_left && b0 + j < n_right) out[(uint64_t(e) * n_right + b0 + j) * n_left + a0 + i] = T::down(v);
+    });
+    __syncthreads();
+  }
+}
+
+__global__ __launch_bounds__(256) void weights_grad_kernel(Plan p, uint32_t shares, const float* d_share, float* dweights) {
+  for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < p.pairs; i += uint64_t(gridDim.x) * 256) {
+    const int32_t at = p.at[i];
+    float s = 0.0f;
+    if (at >= 0)
+      for (uint32_t k = 0; k < shares; ++k) s += d_share[uint64_t(k) * p.pairs + uint32_t(at)];
+    dweights[i] = s;
+  }
+}
+
+// back = down^T dy of every pair: in 32 bits, for the kernel behind it. (One kernel for all three products needs 192 accumulators
+// a lane, so one workgroup a CU: 496 us in a training step of 128 experts, where the two take 340.)
+template <class T, class S>
+__global__ __launch_bounds__(kTileThreads, 2) void back_tile_kernel(Plan p, const u16* dy, uint64_t dy_stride, uint32_t d,
+                                                                    uint32_t f, float* back) {
+  extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
+  constexpr int NI = S::NI, MJ = S::MJ;
+  TileRows t;
+  uint32_t at;
+  if (!tile_of<S>(p, (f + S::kA - 1) / S::kA, t, at)) return;
+  TileColumnsSource<NI, false> w(d, threadIdx.x >> 6 & 1u, reinterpret_cast<const u16*>(p.part[3 * t.e + 2]), f, at * S::kA, f);
+  auto dys = mapped_rows<MJ>(t, dy, dy_stride, d);
+  f32x4 acc[NI][MJ] = {};
+  tile_product<T, NI, MJ, S::NB>(w, dys, d, lds_offset(memory), acc);
+  TypedOut<T, float> o{{back + uint64_t(t.first) * f, f, t.rows, at * S::kA, f}};
+  hand_out<NI, MJ>(memory, acc, o);
+}
+
+// As hidden_grad_any_kernel from gate's and up's products and `back`, 16 NI columns of d_ff.
+template <class T, class S>
+__global__ __launch_bounds__(kTileThreads, 2) void hidden_grad_tile_kernel(Plan p, const u16* x, uint64_t x_stride,
+                                                                           const float* back, const float* weights, uint32_t d,
+                                                                           uint32_t f, uint32_t act, u16* dgu, u16* wh,
+                                                                           float* d_share) {
+  extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
+  constexpr int NI = S::NI, MJ = S::MJ, kHalf = NI / 2;
+  __shared__ float share[S::kB][2];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  TileRows t;
+  uint32_t at;
+  if (!tile_of<S>(p, (f + 16 * NI - 1) / (16 * NI), t, at)) return;
+  const uint32_t f0 = at * 16 * NI;
+  f32x4 gu[NI][MJ] = {};
+  auto ws = gate_up_source<NI>(p, t, d, f, f0);
+  auto xs = mapped_rows<MJ>(t, x, x_stride, d);
+  tile_product<T, NI, MJ, S::NB>(ws, xs, d, lds_offset(memory), gu);
+  float w[MJ];
+  uint32_t pos[MJ];
+#pragma unroll
+  for (int j = 0; j < MJ; ++j) {
+    const uint32_t r = (wave >> 1) * 16 * MJ + 16 * j + (lane & 15u);
+    pos[j] = t.first + (r < t.rows ? r : t.rows - 1);
+    w[j] = weights ? weights[p.pair[pos[j]]] : 1.0f;
+  }
+  f32x4 h[kHalf][MJ];
+#pragma unroll
+  for (int j = 0; j < MJ; ++j) {
+    float sum = 0.0f;
+    f32x4 b[kHalf];
+#pragma unroll
+    for (int i = 0; i < kHalf; ++i) {
+      const uint32_t c = f0 + (wave & 1u) * 8 * NI + 16 * i + (lane >> 4) * 4;
+      b[i] = c < f ? *reinterpret_cast<const f32x4*>(back + uint64_t(pos[j]) * f + c) : f32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int i = 0; i < kHalf; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float g = gu[i][j][q], u = gu[i + kHalf][j][q], a = activate(act, g);
+        sum += a * u * b[i][q];
+        h[i][j][q] = w[j] * a * u;
+        gu[i][j][q] = w[j] * b[i][q] * u * slope(act, g);  // dg, du in the products' places
+        gu[i + kHalf][j][q] = w[j] * b[i][q] * a;
+      }
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (lane < 16) share[(wave >> 1) * 16 * MJ + 16 * j + lane][wave & 1u] = sum;
+  }
+  TypedOut<T, u16> out{{wh + uint64_t(t.first) * f, f, t.rows, f0, f}};
+  hand_out<kHalf, MJ>(memory, h, out);  // (behind its barrier `share` is whole)
+  if (threadIdx.x < t.rows) d_share[uint64_t(at) * p.pairs + t.first + threadIdx.x] = share[threadIdx.x][0] + share[threadIdx.x][1];
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+#pragma unroll
+    for (int i = 0; i < kHalf; ++i)
+#pragma unroll
+      for (int j = 0; j < MJ; ++j) h[i][j] = gu[i + kHalf * half][j];
+    out.out = dgu + uint64_t(t.first) * 2 * f + half * f;
+    out.stride = uint64_t(2) * f;
+    hand_out<kHalf, MJ>(memory, h, out);
+  }
+}
+
+template <class T, class S>
+__global__ __launch_bounds__(kTileThreads, 2) void input_grad_tile_kernel(Plan p, const u16* dgu, uint32_t d, uint32_t f,
+                                                                          float* out) {
+  extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
+  constexpr int NI = S::NI, MJ = S::MJ;
+  TileRows t;
+  uint32_t at;
+  if (!tile_of<S>(p, (d + S::kA - 1) / S::kA, t, at)) return;
+  f32x4 acc[NI][MJ] = {};
+  const auto add = [&](uint32_t half) {
+    TileColumnsSource<NI, false> w(f, threadIdx.x >> 6 & 1u, reinterpret_cast<const u16*>(p.part[3 * t.e + half]), d, at * S::kA, d);
+    auto v = sorted_rows<MJ>(t, dgu + half * f, uint64_t(2) * f, f);
+    tile_product<T, NI, MJ, S::NB>(w, v, f, lds_offset(memory), acc);
+  };
+  add(0);
+  add(1);
+  TypedOut<T, float> o{{out + uint64_t(t.first) * d, d, t.rows, at * S::kA, d}};
+  hand_out<NI, MJ>(memory, acc, o);
+}
+
+// As weight_grad_any_kernel, out[e][b][a]: a tile of columns a of `left` and b of `right` a workgroup, the sum over the expert's
+// pairs. One of the two is read through the rows' map (kMapLeft: left). Columns from n_right on belong to out2 (the
+// gradients of gate and up are one product).
+template <class T, class S, bool kMapLeft>
+__global__ __launch_bounds__(kTileThreads, 2) void weight_grad_tile_kernel(Plan p, const u16* left, uint64_t left_stride,
+                                                                           uint32_t n_left, const u16* right,
+                                                                           uint64_t right_stride, uint32_t n_right,
+                                                                           uint32_t n_outs, u16* out, u16* out2) {
+  extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
+  constexpr int NI = S::NI, MJ = S::MJ;
+  uint32_t* map = reinterpret_cast<uint32_t*>(memory) + S::kLds / 4;
+  const uint32_t wave = threadIdx.x >> 6;
+  const uint32_t ta = (n_left + S::kA - 1) / S::kA, tb = (n_right + S::kB - 1) / S::kB, per = ta * tb * n_outs;
+  const uint32_t e = blockIdx.x / per, in = blockIdx.x % per;
+  const uint32_t a0 = in % ta * S::kA, which = in / ta / tb, b0 = in / ta % tb * S::kB;
+  const uint32_t first = p.first[e], pairs = p.first[e + 1] - first;
+  right += which * n_right;
+  f32x4 acc[NI][MJ] = {};
+  const auto fill = [&](uint32_t from) {  // half of the ring
+    for (uint32_t i = from + threadIdx.x; i < from + kMapRing / 2 && i < pairs; i += kTileThreads)
+      map[i % kMapRing] = p.row[first + i];
+  };
+  const auto refill = [&](uint32_t k) {
+    if (k && k % (kMapRing / 2) == 0 && k + kMapRing / 2 < pairs) fill(k + kMapRing / 2);
+  };
+  if (pairs) {  // (an expert without pairs gets zeros)
+    fill(0);
+    fill(kMapRing / 2);
+    __syncthreads();
+    if constexpr (kMapLeft) {
+      TileColumnsSource<NI, true> l(pairs, wave & 1u, left, left_stride, a0, n_left, map);
+      TileColumnsSource<MJ, false> r(pairs, wave >> 1, right + uint64_t(first) * right_stride, right_stride, b0, n_right);
+      tile_product<T, NI, MJ, S::NB>(l, r, pairs, lds_offset(memory), acc, refill);
+    } else {
+      TileColumnsSource<NI, false> l(pairs, wave & 1u, left + uint64_t(first) * left_stride, left_stride, a0, n_left);
+      TileColumnsSource<MJ, true> r(pairs, wave >> 1, right, right_stride, b0, n_right, map);
+      tile_product<T, NI, MJ, S::NB>(l, r, pairs, lds_offset(memory), acc, refill);
+    }
+  }
+  TypedOut<T, u16> o{{(which ? out2 : out) + (uint64_t(e) * n_right + b0) * n_left, n_left, n_right - b0, a0, n_left}};
+  hand_out<NI, MJ>(memory, acc, o);
+}
+
+// ---- launches ----
+struct Backward {
+  Plan plan;
+  u16 *dgu, *wh;
+  float *share, *out, *back;  // (back and out share their place: out is written behind back's last reader)
+};
+Backward take_backward(Room& r, uint32_t n, uint32_t d, uint32_t f, uint32_t rows, uint32_t top_k) {
+  const uint64_t pairs = uint64_t(rows) * top_k;
+  Backward w;
+  w.plan = take_plan(r, n, uint32_t(pairs), top_k, 64);
+  w.dgu = r.take<u16>(pairs * 2 * f);
+  w.wh = r.take<u16>(pairs * f);
+  w.share = r.take<float>(pairs * ((f + 31) / 32));  // (the narrowest tile's)
+  w.out = w.back = r.take<float>(pairs * (d > f ? d : f));
+  return w;
+}
+
+template <class T, class S>
+int backward_tiles(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_grad_args& a, void* ws, hipStream_t s) {
+  Room room(ws);
+  const Backward w = take_backward(room, e.n, d, f, a.rows, a.top_k);
+  if (int err = launch_plan(e, a.ids, w.plan, S::kB, s)) return err;
+  const auto of = [](uint32_t n, uint32_t each) { return (n + each - 1) / each; };
+  const uint32_t tiles = most_tiles(w.plan.pairs, e.n, S::kB), shares = of(f, S::kA / 2);
+  const u16 *x = static_cast<const u16*>(a.x), *dy = static_cast<const u16*>(a.dy);
+  if (tiles) {
+    hipLaunchKernelGGL((back_tile_kernel<T, S>), dim3(tiles * of(f, S::kA)), dim3(kTileThreads), S::kLds, s, w.plan, dy, a.dy_stride, d,
+                       f, w.back);
+    hipLaunchKernelGGL((hidden_grad_tile_kernel<T, S>), dim3(tiles * shares), dim3(kTileThreads), S::kLds, s, w.plan, x, a.x_stride,
+                       w.back, a.weights, d, f, a.act, w.dgu, w.wh, w.share);
+  }
+  if (a.dx && tiles) {
+    hipLaunchKernelGGL((input_grad_tile_kernel<T, S>), dim3(tiles * of(d, S::kA)), dim3(kTileThreads), S::kLds, s, w.plan, w.dgu, d, f,
+                       w.out);
+    if (int err = launch_combine<T>(w.plan, a.rows, d, w.out, nullptr, nullptr, 0, a.dx, a.dx_stride, s)) return err;
+  }
+  if (a.dweights && tiles)
+    hipLaunchKernelGGL(weights_grad_kernel, dim3(blocks((w.plan.pairs + 255) / 256)), dim3(256), 0, s, w.plan, shares, w.share,
+                       a.dweights);
+  if (a.dgate) {
+    constexpr uint32_t kLds = S::kLds + 4 * kMapRing;
+    hipLaunchKernelGGL((weight_grad_tile_kernel<T, S, true>), dim3(e.n * of(d, S::kA) * of(f, S::kB) * 2), dim3(kTileThreads), kLds, s,
+                       w.plan, x, a.x_stride, d, w.dgu, uint64_t(2) * f, f, 2u, static_cast<u16*>(a.dgate), static_cast<u16*>(a.dup));
+    hipLaunchKernelGGL((weight_grad_tile_kernel<T, S, false>), dim3(e.n * of(f, S::kA) * of(d, S::kB)), dim3(kTileThreads), kLds, s,
+                       w.plan, w.wh, uint64_t(f), f, dy, a.dy_stride, d, 1u, static_cast<u16*>(a.ddown), static_cast<u16*>(nullptr));
+  }
+  return int(hipGetLastError());
+}
+
+template <class T>
+int backward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_grad_args& a, void* ws, hipStream_t s) {
+  if (wide_rows(e, d, f, false, a.x, a.x_stride) && aligned16(a.dy, 2 * a.dy_stride) && a.dy_stride < 1u << 24 && aligned16(a.dgate, 0) && aligned16(a.dup, 0) &&
+      aligned16(a.ddown, 0))
+    return small_tiles(a.rows, a.top_k, e.n) ? backward_tiles<T, SmallTile>(e, d, f, a, ws, s) : backward_tiles<T, BigTile>(e, d, f, a, ws, s);
+  Room room(ws);
+  const Backward w = take_backward(room, e.n, d, f, a.rows, a.top_k);
+  if (int err = launch_plan(e, a.ids, w.plan, 64, s)) return err;
+  const uint32_t tiles = most_tiles(w.plan.pairs, e.n, 64), tf = (f + 63) / 64, td = (d + 63) / 64;
+  const u16 *x = static_cast<const u16*>(a.x), *dy = static_cast<const u16*>(a.dy);
+  if (tiles)
+    hipLaunchKernelGGL((hidden_grad_any_kernel<T>), dim3(tiles * tf), dim3(256), 0, s, w.plan, x, a.x_stride, dy, a.dy_stride,
+                       a.weights, d, f, a.act, w.dgu, w.wh, w.share);
+  if (a.dx && tiles) {
+    hipLaunchKernelGGL((input_grad_any_kernel<T>), dim3(tiles * td), dim3(256), 0, s, w.plan, w.dgu, d, f, w.out);
+    if (int err = launch_combine<T>(w.plan, a.rows, d, w.out, nullptr, nullptr, 0, a.dx, a.dx_stride, s)) return err;
+  }
+  if (a.dweights && tiles)
+    hipLaunchKernelGGL(weights_grad_kernel, dim3(blocks((w.plan.pairs + 255) / 256)), dim3(256), 0, s, w.plan, tf, w.share,
+                       a.dweights);
+  if (a.dgate) {
+    const uint32_t g = blocks(uint64_t(e.n) * tf * td);
+    for (int half = 0; half < 2; ++half)
+      hipLaunchKernelGGL((weight_grad_any_kernel<T>), dim3(g), dim3(256), 0, s, w.plan, x, a.x_stride, true, d,
+                         w.dgu + half * uint64_t(f), uint64_t(2) * f, false, f, static_cast<u16*>(half ? a.dup : a.dgate));
+    hipLaunchKernelGGL((weight_grad_any_kernel<T>), dim3(g), dim3(256), 0, s, w.plan, w.wh, uint64_t(f), false, f, dy,
+                       a.dy_stride, true, d, static_cast<u16*>(a.ddown));
+  }
+  return int(hipGetLastError());
+}
+
+}  // namespace
+}  // namespace op
+
+uint64_t ffn_backward_workspace(uint32_t n, uint32_t d, uint32_t f, uint32_t rows, uint32_t top_k) {
+  op::Room room(nullptr);
+  op::take_backward(room, n, d, f, rows, top_k);
+  return room.bytes;
+}
+int launch_ffn_backward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_grad_args& a, void* ws, hipStream_t stream) {
+  return a.type == TSA_BF16 ? op::backward<op::Bf16>(e, d, f, a, ws, stream) : op::backward<op::F16>(e, d, f, a, ws, stream);
+}
+
+}  // namespace tsa

@@ -170,7 +170,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void linear_tile_kernel(tsa_linear
   f32x4 acc[8][4] = {};
   tile_product<T, 8, 4, 3>(w, x, a.n_in, lds_offset(memory), acc);
   LinearOut<T> out(a, r0, n0);
-  hand_out<8, 4, 2>(memory, acc, out);
+  hand_out<8, 4>(memory, acc, out);
 }
 
 template <class T>
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void linear_q4_tile_kernel(tsa_lin
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[i][j] = TileQ4Source<T>::whole(acc[i][j], acc[i + 4][j]);
   LinearOut<T> out(a, r0, n0);
-  hand_out<4, 4, 4>(memory, v, out);
+  hand_out<4, 4>(memory, v, out);
 }
 
 template <class T>

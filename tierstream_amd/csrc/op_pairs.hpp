@@ -1,0 +1,261 @@
+// What the gated feed-forward blocks' forward and backward passes share: the pairs (row, j) of a call grouped by expert, where
+// experts' weights are, tiles over an expert's pairs, and the sum over a row's pairs.
+#pragma once
+
+#include "op_tile.hpp"
+
+namespace tsa {
+
+// Groups the pairs of `ids` by expert into p (its arrays in the workspace), tiles of rows_per_tile pairs of one expert.
+int launch_plan(const ExpertMap& e, const int32_t* ids, const Plan& p, uint32_t rows_per_tile, hipStream_t s);
+
+namespace op {
+namespace {
+
+// What ss_dg_slot gives for id e (below m.n), with its loads at once instead of one behind the other's test: they stand in
+// front of every product of a decode step.
+__device__ __forceinline__ int32_t slot_of(const ExpertMap& m, uint32_t e) {
+  const ss_dg_device_view& v = m.view;
+  const uint32_t abort = __hip_atomic_load(v.abort, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const uint32_t base = v.unit_base[m.gated], end = v.unit_base[m.gated + 1];
+  const bool in = e < end - base;
+  const int32_t s = in ? __hip_atomic_load(v.slot_of + base + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+  if (abort || !in) return int32_t(v.guard_slot);
+  if (s >= 0) return s;
+  if (v.absent_err) atomicOr(v.absent_err, 1u);  // (null where the view's version has none)
+  return int32_t(v.guard_slot);
+}
+
+__device__ __forceinline__ void part_pointers(const ExpertMap& m, uint32_t e, const char* (&p)[3]) {
+  if (m.form == 2) {
+    const uint64_t s = uint32_t(slot_of(m, e));
+    for (int i = 0; i < 3; ++i) p[i] = static_cast<const char*>(m.view.parts[i].base) + s * m.view.parts[i].stride;
+  } else if (m.form == 1) {
+    for (int i = 0; i < 3; ++i) p[i] = reinterpret_cast<const char*>(m.table[e]) + m.stride[i];
+  } else {
+    for (int i = 0; i < 3; ++i) p[i] = m.part[i] + e * m.stride[i];
+  }
+}
+
+// The expert of a pair, or ~0: an id out of range, or a table entry of 0.
+__device__ __forceinline__ uint32_t expert_of(const ExpertMap& m, const int32_t* ids, uint32_t pair) {
+  const uint32_t e = ids ? uint32_t(ids[pair]) : 0;
+  if (e >= m.n || (m.form == 1 && m.table[e] == 0)) return ~0u;
+  return e;
+}
+
+// One tile's expert and rows (rows_per_tile of the plan); false behind the last tile.
+struct TileRows {
+  uint32_t e, first, rows;
+  const uint32_t* map;
+};
+__device__ __forceinline__ bool tile_rows(const Plan& p, uint32_t tile, uint32_t rows_per_tile, TileRows& t) {
+  if (tile >= *p.n_tiles) return false;
+  t.e = p.tile[2 * tile];
+  t.first = p.tile[2 * tile + 1];
+  const uint32_t end = p.first[t.e + 1];
+  t.rows = end - t.first < rows_per_tile ? end - t.first : rows_per_tile;
+  t.map = p.row + t.first;
+  return true;
+}
+
+// ---- any stride and alignment: 64 x 64 tiles ------------------------------------------------------------------------
+template <class T, bool kQ4, class B>
+__device__ __forceinline__ void weight_tile(const char* w, uint64_t rows, uint32_t n, uint32_t r0, const B& x, TileMemory& m,
+                                            f32x4 (&acc)[2][2]) {
+  if constexpr (kQ4) {
+    const Q4Operand<T> a{reinterpret_cast<const unsigned char*>(w), uint64_t(n / kQ4Block) * kQ4Bytes, uint32_t(rows), n};
+    tile64<T, true>(a, r0, x, 0, n, m, acc);
+  } else {
+    const Operand a{reinterpret_cast<const u16*>(w), n, 1, uint32_t(rows), n, nullptr};
+    tile64<T, false>(a, r0, x, 0, n, m, acc);
+  }
+}
+
+// ---- tiles of pairs of an expert ---------------------------------------------------------------------------------------
+
+// The plan's tile and the a-tile of a workgroup, over the tiles there are (known on the device only).
+template <class S>
+__device__ __forceinline__ bool tile_of(const Plan& p, uint32_t na, TileRows& t, uint32_t& a) {
+  if (blockIdx.x >= na * *p.n_tiles) return false;
+  const TileAt at = tile_at(blockIdx.x, na, *p.n_tiles);
+  a = at.a;
+  return tile_rows(p, at.b, S::kB, t);
+}
+
+// 4 values next to each other a lane, to rows of 16 bits or 32.
+template <class V>
+struct RowsOut {
+  struct Fetched {};
+  V* out;
+  uint64_t stride;
+  uint32_t rows, c0, n_cols, c = 0;
+  __device__ __forceinline__ void columns(uint32_t a) { c = c0 + a; }
+  __device__ __forceinline__ Fetched fetch(uint32_t) const { return {}; }
+  template <class T>
+  __device__ __forceinline__ void put(uint32_t r, f32x4 v) const {
+    if (r >= rows || c >= n_cols) return;  // (columns are a multiple of 8: all four or none)
+    if constexpr (sizeof(V) == 4) {
+      *reinterpret_cast<f32x4*>(out + r * stride + c) = v;
+    } else {
+      bits4 o;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = T::down(v[i]);
+      *reinterpret_cast<bits4*>(out + r * stride + c) = o;
+    }
+  }
+};
+template <class T, class V>
+struct TypedOut : RowsOut<V> {
+  __device__ __forceinline__ void finish(uint32_t r, f32x4 v, const typename RowsOut<V>::Fetched&) const {
+    this->template put<T>(r, v);
+  }
+};
+
+// Gate and up rows of the same 16 NI columns as one operand of 32 NI: each wave gets 8 NI of both.
+template <int NI>
+__device__ __forceinline__ TileRowsSource<NI> gate_up_source(const Plan& p, const TileRows& t, uint32_t d, uint32_t f,
+                                                             uint32_t f0) {
+  const u16 *gate = reinterpret_cast<const u16*>(p.part[3 * t.e]), *up = reinterpret_cast<const u16*>(p.part[3 * t.e + 1]);
+  return TileRowsSource<NI>(d, threadIdx.x >> 6 & 1u, [&](uint32_t r) {
+    const uint32_t c = f0 + r / (16 * NI) * (8 * NI) + r % (8 * NI);
+    return (r & (8 * NI) ? up : gate) + uint64_t(c < f ? c : f - 1) * d;
+  });
+}
+template <int MJ>
+__device__ __forceinline__ TileRowsSource<MJ> mapped_rows(const TileRows& t, const u16* x, uint64_t stride, uint32_t n) {
+  return TileRowsSource<MJ>(n, threadIdx.x >> 7, [&](uint32_t r) { return x + t.map[r < t.rows ? r : t.rows - 1] * stride; });
+}
+template <int MJ>
+__device__ __forceinline__ TileRowsSource<MJ> sorted_rows(const TileRows& t, const u16* x, uint64_t stride, uint32_t n) {
+  return TileRowsSource<MJ>(n, threadIdx.x >> 7,
+                            [&](uint32_t r) { return x + uint64_t(t.first + (r < t.rows ? r : t.rows - 1)) * stride; });
+}
+
+// out_t = residual_t + sum_j w_tj v_{at(t, j)}, in the order of j; kWide columns a thread (a multiple of 4: one access each).
+template <class T, int kWide>
+__global__ __launch_bounds__(256) void combine_kernel(Plan p, uint32_t rows, uint32_t d, const float* v, const float* weights,
+                                                      const u16* residual, uint64_t residual_stride, u16* out,
+                                                      uint64_t out_stride) {
+  const uint32_t per = d / kWide;
+  const uint64_t total = uint64_t(rows) * per;
+  for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += uint64_t(gridDim.x) * 256) {
+    const uint32_t row = uint32_t(i / per), c = uint32_t(i % per) * kWide;
+    float s[kWide];
+    if constexpr (kWide == 4) {
+      const bits4 r = residual ? *reinterpret_cast<const bits4*>(residual + row * residual_stride + c) : bits4{0, 0, 0, 0};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) s[q] = T::up(r[q]);
+    } else {
+      s[0] = residual ? T::up(residual[row * residual_stride + c]) : 0.0f;
+    }
+    for (uint32_t j0 = 0; j0 < p.top_k; j0 += 4) {  // four at once: one after the other each is a memory latency
+      int32_t at[4];
+      float w[4], x[4][kWide];
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        const uint64_t pair = uint64_t(row) * p.top_k + j0 + j;
+        at[j] = j0 + j < p.top_k ? p.at[pair] : -1;
+        w[j] = j0 + j < p.top_k && weights ? weights[pair] : 1.0f;
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        const float* from = v + uint64_t(uint32_t(at[j] < 0 ? 0 : at[j])) * d + c;
+        if constexpr (kWide == 4) {
+          const f32x4 y = at[j] >= 0 ? *reinterpret_cast<const f32x4*>(from) : f32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) x[j][q] = y[q];
+        } else {
+          x[j][0] = at[j] >= 0 ? *from : 0.0f;
+        }
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j)
+        if (at[j] >= 0)
+#pragma unroll
+          for (int q = 0; q < kWide; ++q) s[q] += w[j] * x[j][q];
+    }
+    if constexpr (kWide == 4) {
+      bits4 o;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) o[q] = T::down(s[q]);
+      *reinterpret_cast<bits4*>(out + row * out_stride + c) = o;
+    } else {
+      out[row * out_stride + c] = T::down(s[0]);
+    }
+  }
+}
+
+// ---- the workspace --------------------------------------------------------------------------------------------------
+struct Room {
+  uint64_t bytes = 0;
+  char* base;
+  explicit Room(void* p) : base(static_cast<char*>(p)) {}
+  template <class V>
+  V* take(uint64_t n) {
+    V* p = reinterpret_cast<V*>(base + bytes);
+    bytes += up_to(n * sizeof(V), 256);
+    return p;
+  }
+};
+
+uint32_t most_tiles(uint32_t pairs, uint32_t n, uint32_t rows_per_tile) {
+  return pairs / rows_per_tile + (n < pairs ? n : pairs);
+}
+
+Plan take_plan(Room& r, uint32_t n, uint32_t pairs, uint32_t top_k, uint32_t rows_per_tile) {
+  Plan p;
+  p.part = r.take<const char*>(uint64_t(3) * n);
+  p.first = r.take<uint32_t>(n + 1);
+  p.pair = r.take<uint32_t>(pairs);
+  p.row = r.take<uint32_t>(pairs);
+  p.at = r.take<int32_t>(pairs);
+  p.tile = r.take<uint32_t>(uint64_t(2) * most_tiles(pairs, n, rows_per_tile));
+  p.n_tiles = r.take<uint32_t>(1);
+  p.pairs = pairs;
+  p.top_k = top_k;
+  p.n = n;
+  return p;
+}
+
+uint32_t blocks(uint64_t n) { return uint32_t(n < (1u << 20) ? n : (1u << 20)); }
+
+// Which tile the pairs' products take.
+#include <cstdlib>
+inline bool small_tiles(uint32_t rows, uint32_t top_k, uint32_t n) { const char* e = getenv("TSA_S"); return e && atoi(e); }
+
+template <class T>
+int launch_combine(const Plan& p, uint32_t rows, uint32_t d, const float* v, const float* weights, const void* residual,
+                   uint64_t residual_stride, void* out, uint64_t out_stride, hipStream_t s) {
+  const u16* r = static_cast<const u16*>(residual);
+  u16* o = static_cast<u16*>(out);
+  const uint64_t odd = reinterpret_cast<uintptr_t>(residual) | 2 * residual_stride | reinterpret_cast<uintptr_t>(out) | 2 * out_stride;
+  if (d % 4 == 0 && odd % 8 == 0)
+    hipLaunchKernelGGL((combine_kernel<T, 4>), dim3(blocks((uint64_t(rows) * d / 4 + 255) / 256)), dim3(256), 0, s, p, rows, d, v,
+                       weights, r, residual_stride, o, out_stride);
+  else
+    hipLaunchKernelGGL((combine_kernel<T, 1>), dim3(blocks((uint64_t(rows) * d + 255) / 256)), dim3(256), 0, s, p, rows, d, v,
+                       weights, r, residual_stride, o, out_stride);
+  return int(hipGetLastError());
+}
+
+bool aligned16(const void* p, uint64_t stride_bytes) { return (reinterpret_cast<uintptr_t>(p) | stride_bytes) % 16 == 0; }
+
+// Whether every weight row, x row and row of h starts 16-byte aligned and holds whole groups of 8 values. The addresses of
+// a table's units are the device's: its units are 256-byte aligned, as the library lays them out.
+bool wide_weights(const ExpertMap& e) {
+  for (int p = 0; p < 3; ++p) {
+    if (e.form == 0 && !aligned16(e.part[p], e.stride[p])) return false;
+    if (e.form == 1 && e.stride[p] % 16) return false;
+    if (e.form == 2 && !aligned16(e.view.parts[p].base, e.view.parts[p].stride)) return false;
+  }
+  return true;
+}
+bool wide_rows(const ExpertMap& e, uint32_t d, uint32_t f, bool q4, const void* x, uint64_t x_stride) {
+  if (d % 8 || f % 8 || !aligned16(x, 2 * x_stride) || x_stride >= 1u << 24) return false;
+  return q4 || wide_weights(e);
+}
+
+}  // namespace
+}  // namespace op
+}  // namespace tsa

@@ -5,12 +5,13 @@
 // A step is 32 values of the sum. Its operands are loaded straight to LDS (global_load_lds_dwordx4, NB buffers in turn) and
 // from there to a second set of registers while the step before is multiplied. Two steps, a cache line of every row, are
 // loaded together: by themselves each took the lines' halves from L2 again (a quarter of the time of a long product).
-// With 4 buffers step t (odd) waits for steps t + 1 and t + 2, loaded two steps earlier, and behind its barrier loads t + 3
-// and t + 4 over t - 1 and t, whose reads every wave has done. With 3, so that two workgroups fit a CU, step t (even)
-// loads t + 2 and t + 3 and step t + 1 waits for them.
+// With 3 buffers, so that two workgroups of the big tile fit a CU, step t (even) loads t + 2 and t + 3, behind a barrier and
+// over t - 1 and t, whose reads every wave has done, and step t + 1 waits for them. With more, step t (odd) waits for steps
+// t + 1 and t + 2 and behind its barrier loads t + NB - 1 and t + NB over t - 1 and t.
 //
 // Operands come in two forms. Rows: the values of the sum lie next to each other; a row's 64 bytes a step are 4 pieces,
-// piece c at place c ^ (row / 4 mod 4), so that 16 lanes reading one piece of 16 rows hit all banks. Columns (the operand
+// piece c at place c ^ (row / 2 mod 4), so that the lanes reading one piece of 16 rows hit all banks
+// (with row / 4 in its place the reads took twice the cycles: 4.4e7 of conflicts in one long product, now none). Columns (the operand
 // is transposed in memory): 32 rows of the tile's columns, read with ds_read_b64_tr_b16, which gives each lane of 16 one
 // column of 4 rows; pairs of pieces are permuted by the row so that the 8 rows of a half wave hit all banks. In both, the
 // permutation is made by the loads' addresses: LDS itself is filled in lane order.
@@ -45,10 +46,10 @@ struct TileRowsSource {
   __device__ __forceinline__ TileRowsSource(uint32_t n_, uint32_t half, At&& at) : n(n_) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     mine = __builtin_amdgcn_readfirstlane(wave) * kLoads * 1024;
-    k = ((lane & 3u) ^ (lane >> 4)) * 8;
+    k = ((lane & 3u) ^ ((lane >> 3) & 3u)) * 8;
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) p[j] = at((wave * kLoads + j) * 16 + lane / 4) + k;
-    frag = (half * NF * 16 + (lane & 15u)) * 64 + (((lane >> 4) ^ ((lane >> 2) & 3u)) * 16);
+    frag = (half * NF * 16 + (lane & 15u)) * 64 + (((lane >> 4) ^ ((lane >> 1) & 3u)) * 16);
   }
   // Load j of the next two steps (kCheck: the sum may end inside them); then, after all of them, on to the two behind.
   template <bool kCheck>
@@ -95,8 +96,8 @@ struct TileQ4Source {
     k = second * kQ4Block;
     const uint32_t row = (r / 64) * 128 + r % 64;
     put = row * 64;
-    turn = (row >> 2) & 3u;
-    frag = (half * 128 + (lane & 15u)) * 64 + (((lane >> 4) ^ ((lane >> 2) & 3u)) * 16);
+    turn = (row >> 1) & 3u;
+    frag = (half * 128 + (lane & 15u)) * 64 + (((lane >> 4) ^ ((lane >> 1) & 3u)) * 16);
     fetch();
   }
   __device__ __forceinline__ void fetch() {
@@ -221,6 +222,15 @@ struct TileColumnsSource {
 
 constexpr uint32_t tile_lds(int NI, int MJ, int NB) { return uint32_t(NI + MJ) * 2048u * uint32_t(NB); }
 
+// A tile: 32 NI rows of a, 32 MJ rows of b, NB buffers.
+template <int NI_, int MJ_, int NB_>
+struct TileShape {
+  static constexpr int NI = NI_, MJ = MJ_, NB = NB_;
+  static constexpr uint32_t kA = 32 * NI, kB = 32 * MJ, kLds = tile_lds(NI, MJ, NB);
+};
+typedef TileShape<8, 4, 3> BigTile;
+typedef TileShape<2, 2, 8> SmallTile;
+
 // Every accumulator through an empty statement: what is written before it is not read, and what is read after it not
 // written, on the other side. The compiler counts no wait states behind assembly, so they stand beside it.
 template <int NI, int MJ>
@@ -240,7 +250,7 @@ struct Nothing {
 };
 template <class T, int NI, int MJ, int NB, class A, class B, class F = Nothing>
 __device__ __forceinline__ void tile_product(A& a, B& b, uint32_t n, uint32_t lds, f32x4 (&acc)[NI][MJ], F&& every_two = F{}) {
-  static_assert(NB == 3 || NB == 4, "buffers");
+  static_assert(NB == 3 || (NB >= 4 && NB % 2 == 0), "buffers");
   constexpr int kLoads = A::kLoads + B::kLoads;  // of a step, each thread
   constexpr uint32_t kA = NI * 2048, kBuffer = (NI + MJ) * 2048;
   const auto issue = [&](auto check, int j, uint32_t at0, uint32_t at1) {  // load j of two steps, of both operands
@@ -256,8 +266,9 @@ __device__ __forceinline__ void tile_product(A& a, B& b, uint32_t n, uint32_t ld
   __syncthreads();  // the last product's reads are done
   a.stage(lds, lds + kBuffer);
   issue_all(lds, lds + kBuffer);
-  if (NB == 4) issue_all(lds + 2 * kBuffer, lds + 3 * kBuffer);
-  wait_loads_and_meet<NB == 4 ? 2 * kLoads : 0>();
+#pragma unroll
+  for (int i = 2; i + 1 < NB; i += 2) issue_all(lds + i * kBuffer, lds + (i + 1) * kBuffer);
+  wait_loads_and_meet<NB == 3 ? 0 : (NB - 2) * kLoads>();
   bits8 fa[2][NI], fb[2][MJ];
 #pragma unroll
   for (int i = 0; i < NI; ++i) fa[0][i] = a.read(lds, i);
@@ -272,7 +283,7 @@ __device__ __forceinline__ void tile_product(A& a, B& b, uint32_t n, uint32_t ld
   const auto step = [&](auto now_, auto loads, auto check) {
     constexpr int now = decltype(now_)::value, kFrags = NI + MJ, kPer = NI * MJ / kFrags;
     const uint32_t from = behind(1);
-    const uint32_t to0 = NB == 4 ? behind(3) : behind(2), to1 = lds + at * kBuffer;
+    const uint32_t to0 = NB == 3 ? behind(2) : behind(NB - 1), to1 = lds + at * kBuffer;
 #pragma unroll
     for (int x = 0; x < NI * MJ; ++x) {
       if (x % kPer == 0 && x / kPer < kFrags) {
@@ -293,9 +304,10 @@ __device__ __forceinline__ void tile_product(A& a, B& b, uint32_t n, uint32_t ld
   const auto two_steps = [&](auto check, uint32_t t) {
     using Zero = std::integral_constant<int, 0>;
     using One = std::integral_constant<int, 1>;
-    if (NB == 4) {
+    if (NB != 3) {
       step(Zero{}, std::false_type{}, check);
-      wait_loads_and_meet<0>();
+      wait_loads_and_meet<NB == 3 ? 0 : (NB - 4) * kLoads>();
+      every_two(t * 32);
       step(One{}, std::true_type{}, check);
     } else {
       meet();
@@ -306,7 +318,7 @@ __device__ __forceinline__ void tile_product(A& a, B& b, uint32_t n, uint32_t ld
       step(One{}, std::false_type{}, check);
     }
   };
-  constexpr uint32_t kAhead = NB == 4 ? 6 : 4;  // the last step that two steps from t on load, + 1
+  constexpr uint32_t kAhead = NB == 3 ? 4 : NB + 2;  // the last step that two steps from t on load, + 1
   uint32_t t = 0;
   for (; (t + kAhead) * 32 <= n; t += 2) two_steps(std::false_type{}, t);
   for (; t * 32 < n; t += 2) two_steps(std::true_type{}, t);  // (steps past the end multiply zeros)
@@ -317,11 +329,13 @@ __device__ __forceinline__ void tile_product(A& a, B& b, uint32_t n, uint32_t ld
 
 // Hands a wave's part of a tile to `out`, 4 values of a-rows next to each other at a time, rows counted in the tile: by way
 // of LDS (the wave's own JP fragments of b at a time), so that lanes next to each other have values next to each other.
-// out.columns(a-row): this lane's 4 a-rows, once; out.fetch(b-row) gives what finish() of that row needs from memory, for 8
-// rows before the first finish(b-row, values, fetched): one after the other, each would be a memory latency.
-template <int NI, int MJ, int JP, class Out>
+// out.columns(a-row): this lane's 4 a-rows, once; out.fetch(b-row) gives what finish() of that row needs from memory, for up
+// to 8 rows before the first finish(b-row, values, fetched): one after the other, each would be a memory latency.
+template <int NI, int MJ, class Out>
 __device__ __forceinline__ void hand_out(void* memory, const f32x4 (&acc)[NI][MJ], Out& out) {
+  constexpr int JP = NI == 8 ? MJ / 2 : MJ;                 // (what the buffers hold)
   constexpr uint32_t kLanes = NI * 4, kRows = 64 / kLanes;  // lanes a row, rows at once
+  constexpr uint32_t kBatch = 16 * JP / kRows < 8 ? 16 * JP / kRows : 8;
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   f32x4* mine = static_cast<f32x4*>(memory) + wave * (JP * 16 * kLanes);
   out.columns((wave & 1u) * 16 * NI + (lane % kLanes) * 4);
@@ -335,13 +349,13 @@ __device__ __forceinline__ void hand_out(void* memory, const f32x4 (&acc)[NI][MJ
         mine[(16 * j + (lane & 15u)) * kLanes + ((4 * i + (lane >> 4)) ^ ((lane & 15u) % kLanes))] = acc[i][j0 + j];
     __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
-    for (uint32_t r0 = lane / kLanes; r0 < 16 * JP; r0 += 8 * kRows) {
+    for (uint32_t r0 = lane / kLanes; r0 < 16 * JP; r0 += kBatch * kRows) {
       const uint32_t base = (wave >> 1) * 16 * MJ + 16 * j0 + r0;
-      typename Out::Fetched got[8];
+      typename Out::Fetched got[kBatch];
 #pragma unroll
-      for (uint32_t x = 0; x < 8; ++x) got[x] = out.fetch(base + x * kRows);
+      for (uint32_t x = 0; x < kBatch; ++x) got[x] = out.fetch(base + x * kRows);
 #pragma unroll
-      for (uint32_t x = 0; x < 8; ++x) {
+      for (uint32_t x = 0; x < kBatch; ++x) {
         const uint32_t r = r0 + x * kRows;
         out.finish(base + x * kRows, mine[r * kLanes + ((lane % kLanes) ^ ((r & 15u) % kLanes))], got[x]);
       }
