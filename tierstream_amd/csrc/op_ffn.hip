@@ -300,7 +300,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void gate_up_q4_tile_kernel(Plan p
   extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
   TileRows t;
   uint32_t at;
-  if (!tile_of<BigTile>(p, (f + 63) / 64, t, at)) return;
+  if (!tile_of<WideTile>(p, (f + 63) / 64, t, at)) return;
   const char *gate = p.part[3 * t.e], *up = p.part[3 * t.e + 1];
   TileQ4Source<T> w(d, threadIdx.x >> 6 & 1u, [&](uint32_t r) {  // of each wave's 64 rows: 32 gate, 32 up
     const uint32_t c = at * 64 + (r >> 6) * 32 + (r & 31u);
@@ -327,7 +327,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void down_q4_tile_kernel(Plan p, c
   extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
   TileRows t;
   uint32_t at;
-  if (!tile_of<BigTile>(p, (d + 127) / 128, t, at)) return;
+  if (!tile_of<WideTile>(p, (d + 127) / 128, t, at)) return;
   const unsigned char* down = reinterpret_cast<const unsigned char*>(p.part[3 * t.e + 2]);
   TileQ4Source<T> w(f, threadIdx.x >> 6 & 1u, [&](uint32_t r) {
     const uint32_t c = at * 128 + r;
@@ -437,7 +437,7 @@ int forward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& a, v
   if (wide_rows(e, d, f, kQ4, a.x, a.x_stride)) {
     if constexpr (!kQ4)
       if (small_tiles(a.rows, a.top_k, e.n)) return forward_tiles<T, false, SmallTile>(e, d, f, a, ws, s);
-    return forward_tiles<T, kQ4, BigTile>(e, d, f, a, ws, s);
+    return forward_tiles<T, kQ4, std::conditional_t<kQ4, WideTile, BigTile>>(e, d, f, a, ws, s);
   }
   Room room(ws);
   const Forward w = take_forward(room, e.n, d, f, a.rows, a.top_k);

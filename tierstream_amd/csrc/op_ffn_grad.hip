@@ -146,7 +146,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void hidden_grad_tile_kernel(Plan 
                                                                            float* d_share) {
   extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
   constexpr int NI = S::NI, MJ = S::MJ, kHalf = NI / 2;
-  __shared__ float share[S::kB][2];
+  float* share = reinterpret_cast<float*>(memory) + S::kLds / 4 - 2 * S::kB;  // (behind what hand_out uses)
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   TileRows t;
   uint32_t at;
@@ -165,6 +165,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void hidden_grad_tile_kernel(Plan 
     w[j] = weights ? weights[p.pair[pos[j]]] : 1.0f;
   }
   f32x4 h[kHalf][MJ];
+  __syncthreads();  // the product's reads are done
 #pragma unroll
   for (int j = 0; j < MJ; ++j) {
     float sum = 0.0f;
@@ -186,11 +187,11 @@ __global__ __launch_bounds__(kTileThreads, 2) void hidden_grad_tile_kernel(Plan 
       }
     sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
-    if (lane < 16) share[(wave >> 1) * 16 * MJ + 16 * j + lane][wave & 1u] = sum;
+    if (lane < 16) share[2 * ((wave >> 1) * 16 * MJ + 16 * j + lane) + (wave & 1u)] = sum;
   }
   TypedOut<T, u16> out{{wh + uint64_t(t.first) * f, f, t.rows, f0, f}};
   hand_out<kHalf, MJ>(memory, h, out);  // (behind its barrier `share` is whole)
-  if (threadIdx.x < t.rows) d_share[uint64_t(at) * p.pairs + t.first + threadIdx.x] = share[threadIdx.x][0] + share[threadIdx.x][1];
+  if (threadIdx.x < t.rows) d_share[uint64_t(at) * p.pairs + t.first + threadIdx.x] = share[2 * threadIdx.x] + share[2 * threadIdx.x + 1];
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
 #pragma unroll
@@ -283,7 +284,7 @@ Backward take_backward(Room& r, uint32_t n, uint32_t d, uint32_t f, uint32_t row
   return w;
 }
 
-template <class T, class S>
+template <class T, class S, class W>
 int backward_tiles(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_grad_args& a, void* ws, hipStream_t s) {
   Room room(ws);
   const Backward w = take_backward(room, e.n, d, f, a.rows, a.top_k);
@@ -306,10 +307,10 @@ int backward_tiles(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_gra
     hipLaunchKernelGGL(weights_grad_kernel, dim3(blocks((w.plan.pairs + 255) / 256)), dim3(256), 0, s, w.plan, shares, w.share,
                        a.dweights);
   if (a.dgate) {
-    constexpr uint32_t kLds = S::kLds + 4 * kMapRing;
-    hipLaunchKernelGGL((weight_grad_tile_kernel<T, S, true>), dim3(e.n * of(d, S::kA) * of(f, S::kB) * 2), dim3(kTileThreads), kLds, s,
+    constexpr uint32_t kLds = W::kLds + 4 * kMapRing;
+    hipLaunchKernelGGL((weight_grad_tile_kernel<T, W, true>), dim3(e.n * of(d, W::kA) * of(f, W::kB) * 2), dim3(kTileThreads), kLds, s,
                        w.plan, x, a.x_stride, d, w.dgu, uint64_t(2) * f, f, 2u, static_cast<u16*>(a.dgate), static_cast<u16*>(a.dup));
-    hipLaunchKernelGGL((weight_grad_tile_kernel<T, S, false>), dim3(e.n * of(f, S::kA) * of(d, S::kB)), dim3(kTileThreads), kLds, s,
+    hipLaunchKernelGGL((weight_grad_tile_kernel<T, W, false>), dim3(e.n * of(f, W::kA) * of(d, W::kB)), dim3(kTileThreads), kLds, s,
                        w.plan, w.wh, uint64_t(f), f, dy, a.dy_stride, d, 1u, static_cast<u16*>(a.ddown), static_cast<u16*>(nullptr));
   }
   return int(hipGetLastError());
@@ -319,7 +320,7 @@ template <class T>
 int backward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_grad_args& a, void* ws, hipStream_t s) {
   if (wide_rows(e, d, f, false, a.x, a.x_stride) && aligned16(a.dy, 2 * a.dy_stride) && a.dy_stride < 1u << 24 && aligned16(a.dgate, 0) && aligned16(a.dup, 0) &&
       aligned16(a.ddown, 0))
-    return small_tiles(a.rows, a.top_k, e.n) ? backward_tiles<T, SmallTile>(e, d, f, a, ws, s) : backward_tiles<T, BigTile>(e, d, f, a, ws, s);
+    return small_tiles(a.rows, a.top_k, e.n) ? backward_tiles<T, SmallTile, SmallTile>(e, d, f, a, ws, s) : backward_tiles<T, BigTile, WideTile>(e, d, f, a, ws, s);
   Room room(ws);
   const Backward w = take_backward(room, e.n, d, f, a.rows, a.top_k);
   if (int err = launch_plan(e, a.ids, w.plan, 64, s)) return err;

@@ -150,33 +150,34 @@ int launch_few(const tsa_linear_args& a, hipStream_t stream) {
   return launch_few<T, W, 2, 4>(a, stream);
 }
 
-// Many rows: tiles of 256 weight rows and 128 rows of x, two workgroups a CU: one's products run under the other's epilogue.
-// (Tiles of 256 x 256, one a CU, take less from L2 and LDS, but their epilogue stands alone: 575 us where these take 528,
-// 2047 rows through 4096 x 28672 with bias, tanh gelu and residual.)
-template <class T>
+// Many rows: big tiles, two workgroups a CU: one's products run under the other's epilogue. (Tiles of 256 x 256, one a CU,
+// take less from L2 and LDS, but their epilogue stands alone: 575 us where 256 x 128 took 528, 2047 rows through 4096 x 28672
+// with bias, tanh gelu and residual.)
+template <class T, class S>
 __global__ __launch_bounds__(kTileThreads, 2) void linear_tile_kernel(tsa_linear_args a) {
-  extern __shared__ f32x4 memory[];
+  extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
+  constexpr int NI = S::NI, MJ = S::MJ;
   const uint32_t wave = threadIdx.x >> 6;
-  const TileAt t = tile_at(blockIdx.x, (a.n_out + 255) / 256, (a.rows + 127) / 128);
-  const uint32_t n0 = t.a * 256, r0 = t.b * 128;
-  TileRowsSource<8> w(a.n_in, wave & 1u, [&](uint32_t r) {
+  const TileAt t = tile_at(blockIdx.x, (a.n_out + S::kA - 1) / S::kA, (a.rows + S::kB - 1) / S::kB);
+  const uint32_t n0 = t.a * S::kA, r0 = t.b * S::kB;
+  TileRowsSource<NI> w(a.n_in, wave & 1u, [&](uint32_t r) {
     const uint32_t n = n0 + r;
     return static_cast<const u16*>(a.w) + (n < a.n_out ? n : a.n_out - 1) * a.w_stride;
   });
-  TileRowsSource<4> x(a.n_in, wave >> 1, [&](uint32_t r) {
+  TileRowsSource<MJ> x(a.n_in, wave >> 1, [&](uint32_t r) {
     const uint32_t row = r0 + r;
     return static_cast<const u16*>(a.x) + (row < a.rows ? row : a.rows - 1) * a.x_stride;
   });
-  f32x4 acc[8][4] = {};
-  tile_product<T, 8, 4, 3>(w, x, a.n_in, lds_offset(memory), acc);
+  f32x4 acc[NI][MJ] = {};
+  tile_product<T, NI, MJ, S::NB>(w, x, a.n_in, lds_offset(memory), acc);
   LinearOut<T> out(a, r0, n0);
-  hand_out<8, 4>(memory, acc, out);
+  hand_out<NI, MJ>(memory, acc, out);
 }
 
-template <class T>
+template <class T, class S>
 int launch_tile(const tsa_linear_args& a, hipStream_t stream) {
-  const uint32_t tiles = (a.n_out + 255) / 256 * ((a.rows + 127) / 128);
-  hipLaunchKernelGGL((linear_tile_kernel<T>), dim3(tiles), dim3(kTileThreads), tile_lds(8, 4, 3), stream, a);
+  const uint32_t tiles = (a.n_out + S::kA - 1) / S::kA * ((a.rows + S::kB - 1) / S::kB);
+  hipLaunchKernelGGL((linear_tile_kernel<T, S>), dim3(tiles), dim3(kTileThreads), S::kLds, stream, a);
   return int(hipGetLastError());
 }
 
@@ -276,7 +277,8 @@ int launch_linear(const tsa_linear_args& a0, void* workspace, hipStream_t stream
   }
   a.n_in = wide;  // (packed rows end in zeros; unpacked ones are whole)
   if (q4) return bf16 ? op::launch_q4_tile<op::Bf16>(a, stream) : op::launch_q4_tile<op::F16>(a, stream);
-  return bf16 ? op::launch_tile<op::Bf16>(a, stream) : op::launch_tile<op::F16>(a, stream);
+  if (getenv("TSA_M") && atoi(getenv("TSA_M")) == 1) return bf16 ? op::launch_tile<op::Bf16, op::WideTile>(a, stream) : op::launch_tile<op::F16, op::WideTile>(a, stream);
+  return bf16 ? op::launch_tile<op::Bf16, op::BigTile>(a, stream) : op::launch_tile<op::F16, op::BigTile>(a, stream);
 }
 
 }  // namespace tsa

@@ -119,7 +119,7 @@ __device__ __forceinline__ TileRowsSource<NI> gate_up_source(const Plan& p, cons
   const u16 *gate = reinterpret_cast<const u16*>(p.part[3 * t.e]), *up = reinterpret_cast<const u16*>(p.part[3 * t.e + 1]);
   return TileRowsSource<NI>(d, threadIdx.x >> 6 & 1u, [&](uint32_t r) {
     const uint32_t c = f0 + r / (16 * NI) * (8 * NI) + r % (8 * NI);
-    return (r & (8 * NI) ? up : gate) + uint64_t(c < f ? c : f - 1) * d;
+    return (r % (16 * NI) >= 8 * NI ? up : gate) + uint64_t(c < f ? c : f - 1) * d;
   });
 }
 template <int MJ>

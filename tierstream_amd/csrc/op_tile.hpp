@@ -166,12 +166,15 @@ template <int NF, bool kMap>
 struct TileColumnsSource {
   static constexpr int kLoads = NF / 2;
   static constexpr uint32_t kPieces = 4 * NF;  // 16-byte pieces of a row
+  static constexpr bool kEven = (kPieces & (kPieces - 1)) == 0;  // rows of 256 bytes or a power of two of it; else of 128 more
   uint64_t base;
   uint32_t offset[kLoads];  // bytes: of the lane's column, and without a map of its row
-  uint32_t stride, k, n, mine, frag;
+  uint32_t stride, k, n, mine, frag[kEven ? 1 : NF];
   const uint32_t* map;
 
-  static __device__ __forceinline__ uint32_t turn(uint32_t kk) { return (((kk & 3u) | ((kk >> 3) & 1u) << 2) << 1) & (kPieces - 1); }
+  static __device__ __forceinline__ uint32_t turn(uint32_t kk) {
+    return kEven ? (((kk & 3u) | ((kk >> 3) & 1u) << 2) << 1) & (kPieces - 1) : ((kk >> 1 & 1u) | ((kk >> 3) & 1u) << 1) << 1;
+  }
   __device__ __forceinline__ TileColumnsSource(uint32_t n_, uint32_t half, const u16* at, uint64_t stride_, uint32_t first,
                                                uint32_t n_cols, const uint32_t* map_ = nullptr)
       : base(uniform(reinterpret_cast<uint64_t>(at))), stride(uint32_t(stride_) * 2), k(0), n(n_), map(map_) {
@@ -184,7 +187,9 @@ struct TileColumnsSource {
       offset[j] = (c < n_cols ? c : n_cols - 8) * 2 + (kMap ? 0 : i / kPieces * stride);
     }
     const uint32_t kk = (lane >> 4) * 8 + ((lane & 15u) >> 2);
-    frag = kk * (kPieces * 16) + ((half * NF * 2 + ((lane & 3u) >> 1)) ^ turn(kk)) * 16 + (lane & 1u) * 8;
+#pragma unroll
+    for (int i = 0; i < (kEven ? 1 : NF); ++i)
+      frag[i] = kk * (kPieces * 16) + ((half * NF * 2 + 2 * i + ((lane & 3u) >> 1)) ^ turn(kk)) * 16 + (lane & 1u) * 8;
   }
   __device__ __forceinline__ uint32_t row_of(int j) const {  // of the lane's piece, in its step
     return (mine + j * 1024 + (threadIdx.x & 63u) * 16) / (kPieces * 16);
@@ -213,7 +218,7 @@ struct TileColumnsSource {
   }
   __device__ __forceinline__ void stage(uint32_t, uint32_t) {}
   __device__ __forceinline__ bits8 read(uint32_t lds, int i) const {
-    const uint32_t at = (lds + frag) ^ (32u * i);
+    const uint32_t at = kEven ? (lds + frag[0]) ^ (32u * i) : lds + frag[kEven ? 0 : i];
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4_t*>(at));
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4_t*>(at + 4 * kPieces * 16));
     return __builtin_bit_cast(bits8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -228,7 +233,8 @@ struct TileShape {
   static constexpr int NI = NI_, MJ = MJ_, NB = NB_;
   static constexpr uint32_t kA = 32 * NI, kB = 32 * MJ, kLds = tile_lds(NI, MJ, NB);
 };
-typedef TileShape<8, 4, 3> BigTile;
+typedef TileShape<6, 4, 4> BigTile;
+typedef TileShape<8, 4, 3> WideTile;
 typedef TileShape<2, 2, 8> SmallTile;
 
 // Every accumulator through an empty statement: what is written before it is not read, and what is read after it not
@@ -333,9 +339,13 @@ __device__ __forceinline__ void tile_product(A& a, B& b, uint32_t n, uint32_t ld
 // to 8 rows before the first finish(b-row, values, fetched): one after the other, each would be a memory latency.
 template <int NI, int MJ, class Out>
 __device__ __forceinline__ void hand_out(void* memory, const f32x4 (&acc)[NI][MJ], Out& out) {
-  constexpr int JP = NI == 8 ? MJ / 2 : MJ;                 // (what the buffers hold)
-  constexpr uint32_t kLanes = NI * 4, kRows = 64 / kLanes;  // lanes a row, rows at once
+  constexpr int JP = NI >= 6 ? MJ / 2 : MJ;  // (what the buffers hold)
+  constexpr uint32_t kLanes = NI * 4, kRows = kLanes > 16 ? (kLanes > 32 ? 1 : 2) : kLanes > 8 ? 4 : 64 / kLanes;  // lanes a row, rows at once
   constexpr uint32_t kBatch = 16 * JP / kRows < 8 ? 16 * JP / kRows : 8;
+  // Piece p of row r: turned by the row, so that both ways hit all banks.
+  const auto place = [](uint32_t p, uint32_t r) {
+    return r * kLanes + ((kLanes & (kLanes - 1)) == 0 ? p ^ (r & 15u) % kLanes : (p + (r & 15u)) % kLanes);
+  };
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   f32x4* mine = static_cast<f32x4*>(memory) + wave * (JP * 16 * kLanes);
   out.columns((wave & 1u) * 16 * NI + (lane % kLanes) * 4);
@@ -345,21 +355,19 @@ __device__ __forceinline__ void hand_out(void* memory, const f32x4 (&acc)[NI][MJ
 #pragma unroll
     for (int j = 0; j < JP; ++j)
 #pragma unroll
-      for (int i = 0; i < NI; ++i)  // (piece p of row r at p ^ r mod 16: both ways hit all banks)
-        mine[(16 * j + (lane & 15u)) * kLanes + ((4 * i + (lane >> 4)) ^ ((lane & 15u) % kLanes))] = acc[i][j0 + j];
+      for (int i = 0; i < NI; ++i) mine[place(4 * i + (lane >> 4), 16 * j + (lane & 15u))] = acc[i][j0 + j];
     __builtin_amdgcn_wave_barrier();
+    if (lane < kLanes * kRows)
 #pragma unroll 1
-    for (uint32_t r0 = lane / kLanes; r0 < 16 * JP; r0 += kBatch * kRows) {
-      const uint32_t base = (wave >> 1) * 16 * MJ + 16 * j0 + r0;
-      typename Out::Fetched got[kBatch];
+      for (uint32_t r0 = lane / kLanes; r0 < 16 * JP; r0 += kBatch * kRows) {
+        const uint32_t base = (wave >> 1) * 16 * MJ + 16 * j0 + r0;
+        typename Out::Fetched got[kBatch];
 #pragma unroll
-      for (uint32_t x = 0; x < kBatch; ++x) got[x] = out.fetch(base + x * kRows);
+        for (uint32_t x = 0; x < kBatch; ++x) got[x] = out.fetch(base + x * kRows);
 #pragma unroll
-      for (uint32_t x = 0; x < kBatch; ++x) {
-        const uint32_t r = r0 + x * kRows;
-        out.finish(base + x * kRows, mine[r * kLanes + ((lane % kLanes) ^ ((r & 15u) % kLanes))], got[x]);
+        for (uint32_t x = 0; x < kBatch; ++x)
+          out.finish(base + x * kRows, mine[place(lane % kLanes, r0 + x * kRows)], got[x]);
       }
-    }
     __builtin_amdgcn_wave_barrier();
   }
 }
