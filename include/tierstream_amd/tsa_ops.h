@@ -75,8 +75,8 @@ typedef struct tsa_linear_args {
   uint32_t act;
   uint32_t reserved;
 } tsa_linear_args;
-/* Workspace bytes of a call (0: none is used): where more than 64 rows are to be multiplied and rows of x or w do not start
- * 16-byte aligned or are no multiple of 8 values, these are packed first. Sizes are below 2^24, rows x n_out below 2^37. */
+/* Workspace bytes of a call (0: none is used): where more than a few rows are to be multiplied and rows of x or w do not
+ * start 16-byte aligned or are no multiple of 8 values, these are packed first. Sizes are below 2^24, rows x n_out below 2^37. */
 SS_API uint64_t tsa_linear_workspace(const tsa_linear_args* a);
 SS_API ss_status tsa_linear(const tsa_linear_args* a, void* workspace, uint64_t workspace_bytes, void* stream);
 

@@ -270,8 +270,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void gate_up_tile_kernel(Plan p, c
     for (int j = 0; j < MJ; ++j)
 #pragma unroll
       for (int q = 0; q < 4; ++q) v[i][j][q] = activate(act, acc[i][j][q]) * acc[i + NI / 2][j][q];
-  TypedOut<T, u16> out{{h + uint64_t(t.first) * f, f, t.rows, at * 16 * NI, f}};
-  hand_out<NI / 2, MJ>(memory, v, out);
+  hand_out_bits<T, NI / 2, MJ>(memory, v, h + uint64_t(t.first) * f + at * 16 * NI, f, t.rows, f - at * 16 * NI);
 }
 
 template <class T, class S>
@@ -289,7 +288,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void down_tile_kernel(Plan p, cons
   auto hs = sorted_rows<MJ>(t, h, f, f);
   f32x4 acc[NI][MJ] = {};
   tile_product<T, NI, MJ, S::NB>(w, hs, f, lds_offset(memory), acc);
-  TypedOut<T, float> o{{out + uint64_t(t.first) * d, d, t.rows, at * S::kA, d}};
+  FloatRows o{out + uint64_t(t.first) * d, d, t.rows, at * S::kA, d};
   hand_out<NI, MJ>(memory, acc, o);
 }
 
@@ -318,8 +317,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void gate_up_q4_tile_kernel(Plan p
 #pragma unroll
       for (int q = 0; q < 4; ++q) v[i][j][q] = activate(act, g[q]) * u[q];
     }
-  TypedOut<T, u16> out{{h + uint64_t(t.first) * f, f, t.rows, at * 64, f}};
-  hand_out<2, 4>(memory, v, out);
+  hand_out_bits<T, 2, 4>(memory, v, h + uint64_t(t.first) * f + at * 64, f, t.rows, f - at * 64);
 }
 
 template <class T>
@@ -341,7 +339,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void down_q4_tile_kernel(Plan p, c
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[i][j] = TileQ4Source<T>::whole(acc[i][j], acc[i + 4][j]);
-  TypedOut<T, float> o{{out + uint64_t(t.first) * d, d, t.rows, at * 128, d}};
+  FloatRows o{out + uint64_t(t.first) * d, d, t.rows, at * 128, d};
   hand_out<4, 4>(memory, v, o);
 }
 
@@ -397,12 +395,13 @@ int forward_few(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& 
   return launch_combine<T>(w.plan, a.rows, d, w.out, a.weights, a.residual, a.residual_stride, a.y, a.y_stride, s);
 }
 
-template <class T, class W, bool kTail>
-int forward_stream(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& a, void* ws, hipStream_t s) {
-  if (a.rows == 1) return forward_one<T, W, kTail>(e, d, f, a, ws, s);
+// 4-bit weights, few rows: up to so many pairs an expert (if all are asked for alike) as CT tiles of 16 hold.
+template <class T, bool kTail>
+int forward_few_q4(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& a, void* ws, hipStream_t s) {
+  typedef RowsQ4<T> W;
   Room room(ws);
   const Forward w = take_forward(room, e.n, d, f, a.rows, a.top_k);
-  const uint32_t each = w.plan.pairs / e.n;  // pairs of an expert if all are asked for alike
+  const uint32_t each = w.plan.pairs / e.n;
   if (each <= 8) return forward_few<T, W, 1, kTail>(e, d, f, a, w, s);
   if (each <= 24) return forward_few<T, W, 2, kTail>(e, d, f, a, w, s);
   return forward_few<T, W, 4, kTail>(e, d, f, a, w, s);
@@ -414,14 +413,17 @@ int forward_tiles(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args
   const Forward w = take_forward(room, e.n, d, f, a.rows, a.top_k);
   if (int err = launch_plan(e, a.ids, w.plan, S::kB, s)) return err;
   const uint32_t tiles = most_tiles(w.plan.pairs, e.n, S::kB);
-  constexpr uint32_t kF = kQ4 ? S::kA / 4 : S::kA / 2, kD = kQ4 ? S::kA / 2 : S::kA;  // columns a tile
+  // Gate and up as wide as they come, 1850 us in a prompt of 4001 rows where 192 rows a tile take 1955; down, whose sums are longer
+  // and whose tiles are fewer, 192 rows: 1093 us, 1240.
+  typedef std::conditional_t<std::is_same_v<S, BigTile>, WideTile, S> U;
+  constexpr uint32_t kF = kQ4 ? U::kA / 4 : U::kA / 2, kD = kQ4 ? S::kA / 2 : S::kA;  // columns a tile
   const dim3 up(tiles * ((f + kF - 1) / kF)), down(tiles * ((d + kD - 1) / kD));
   const u16* x = static_cast<const u16*>(a.x);
   if constexpr (kQ4) {
     hipLaunchKernelGGL((gate_up_q4_tile_kernel<T>), up, dim3(kTileThreads), S::kLds, s, w.plan, x, a.x_stride, d, f, a.act, w.h);
     hipLaunchKernelGGL((down_q4_tile_kernel<T>), down, dim3(kTileThreads), S::kLds, s, w.plan, w.h, d, f, w.out);
   } else {
-    hipLaunchKernelGGL((gate_up_tile_kernel<T, S>), up, dim3(kTileThreads), S::kLds, s, w.plan, x, a.x_stride, d, f, a.act, w.h);
+    hipLaunchKernelGGL((gate_up_tile_kernel<T, U>), up, dim3(kTileThreads), U::kLds, s, w.plan, x, a.x_stride, d, f, a.act, w.h);
     hipLaunchKernelGGL((down_tile_kernel<T, S>), down, dim3(kTileThreads), S::kLds, s, w.plan, w.h, d, f, w.out);
   }
   return launch_combine<T>(w.plan, a.rows, d, w.out, a.weights, a.residual, a.residual_stride, a.y, a.y_stride, s);
@@ -430,13 +432,17 @@ int forward_tiles(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args
 template <class T, bool kQ4>
 int forward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& a, void* ws, hipStream_t s) {
   typedef std::conditional_t<kQ4, RowsQ4<T>, Rows16<T>> W;
-  if constexpr (kQ4)
+  const bool tail = d % kChunk || f % kChunk;
+  if constexpr (kQ4) {
     if (a.rows == 1 && d % 256 == 0 && f % 256 == 0 && aligned16(a.x, 0) && wide_weights(e)) return forward_one_q4<T>(e, d, f, a, ws, s);
-  if (uint64_t(a.rows) * a.top_k <= uint64_t(64) * e.n)
-    return d % kChunk || f % kChunk ? forward_stream<T, W, true>(e, d, f, a, ws, s) : forward_stream<T, W, false>(e, d, f, a, ws, s);
+    if (a.rows > 1 && uint64_t(a.rows) * a.top_k <= uint64_t(64) * e.n)
+      return tail ? forward_few_q4<T, true>(e, d, f, a, ws, s) : forward_few_q4<T, false>(e, d, f, a, ws, s);
+  }
+  // (Two rows of 16-bit weights and more are no slower in small tiles: 32 rows, 8 of 128 experts, 146 us and 156 streamed.)
+  if (a.rows == 1) return tail ? forward_one<T, W, true>(e, d, f, a, ws, s) : forward_one<T, W, false>(e, d, f, a, ws, s);
   if (wide_rows(e, d, f, kQ4, a.x, a.x_stride)) {
     if constexpr (!kQ4)
-      if (small_tiles(a.rows, a.top_k, e.n)) return forward_tiles<T, false, SmallTile>(e, d, f, a, ws, s);
+      if (small_tiles(a.rows, a.top_k, e.n, d, f)) return forward_tiles<T, false, SmallTile>(e, d, f, a, ws, s);
     return forward_tiles<T, kQ4, std::conditional_t<kQ4, WideTile, BigTile>>(e, d, f, a, ws, s);
   }
   Room room(ws);

@@ -134,7 +134,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void back_tile_kernel(Plan p, cons
   auto dys = mapped_rows<MJ>(t, dy, dy_stride, d);
   f32x4 acc[NI][MJ] = {};
   tile_product<T, NI, MJ, S::NB>(w, dys, d, lds_offset(memory), acc);
-  TypedOut<T, float> o{{back + uint64_t(t.first) * f, f, t.rows, at * S::kA, f}};
+  FloatRows o{back + uint64_t(t.first) * f, f, t.rows, at * S::kA, f};
   hand_out<NI, MJ>(memory, acc, o);
 }
 
@@ -189,8 +189,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void hidden_grad_tile_kernel(Plan 
     sum += __shfl_xor(sum, 32, 64);
     if (lane < 16) share[2 * ((wave >> 1) * 16 * MJ + 16 * j + lane) + (wave & 1u)] = sum;
   }
-  TypedOut<T, u16> out{{wh + uint64_t(t.first) * f, f, t.rows, f0, f}};
-  hand_out<kHalf, MJ>(memory, h, out);  // (behind its barrier `share` is whole)
+  hand_out_bits<T, kHalf, MJ>(memory, h, wh + uint64_t(t.first) * f + f0, f, t.rows, f - f0);  // (behind its barrier `share` is whole)
   if (threadIdx.x < t.rows) d_share[uint64_t(at) * p.pairs + t.first + threadIdx.x] = share[2 * threadIdx.x] + share[2 * threadIdx.x + 1];
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
@@ -198,9 +197,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void hidden_grad_tile_kernel(Plan 
     for (int i = 0; i < kHalf; ++i)
 #pragma unroll
       for (int j = 0; j < MJ; ++j) h[i][j] = gu[i + kHalf * half][j];
-    out.out = dgu + uint64_t(t.first) * 2 * f + half * f;
-    out.stride = uint64_t(2) * f;
-    hand_out<kHalf, MJ>(memory, h, out);
+    hand_out_bits<T, kHalf, MJ>(memory, h, dgu + uint64_t(t.first) * 2 * f + half * f + f0, uint64_t(2) * f, t.rows, f - f0);
   }
 }
 
@@ -220,7 +217,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void input_grad_tile_kernel(Plan p
   };
   add(0);
   add(1);
-  TypedOut<T, float> o{{out + uint64_t(t.first) * d, d, t.rows, at * S::kA, d}};
+  FloatRows o{out + uint64_t(t.first) * d, d, t.rows, at * S::kA, d};
   hand_out<NI, MJ>(memory, acc, o);
 }
 
@@ -263,8 +260,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void weight_grad_tile_kernel(Plan 
       tile_product<T, NI, MJ, S::NB>(l, r, pairs, lds_offset(memory), acc, refill);
     }
   }
-  TypedOut<T, u16> o{{(which ? out2 : out) + (uint64_t(e) * n_right + b0) * n_left, n_left, n_right - b0, a0, n_left}};
-  hand_out<NI, MJ>(memory, acc, o);
+  hand_out_bits<T, NI, MJ>(memory, acc, (which ? out2 : out) + (uint64_t(e) * n_right + b0) * n_left + a0, n_left, n_right - b0,
+                           n_left - a0);
 }
 
 // ---- launches ----
@@ -320,7 +317,15 @@ template <class T>
 int backward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_grad_args& a, void* ws, hipStream_t s) {
   if (wide_rows(e, d, f, false, a.x, a.x_stride) && aligned16(a.dy, 2 * a.dy_stride) && a.dy_stride < 1u << 24 && aligned16(a.dgate, 0) && aligned16(a.dup, 0) &&
       aligned16(a.ddown, 0))
-    return small_tiles(a.rows, a.top_k, e.n) ? backward_tiles<T, SmallTile, SmallTile>(e, d, f, a, ws, s) : backward_tiles<T, BigTile, WideTile>(e, d, f, a, ws, s);
+  {
+    // The weights' gradients choose by themselves: 4 experts of 512 x 1024 (64 wide tiles) 173 us in all with wide tiles and 141
+    // with small ones, one of 2048 x 2048 (128) 107 and 112, 8 of 4096 x 2048 (2048) 337 and 480.
+    const bool small = small_tiles(a.rows, a.top_k, e.n, d, f);
+    const bool small_out = uint64_t(e.n) * ((d + WideTile::kA - 1) / WideTile::kA) * ((f + WideTile::kB - 1) / WideTile::kB) < 100;
+    if (small)
+      return small_out ? backward_tiles<T, SmallTile, SmallTile>(e, d, f, a, ws, s) : backward_tiles<T, SmallTile, WideTile>(e, d, f, a, ws, s);
+    return small_out ? backward_tiles<T, BigTile, SmallTile>(e, d, f, a, ws, s) : backward_tiles<T, BigTile, WideTile>(e, d, f, a, ws, s);
+  }
   Room room(ws);
   const Backward w = take_backward(room, e.n, d, f, a.rows, a.top_k);
   if (int err = launch_plan(e, a.ids, w.plan, 64, s)) return err;

@@ -145,9 +145,11 @@ int launch_few(const tsa_linear_args& a, hipStream_t stream) {
 
 template <class T, class W>
 int launch_few(const tsa_linear_args& a, hipStream_t stream) {
-  if (a.rows <= 16) return launch_few<T, W, 1, 1>(a, stream);
-  if (a.rows <= 32) return launch_few<T, W, 2, 2>(a, stream);
-  return launch_few<T, W, 2, 4>(a, stream);
+  if constexpr (std::is_same_v<W, RowsQ4<T>>) {
+    if (a.rows > 32) return launch_few<T, W, 2, 4>(a, stream);
+    if (a.rows > 16) return launch_few<T, W, 2, 2>(a, stream);
+  }
+  return launch_few<T, W, 1, 1>(a, stream);
 }
 
 // Many rows: big tiles, two workgroups a CU: one's products run under the other's epilogue. (Tiles of 256 x 256, one a CU,
@@ -230,13 +232,18 @@ bool aligned16(const void* p, uint64_t stride) { return reinterpret_cast<uintptr
 }  // namespace
 }  // namespace op
 
-constexpr uint32_t kFewRows = 64;  // up to here the weights are streamed, in tiles beyond
-
-// What a call with more rows packs first: x, the weights, neither or both.
+// Whether the weights are streamed. 4-bit ones up to 64 rows of x (17, 32 and 64 rows, 7168 x 2048: 45, 54 and 81 us, tiles 155 to
+// 172). 16-bit ones up to 16, of x's rows above 4 only where small tiles are too few to keep up: 17 rows, 4096 x 28672: 73 us
+// and 48 in tiles; 16 rows: 66 and 48, 7168 x 2048 19 and 27; 4 rows: 50 and 48.
 namespace {
-bool pack_x(const tsa_linear_args& a) { return a.rows > kFewRows && (a.n_in % 8 || !op::aligned16(a.x, a.x_stride)); }
+bool streamed(const tsa_linear_args& a) {
+  if (a.w_type == TSA_Q4) return a.rows <= 64;
+  return a.rows <= 4 || (a.rows <= 16 && (a.n_out < 16384 || a.n_in % 8 || !op::aligned16(a.x, a.x_stride) || !op::aligned16(a.w, a.w_stride)));
+}
+// What a call in tiles packs first: x, the weights, neither or both.
+bool pack_x(const tsa_linear_args& a) { return !streamed(a) && (a.n_in % 8 || !op::aligned16(a.x, a.x_stride)); }
 bool pack_w(const tsa_linear_args& a) {
-  return a.rows > kFewRows && a.w_type != TSA_Q4 && (a.n_in % 8 || !op::aligned16(a.w, a.w_stride));
+  return !streamed(a) && a.w_type != TSA_Q4 && (a.n_in % 8 || !op::aligned16(a.w, a.w_stride));
 }
 int pack(const void* from, uint64_t stride, uint32_t rows, uint32_t n, void* to, hipStream_t stream) {
   const uint32_t wide = uint32_t(up_to(n, 8));
@@ -257,7 +264,7 @@ int launch_linear(const tsa_linear_args& a0, void* workspace, hipStream_t stream
   const bool bf16 = a.x_type == TSA_BF16, q4 = a.w_type == TSA_Q4;
   if (a.rows == 1 && q4 && a.n_in % 256 == 0 && op::aligned16(a.w, 0) && op::aligned16(a.x, 0))
     return bf16 ? op::launch_q4<op::Bf16>(a, stream) : op::launch_q4<op::F16>(a, stream);
-  if (a.rows <= kFewRows) {
+  if (streamed(a)) {
     if (bf16) return q4 ? op::launch_few<op::Bf16, op::RowsQ4<op::Bf16>>(a, stream) : op::launch_few<op::Bf16, op::Rows16<op::Bf16>>(a, stream);
     return q4 ? op::launch_few<op::F16, op::RowsQ4<op::F16>>(a, stream) : op::launch_few<op::F16, op::Rows16<op::F16>>(a, stream);
   }
@@ -277,8 +284,11 @@ int launch_linear(const tsa_linear_args& a0, void* workspace, hipStream_t stream
   }
   a.n_in = wide;  // (packed rows end in zeros; unpacked ones are whole)
   if (q4) return bf16 ? op::launch_q4_tile<op::Bf16>(a, stream) : op::launch_q4_tile<op::F16>(a, stream);
-  if (getenv("TSA_M") && atoi(getenv("TSA_M")) == 1) return bf16 ? op::launch_tile<op::Bf16, op::WideTile>(a, stream) : op::launch_tile<op::F16, op::WideTile>(a, stream);
-  return bf16 ? op::launch_tile<op::Bf16, op::BigTile>(a, stream) : op::launch_tile<op::F16, op::BigTile>(a, stream);
+  // Few wide tiles leave each alone on its CU, waiting for its loads. Wide and small: 1000 rows, 4096 x 4096 (128 wide tiles) 91
+  // and 59 us, 256 rows, 4096 x 28672 (224) 129 and 135, 1000 rows, 4096 x 8192 (256) 104 and 126.
+  if (uint64_t((a.n_out + op::WideTile::kA - 1) / op::WideTile::kA) * ((a.rows + op::WideTile::kB - 1) / op::WideTile::kB) < 224)
+    return bf16 ? op::launch_tile<op::Bf16, op::SmallTile>(a, stream) : op::launch_tile<op::F16, op::SmallTile>(a, stream);
+  return bf16 ? op::launch_tile<op::Bf16, op::WideTile>(a, stream) : op::launch_tile<op::F16, op::WideTile>(a, stream);
 }
 
 }  // namespace tsa

@@ -83,32 +83,16 @@ __device__ __forceinline__ bool tile_of(const Plan& p, uint32_t na, TileRows& t,
   return tile_rows(p, at.b, S::kB, t);
 }
 
-// 4 values next to each other a lane, to rows of 16 bits or 32.
-template <class V>
-struct RowsOut {
+// 4 values next to each other a lane, to rows of 32 bits.
+struct FloatRows {
   struct Fetched {};
-  V* out;
+  float* out;
   uint64_t stride;
   uint32_t rows, c0, n_cols, c = 0;
   __device__ __forceinline__ void columns(uint32_t a) { c = c0 + a; }
   __device__ __forceinline__ Fetched fetch(uint32_t) const { return {}; }
-  template <class T>
-  __device__ __forceinline__ void put(uint32_t r, f32x4 v) const {
-    if (r >= rows || c >= n_cols) return;  // (columns are a multiple of 8: all four or none)
-    if constexpr (sizeof(V) == 4) {
-      *reinterpret_cast<f32x4*>(out + r * stride + c) = v;
-    } else {
-      bits4 o;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = T::down(v[i]);
-      *reinterpret_cast<bits4*>(out + r * stride + c) = o;
-    }
-  }
-};
-template <class T, class V>
-struct TypedOut : RowsOut<V> {
-  __device__ __forceinline__ void finish(uint32_t r, f32x4 v, const typename RowsOut<V>::Fetched&) const {
-    this->template put<T>(r, v);
+  __device__ __forceinline__ void finish(uint32_t r, f32x4 v, const Fetched&) const {
+    if (r < rows && c < n_cols) *reinterpret_cast<f32x4*>(out + r * stride + c) = v;  // (columns are a multiple of 8)
   }
 };
 
@@ -220,9 +204,16 @@ Plan take_plan(Room& r, uint32_t n, uint32_t pairs, uint32_t top_k, uint32_t row
 
 uint32_t blocks(uint64_t n) { return uint32_t(n < (1u << 20) ? n : (1u << 20)); }
 
-// Which tile the pairs' products take.
-#include <cstdlib>
-inline bool small_tiles(uint32_t rows, uint32_t top_k, uint32_t n) { const char* e = getenv("TSA_S"); return e && atoi(e); }
+// Which tile the pairs' products take. A big tile's workgroup alone on a CU waits for its loads: below about 150 of them (128
+// pairs by 192 columns, half a tile more for every expert) small ones are as fast or faster, above they read too much; and
+// with fewer than about 24 pairs an expert most of a big tile is empty. Big and small, forward: 600 rows, 2 of 8 experts of
+// 2048 x 1024 (147): 78 and 62 us; 1200 rows, 2048 x 2048 (253): 141 and 179; 400 rows of one expert of 4096 x 8192 (88): 241 and
+// 196; 8 of 128 experts of 2048 x 768, 32 rows: 160 and 146, 256: 284 and 269, 512: 298 and 308. Gradients: 300 rows of one
+// expert of 2048 x 2048 (33): 165 and 107 us; 2000 rows, 2048 x 4096 (176): 392 and 470.
+inline bool small_tiles(uint32_t rows, uint32_t top_k, uint32_t n, uint32_t d, uint32_t f) {
+  const uint64_t pairs = uint64_t(rows) * top_k, tiles = pairs / 128 + (n < pairs ? n + 1 : pairs + 1) / 2;
+  return pairs < uint64_t(24) * n || tiles * (((d < f ? d : f) + BigTile::kA - 1) / BigTile::kA) < 150;
+}
 
 template <class T>
 int launch_combine(const Plan& p, uint32_t rows, uint32_t d, const float* v, const float* weights, const void* residual,
