@@ -344,6 +344,20 @@ __global__ __launch_bounds__(kTileThreads, 2) void down_q4_tile_kernel(Plan p, c
 }
 
 // ---- launches ----
+template <class T, int kWide>
+__global__ __launch_bounds__(256) void combine_kernel(Combine c) {
+  combine<T, kWide>(c, blockIdx.x);
+}
+
+template <class T>
+int launch_combine(const Plan& p, uint32_t d, const float* v, const tsa_ffn_args& a, hipStream_t s) {
+  bool wide;
+  const Combine c = combine_of(p, a.rows, d, v, a.weights, a.residual, a.residual_stride, a.y, a.y_stride, wide);
+  if (wide) hipLaunchKernelGGL((combine_kernel<T, 4>), dim3(c.n_blocks), dim3(256), 0, s, c);
+  else hipLaunchKernelGGL((combine_kernel<T, 1>), dim3(c.n_blocks), dim3(256), 0, s, c);
+  return int(hipGetLastError());
+}
+
 struct Forward {
   Plan plan;
   u16* h;
@@ -392,7 +406,7 @@ int forward_few(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& 
   const uint32_t w2 = stream_waves(uint64_t(td) * tiles, chunks_of(f), most_waves(CT));
   hipLaunchKernelGGL((down_few_kernel<T, W, CT, kTail>), dim3(td, tiles), dim3(64 * w2), w2 * CT * 2048, s, w.plan, w.h, d, f,
                      w.out);
-  return launch_combine<T>(w.plan, a.rows, d, w.out, a.weights, a.residual, a.residual_stride, a.y, a.y_stride, s);
+  return launch_combine<T>(w.plan, d, w.out, a, s);
 }
 
 // 4-bit weights, few rows: up to so many pairs an expert (if all are asked for alike) as CT tiles of 16 hold.
@@ -426,7 +440,7 @@ int forward_tiles(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args
     hipLaunchKernelGGL((gate_up_tile_kernel<T, U>), up, dim3(kTileThreads), U::kLds, s, w.plan, x, a.x_stride, d, f, a.act, w.h);
     hipLaunchKernelGGL((down_tile_kernel<T, S>), down, dim3(kTileThreads), S::kLds, s, w.plan, w.h, d, f, w.out);
   }
-  return launch_combine<T>(w.plan, a.rows, d, w.out, a.weights, a.residual, a.residual_stride, a.y, a.y_stride, s);
+  return launch_combine<T>(w.plan, d, w.out, a, s);
 }
 
 template <class T, bool kQ4>
@@ -452,7 +466,7 @@ int forward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& a, v
   hipLaunchKernelGGL((gate_up_any_kernel<T, kQ4>), dim3(tiles * ((f + 63) / 64)), dim3(256), 0, s, w.plan,
                      static_cast<const u16*>(a.x), a.x_stride, d, f, a.act, w.h);
   hipLaunchKernelGGL((down_any_kernel<T, kQ4>), dim3(tiles * ((d + 63) / 64)), dim3(256), 0, s, w.plan, w.h, d, f, w.out);
-  return launch_combine<T>(w.plan, a.rows, d, w.out, a.weights, a.residual, a.residual_stride, a.y, a.y_stride, s);
+  return launch_combine<T>(w.plan, d, w.out, a, s);
 }
 
 }  // namespace

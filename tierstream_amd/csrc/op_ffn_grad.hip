@@ -110,14 +110,28 @@ __global__ __launch_bounds__(256) void weight_grad_any_kernel(Plan p, const u16*
   }
 }
 
-__global__ __launch_bounds__(256) void weights_grad_kernel(Plan p, uint32_t shares, const float* d_share, float* dweights) {
-  for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < p.pairs; i += uint64_t(gridDim.x) * 256) {
+// d w of every pair: its shares, in their order.
+struct WeightShares {
+  uint32_t n = 0;
+  const float* share = nullptr;
+  float* dweights = nullptr;
+};
+__device__ __forceinline__ void weights_grad(const Plan& p, const WeightShares& w, uint32_t block, uint32_t n_blocks) {
+  for (uint64_t i = uint64_t(block) * 256 + threadIdx.x; i < p.pairs; i += uint64_t(n_blocks) * 256) {
     const int32_t at = p.at[i];
     float s = 0.0f;
     if (at >= 0)
-      for (uint32_t k = 0; k < shares; ++k) s += d_share[uint64_t(k) * p.pairs + uint32_t(at)];
-    dweights[i] = s;
+#pragma unroll 4
+      for (uint32_t k = 0; k < w.n; ++k) s += w.share[uint64_t(k) * p.pairs + uint32_t(at)];
+    w.dweights[i] = s;
   }
+}
+
+// dx by the first blocks, d w by the others: two sums that need nothing of each other.
+template <class T, int kWide>
+__global__ __launch_bounds__(256) void sums_kernel(Combine c, Plan p, WeightShares w) {
+  if (blockIdx.x < c.n_blocks) combine<T, kWide>(c, blockIdx.x);
+  else weights_grad(p, w, blockIdx.x - c.n_blocks, gridDim.x - c.n_blocks);
 }
 
 // back = down^T dy of every pair: in 32 bits, for the kernel behind it. (One kernel for all three products needs 192 accumulators
@@ -225,16 +239,14 @@ __global__ __launch_bounds__(kTileThreads, 2) void input_grad_tile_kernel(Plan p
 // pairs. One of the two is read through the rows' map (kMapLeft: left). Columns from n_right on belong to out2 (the
 // gradients of gate and up are one product).
 template <class T, class S, bool kMapLeft>
-__global__ __launch_bounds__(kTileThreads, 2) void weight_grad_tile_kernel(Plan p, const u16* left, uint64_t left_stride,
-                                                                           uint32_t n_left, const u16* right,
-                                                                           uint64_t right_stride, uint32_t n_right,
-                                                                           uint32_t n_outs, u16* out, u16* out2) {
-  extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
+__device__ __forceinline__ void weight_grad_tile(f32x4* memory, uint32_t block, const Plan& p, const u16* left, uint64_t left_stride,
+                                                 uint32_t n_left, const u16* right, uint64_t right_stride, uint32_t n_right,
+                                                 uint32_t n_outs, u16* out, u16* out2) {
   constexpr int NI = S::NI, MJ = S::MJ;
   uint32_t* map = reinterpret_cast<uint32_t*>(memory) + S::kLds / 4;
   const uint32_t wave = threadIdx.x >> 6;
   const uint32_t ta = (n_left + S::kA - 1) / S::kA, tb = (n_right + S::kB - 1) / S::kB, per = ta * tb * n_outs;
-  const uint32_t e = blockIdx.x / per, in = blockIdx.x % per;
+  const uint32_t e = block / per, in = block % per;
   const uint32_t a0 = in % ta * S::kA, which = in / ta / tb, b0 = in / ta % tb * S::kB;
   const uint32_t first = p.first[e], pairs = p.first[e + 1] - first;
   right += which * n_right;
@@ -264,6 +276,19 @@ __global__ __launch_bounds__(kTileThreads, 2) void weight_grad_tile_kernel(Plan 
                            n_left - a0);
 }
 
+// The gradients of gate and up by the first `n_up` workgroups, down's by the others.
+template <class T, class S>
+__global__ __launch_bounds__(kTileThreads, 2) void weight_grad_tile_kernel(Plan p, uint32_t n_up, const u16* x, uint64_t x_stride,
+                                                                           const u16* dy, uint64_t dy_stride, uint32_t d,
+                                                                           uint32_t f, const u16* dgu, const u16* wh, u16* dgate,
+                                                                           u16* dup, u16* ddown) {
+  extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
+  if (blockIdx.x < n_up)
+    weight_grad_tile<T, S, true>(memory, blockIdx.x, p, x, x_stride, d, dgu, uint64_t(2) * f, f, 2, dgate, dup);
+  else
+    weight_grad_tile<T, S, false>(memory, blockIdx.x - n_up, p, wh, f, f, dy, dy_stride, d, 1, ddown, nullptr);
+}
+
 // ---- launches ----
 struct Backward {
   Plan plan;
@@ -281,6 +306,22 @@ Backward take_backward(Room& r, uint32_t n, uint32_t d, uint32_t f, uint32_t row
   return w;
 }
 
+template <class T>
+int launch_sums(const Backward& w, const tsa_ffn_grad_args& a, uint32_t d, uint32_t shares, hipStream_t s) {
+  bool wide = true;
+  Combine c;
+  if (a.dx) c = combine_of(w.plan, a.rows, d, w.out, nullptr, nullptr, 0, a.dx, a.dx_stride, wide);
+  WeightShares g;
+  g.n = shares;
+  g.share = w.share;
+  g.dweights = a.dweights;
+  const uint32_t n = c.n_blocks + (a.dweights ? blocks((w.plan.pairs + 255) / 256) : 0);
+  if (n == 0) return 0;
+  if (wide) hipLaunchKernelGGL((sums_kernel<T, 4>), dim3(n), dim3(256), 0, s, c, w.plan, g);
+  else hipLaunchKernelGGL((sums_kernel<T, 1>), dim3(n), dim3(256), 0, s, c, w.plan, g);
+  return int(hipGetLastError());
+}
+
 template <class T, class S, class W>
 int backward_tiles(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_grad_args& a, void* ws, hipStream_t s) {
   Room room(ws);
@@ -295,20 +336,16 @@ int backward_tiles(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_gra
     hipLaunchKernelGGL((hidden_grad_tile_kernel<T, S>), dim3(tiles * shares), dim3(kTileThreads), S::kLds, s, w.plan, x, a.x_stride,
                        w.back, a.weights, d, f, a.act, w.dgu, w.wh, w.share);
   }
-  if (a.dx && tiles) {
+  if (a.dx && tiles)
     hipLaunchKernelGGL((input_grad_tile_kernel<T, S>), dim3(tiles * of(d, S::kA)), dim3(kTileThreads), S::kLds, s, w.plan, w.dgu, d, f,
                        w.out);
-    if (int err = launch_combine<T>(w.plan, a.rows, d, w.out, nullptr, nullptr, 0, a.dx, a.dx_stride, s)) return err;
-  }
-  if (a.dweights && tiles)
-    hipLaunchKernelGGL(weights_grad_kernel, dim3(blocks((w.plan.pairs + 255) / 256)), dim3(256), 0, s, w.plan, shares, w.share,
-                       a.dweights);
+  if (tiles)
+    if (int err = launch_sums<T>(w, a, d, shares, s)) return err;
   if (a.dgate) {
-    constexpr uint32_t kLds = W::kLds + 4 * kMapRing;
-    hipLaunchKernelGGL((weight_grad_tile_kernel<T, W, true>), dim3(e.n * of(d, W::kA) * of(f, W::kB) * 2), dim3(kTileThreads), kLds, s,
-                       w.plan, x, a.x_stride, d, w.dgu, uint64_t(2) * f, f, 2u, static_cast<u16*>(a.dgate), static_cast<u16*>(a.dup));
-    hipLaunchKernelGGL((weight_grad_tile_kernel<T, W, false>), dim3(e.n * of(f, W::kA) * of(d, W::kB)), dim3(kTileThreads), kLds, s,
-                       w.plan, w.wh, uint64_t(f), f, dy, a.dy_stride, d, 1u, static_cast<u16*>(a.ddown), static_cast<u16*>(nullptr));
+    const uint32_t n_up = e.n * of(d, W::kA) * of(f, W::kB) * 2, n_down = e.n * of(f, W::kA) * of(d, W::kB);
+    hipLaunchKernelGGL((weight_grad_tile_kernel<T, W>), dim3(n_up + n_down), dim3(kTileThreads), W::kLds + 4 * kMapRing, s, w.plan, n_up,
+                       x, a.x_stride, dy, a.dy_stride, d, f, w.dgu, w.wh, static_cast<u16*>(a.dgate), static_cast<u16*>(a.dup),
+                       static_cast<u16*>(a.ddown));
   }
   return int(hipGetLastError());
 }
@@ -316,8 +353,7 @@ int backward_tiles(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_gra
 template <class T>
 int backward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_grad_args& a, void* ws, hipStream_t s) {
   if (wide_rows(e, d, f, false, a.x, a.x_stride) && aligned16(a.dy, 2 * a.dy_stride) && a.dy_stride < 1u << 24 && aligned16(a.dgate, 0) && aligned16(a.dup, 0) &&
-      aligned16(a.ddown, 0))
-  {
+      aligned16(a.ddown, 0)) {
     // The weights' gradients choose by themselves: 4 experts of 512 x 1024 (64 wide tiles) 173 us in all with wide tiles and 141
     // with small ones, one of 2048 x 2048 (128) 107 and 112, 8 of 4096 x 2048 (2048) 337 and 480.
     const bool small = small_tiles(a.rows, a.top_k, e.n, d, f);
@@ -334,13 +370,10 @@ int backward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_grad_args
   if (tiles)
     hipLaunchKernelGGL((hidden_grad_any_kernel<T>), dim3(tiles * tf), dim3(256), 0, s, w.plan, x, a.x_stride, dy, a.dy_stride,
                        a.weights, d, f, a.act, w.dgu, w.wh, w.share);
-  if (a.dx && tiles) {
+  if (a.dx && tiles)
     hipLaunchKernelGGL((input_grad_any_kernel<T>), dim3(tiles * td), dim3(256), 0, s, w.plan, w.dgu, d, f, w.out);
-    if (int err = launch_combine<T>(w.plan, a.rows, d, w.out, nullptr, nullptr, 0, a.dx, a.dx_stride, s)) return err;
-  }
-  if (a.dweights && tiles)
-    hipLaunchKernelGGL(weights_grad_kernel, dim3(blocks((w.plan.pairs + 255) / 256)), dim3(256), 0, s, w.plan, tf, w.share,
-                       a.dweights);
+  if (tiles)
+    if (int err = launch_sums<T>(w, a, d, tf, s)) return err;
   if (a.dgate) {
     const uint32_t g = blocks(uint64_t(e.n) * tf * td);
     for (int half = 0; half < 2; ++half)

@@ -117,13 +117,26 @@ __device__ __forceinline__ TileRowsSource<MJ> sorted_rows(const TileRows& t, con
 }
 
 // out_t = residual_t + sum_j w_tj v_{at(t, j)}, in the order of j; kWide columns a thread (a multiple of 4: one access each).
+// By blocks first.. of `n_blocks` of 256 threads.
+struct Combine {
+  Plan p;
+  uint32_t rows = 0, d = 0, n_blocks = 0;
+  const float *v = nullptr, *weights = nullptr;
+  const u16* residual = nullptr;
+  uint64_t residual_stride = 0;
+  u16* out = nullptr;
+  uint64_t out_stride = 0;
+};
 template <class T, int kWide>
-__global__ __launch_bounds__(256) void combine_kernel(Plan p, uint32_t rows, uint32_t d, const float* v, const float* weights,
-                                                      const u16* residual, uint64_t residual_stride, u16* out,
-                                                      uint64_t out_stride) {
-  const uint32_t per = d / kWide;
-  const uint64_t total = uint64_t(rows) * per;
-  for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += uint64_t(gridDim.x) * 256) {
+__device__ __forceinline__ void combine(const Combine& a, uint32_t block) {
+  const Plan& p = a.p;
+  const float *v = a.v, *weights = a.weights;
+  const u16* residual = a.residual;
+  u16* out = a.out;
+  const uint64_t residual_stride = a.residual_stride, out_stride = a.out_stride;
+  const uint32_t d = a.d, per = d / kWide;
+  const uint64_t total = uint64_t(a.rows) * per;
+  for (uint64_t i = uint64_t(block) * 256 + threadIdx.x; i < total; i += uint64_t(a.n_blocks) * 256) {
     const uint32_t row = uint32_t(i / per), c = uint32_t(i % per) * kWide;
     float s[kWide];
     if constexpr (kWide == 4) {
@@ -215,19 +228,23 @@ inline bool small_tiles(uint32_t rows, uint32_t top_k, uint32_t n, uint32_t d, u
   return pairs < uint64_t(24) * n || tiles * (((d < f ? d : f) + BigTile::kA - 1) / BigTile::kA) < 150;
 }
 
-template <class T>
-int launch_combine(const Plan& p, uint32_t rows, uint32_t d, const float* v, const float* weights, const void* residual,
-                   uint64_t residual_stride, void* out, uint64_t out_stride, hipStream_t s) {
-  const u16* r = static_cast<const u16*>(residual);
-  u16* o = static_cast<u16*>(out);
+// The sum's arguments; wide: whether four columns a thread can be.
+inline Combine combine_of(const Plan& p, uint32_t rows, uint32_t d, const float* v, const float* weights, const void* residual,
+                          uint64_t residual_stride, void* out, uint64_t out_stride, bool& wide) {
   const uint64_t odd = reinterpret_cast<uintptr_t>(residual) | 2 * residual_stride | reinterpret_cast<uintptr_t>(out) | 2 * out_stride;
-  if (d % 4 == 0 && odd % 8 == 0)
-    hipLaunchKernelGGL((combine_kernel<T, 4>), dim3(blocks((uint64_t(rows) * d / 4 + 255) / 256)), dim3(256), 0, s, p, rows, d, v,
-                       weights, r, residual_stride, o, out_stride);
-  else
-    hipLaunchKernelGGL((combine_kernel<T, 1>), dim3(blocks((uint64_t(rows) * d + 255) / 256)), dim3(256), 0, s, p, rows, d, v,
-                       weights, r, residual_stride, o, out_stride);
-  return int(hipGetLastError());
+  wide = d % 4 == 0 && odd % 8 == 0;
+  Combine c;
+  c.p = p;
+  c.rows = rows;
+  c.d = d;
+  c.n_blocks = blocks((uint64_t(rows) * (wide ? d / 4 : d) + 255) / 256);
+  c.v = v;
+  c.weights = weights;
+  c.residual = static_cast<const u16*>(residual);
+  c.residual_stride = residual_stride;
+  c.out = static_cast<u16*>(out);
+  c.out_stride = out_stride;
+  return c;
 }
 
 bool aligned16(const void* p, uint64_t stride_bytes) { return (reinterpret_cast<uintptr_t>(p) | stride_bytes) % 16 == 0; }

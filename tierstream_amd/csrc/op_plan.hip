@@ -7,49 +7,59 @@ namespace {
 
 constexpr uint32_t kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
 
-// Sum of v over the threads before this one, and over all of them (kPlanThreads threads).
-__device__ __forceinline__ uint32_t scan(uint32_t v, uint32_t* buf, uint32_t* total) {
-  const uint32_t t = threadIdx.x;
-  buf[t] = v;
-  __syncthreads();
-  for (uint32_t s = 1; s < kPlanThreads; s <<= 1) {
-    const uint32_t o = t >= s ? buf[t - s] : 0;
-    __syncthreads();
-    buf[t] += o;
-    __syncthreads();
+constexpr int kBatch = 4;  // ids of so many times 64 pairs are loaded at once
+
+// Inclusive sum over a wave's lanes.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  const uint32_t lane = threadIdx.x & 63u;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const uint32_t o = __shfl_up(v, s, 64);
+    if (lane >= uint32_t(s)) v += o;
   }
-  const uint32_t r = buf[t] - v;
-  *total = buf[kPlanThreads - 1];
-  __syncthreads();
-  return r;
+  return v;
 }
 
 // Groups the pairs by expert, stably: each wave counts its stretch of pairs per expert, the counts are summed over
 // experts and waves, then each wave places its stretch 64 pairs at a time, a pair behind those of its expert in lower
-// lanes. `rows_per_tile` sorted positions of one expert make a tile.
+// lanes. `rows_per_tile` sorted positions of one expert make a tile. Bound by its latencies: the ids' (twice where a stretch is
+// longer than kBatch), three barriers, a slot's look-up: 256 pairs 5 us, 16384 10 us.
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(ExpertMap m, const int32_t* ids, Plan p, uint32_t rows_per_tile) {
-  extern __shared__ uint32_t lds[];
-  uint32_t* buf = lds;                    // [kPlanThreads]
-  uint32_t* count = lds + kPlanThreads;   // [kPlanWaves][n]
+  extern __shared__ uint32_t count[];  // [kPlanWaves][n]
+  __shared__ uint32_t totals[kPlanWaves][2];
   const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6, n = m.n;
+  const uint32_t stretch = (p.pairs + 64 * kPlanWaves - 1) / (64 * kPlanWaves);  // of 64 pairs, a wave
+  const uint32_t from = wave * stretch * 64 + lane;                              // (pairs are below 2^24)
+  uint32_t e[kBatch];
+  const auto load = [&](uint32_t i) {
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const uint32_t pair = from + (i + b) * 64;
+      e[b] = i + b < stretch && pair < p.pairs ? expert_of(m, ids, pair) : ~0u;
+    }
+  };
+  load(0);
   for (uint32_t i = t; i < kPlanWaves * n; i += kPlanThreads) count[i] = 0;
   __syncthreads();
-  const uint32_t stretch = ((p.pairs + kPlanThreads - 1) / kPlanThreads) * 64;
-  const uint64_t from = uint64_t(wave) * stretch;
-  for (uint32_t i = 0; i < stretch; i += 64) {
-    const uint64_t pair = from + i + lane;
-    if (pair >= p.pairs) break;
-    const uint32_t e = expert_of(m, ids, uint32_t(pair));
-    if (e != ~0u) atomicAdd(&count[wave * n + e], 1u);
+  for (uint32_t i = 0; i < stretch; i += kBatch) {
+    if (i) load(i);
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b)
+      if (e[b] != ~0u) atomicAdd(&count[wave * n + e[b]], 1u);
   }
   __syncthreads();
   uint32_t mine = 0;
   if (t < n)
     for (uint32_t w = 0; w < kPlanWaves; ++w) mine += count[w * n + t];
-  uint32_t all, tiles;
-  const uint32_t first = scan(mine, buf, &all);
+  const char* parts[3] = {};
+  if (mine) part_pointers(m, t, parts);
   const uint32_t n_tiles = (mine + rows_per_tile - 1) / rows_per_tile;
-  const uint32_t tile0 = scan(n_tiles, buf, &tiles);
+  uint32_t first = wave_scan(mine), tile = wave_scan(n_tiles);
+  if (lane == 63) totals[wave][0] = first, totals[wave][1] = tile;
+  __syncthreads();
+  first -= mine;
+  tile -= n_tiles;
+  for (uint32_t w = 0; w < wave; ++w) first += totals[w][0], tile += totals[w][1];
   if (t < n) {
     p.first[t] = first;
     uint32_t at = first;
@@ -58,43 +68,43 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(ExpertMap m, const i
       count[w * n + t] = at;
       at += c;
     }
-    if (mine) {
-      const char* q[3];
-      part_pointers(m, t, q);
-      for (int i = 0; i < 3; ++i) p.part[3 * t + i] = q[i];
-    }
     for (uint32_t i = 0; i < n_tiles; ++i) {
-      p.tile[2 * (tile0 + i)] = t;
-      p.tile[2 * (tile0 + i) + 1] = first + i * rows_per_tile;
+      p.tile[2 * (tile + i)] = t;
+      p.tile[2 * (tile + i) + 1] = first + i * rows_per_tile;
     }
-  }
-  if (t == 0) {
-    p.first[n] = all;
-    *p.n_tiles = tiles;
+    if (t == n - 1) {
+      p.first[n] = first + mine;
+      *p.n_tiles = tile + n_tiles;
+    }
+    if (mine)
+      for (int i = 0; i < 3; ++i) p.part[3 * t + i] = parts[i];
   }
   __syncthreads();
-  for (uint32_t i = 0; i < stretch; i += 64) {
-    const uint64_t pair = from + i + lane;
-    if (from + i >= p.pairs) break;
-    const bool on = pair < p.pairs;
-    const uint32_t e = on ? expert_of(m, ids, uint32_t(pair)) : ~0u;
-    uint64_t same = __ballot(e != ~0u);
-    for (uint32_t b = 0; b < 9; ++b) {  // (n <= 512)
-      const uint64_t set = __ballot((e >> b) & 1u);
-      same &= (e >> b) & 1u ? set : ~set;
+  if (stretch > kBatch) load(0);
+  for (uint32_t i = 0; i < stretch; i += kBatch) {
+    if (i) load(i);
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const uint32_t pair = from + (i + b) * 64;
+      if (i + b >= stretch || pair - lane >= p.pairs) break;
+      uint64_t same = __ballot(e[b] != ~0u);
+      for (uint32_t bit = 0; bit < 9; ++bit) {  // (n <= 512)
+        const uint64_t set = __ballot((e[b] >> bit) & 1u);
+        same &= (e[b] >> bit) & 1u ? set : ~set;
+      }
+      uint32_t at = 0;
+      if (e[b] != ~0u) {
+        at = __hip_atomic_load(&count[wave * n + e[b]], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) +
+             uint32_t(__popcll(same & ((1ull << lane) - 1)));
+        p.pair[at] = pair;
+        p.row[at] = pair / p.top_k;
+      }
+      __builtin_amdgcn_wave_barrier();
+      if (e[b] != ~0u && (same >> lane) == 1)  // the last lane of its expert
+        __hip_atomic_store(&count[wave * n + e[b]], at + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      __builtin_amdgcn_wave_barrier();
+      if (pair < p.pairs) p.at[pair] = e[b] != ~0u ? int32_t(at) : -1;
     }
-    uint32_t at = 0;
-    if (e != ~0u) {
-      at = __hip_atomic_load(&count[wave * n + e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) +
-           uint32_t(__popcll(same & ((1ull << lane) - 1)));
-      p.pair[at] = uint32_t(pair);
-      p.row[at] = uint32_t(pair) / p.top_k;
-    }
-    __builtin_amdgcn_wave_barrier();
-    if (e != ~0u && (same >> lane) == 1)  // the last lane of its expert
-      __hip_atomic_store(&count[wave * n + e], at + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-    __builtin_amdgcn_wave_barrier();
-    if (on) p.at[pair] = e != ~0u ? int32_t(at) : -1;
   }
 }
 
@@ -102,7 +112,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(ExpertMap m, const i
 }  // namespace op
 
 int launch_plan(const ExpertMap& e, const int32_t* ids, const Plan& p, uint32_t rows_per_tile, hipStream_t s) {
-  hipLaunchKernelGGL(op::plan_kernel, dim3(1), dim3(op::kPlanThreads), 4 * (op::kPlanThreads + op::kPlanWaves * e.n), s, e, ids, p,
+  hipLaunchKernelGGL(op::plan_kernel, dim3(1), dim3(op::kPlanThreads), 4 * op::kPlanWaves * e.n, s, e, ids, p,
                      rows_per_tile);
   return int(hipGetLastError());
 }
