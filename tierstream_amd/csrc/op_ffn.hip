@@ -292,30 +292,32 @@ __global__ __launch_bounds__(kTileThreads, 2) void down_tile_kernel(Plan p, cons
   hand_out<NI, MJ>(memory, acc, o);
 }
 
-// The two with 4-bit weights: 32 columns of gate and up, 64 of down a tile.
+// The two with 4-bit weights: 64 columns of gate and up, 128 of down a tile.
 template <class T>
 __global__ __launch_bounds__(kTileThreads, 2) void gate_up_q4_tile_kernel(Plan p, const u16* x, uint64_t x_stride, uint32_t d,
                                                                           uint32_t f, uint32_t act, u16* h) {
   extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
   TileRows t;
   uint32_t at;
-  if (!tile_of<MiddleTile>(p, (f + 31) / 32, t, at)) return;
+  if (!tile_of<WideTile>(p, (f + 63) / 64, t, at)) return;
   const char *gate = p.part[3 * t.e], *up = p.part[3 * t.e + 1];
-  TileQ4Source<T, 4> w(d, threadIdx.x >> 6 & 1u, [&](uint32_t r) {  // of each wave's 32 rows: 16 gate, 16 up
-    const uint32_t c = at * 32 + (r >> 5) * 16 + (r & 15u);
-    return reinterpret_cast<const unsigned char*>(r & 16u ? up : gate) + uint64_t(c < f ? c : f - 1) * (d / kQ4Block * kQ4Bytes);
+  TileQ4Source<T> w(d, threadIdx.x >> 6 & 1u, [&](uint32_t r) {  // of each wave's 64 rows: 32 gate, 32 up
+    const uint32_t c = at * 64 + (r >> 6) * 32 + (r & 31u);
+    return reinterpret_cast<const unsigned char*>(r & 32u ? up : gate) + uint64_t(c < f ? c : f - 1) * (d / kQ4Block * kQ4Bytes);
   });
   auto xs = mapped_rows<4>(t, x, x_stride, d);
-  f32x4 acc[4][4] = {};
-  tile_product<T, 4, 4, 4>(w, xs, d, lds_offset(memory), acc);
-  f32x4 v[1][4];
+  f32x4 acc[8][4] = {};
+  tile_product<T, 8, 4, 3>(w, xs, d, lds_offset(memory), acc);
+  f32x4 v[2][4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const f32x4 g = TileQ4Source<T, 4>::whole(acc[0][j], acc[2][j]), u = TileQ4Source<T, 4>::whole(acc[1][j], acc[3][j]);
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v[0][j][q] = activate(act, g[q]) * u[q];
-  }
-  hand_out_bits<T, 1, 4>(memory, v, h + uint64_t(t.first) * f + at * 32, f, t.rows, f - at * 32);
+    for (int j = 0; j < 4; ++j) {
+      const f32x4 g = TileQ4Source<T>::whole(acc[i][j], acc[i + 4][j]), u = TileQ4Source<T>::whole(acc[i + 2][j], acc[i + 6][j]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[i][j][q] = activate(act, g[q]) * u[q];
+    }
+  hand_out_bits<T, 2, 4>(memory, v, h + uint64_t(t.first) * f + at * 64, f, t.rows, f - at * 64);
 }
 
 template <class T>
@@ -323,22 +325,22 @@ __global__ __launch_bounds__(kTileThreads, 2) void down_q4_tile_kernel(Plan p, c
   extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
   TileRows t;
   uint32_t at;
-  if (!tile_of<MiddleTile>(p, (d + 63) / 64, t, at)) return;
+  if (!tile_of<WideTile>(p, (d + 127) / 128, t, at)) return;
   const unsigned char* down = reinterpret_cast<const unsigned char*>(p.part[3 * t.e + 2]);
-  TileQ4Source<T, 4> w(f, threadIdx.x >> 6 & 1u, [&](uint32_t r) {
-    const uint32_t c = at * 64 + r;
+  TileQ4Source<T> w(f, threadIdx.x >> 6 & 1u, [&](uint32_t r) {
+    const uint32_t c = at * 128 + r;
     return down + uint64_t(c < d ? c : d - 1) * (f / kQ4Block * kQ4Bytes);
   });
   auto hs = sorted_rows<4>(t, h, f, f);
-  f32x4 acc[4][4] = {};
-  tile_product<T, 4, 4, 4>(w, hs, f, lds_offset(memory), acc);
-  f32x4 v[2][4];
+  f32x4 acc[8][4] = {};
+  tile_product<T, 8, 4, 3>(w, hs, f, lds_offset(memory), acc);
+  f32x4 v[4][4];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[i][j] = TileQ4Source<T, 4>::whole(acc[i][j], acc[i + 2][j]);
-  FloatRows o{out + uint64_t(t.first) * d, d, t.rows, at * 64, d};
-  hand_out<2, 4>(memory, v, o);
+    for (int j = 0; j < 4; ++j) v[i][j] = TileQ4Source<T>::whole(acc[i][j], acc[i + 4][j]);
+  FloatRows o{out + uint64_t(t.first) * d, d, t.rows, at * 128, d};
+  hand_out<4, 4>(memory, v, o);
 }
 
 // ---- launches ----
@@ -425,14 +427,17 @@ int forward_tiles(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args
   const Forward w = take_forward(room, e.n, d, f, a.rows, a.top_k);
   if (int err = launch_plan(e, a.ids, w.plan, S::kB, s)) return err;
   const uint32_t tiles = most_tiles(w.plan.pairs, e.n, S::kB);
-  constexpr uint32_t kF = kQ4 ? S::kA / 4 : S::kA / 2, kD = kQ4 ? S::kA / 2 : S::kA;  // columns a tile
+  // Gate and up as wide as they come, 1850 us in a prompt of 4001 rows where 192 rows a tile take 1955; down, whose sums are longer
+  // and whose tiles are fewer, 192 rows: 1093 us, 1240.
+  typedef std::conditional_t<std::is_same_v<S, BigTile>, WideTile, S> U;
+  constexpr uint32_t kF = kQ4 ? U::kA / 4 : U::kA / 2, kD = kQ4 ? S::kA / 2 : S::kA;  // columns a tile
   const dim3 up(tiles * ((f + kF - 1) / kF)), down(tiles * ((d + kD - 1) / kD));
   const u16* x = static_cast<const u16*>(a.x);
   if constexpr (kQ4) {
     hipLaunchKernelGGL((gate_up_q4_tile_kernel<T>), up, dim3(kTileThreads), S::kLds, s, w.plan, x, a.x_stride, d, f, a.act, w.h);
     hipLaunchKernelGGL((down_q4_tile_kernel<T>), down, dim3(kTileThreads), S::kLds, s, w.plan, w.h, d, f, w.out);
   } else {
-    hipLaunchKernelGGL((gate_up_tile_kernel<T, S>), up, dim3(kTileThreads), S::kLds, s, w.plan, x, a.x_stride, d, f, a.act, w.h);
+    hipLaunchKernelGGL((gate_up_tile_kernel<T, U>), up, dim3(kTileThreads), U::kLds, s, w.plan, x, a.x_stride, d, f, a.act, w.h);
     hipLaunchKernelGGL((down_tile_kernel<T, S>), down, dim3(kTileThreads), S::kLds, s, w.plan, w.h, d, f, w.out);
   }
   return launch_combine<T>(w.plan, d, w.out, a, s);
@@ -452,7 +457,7 @@ int forward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& a, v
   if (wide_rows(e, d, f, kQ4, a.x, a.x_stride)) {
     if constexpr (!kQ4)
       if (small_tiles(a.rows, a.top_k, e.n, d, f)) return forward_tiles<T, false, SmallTile>(e, d, f, a, ws, s);
-    return forward_tiles<T, kQ4, std::conditional_t<kQ4, MiddleTile, BigTile>>(e, d, f, a, ws, s);
+    return forward_tiles<T, kQ4, std::conditional_t<kQ4, WideTile, BigTile>>(e, d, f, a, ws, s);
   }
   Room room(ws);
   const Forward w = take_forward(room, e.n, d, f, a.rows, a.top_k);

@@ -357,10 +357,10 @@ int backward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_grad_args
     // The weights' gradients choose by themselves: 4 experts of 512 x 1024 (64 wide tiles) 173 us in all with wide tiles and 141
     // with small ones, one of 2048 x 2048 (128) 107 and 112, 8 of 4096 x 2048 (2048) 337 and 480.
     const bool small = small_tiles(a.rows, a.top_k, e.n, d, f);
-    const bool small_out = uint64_t(e.n) * ((d + MiddleTile::kA - 1) / MiddleTile::kA) * ((f + MiddleTile::kB - 1) / MiddleTile::kB) < 100;
+    const bool small_out = uint64_t(e.n) * ((d + WideTile::kA - 1) / WideTile::kA) * ((f + WideTile::kB - 1) / WideTile::kB) < 100;
     if (small)
-      return small_out ? backward_tiles<T, SmallTile, SmallTile>(e, d, f, a, ws, s) : backward_tiles<T, SmallTile, MiddleTile>(e, d, f, a, ws, s);
-    return small_out ? backward_tiles<T, BigTile, SmallTile>(e, d, f, a, ws, s) : backward_tiles<T, BigTile, MiddleTile>(e, d, f, a, ws, s);
+      return small_out ? backward_tiles<T, SmallTile, SmallTile>(e, d, f, a, ws, s) : backward_tiles<T, SmallTile, WideTile>(e, d, f, a, ws, s);
+    return small_out ? backward_tiles<T, BigTile, SmallTile>(e, d, f, a, ws, s) : backward_tiles<T, BigTile, WideTile>(e, d, f, a, ws, s);
   }
   Room room(ws);
   const Backward w = take_backward(room, e.n, d, f, a.rows, a.top_k);

@@ -183,14 +183,14 @@ int launch_tile(const tsa_linear_args& a, hipStream_t stream) {
   return int(hipGetLastError());
 }
 
-// The same with 4-bit weights, 64 rows of them a tile.
+// The same with 4-bit weights, 128 rows of them a tile.
 template <class T>
 __global__ __launch_bounds__(kTileThreads, 2) void linear_q4_tile_kernel(tsa_linear_args a) {
-  extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
+  extern __shared__ f32x4 memory[];
   const uint32_t wave = threadIdx.x >> 6;
-  const TileAt t = tile_at(blockIdx.x, (a.n_out + 63) / 64, (a.rows + 127) / 128);
-  const uint32_t n0 = t.a * 64, r0 = t.b * 128;
-  TileQ4Source<T, 4> w(a.n_in, wave & 1u, [&](uint32_t r) {
+  const TileAt t = tile_at(blockIdx.x, (a.n_out + 127) / 128, (a.rows + 127) / 128);
+  const uint32_t n0 = t.a * 128, r0 = t.b * 128;
+  TileQ4Source<T> w(a.n_in, wave & 1u, [&](uint32_t r) {
     const uint32_t n = n0 + r;
     return static_cast<const unsigned char*>(a.w) + uint64_t(n < a.n_out ? n : a.n_out - 1) * (a.n_in / kQ4Block * kQ4Bytes);
   });
@@ -198,21 +198,21 @@ __global__ __launch_bounds__(kTileThreads, 2) void linear_q4_tile_kernel(tsa_lin
     const uint32_t row = r0 + r;
     return static_cast<const u16*>(a.x) + (row < a.rows ? row : a.rows - 1) * a.x_stride;
   });
-  f32x4 acc[4][4] = {};
-  tile_product<T, 4, 4, 4>(w, x, a.n_in, lds_offset(memory), acc);
-  f32x4 v[2][4];
+  f32x4 acc[8][4] = {};
+  tile_product<T, 8, 4, 3>(w, x, a.n_in, lds_offset(memory), acc);
+  f32x4 v[4][4];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[i][j] = TileQ4Source<T, 4>::whole(acc[i][j], acc[i + 2][j]);
+    for (int j = 0; j < 4; ++j) v[i][j] = TileQ4Source<T>::whole(acc[i][j], acc[i + 4][j]);
   LinearOut<T> out(a, r0, n0);
-  hand_out<2, 4>(memory, v, out);
+  hand_out<4, 4>(memory, v, out);
 }
 
 template <class T>
 int launch_q4_tile(const tsa_linear_args& a, hipStream_t stream) {
-  const uint32_t tiles = (a.n_out + 63) / 64 * ((a.rows + 127) / 128);
-  hipLaunchKernelGGL((linear_q4_tile_kernel<T>), dim3(tiles), dim3(kTileThreads), MiddleTile::kLds, stream, a);
+  const uint32_t tiles = (a.n_out + 127) / 128 * ((a.rows + 127) / 128);
+  hipLaunchKernelGGL((linear_q4_tile_kernel<T>), dim3(tiles), dim3(kTileThreads), tile_lds(8, 4, 3), stream, a);
   return int(hipGetLastError());
 }
 
@@ -286,9 +286,9 @@ int launch_linear(const tsa_linear_args& a0, void* workspace, hipStream_t stream
   if (q4) return bf16 ? op::launch_q4_tile<op::Bf16>(a, stream) : op::launch_q4_tile<op::F16>(a, stream);
   // Few wide tiles leave each alone on its CU, waiting for its loads. Wide and small: 1000 rows, 4096 x 4096 (128 wide tiles) 91
   // and 59 us, 256 rows, 4096 x 28672 (224) 129 and 135, 1000 rows, 4096 x 8192 (256) 104 and 126.
-  if (uint64_t((a.n_out + op::BigTile::kA - 1) / op::BigTile::kA) * ((a.rows + op::BigTile::kB - 1) / op::BigTile::kB) < 224)
+  if (uint64_t((a.n_out + op::WideTile::kA - 1) / op::WideTile::kA) * ((a.rows + op::WideTile::kB - 1) / op::WideTile::kB) < 224)
     return bf16 ? op::launch_tile<op::Bf16, op::SmallTile>(a, stream) : op::launch_tile<op::F16, op::SmallTile>(a, stream);
-  return bf16 ? op::launch_tile<op::Bf16, op::BigTile>(a, stream) : op::launch_tile<op::F16, op::BigTile>(a, stream);
+  return bf16 ? op::launch_tile<op::Bf16, op::WideTile>(a, stream) : op::launch_tile<op::F16, op::WideTile>(a, stream);
 }
 
 }  // namespace tsa

@@ -1,17 +1,20 @@
-// Products with many rows: tiles of 32 NI rows of `a` times 32 MJ rows of `b`, by four waves (2 x 2, each 16 NI x 16 MJ) whose
-// accumulators stay in registers. Both operands go through LDS, two workgroups to a CU.
+// Products with many rows: tiles of 32 NI rows of `a` times 32 MJ rows of `b`, by four waves (2 x 2, each 16 NI x 16 MJ), one
+// to a SIMD, whose accumulators take half of its registers. Both operands go through LDS: a wave of 128 x 128 reads 32 KiB
+// there for 64 matrix instructions, half of what LDS gives in that time.
 //
-// A step is 32 values of the sum, a pair of steps the 64 of a cache line of every row. A pair's operands are loaded straight to
-// LDS (global_load_lds_dwordx4, NB / 2 buffers of a pair in turn) and from there, a step ahead, to a second set of registers.
-// The second step of a pair starts with the wait for the next pair's loads and the pair's one barrier, behind which every wave
-// has read its own pair, and loads the pair NB / 2 ahead over it.
+// A step is 32 values of the sum. Its operands are loaded straight to LDS (global_load_lds_dwordx4, NB buffers in turn) and
+// from there to a second set of registers while the step before is multiplied. Two steps, a cache line of every row, are
+// loaded together: by themselves each took the lines' halves from L2 again (a quarter of the time of a long product).
+// With 3 buffers, so that two workgroups of the big tile fit a CU, step t (even) loads t + 2 and t + 3, behind a barrier and
+// over t - 1 and t, whose reads every wave has done, and step t + 1 waits for them. With more, step t (odd) waits for steps
+// t + 1 and t + 2 and behind its barrier loads t + NB - 1 and t + NB over t - 1 and t.
 //
-// Operands come in two forms. Rows: the values of the sum lie next to each other; a pair's 128 bytes of a row are 8 pieces,
-// piece c at place c ^ (row mod 8), so that the lanes reading one piece of 16 rows hit all banks (c ^ (row / 4 mod 4) in rows of
-// 64 bytes: twice the cycles, 4.4e7 of conflicts in one long product). Columns (the operand is transposed in memory): 32
-// rows of the tile's columns a step, read with ds_read_b64_tr_b16, which gives each lane of 16 one column of 4 rows; pairs of
-// pieces are permuted by the row so that the 8 rows of a half wave hit all banks. In both, the permutation is made by the
-// loads' addresses: LDS itself is filled in lane order.
+// Operands come in two forms. Rows: the values of the sum lie next to each other; a row's 64 bytes a step are 4 pieces,
+// piece c at place c ^ (row / 2 mod 4), so that the lanes reading one piece of 16 rows hit all banks
+// (with row / 4 in its place the reads took twice the cycles: 4.4e7 of conflicts in one long product, now none). Columns (the operand
+// is transposed in memory): 32 rows of the tile's columns, read with ds_read_b64_tr_b16, which gives each lane of 16 one
+// column of 4 rows; pairs of pieces are permuted by the row so that the 8 rows of a half wave hit all banks. In both, the
+// permutation is made by the loads' addresses: LDS itself is filled in lane order.
 #pragma once
 
 #include "op_device.hpp"
@@ -25,6 +28,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4_t;
 typedef __attribute__((address_space(3))) const bits8 lds_bits8_t;
 
+__device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void wait_loads_and_meet() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
@@ -33,41 +37,45 @@ __device__ __forceinline__ void wait_loads_and_meet() {
 // An operand of 32 NF rows, in rows: at(r) gives row r's first value (any valid row for r behind the last).
 template <int NF>
 struct TileRowsSource {
-  static constexpr int kLoads = NF;  // of a pair, each thread: 8 rows of 128 bytes each
+  static constexpr int kLoads = NF / 2;
   const u16* p[kLoads];
   uint32_t k, n, mine;
-  uint32_t frag;  // this lane's place of its wave's first fragment, first step
+  uint32_t frag;  // this lane's place of its wave's first fragment
 
   template <class At>
   __device__ __forceinline__ TileRowsSource(uint32_t n_, uint32_t half, At&& at) : n(n_) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     mine = __builtin_amdgcn_readfirstlane(wave) * kLoads * 1024;
-    k = ((lane & 7u) ^ (lane >> 3)) * 8;
+    k = ((lane & 3u) ^ ((lane >> 3) & 3u)) * 8;
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) p[j] = at((wave * kLoads + j) * 8 + lane / 8) + k;
-    frag = (half * NF * 16 + (lane & 15u)) * 128 + ((lane >> 4) ^ (lane & 7u)) * 16;
+    for (int j = 0; j < kLoads; ++j) p[j] = at((wave * kLoads + j) * 16 + lane / 4) + k;
+    frag = (half * NF * 16 + (lane & 15u)) * 64 + (((lane >> 4) ^ ((lane >> 1) & 3u)) * 16);
   }
-  // Load j of the next pair (kCheck: the sum may end inside it); then, after all of them, on to the one behind.
+  // Load j of the next two steps (kCheck: the sum may end inside them); then, after all of them, on to the two behind.
   template <bool kCheck>
-  __device__ __forceinline__ void issue(int j, uint32_t lds) {
-    load_to_lds(!kCheck || k < n ? static_cast<const void*>(p[j]) : &kZeroPiece, lds + mine + j * 1024);
+  __device__ __forceinline__ void issue(int j, uint32_t lds0, uint32_t lds1) {
+    if (kCheck) {
+      load_to_lds(k < n ? static_cast<const void*>(p[j]) : &kZeroPiece, lds0 + mine + j * 1024);
+      load_to_lds(k + 32 < n ? static_cast<const void*>(p[j] + 32) : &kZeroPiece, lds1 + mine + j * 1024);
+    } else {
+      load_to_lds(p[j], lds0 + mine + j * 1024);
+      load_to_lds(p[j] + 32, lds1 + mine + j * 1024);
+    }
     p[j] += 64;
   }
   __device__ __forceinline__ void advance() { k += 64; }
-  __device__ __forceinline__ void stage(uint32_t) {}
-  // Fragment i of step kStep of the pair at lds (a multiple of 2048 from LDS' 1024-byte aligned start).
-  template <int kStep>
+  __device__ __forceinline__ void stage(uint32_t, uint32_t) {}
   __device__ __forceinline__ bits8 read(uint32_t lds, int i) const {
-    return *reinterpret_cast<lds_bits8_t*>(((lds + frag) ^ (64u * kStep)) + i * 2048);
+    return *reinterpret_cast<lds_bits8_t*>(lds + frag + i * 1024);
   }
 };
 
-// Rows of 4-bit blocks: 16 NI weight rows as 32 NI rows of the tile, 8 NI of each wave's half the values' leading 16 bits and 8 NI
+// Rows of 4-bit blocks: 128 weight rows as 256 rows of the tile, 64 of each wave's half the values' leading 16 bits and 64
 // what is left of them. A value (q - 8) s has 15 bits, so both together are exact: bf16 takes the value itself, half
 // precision an eighth of it (no scale overflows) and 2^12 times the rest (none underflows). whole() joins the two sums.
-// Each of the first 32 NI threads takes one block of a row every pair: from memory to registers a pair ahead, then to LDS in
-// the places where loads put rows.
-template <class T, int NI>
+// A thread takes one block of a row every two steps: from memory to registers two steps ahead, then to LDS in the places
+// where loads put rows.
+template <class T>
 struct TileQ4Source {
   static constexpr int kLoads = 0;
   static constexpr bool kHalf = std::is_same_v<T, F16>;
@@ -84,14 +92,12 @@ struct TileQ4Source {
   template <class At>
   __device__ __forceinline__ TileQ4Source(uint32_t n_, uint32_t half, At&& at) : n(n_) {
     const uint32_t lane = threadIdx.x & 63u, r = threadIdx.x / 2, second = threadIdx.x & 1u;
-    const bool on = r < 16 * NI;
-    p = at(on ? r : 0) + second * kQ4Bytes;
+    p = at(r) + second * kQ4Bytes;
     k = second * kQ4Block;
-    if (!on) n = 0;  // (fetches zeros, stores nothing)
-    const uint32_t row = r / (8 * NI) * (16 * NI) + r % (8 * NI);
-    put = on ? row * 128 : ~0u;
-    turn = (4 * second) ^ (row & 7u);
-    frag = (half * NI * 16 + (lane & 15u)) * 128 + ((lane >> 4) ^ (lane & 7u)) * 16;
+    const uint32_t row = (r / 64) * 128 + r % 64;
+    put = row * 64;
+    turn = (row >> 1) & 3u;
+    frag = (half * 128 + (lane & 15u)) * 64 + (((lane >> 4) ^ ((lane >> 1) & 3u)) * 16);
     fetch();
   }
   __device__ __forceinline__ void fetch() {
@@ -106,12 +112,11 @@ struct TileQ4Source {
     k += 2 * kQ4Block;
   }
   template <bool kCheck>
-  __device__ __forceinline__ void issue(int, uint32_t) {}
+  __device__ __forceinline__ void issue(int, uint32_t, uint32_t) {}
   __device__ __forceinline__ void advance() {}
-  // The fetched blocks to a pair's buffer, and the next ones from memory.
-  __device__ __forceinline__ void stage(uint32_t lds) {
-    if (put != ~0u) {
-    const uint32_t to = lds + put;
+  // The fetched blocks to the buffers of their two steps, and the next ones from memory.
+  __device__ __forceinline__ void stage(uint32_t lds0, uint32_t lds1) {
+    const uint32_t to = (threadIdx.x & 1u ? lds1 : lds0) + put;
     const float s = F16::up(scale) * (kHalf ? 0.125f : 1.0f), s8 = -8.0f * s;
 #pragma unroll
     for (uint32_t c = 0; c < 4; ++c) {  // values 8 c..: bytes 8 (c mod 2).. of the block, low halves first
@@ -124,14 +129,12 @@ struct TileQ4Source {
         lo[i] = T::down((w - T::up(hi[i])) * (kHalf ? 4096.0f : 1.0f));
       }
       *reinterpret_cast<lds_put_t*>(to + ((c ^ turn) * 16)) = hi;
-      *reinterpret_cast<lds_put_t*>(to + 8 * NI * 128 + ((c ^ turn) * 16)) = lo;
-    }
+      *reinterpret_cast<lds_put_t*>(to + 64 * 64 + ((c ^ turn) * 16)) = lo;
     }
     fetch();
   }
-  template <int kStep>
   __device__ __forceinline__ bits8 read(uint32_t lds, int i) const {
-    return *reinterpret_cast<lds_bits8_t*>(((lds + frag) ^ (64u * kStep)) + i * 2048);
+    return *reinterpret_cast<lds_bits8_t*>(lds + frag + i * 1024);
   }
   static __device__ __forceinline__ f32x4 whole(f32x4 hi, f32x4 lo) {
     return kHalf ? (hi + lo * (1.0f / 4096)) * 8.0f : hi + lo;
@@ -161,11 +164,11 @@ constexpr uint32_t kMapRing = 2048;
 // first one's with the fragment's number in three bits that the permutation turns.
 template <int NF, bool kMap>
 struct TileColumnsSource {
-  static constexpr int kEach = NF / 2, kLoads = 2 * kEach;  // of a step and of a pair, each thread
-  static constexpr uint32_t kPieces = 4 * NF;                // 16-byte pieces of a row
+  static constexpr int kLoads = NF / 2;
+  static constexpr uint32_t kPieces = 4 * NF;  // 16-byte pieces of a row
   static constexpr bool kEven = (kPieces & (kPieces - 1)) == 0;  // rows of 256 bytes or a power of two of it; else of 128 more
   uint64_t base;
-  uint32_t offset[kEach];  // bytes: of the lane's column, and without a map of its row
+  uint32_t offset[kLoads];  // bytes: of the lane's column, and without a map of its row
   uint32_t stride, k, n, mine, frag[kEven ? 1 : NF];
   const uint32_t* map;
 
@@ -176,10 +179,10 @@ struct TileColumnsSource {
                                                uint32_t n_cols, const uint32_t* map_ = nullptr)
       : base(uniform(reinterpret_cast<uint64_t>(at))), stride(uint32_t(stride_) * 2), k(0), n(n_), map(map_) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    mine = __builtin_amdgcn_readfirstlane(wave) * kEach * 1024;
+    mine = __builtin_amdgcn_readfirstlane(wave) * kLoads * 1024;
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      const uint32_t i = (wave * kEach + j) * 64 + lane;
+    for (int j = 0; j < kLoads; ++j) {
+      const uint32_t i = (wave * kLoads + j) * 64 + lane;
       const uint32_t c = first + ((i % kPieces) ^ turn(i / kPieces)) * 8;
       offset[j] = (c < n_cols ? c : n_cols - 8) * 2 + (kMap ? 0 : i / kPieces * stride);
     }
@@ -191,29 +194,30 @@ struct TileColumnsSource {
   __device__ __forceinline__ uint32_t row_of(int j) const {  // of the lane's piece, in its step
     return (mine + j * 1024 + (threadIdx.x & 63u) * 16) / (kPieces * 16);
   }
-  // Load j of the next pair, as TileRowsSource's: of its first step the even ones.
+  // Load j of the next two steps, as TileRowsSource's.
   template <bool kCheck>
-  __device__ __forceinline__ void issue(int j, uint32_t lds) {
-    const uint32_t s = j & 1, to = lds + s * (NF * 2048) + mine + j / 2 * 1024;
-    if constexpr (kMap || kCheck) {
-      const uint32_t row = k + 32 * s + row_of(j / 2);
-      const bool in = !kCheck || row < n;
-      uint64_t g = base + offset[j / 2];
-      if constexpr (kMap) g += uint64_t(map[in ? row % kMapRing : 0]) * stride;
-      else g += uint64_t(32 * s) * stride;
-      load_to_lds(in ? reinterpret_cast<const void*>(g) : &kZeroPiece, to);
-    } else {
-      load_offset_to_lds(base + uint64_t(32 * s) * stride, offset[j / 2], to);
+  __device__ __forceinline__ void issue(int j, uint32_t lds0, uint32_t lds1) {
+#pragma unroll
+    for (uint32_t s = 0; s < 2; ++s) {
+      const uint32_t to = (s ? lds1 : lds0) + mine + j * 1024;
+      if constexpr (kMap || kCheck) {
+        const uint32_t row = k + 32 * s + row_of(j);
+        const bool in = !kCheck || row < n;
+        uint64_t g = base + offset[j];
+        if constexpr (kMap) g += uint64_t(map[in ? row % kMapRing : 0]) * stride;
+        else g += uint64_t(32 * s) * stride;
+        load_to_lds(in ? reinterpret_cast<const void*>(g) : &kZeroPiece, to);
+      } else {
+        load_offset_to_lds(base + uint64_t(32 * s) * stride, offset[j], to);
+      }
     }
   }
   __device__ __forceinline__ void advance() {
     k += 64;
     if (!kMap) base += uint64_t(64) * stride;
   }
-  __device__ __forceinline__ void stage(uint32_t) {}
-  template <int kStep>
+  __device__ __forceinline__ void stage(uint32_t, uint32_t) {}
   __device__ __forceinline__ bits8 read(uint32_t lds, int i) const {
-    lds += kStep * (NF * 2048);
     const uint32_t at = kEven ? (lds + frag[0]) ^ (32u * i) : lds + frag[kEven ? 0 : i];
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4_t*>(at));
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4_t*>(at + 4 * kPieces * 16));
@@ -229,8 +233,8 @@ struct TileShape {
   static constexpr int NI = NI_, MJ = MJ_, NB = NB_;
   static constexpr uint32_t kA = 32 * NI, kB = 32 * MJ, kLds = tile_lds(NI, MJ, NB);
 };
-typedef TileShape<6, 4, 4> BigTile;     // 80 KiB of LDS: two to a CU
-typedef TileShape<4, 4, 4> MiddleTile;  // 64 KiB
+typedef TileShape<6, 4, 4> BigTile;
+typedef TileShape<8, 4, 3> WideTile;
 typedef TileShape<2, 2, 8> SmallTile;
 
 // Every accumulator through an empty statement: what is written before it is not read, and what is read after it not
@@ -245,70 +249,85 @@ __device__ __forceinline__ void settle(f32x4 (&acc)[NI][MJ]) {
 
 // acc[i][j] += a's rows 16 i.. of this wave's half times b's rows 16 j.. of its half, over the sources' n values. Lane l
 // holds a-rows 4 (l / 16) + 0..3 and b-row l % 16 of each.
-// every_pair(k): behind the barrier of the pair at value k of the sum, when every wave has issued the loads of the NB / 2 pairs
-// from it on.
+// every_two(k): behind the barrier of each second step (3 buffers), when every wave has issued the loads of the values below
+// k + 64.
 struct Nothing {
   __device__ __forceinline__ void operator()(uint32_t) const {}
 };
 template <class T, int NI, int MJ, int NB, class A, class B, class F = Nothing>
-__device__ __forceinline__ void tile_product(A& a, B& b, uint32_t n, uint32_t lds, f32x4 (&acc)[NI][MJ], F&& every_pair = F{}) {
-  static_assert(NB >= 4 && NB % 2 == 0, "buffers of two steps");
-  using Zero = std::integral_constant<int, 0>;
-  using One = std::integral_constant<int, 1>;
-  constexpr int kPairs = NB / 2, kLoads = A::kLoads + B::kLoads;  // loads of a pair, each thread
-  constexpr uint32_t kA = NI * 4096, kPair = (NI + MJ) * 4096;
-  const auto issue = [&](auto check, int j, uint32_t to) {
-    if (j < A::kLoads) a.template issue<decltype(check)::value>(j, to);
-    else b.template issue<decltype(check)::value>(j - A::kLoads, to + kA);
+__device__ __forceinline__ void tile_product(A& a, B& b, uint32_t n, uint32_t lds, f32x4 (&acc)[NI][MJ], F&& every_two = F{}) {
+  static_assert(NB == 3 || (NB >= 4 && NB % 2 == 0), "buffers");
+  constexpr int kLoads = A::kLoads + B::kLoads;  // of a step, each thread
+  constexpr uint32_t kA = NI * 2048, kBuffer = (NI + MJ) * 2048;
+  const auto issue = [&](auto check, int j, uint32_t at0, uint32_t at1) {  // load j of two steps, of both operands
+    if (j < A::kLoads) a.template issue<decltype(check)::value>(j, at0, at1);
+    else b.template issue<decltype(check)::value>(j - A::kLoads, at0 + kA, at1 + kA);
   };
-  __syncthreads();  // the last product's reads are done
+  const auto issue_all = [&](uint32_t at0, uint32_t at1) {
 #pragma unroll
-  for (int i = 0; i < kPairs; ++i) {
-    a.stage(lds + i * kPair);
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) issue(std::true_type{}, j, lds + i * kPair);
+    for (int j = 0; j < kLoads; ++j) issue(std::true_type{}, j, at0, at1);
     a.advance();
     b.advance();
-  }
-  wait_loads_and_meet<(kPairs - 1) * kLoads>();
+  };
+  __syncthreads();  // the last product's reads are done
+  a.stage(lds, lds + kBuffer);
+  issue_all(lds, lds + kBuffer);
+#pragma unroll
+  for (int i = 2; i + 1 < NB; i += 2) issue_all(lds + i * kBuffer, lds + (i + 1) * kBuffer);
+  wait_loads_and_meet<NB == 3 ? 0 : (NB - 2) * kLoads>();
   bits8 fa[2][NI], fb[2][MJ];
 #pragma unroll
-  for (int i = 0; i < NI; ++i) fa[0][i] = a.template read<0>(lds, i);
+  for (int i = 0; i < NI; ++i) fa[0][i] = a.read(lds, i);
 #pragma unroll
-  for (int j = 0; j < MJ; ++j) fb[0][j] = b.template read<0>(lds + kA, j);
+  for (int j = 0; j < MJ; ++j) fb[0][j] = b.read(lds + kA, j);
   settle(acc);
   asm volatile("s_nop 7");
+  uint32_t at = 0;  // this step's buffer
+  const auto behind = [&](uint32_t steps) { return lds + (at + steps >= NB ? at + steps - NB : at + steps) * kBuffer; };
   // A step, product by product: a read of the next step's operands every kPer, the loads in between. Left to itself the
   // compiler puts the reads behind the last product, where nothing hides them.
-  const auto step = [&](auto now_, auto check, uint32_t from, uint32_t to) {
+  const auto step = [&](auto now_, auto loads, auto check) {
     constexpr int now = decltype(now_)::value, kFrags = NI + MJ, kPer = NI * MJ / kFrags;
+    const uint32_t from = behind(1);
+    const uint32_t to0 = NB == 3 ? behind(2) : behind(NB - 1), to1 = lds + at * kBuffer;
 #pragma unroll
     for (int x = 0; x < NI * MJ; ++x) {
       if (x % kPer == 0 && x / kPer < kFrags) {
         const int r = x / kPer;
-        if (r < MJ) fb[now ^ 1][r] = b.template read<now ^ 1>(from + kA, r);
-        else fa[now ^ 1][r - MJ] = a.template read<now ^ 1>(from, r - MJ);
-        if (now == 1 && r < kLoads) issue(check, r, to);
+        if (r < MJ) fb[now ^ 1][r] = b.read(from + kA, r);
+        else fa[now ^ 1][r - MJ] = a.read(from, r - MJ);
+        if (decltype(loads)::value && r % 2 == 0 && r / 2 < kLoads) issue(check, r / 2, to0, to1);
       }
       T::mfma_in_place(acc[x / MJ][x % MJ], fa[now][x / MJ], fb[now][x % MJ]);
       if (x % kPer == kPer - 1) __builtin_amdgcn_sched_barrier(0);
     }
+    if (decltype(loads)::value) {
+      a.advance();
+      b.advance();
+    }
+    at = at + 1 == NB ? 0 : at + 1;
   };
-  uint32_t at = 0, k = 0;  // this pair's buffer, its first value
-  const auto pair = [&](auto check) {
-    const uint32_t here = lds + at * kPair;
-    at = at + 1 == kPairs ? 0 : at + 1;
-    step(Zero{}, check, here, 0);
-    wait_loads_and_meet<(kPairs - 2) * kLoads>();
-    every_pair(k);
-    a.stage(here);
-    step(One{}, check, lds + at * kPair, here);
-    a.advance();
-    b.advance();
-    k += 64;
+  const auto two_steps = [&](auto check, uint32_t t) {
+    using Zero = std::integral_constant<int, 0>;
+    using One = std::integral_constant<int, 1>;
+    if (NB != 3) {
+      step(Zero{}, std::false_type{}, check);
+      wait_loads_and_meet<NB == 3 ? 0 : (NB - 4) * kLoads>();
+      every_two(t * 32);
+      step(One{}, std::true_type{}, check);
+    } else {
+      meet();
+      every_two(t * 32);
+      a.stage(behind(2), lds + at * kBuffer);
+      step(Zero{}, std::true_type{}, check);
+      wait_loads_and_meet<0>();
+      step(One{}, std::false_type{}, check);
+    }
   };
-  while (k + 64 * (kPairs + 1) <= n) pair(std::false_type{});  // (the pair that is loaded is whole)
-  while (k < n) pair(std::true_type{});                        // (steps past the end multiply zeros)
+  constexpr uint32_t kAhead = NB == 3 ? 4 : NB + 2;  // the last step that two steps from t on load, + 1
+  uint32_t t = 0;
+  for (; (t + kAhead) * 32 <= n; t += 2) two_steps(std::false_type{}, t);
+  for (; t * 32 < n; t += 2) two_steps(std::true_type{}, t);  // (steps past the end multiply zeros)
   // The loads past the end have landed, and the last results are written before anything reads them (18 wait states).
   asm volatile("s_waitcnt vmcnt(0)\n\ts_nop 15\n\ts_nop 3" ::: "memory");
   settle(acc);
