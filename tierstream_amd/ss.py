@@ -225,6 +225,10 @@ def _declare() -> C.CDLL:
         "tsa_test_score_profile_check": (st, [C.c_char_p, u64, C.POINTER(u32), u32, C.c_char_p, C.c_char_p, u32]),
         "ss_dg_get_device_view_sized": (st, [vp, C.POINTER(SsDgDeviceView), u32]),
         "ss_dg_gated_index": (C.c_int, [vp, C.c_int]),
+        "ss_dg_enqueue_begin": (st, [vp, vp]),
+        "ss_dg_enqueue_export": (st, [vp, C.c_int, vp, C.c_int, C.c_int, vp]),
+        "ss_dg_enqueue_wait": (st, [vp, C.c_int, vp]),
+        "ss_dg_enqueue_end": (st, [vp, vp]),
         "ss_dg_residency": (st, [vp, vp, u32, C.POINTER(u32)]),
         "ss_dg_set_clean_evict": (st, [vp, u32]),
         "ss_source_direct": (C.c_int, [vp, C.c_int]),
@@ -515,6 +519,25 @@ class Ctx:
         v = SsDgDeviceView()
         check(_declare().ss_dg_get_device_view_sized(self.h, C.byref(v), C.sizeof(v)))
         return v
+
+    # A device-gated token: begin(), the enqueued calls (or a graph that captured them), end().
+    def begin(self):
+        check(_declare().ss_begin(self.h, None, 0))
+
+    def end(self):
+        check(_declare().ss_end(self.h))
+
+    def dg_enqueue_begin(self, stream):
+        check(_declare().ss_dg_enqueue_begin(self.h, stream))
+
+    def dg_enqueue_export(self, g: int, ids_dev: int, n: int, stream, n_pred: int = 0):
+        check(_declare().ss_dg_enqueue_export(self.h, g, ids_dev, n, n_pred, stream))
+
+    def dg_enqueue_wait(self, g: int, stream):
+        check(_declare().ss_dg_enqueue_wait(self.h, g, stream))
+
+    def dg_enqueue_end(self, stream):
+        check(_declare().ss_dg_enqueue_end(self.h, stream))
 
     def verify_failures(self) -> int:
         return int(_declare().tsa_test_verify_failures(self.h))
