@@ -363,6 +363,19 @@ def test_ffn_without_ids(ops, rows):
     near(y, want)
 
 
+@pytest.mark.parametrize("rows,n,k,where", [(1025, 3, 2, "stacked"), (5003, 400, 7, "table"), (70001, 5, 2, "arena")])
+def test_ffn_many_pairs(ops, rows, n, k, where):
+    """Pairs for more than one workgroup to group: a few over one's share, a ragged last one, more than 64 shares."""
+    g = gen(n)
+    layer = Layer(ops, g, where, n, 64, 72, "bf16")
+    x = mat(g, rows, 64, "bf16")
+    ids, w = choices(g, rows, n, k)
+    t, y = guarded(rows, 64, "bf16")
+    ops.ffn(layer.e, x, y, ids=ids, weights=w, workspace=room(ops.ffn_workspace(layer.e, rows, k)), stream=stream())
+    near(y, ffn64(layer, x, ids, w, None, "silu"))
+    untouched(t, rows, 64)
+
+
 def test_ffn_absent_table_entries_and_empty_calls(ops):
     g = gen(1)
     layer = Layer(ops, g, "table", 4, 128, 96, "bf16")

@@ -37,7 +37,8 @@ struct Plan {
   int32_t* at = nullptr;           // [pairs]: pair -> sorted position, -1 where the id adds nothing
   uint32_t* tile = nullptr;        // [tiles][2]: expert, first sorted position
   uint32_t* n_tiles = nullptr;
-  uint32_t pairs = 0, top_k = 1, n = 0;
+  uint32_t* counts = nullptr;      // [groups][n]: an expert's pairs in each workgroup's stretch of pairs
+  uint32_t pairs = 0, top_k = 1, n = 0, groups = 1, stretch = 0;
 };
 
 int launch_route(const tsa_route_args& a, hipStream_t stream);

@@ -200,6 +200,9 @@ uint32_t most_tiles(uint32_t pairs, uint32_t n, uint32_t rows_per_tile) {
   return pairs / rows_per_tile + (n < pairs ? n : pairs);
 }
 
+// Pairs that one workgroup groups (a multiple of 1024); of more than 64 times as many, 64 share them.
+constexpr uint32_t kPlanOne = 2048;
+
 Plan take_plan(Room& r, uint32_t n, uint32_t pairs, uint32_t top_k, uint32_t rows_per_tile) {
   Plan p;
   p.part = r.take<const char*>(uint64_t(3) * n);
@@ -210,6 +213,10 @@ Plan take_plan(Room& r, uint32_t n, uint32_t pairs, uint32_t top_k, uint32_t row
   p.tile = r.take<uint32_t>(uint64_t(2) * most_tiles(pairs, n, rows_per_tile));
   p.n_tiles = r.take<uint32_t>(1);
   p.pairs = pairs;
+  p.stretch = pairs > kPlanOne ? kPlanOne : pairs;
+  if (pairs > 64 * kPlanOne) p.stretch = (pairs / 64 + kPlanOne) / 1024 * 1024;
+  p.groups = pairs > kPlanOne ? (pairs + p.stretch - 1) / p.stretch : 1;
+  p.counts = r.take<uint32_t>(p.groups > 1 ? uint64_t(p.groups) * n : 0);
   p.top_k = top_k;
   p.n = n;
   return p;

@@ -1,4 +1,4 @@
-// Groups the pairs of a call by expert (one workgroup: a call has at most 2^24 pairs, a decode step a few hundred).
+// Groups the pairs of a call by expert.
 #include "op_pairs.hpp"
 
 namespace tsa {
@@ -20,16 +20,32 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
   return v;
 }
 
+// Pairs of each expert in one workgroup's stretch of pairs, for the kernel below.
+__global__ __launch_bounds__(kPlanThreads) void count_kernel(ExpertMap m, const int32_t* ids, Plan p) {
+  extern __shared__ uint32_t count[];  // [n]
+  for (uint32_t i = threadIdx.x; i < m.n; i += kPlanThreads) count[i] = 0;
+  __syncthreads();
+  const uint32_t from = blockIdx.x * p.stretch, to = p.pairs - from < p.stretch ? p.pairs : from + p.stretch;
+  for (uint32_t pair = from + threadIdx.x; pair < to; pair += kPlanThreads) {
+    const uint32_t e = expert_of(m, ids, pair);
+    if (e != ~0u) atomicAdd(&count[e], 1u);
+  }
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < m.n; i += kPlanThreads) p.counts[blockIdx.x * m.n + i] = count[i];
+}
+
 // Groups the pairs by expert, stably: each wave counts its stretch of pairs per expert, the counts are summed over
 // experts and waves, then each wave places its stretch 64 pairs at a time, a pair behind those of its expert in lower
-// lanes. `rows_per_tile` sorted positions of one expert make a tile. Bound by its latencies: the ids' (twice where a stretch is
-// longer than kBatch), three barriers, a slot's look-up: 256 pairs 5 us, 16384 10 us.
+// lanes. `rows_per_tile` sorted positions of one expert make a tile. A few hundred pairs: bound by its latencies (the ids', three
+// barriers, a slot's look-up), 5 us. Many: by the instructions and scattered stores of a CU, so above kPlanOne pairs
+// every kPlanOne of them have a workgroup, which counts on those in front of it in p.counts and writes the places of
+// its own pairs, the first one also the experts' and the tiles' (16384 pairs: 13 us for both kernels, one workgroup 31).
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(ExpertMap m, const int32_t* ids, Plan p, uint32_t rows_per_tile) {
   extern __shared__ uint32_t count[];  // [kPlanWaves][n]
   __shared__ uint32_t totals[kPlanWaves][2];
   const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6, n = m.n;
-  const uint32_t stretch = (p.pairs + 64 * kPlanWaves - 1) / (64 * kPlanWaves);  // of 64 pairs, a wave
-  const uint32_t from = wave * stretch * 64 + lane;                              // (pairs are below 2^24)
+  const uint32_t stretch = (p.stretch + 64 * kPlanWaves - 1) / (64 * kPlanWaves);  // of 64 pairs, a wave
+  const uint32_t from = blockIdx.x * p.stretch + wave * stretch * 64 + lane;       // (pairs are below 2^24)
   uint32_t e[kBatch];
   const auto load = [&](uint32_t i) {
 #pragma unroll
@@ -51,8 +67,18 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(ExpertMap m, const i
   uint32_t mine = 0;
   if (t < n)
     for (uint32_t w = 0; w < kPlanWaves; ++w) mine += count[w * n + t];
+  uint32_t before = 0;  // of the workgroups in front
+  if (p.groups > 1 && t < n) {
+    mine = 0;
+#pragma unroll 8
+    for (uint32_t g = 0; g < p.groups; ++g) {
+      const uint32_t c = p.counts[g * n + t];
+      before += g < blockIdx.x ? c : 0;
+      mine += c;
+    }
+  }
   const char* parts[3] = {};
-  if (mine) part_pointers(m, t, parts);
+  if (mine && blockIdx.x == 0) part_pointers(m, t, parts);
   const uint32_t n_tiles = (mine + rows_per_tile - 1) / rows_per_tile;
   uint32_t first = wave_scan(mine), tile = wave_scan(n_tiles);
   if (lane == 63) totals[wave][0] = first, totals[wave][1] = tile;
@@ -61,13 +87,15 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(ExpertMap m, const i
   tile -= n_tiles;
   for (uint32_t w = 0; w < wave; ++w) first += totals[w][0], tile += totals[w][1];
   if (t < n) {
-    p.first[t] = first;
-    uint32_t at = first;
+    uint32_t at = first + before;
     for (uint32_t w = 0; w < kPlanWaves; ++w) {
       const uint32_t c = count[w * n + t];
       count[w * n + t] = at;
       at += c;
     }
+  }
+  if (t < n && blockIdx.x == 0) {
+    p.first[t] = first;
     for (uint32_t i = 0; i < n_tiles; ++i) {
       p.tile[2 * (tile + i)] = t;
       p.tile[2 * (tile + i) + 1] = first + i * rows_per_tile;
@@ -112,8 +140,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(ExpertMap m, const i
 }  // namespace op
 
 int launch_plan(const ExpertMap& e, const int32_t* ids, const Plan& p, uint32_t rows_per_tile, hipStream_t s) {
-  hipLaunchKernelGGL(op::plan_kernel, dim3(1), dim3(op::kPlanThreads), 4 * op::kPlanWaves * e.n, s, e, ids, p,
-                     rows_per_tile);
+  if (p.groups > 1) hipLaunchKernelGGL(op::count_kernel, dim3(p.groups), dim3(op::kPlanThreads), 4 * e.n, s, e, ids, p);
+  hipLaunchKernelGGL(op::plan_kernel, dim3(p.groups), dim3(op::kPlanThreads), 4 * op::kPlanWaves * e.n, s, e, ids, p, rows_per_tile);
   return int(hipGetLastError());
 }
 
