@@ -272,7 +272,7 @@ __device__ __forceinline__ void weight_grad_tile(f32x4* memory, uint32_t block, 
       tile_product<T, NI, MJ, S::NB>(l, r, pairs, lds_offset(memory), acc, refill);
     }
   }
-  hand_out_bits<T, NI, MJ>(memory, acc, (which ? out2 : out) + (uint64_t(e) * n_right + b0) * n_left + a0, n_left, n_right - b0,
+  hand_out_bits<T, NI, MJ, true>(memory, acc, (which ? out2 : out) + (uint64_t(e) * n_right + b0) * n_left + a0, n_left, n_right - b0,
                            n_left - a0);
 }
 

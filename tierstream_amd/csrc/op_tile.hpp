@@ -375,8 +375,9 @@ __device__ __forceinline__ void hand_out(void* memory, const f32x4 (&acc)[NI][MJ
 // A wave's part of a tile as 16-bit values to rows of `out`: through LDS as hand_out, 8 values a lane. out: the tile's first row
 // and column, 16-byte aligned; rows and columns there are (columns a multiple of 8). With 4 bytes a value in LDS and 8-byte
 // stores the weights' gradients of a training step of 128 experts took 535 us; straight from the registers (16 rows of 32 bytes
-// a store) 644.
-template <class T, int NI, int MJ>
+// a store) 644. kOnce: nothing that follows soon reads them, so they pass the caches by (1.2 GB of gradients: 492 and 461 us, and the
+// next call finds its inputs there: its first product 157 and 122).
+template <class T, int NI, int MJ, bool kOnce = false>
 __device__ __forceinline__ void hand_out_bits(void* memory, const f32x4 (&acc)[NI][MJ], u16* out, uint64_t stride, uint32_t rows,
                                               uint32_t cols) {
   constexpr uint32_t kPieces = 2 * NI, kRows = kPieces > 8 ? 4 : kPieces > 4 ? 8 : 64 / kPieces;  // pieces a row, rows at once
@@ -401,7 +402,10 @@ __device__ __forceinline__ void hand_out_bits(void* memory, const f32x4 (&acc)[N
 #pragma unroll 4
     for (uint32_t r0 = 0; r0 < 16 * MJ; r0 += kRows) {
       const uint32_t r = r0 + lane / kPieces, row = (wave >> 1) * 16 * MJ + r;
-      if (row < rows) *reinterpret_cast<bits8*>(out + row * stride + c) = mine[place(lane % kPieces, r)];
+      bits8* to = reinterpret_cast<bits8*>(out + row * stride + c);
+      if (row >= rows) continue;
+      if constexpr (kOnce) __builtin_nontemporal_store(mine[place(lane % kPieces, r)], to);
+      else *to = mine[place(lane % kPieces, r)];
     }
 }
 
