@@ -273,6 +273,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void gate_up_tile_kernel(Plan p, c
   hand_out_bits<T, NI / 2, MJ>(memory, v, h + uint64_t(t.first) * f + at * 16 * NI, f, t.rows, f - at * 16 * NI);
 }
 
+// (With small tiles, a step of 32 rows through 8 of 128 experts of 2048 x 768: gate and up 84 us, 5.1 TB/s of weights, down 48, 4.5;
+// with big ones a prompt of 4001 rows through 2 of 8 experts of 4096 x 14336: 1880 and 1060 us, 1000 and 890 TFLOP/s.)
 template <class T, class S>
 __global__ __launch_bounds__(kTileThreads, 2) void down_tile_kernel(Plan p, const u16* h, uint32_t d, uint32_t f, float* out) {
   extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];

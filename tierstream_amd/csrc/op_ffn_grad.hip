@@ -135,7 +135,9 @@ __global__ __launch_bounds__(256) void sums_kernel(Combine c, Plan p, WeightShar
 }
 
 // back = down^T dy of every pair: in 32 bits, for the kernel behind it. (One kernel for all three products needs 192 accumulators
-// a lane, so one workgroup a CU: 496 us in a training step of 128 experts, where the two take 340.)
+// a lane, so one workgroup a CU: 496 us in a training step of 128 experts of 2048 x 768 with 16384 pairs, where the two take 413:
+// 123 and 290. The input's gradient takes 237 there, the sums over pairs 27. All three products are bound by their loads, 2.8
+// to 3.4 TB/s of weights: leaving out the empty half of short tiles changes nothing, nor do tiles of half the rows.)
 template <class T, class S>
 __global__ __launch_bounds__(kTileThreads, 2) void back_tile_kernel(Plan p, const u16* dy, uint64_t dy_stride, uint32_t d,
                                                                     uint32_t f, float* back) {
@@ -237,7 +239,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void input_grad_tile_kernel(Plan p
 
 // As weight_grad_any_kernel, out[e][b][a]: a tile of columns a of `left` and b of `right` a workgroup, the sum over the expert's
 // pairs. One of the two is read through the rows' map (kMapLeft: left). Columns from n_right on belong to out2 (the
-// gradients of gate and up are one product).
+// gradients of gate and up are one product). 128 experts of 2048 x 768 (1.2 GB written): 454 us, 2.7 TB/s: a sum of 128 pairs is
+// 4 steps, so a tile is its first loads and its stores. Tiles of 128 x 128, three a CU: 523 for 492; an expert's on one XCD: 560.
 template <class T, class S, bool kMapLeft>
 __device__ __forceinline__ void weight_grad_tile(f32x4* memory, uint32_t block, const Plan& p, const u16* left, uint64_t left_stride,
                                                  uint32_t n_left, const u16* right, uint64_t right_stride, uint32_t n_right,
