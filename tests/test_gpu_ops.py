@@ -211,6 +211,14 @@ def test_linear(ops, rows, n_in, n_out, kind, weights):
         untouched(t, rows, n_out)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,n_in,n_out,weights", [(2050, 136, 3601, "same"), (1793, 72, 4096, "same"), (290, 96, 4096, "q4"),
+                                                     (449, 1056, 2501, "q4")])
+def test_linear_many_tiles(ops, rows, n_in, n_out, weights, kind):
+    """Enough tiles for the largest ones: ragged in both directions, short and long sums."""
+    test_linear(ops, rows, n_in, n_out, kind, weights)
+
+
 @pytest.mark.parametrize("pad,shift", [(0, 0), (1, 0), (3, 1), (8, 4), (0, 1)])
 @pytest.mark.parametrize("rows,n_in,n_out", [(1, 1, 1), (1, 129, 40), (5, 63, 17), (33, 515, 70), (64, 255, 33), (70, 1001, 65), (140, 264, 300)])
 def test_linear_any_alignment(ops, pad, shift, rows, n_in, n_out):
@@ -363,6 +371,14 @@ def test_ffn_without_ids(ops, rows):
     near(y, want)
 
 
+@pytest.mark.parametrize("rows,n,k,d,f,weights", [(2501, 3, 2, 768, 776, "same"), (1100, 1, 1, 1024, 1024, "q4"), (701, 3, 2, 992, 1056, "q4")])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("where", ["stacked", "arena"])
+def test_ffn_many_tiles(ops, rows, n, k, d, f, kind, weights, where):
+    """Enough tiles for the largest ones."""
+    test_ffn(ops, rows, n, k, d, f, kind, kind if weights == "same" else weights, where)
+
+
 @pytest.mark.parametrize("rows,n,k,where", [(1025, 3, 2, "stacked"), (5003, 400, 7, "table"), (70001, 5, 2, "arena")])
 def test_ffn_many_pairs(ops, rows, n, k, where):
     """Pairs for more than one workgroup to group: a few over one's share, a ragged last one, more than 64 shares."""
@@ -437,6 +453,12 @@ def test_ffn_backward(ops, rows, n, k, d, f, kind, where):
     dx2 = torch.empty((rows, d), dtype=dx.dtype, device="cuda")  # the input's alone: the same bits
     ops.ffn_backward(layer.e, x, dy, dx2, ids=ids, weights=w, act=act, workspace=ws.zero_(), stream=stream())
     assert torch.equal(dx, dx2)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_ffn_backward_many_tiles(ops, kind):
+    """Enough tiles for the largest ones, and sums over more pairs than one filling of a tile's map of rows holds."""
+    test_ffn_backward(ops, 3001, 2, 2, 1024, 1672, kind, "arena")
 
 
 def test_ffn_backward_odd_sizes_and_dense(ops):

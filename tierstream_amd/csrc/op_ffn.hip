@@ -411,6 +411,20 @@ int forward_few(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& 
   return launch_combine<T>(w.plan, d, w.out, a, s);
 }
 
+// Whether 4-bit weights are streamed: up to 24 pairs an expert; more where a product's workgroups, taken one after the other as in the
+// linear product (11 ns a value of the sum, 256 at a time), end before its tiles (25 ns, 512 at a time), with half a tile of
+// rows more for every expert. Streamed and in tiles: one expert of 4096 x 4096, 96 rows 136 and 212 us, 256 rows 272 and 213; 3 of
+// 2048 x 2048, 200 rows 82 and 117; 8 of 16 of 1024 x 2048, 64 rows (32 pairs each) 122 and 107.
+bool stream_few(uint32_t n, uint32_t d, uint32_t f, uint32_t rows, uint32_t top_k, bool tiles) {
+  const uint64_t pairs = uint64_t(rows) * top_k, short_tiles = (n + 1) / 2;
+  if (pairs <= uint64_t(tiles ? 24 : 64) * n) return true;
+  if (!tiles) return false;
+  const uint64_t r = pairs / 64 + short_tiles, t = pairs / 128 + short_tiles;
+  const auto turns = [](uint64_t groups, uint64_t at_once) { return double(groups > at_once ? groups : at_once) / double(at_once); };
+  return 11.0 * (turns(r * (f / 16), 256) * d + turns(r * (d / 32), 256) * f) <=
+         25.0 * (turns(t * ((f + 63) / 64), 512) * d + turns(t * ((d + 127) / 128), 512) * f);
+}
+
 // 4-bit weights, few rows: up to so many pairs an expert (if all are asked for alike) as CT tiles of 16 hold.
 template <class T, bool kTail>
 int forward_few_q4(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& a, void* ws, hipStream_t s) {
@@ -451,7 +465,7 @@ int forward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& a, v
   const bool tail = d % kChunk || f % kChunk;
   if constexpr (kQ4) {
     if (a.rows == 1 && d % 256 == 0 && f % 256 == 0 && aligned16(a.x, 0) && wide_weights(e)) return forward_one_q4<T>(e, d, f, a, ws, s);
-    if (a.rows > 1 && uint64_t(a.rows) * a.top_k <= uint64_t(64) * e.n)
+    if (a.rows > 1 && stream_few(e.n, d, f, a.rows, a.top_k, wide_rows(e, d, f, true, a.x, a.x_stride)))
       return tail ? forward_few_q4<T, true>(e, d, f, a, ws, s) : forward_few_q4<T, false>(e, d, f, a, ws, s);
   }
   // (Two rows of 16-bit weights and more are no slower in small tiles: 32 rows, 8 of 128 experts, 146 us and 156 streamed.)

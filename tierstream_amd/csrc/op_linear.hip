@@ -232,12 +232,19 @@ bool aligned16(const void* p, uint64_t stride) { return reinterpret_cast<uintptr
 }  // namespace
 }  // namespace op
 
-// Whether the weights are streamed. 4-bit ones up to 64 rows of x (17, 32 and 64 rows, 7168 x 2048: 45, 54 and 81 us, tiles 155 to
-// 172). 16-bit ones up to 16, of x's rows above 4 only where small tiles are too few to keep up: 17 rows, 4096 x 28672: 73 us
-// and 48 in tiles; 16 rows: 66 and 48, 7168 x 2048 19 and 27; 4 rows: 50 and 48.
+// Whether the weights are streamed. 16-bit ones up to 16 rows of x, above 4 only where small tiles are too few to keep up: 17 rows,
+// 4096 x 28672: 73 us and 48 in tiles; 16 rows: 66 and 48, 7168 x 2048 19 and 27; 4 rows: 50 and 48. 4-bit ones by what the
+// workgroups take one after the other: of 32 weight rows and 64 rows of x 11 ns a value of the sum (32 rows of x: 6), 256 of
+// them at a time; a tile, half of whose time is unpacking, 25 ns, 512 at a time. Streamed and in tiles: 128 rows, 7168 x 2048
+// (128 workgroups, 16 tiles) 81 and 178 us, 512 (512, 64) 152 and 178; 192 rows, 2048 x 7168 (672, 112) 69 and 60; 64 rows,
+// 4096 x 28672 (896, 224) 173 and 111, 17 rows 96 and 109.
 namespace {
 bool streamed(const tsa_linear_args& a) {
-  if (a.w_type == TSA_Q4) return a.rows <= 64;
+  if (a.w_type == TSA_Q4) {
+    const auto of = [](uint32_t n, uint32_t each) { return uint64_t(n + each - 1) / each; };
+    const uint64_t groups = of(a.n_out, 32) * of(a.rows, a.rows > 32 ? 64 : 32), tiles = of(a.n_out, 128) * of(a.rows, 128);
+    return a.rows <= 16 || (groups > 256 ? groups : 256) * (a.rows > 32 ? 10 : 6) <= (tiles > 512 ? tiles : 512) * 11;
+  }
   return a.rows <= 4 || (a.rows <= 16 && (a.n_out < 16384 || a.n_in % 8 || !op::aligned16(a.x, a.x_stride) || !op::aligned16(a.w, a.w_stride)));
 }
 // What a call in tiles packs first: x, the weights, neither or both.

@@ -1,4 +1,4 @@
-// Products of weights with few rows of x (at most 64): bound by the bytes of the weights, which cross memory once and go
+// Products of weights with few rows of x: bound by the bytes of the weights, which cross memory once and go
 // straight to registers in the layout the matrix instruction takes, without LDS.
 //
 // The result column of v_mfma_f32_16x16x32 (operand b) is a weight row, the result row (operand a) a row of x: lane l holds
