@@ -219,6 +219,12 @@ def test_linear_many_tiles(ops, rows, n_in, n_out, weights, kind):
     test_linear(ops, rows, n_in, n_out, kind, weights)
 
 
+@pytest.mark.parametrize("n_in", [32767, 32768, 32769, 40000])
+def test_linear_long_rows(ops, n_in):
+    """One row of x up to what is staged of it, and beyond."""
+    test_linear(ops, 1, n_in, 37, "bf16", "same")
+
+
 @pytest.mark.parametrize("pad,shift", [(0, 0), (1, 0), (3, 1), (8, 4), (0, 1)])
 @pytest.mark.parametrize("rows,n_in,n_out", [(1, 1, 1), (1, 129, 40), (5, 63, 17), (33, 515, 70), (64, 255, 33), (70, 1001, 65), (140, 264, 300)])
 def test_linear_any_alignment(ops, pad, shift, rows, n_in, n_out):
@@ -377,6 +383,12 @@ def test_ffn_without_ids(ops, rows):
 def test_ffn_many_tiles(ops, rows, n, k, d, f, kind, weights, where):
     """Enough tiles for the largest ones."""
     test_ffn(ops, rows, n, k, d, f, kind, kind if weights == "same" else weights, where)
+
+
+@pytest.mark.parametrize("n,k,d,f", [(4, 3, 72, 10880), (4, 3, 64, 10923), (4, 4, 128, 8192), (2, 1, 33000, 48)])
+def test_ffn_one_long_row(ops, n, k, d, f):
+    """One row whose x, or whose h of all experts, is as long as what is staged of it, or longer."""
+    test_ffn(ops, 1, n, k, d, f, "bf16", "bf16", "stacked")
 
 
 @pytest.mark.parametrize("rows,n,k,where", [(1025, 3, 2, "stacked"), (5003, 400, 7, "table"), (70001, 5, 2, "arena")])

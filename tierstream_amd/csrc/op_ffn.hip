@@ -58,7 +58,7 @@ __device__ __forceinline__ bool resolve(const ExpertMap& m, uint32_t e, const ch
 }
 
 // One row of x: pair j is blockIdx.y, h_j = w_j act(gate x) (up x) for 16 columns a workgroup.
-template <class T, class W, bool kTail>
+template <class T, class W, bool kTail, bool kStaged>
 __global__ __launch_bounds__(64 * most_waves(1)) void gate_up_one_kernel(ExpertMap m, const int32_t* ids, const float* weights,
                                                                          const u16* x, uint32_t d, uint32_t f, uint32_t act,
                                                                          u16* h) {
@@ -68,12 +68,23 @@ __global__ __launch_bounds__(64 * most_waves(1)) void gate_up_one_kernel(ExpertM
   if (!resolve(m, expert_of(m, ids, blockIdx.y), p)) return;
   const uint32_t c0 = blockIdx.x * 16 + (lane & 15u), col = c0 < f ? c0 : f - 1;
   f32x4 acc[2][1] = {};
-  stream_chunks<W, 2, 1, kTail>((d + kChunk - 1) / kChunk, wave, waves, [&](uint32_t c, W (&w)[2], const u16* (&row)[1]) {
+  const auto at = [&](uint32_t c, W (&w)[2]) {
     w[0] = W(p[0], d, col, d);
     w[1] = W(p[1], d, col, d);
-    row[0] = x;
     return c * kChunk;
-  }, acc);
+  };
+  if constexpr (kStaged) {
+    u16* xs = reinterpret_cast<u16*>(part + waves * 128);
+    stream_one<T, 2, kTail>((d + kChunk - 1) / kChunk, wave, waves, lds_offset(xs), at, [&] {
+      stage_row(xs, x, d);
+      __syncthreads();
+    }, acc);
+  } else {
+    stream_chunks<W, 2, 1, kTail>((d + kChunk - 1) / kChunk, wave, waves, [&](uint32_t c, W (&w)[2], const u16* (&row)[1]) {
+      row[0] = x;
+      return at(c, w);
+    }, acc);
+  }
   const f32x4 v[2] = {acc[0][0], acc[1][0]};
   join_waves<2>(part, v, wave, waves, [&](auto&& sum) {
     if (wave != 0) return;
@@ -104,7 +115,7 @@ __device__ __forceinline__ void find_live(const ExpertMap& m, const int32_t* ids
 }
 
 // y = residual + sum_j down_j h_j: one row over the chunks of all its experts.
-template <class T, class W, bool kTail>
+template <class T, class W, bool kTail, bool kStaged>
 __global__ __launch_bounds__(64 * most_waves(1)) void down_one_kernel(ExpertMap m, const int32_t* ids, uint32_t top_k,
                                                                       const u16* h, uint32_t d, uint32_t f,
                                                                       const u16* residual, u16* y) {
@@ -114,12 +125,24 @@ __global__ __launch_bounds__(64 * most_waves(1)) void down_one_kernel(ExpertMap 
   find_live(m, ids, top_k, 2, live);
   const uint32_t c0 = blockIdx.x * 16 + (lane & 15u), col = c0 < d ? c0 : d - 1, per = (f + kChunk - 1) / kChunk;
   f32x4 acc[1][1] = {};
-  stream_chunks<W, 1, 1, kTail>(live.n * per, wave, waves, [&](uint32_t c, W (&w)[1], const u16* (&row)[1]) {
-    const uint32_t j = c / per;
-    w[0] = W(live.part[j], f, col, f);
-    row[0] = h + uint64_t(live.from[j]) * f;
-    return (c - j * per) * kChunk;
-  }, acc);
+  if constexpr (kStaged) {
+    u16* xs = reinterpret_cast<u16*>(part + waves * 64);
+    stream_one<T, 1, kTail>(live.n * per, wave, waves, lds_offset(xs), [&](uint32_t c, W (&w)[1]) {
+      const uint32_t j = c / per;
+      w[0] = W(live.part[j], f, col, f);
+      return (c - j * per) * kChunk;
+    }, [&] {
+      for (uint32_t j = 0; j < live.n; ++j) stage_row(xs + j * per * kChunk, h + uint64_t(live.from[j]) * f, f);
+      __syncthreads();
+    }, acc);
+  } else {
+    stream_chunks<W, 1, 1, kTail>(live.n * per, wave, waves, [&](uint32_t c, W (&w)[1], const u16* (&row)[1]) {
+      const uint32_t j = c / per;
+      w[0] = W(live.part[j], f, col, f);
+      row[0] = h + uint64_t(live.from[j]) * f;
+      return (c - j * per) * kChunk;
+    }, acc);
+  }
   const f32x4 v[1] = {acc[0][0]};
   join_waves<1>(part, v, wave, waves, [&](auto&& sum) {
     if (wave != 0) return;
@@ -377,11 +400,21 @@ int forward_one(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_args& 
   u16* h = static_cast<u16*>(ws);
   const uint32_t tf = (f + 15) / 16, td = (d + 15) / 16;
   const uint32_t w1 = stream_waves(uint64_t(tf) * a.top_k, chunks_of(d), 16);
-  hipLaunchKernelGGL((gate_up_one_kernel<T, W, kTail>), dim3(tf, a.top_k), dim3(64 * w1), w1 * 2048, s, e, a.ids, a.weights,
-                     static_cast<const u16*>(a.x), d, f, a.act, h);
+  const auto up = [&](auto staged) {
+    hipLaunchKernelGGL((gate_up_one_kernel<T, W, kTail, decltype(staged)::value>), dim3(tf, a.top_k), dim3(64 * w1),
+                       w1 * 2048 + (staged ? staged_bytes(d) : 0), s, e, a.ids, a.weights, static_cast<const u16*>(a.x), d, f, a.act, h);
+  };
   const uint32_t w2 = stream_waves(td, uint64_t(chunks_of(f)) * a.top_k, 16);
-  hipLaunchKernelGGL((down_one_kernel<T, W, kTail>), dim3(td), dim3(64 * w2), w2 * 1024, s, e, a.ids, a.top_k, h, d, f,
-                     static_cast<const u16*>(a.residual), static_cast<u16*>(a.y));
+  const auto down = [&](auto staged) {
+    hipLaunchKernelGGL((down_one_kernel<T, W, kTail, decltype(staged)::value>), dim3(td), dim3(64 * w2),
+                       w2 * 1024 + (staged ? a.top_k * staged_bytes(f) : 0), s, e, a.ids, a.top_k, h, d, f,
+                       static_cast<const u16*>(a.residual), static_cast<u16*>(a.y));
+  };
+  constexpr std::bool_constant<std::is_same_v<W, Rows16<T>>> k16{};
+  if (k16 && staged_bytes(d) <= kStagedBytes) up(k16);
+  else up(std::false_type{});
+  if (k16 && a.top_k * staged_bytes(f) <= kStagedBytes) down(k16);
+  else down(std::false_type{});
   return int(hipGetLastError());
 }
 

@@ -71,6 +71,29 @@ struct LinearOut {
   }
 };
 
+// One row of 16-bit weights by 16 a workgroup, x in LDS.
+template <class T, bool kTail>
+__global__ __launch_bounds__(64 * most_waves(1)) void linear_one_kernel(tsa_linear_args a) {
+  extern __shared__ f32x4 part[];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const uint32_t n = blockIdx.x * 16 + (lane & 15u);
+  u16* xs = reinterpret_cast<u16*>(part + waves * 64);
+  f32x4 acc[1][1] = {};
+  stream_one<T, 1, kTail>((a.n_in + kChunk - 1) / kChunk, wave, waves, lds_offset(xs), [&](uint32_t c, Rows16<T> (&w)[1]) {
+    w[0] = Rows16<T>(a.w, a.w_stride, n < a.n_out ? n : a.n_out - 1, a.n_in);
+    return c * kChunk;
+  }, [&] {
+    stage_row(xs, static_cast<const u16*>(a.x), a.n_in);
+    __syncthreads();
+  }, acc);
+  const f32x4 v[1] = {acc[0][0]};
+  join_waves<1>(part, v, wave, waves, [&](auto&& sum) {
+    if (wave != 0) return;
+    const float s = sum(0)[0];
+    if (lane < 16 && n < a.n_out) finish_linear(a, 0, n, s);
+  });
+}
+
 // Few rows: a workgroup takes 16 R weight rows and 16 CT rows of x.
 template <class T, class W, int R, int CT, bool kTail>
 __global__ __launch_bounds__(64 * most_waves(CT)) void linear_few_kernel(tsa_linear_args a) {
@@ -148,6 +171,12 @@ int launch_few(const tsa_linear_args& a, hipStream_t stream) {
   if constexpr (std::is_same_v<W, RowsQ4<T>>) {
     if (a.rows > 32) return launch_few<T, W, 2, 4>(a, stream);
     if (a.rows > 16) return launch_few<T, W, 2, 2>(a, stream);
+  } else if (a.rows == 1 && staged_bytes(a.n_in) <= kStagedBytes) {
+    const uint32_t tn = (a.n_out + 15) / 16, waves = stream_waves(tn, chunks_of(a.n_in), most_waves(1));
+    const uint32_t lds = waves * 1024 + uint32_t(staged_bytes(a.n_in));
+    if (a.n_in % kChunk) hipLaunchKernelGGL((linear_one_kernel<T, true>), dim3(tn), dim3(64 * waves), lds, stream, a);
+    else hipLaunchKernelGGL((linear_one_kernel<T, false>), dim3(tn), dim3(64 * waves), lds, stream, a);
+    return int(hipGetLastError());
   }
   return launch_few<T, W, 1, 1>(a, stream);
 }

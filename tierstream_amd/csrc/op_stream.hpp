@@ -7,10 +7,10 @@
 // in one load: values 4 (l / 16) + 0..3 from their low halves, 16 more from their high ones.
 //
 // The waves of a workgroup take turns along the row in chunks of 128 values, each with the next chunk's loads in flight
-// while it multiplies this one's, and add up through LDS. x is read from the caches.
+// while it multiplies this one's, and add up through LDS. x is read from the caches, or if it is one row from LDS.
 //
-// One row through 4096 x 28672 (235 MB of 16-bit weights): 46 us, 5.1 TB/s; two experts of 4096 x 14336: gate and up (470 MB) 86 us,
-// 5.4 TB/s, down (235 MB) 53 us, 4.4. A lane keeps one row, so an instruction reads 64 bytes of each of 16; a second chunk in
+// One row through 4096 x 28672 (235 MB of 16-bit weights): 43 us, 5.5 TB/s; two experts of 4096 x 14336: gate and up (470 MB) 83 us,
+// 5.7 TB/s, down (235 MB) 49 us, 4.8. A lane keeps one row, so an instruction reads 64 bytes of each of 16; a second chunk in
 // flight, twice or half the waves, or another first chunk in every workgroup gives the same or up to 10 % less.
 #pragma once
 
@@ -205,6 +205,52 @@ __device__ __forceinline__ void stream_chunks(uint32_t n_chunks, uint32_t wave, 
   }
   multiply(now);
 }
+
+// The same for one row of x that lies in LDS from `row` on, chunk after chunk: stage() puts it there and meets the other waves,
+// behind the first chunk's loads. (From the caches a row of x is as many loads as one of weights: 46.5 us for 43.2, 4096 x 28672;
+// down of two experts of 14336 x 4096 53.4 for 48.8.)
+template <class T, int R, bool kTail, class At, class Stage>
+__device__ __forceinline__ void stream_one(uint32_t n_chunks, uint32_t wave, uint32_t waves, uint32_t row, At&& at, Stage&& stage, f32x4 (&acc)[R][1]) {
+  typedef Rows16<T> W;
+  struct Step {
+    typename W::Chunk c[R];
+    uint32_t x;
+  };
+  typedef __attribute__((address_space(3))) const bits8 lds_bits8_t;
+  auto load = [&](Step& b, uint32_t c) {
+    W w[R];
+    const uint32_t k = at(c, w);
+    b.x = row + c * (kChunk * 2);
+#pragma unroll
+    for (int r = 0; r < R; ++r) w[r].template load<kTail>(b.c[r], k);
+  };
+  auto multiply = [&](const Step& b) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const bits8 x[1] = {*reinterpret_cast<lds_bits8_t*>(b.x + (threadIdx.x & 48u) + 64 * s)};
+      W::template multiply<R, 1>(b.c, s, x, acc);
+    }
+  };
+  uint32_t c = wave;
+  Step now;
+  if (c < n_chunks) load(now, c);
+  stage();
+  if (c >= n_chunks) return;
+  for (; c + waves < n_chunks; c += waves) {
+    Step next;
+    load(next, c + waves);
+    multiply(now);
+    now = next;
+  }
+  multiply(now);
+}
+// A row of n values to LDS by all threads, zeros behind it up to whole chunks.
+__device__ __forceinline__ void stage_row(u16* to, const u16* row, uint32_t n) {
+  for (uint32_t i = threadIdx.x * 8; i < (n + kChunk - 1) / kChunk * kChunk; i += blockDim.x * 8)
+    *reinterpret_cast<bits8*>(to + i) = load_end(row + i, int(n) - int(i));
+}
+constexpr uint32_t kStagedBytes = 64 * 1024;  // of x, at most: two workgroups a CU
+inline uint64_t staged_bytes(uint32_t n) { return uint64_t(n + kChunk - 1) / kChunk * kChunk * 2; }
 
 // The waves' sums added in their order: part[wave][i][lane], i over the wave's V vectors; thread (wave, lane) calls
 // f(i, lane, sum) for i = wave, wave + waves, ... of `use` vectors.
