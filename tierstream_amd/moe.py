@@ -130,10 +130,13 @@ class Model:
 
 
 class Decoder:
-    """Tokens one at a time, the experts of `model` read from a device-gated context over its written source."""
+    """Tokens one at a time, the experts of `model` read from a device-gated context over its written source. The model may be
+    trained on: the decoder keeps the weights it was made with, as the source does (a step gives the model new tensors, and
+    the captured graph goes on reading these)."""
 
     def __init__(self, model: Model, desc_json: str):
-        self.model, s, shape = model, model.s, wl.dg_shape(model.workload())
+        s, shape = model.s, wl.dg_shape(model.workload())
+        self.embedding, self.w = model.embedding, {"head": model.w["head"], **{f"router{L}": model.w[f"router{L}"] for L in range(s.layers)}}
         self.desc, budget = ss.Desc(desc_json), ss.budget(**shape.budget)
         self.plan = ss.Plan(self.desc, budget)
         self.ctx = ss.Ctx(self.desc, budget, self.plan, ss.options(**shape.options, verify_hash=2, dg_wait_timeout_ms=5000))
@@ -145,8 +148,8 @@ class Decoder:
         self.weights = _empty(1, s.top_k, dtype=torch.float32)
         self.logits = _empty(1, s.vocab, dtype=torch.float32)
         self.room = _workspace(max(ops.ffn_workspace(self.experts[0], 1, s.top_k),
-                                   ops.linear_workspace(self.x[0], model.w["head"], self.logits),
-                                   ops.linear_workspace(self.x[0], model.w["router0"], self.scores)))
+                                   ops.linear_workspace(self.x[0], self.w["head"], self.logits),
+                                   ops.linear_workspace(self.x[0], self.w["router0"], self.scores)))
         self.stream, self.graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
         torch.cuda.synchronize()
         # (the library's threads go on with their own calls while this one captures)
@@ -154,12 +157,12 @@ class Decoder:
             self._enqueue(torch.cuda.current_stream().cuda_stream)
 
     def _enqueue(self, h):
-        w, x = self.model.w, self.x
+        w, x = self.w, self.x
         self.ctx.dg_enqueue_begin(h)
         for L, e in enumerate(self.experts):
             ops.linear(x[L], w[f"router{L}"], self.scores, workspace=self.room, stream=h)
             ops.route(self.scores, self.ids[L], self.weights, stream=h)
-            self.ctx.dg_enqueue_export(e.s.gated, self.ids[L].data_ptr(), self.model.s.top_k, h)
+            self.ctx.dg_enqueue_export(e.s.gated, self.ids[L].data_ptr(), self.ids[L].numel(), h)
             self.ctx.dg_enqueue_wait(e.s.gated, h)
             ops.ffn(e, x[L], x[L + 1], ids=self.ids[L], weights=self.weights, residual=x[L], workspace=self.room, stream=h)
         self.ctx.dg_enqueue_end(h)
@@ -168,7 +171,7 @@ class Decoder:
     def token(self, token: int) -> int:
         """The likeliest token behind `token`."""
         with torch.cuda.stream(self.stream):
-            self.x[0].copy_(self.model.embedding[token:token + 1])
+            self.x[0].copy_(self.embedding[token:token + 1])
             self.ctx.begin()
             try:
                 self.graph.replay()
