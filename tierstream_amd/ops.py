@@ -1,6 +1,7 @@
 """The model operators of include/tierstream_amd/tsa_ops.h, on any 2-D array objects that have data_ptr(), shape, stride()
-and dtype as torch's tensors have (torch itself is not imported). Streams are hipStream_t handles
-(torch.cuda.current_stream().cuda_stream); outputs and workspaces are the caller's. Errors are raised as SsError.
+and dtype as torch's tensors have (torch itself is not imported), all in device memory: what says by is_cuda that it is
+elsewhere is refused. Streams are hipStream_t handles (torch.cuda.current_stream().cuda_stream); outputs and workspaces are
+the caller's. Errors are raised as SsError, arrays that do not fit together or are not the device's as ValueError.
 
     ops.route(logits, ids, weights, stream=s)                       # ids for ss_dg_enqueue_export and for ops.ffn
     e = ops.Experts.in_arena(ctx.dg_view(), g, n, d, f, "bf16")     # the slots of gated layer g
@@ -87,11 +88,18 @@ def _type(t) -> int:
     return kind
 
 
+def _device(t, what: str) -> None:
+    """A kernel takes an address as it is: one of the host's would fault the device."""
+    if not getattr(t, "is_cuda", True):
+        raise ValueError(f"{what}: not in device memory")
+
+
 def _mat(t, rows: int, cols: int, what: str, kind: int | None = None):
     """(pointer, row stride) of a matrix with contiguous rows."""
     stride = t.stride()
     if t.shape != (rows, cols) or (cols > 1 and stride[1] != 1):
         raise ValueError(f"{what}: a [{rows}][{cols}] matrix with contiguous rows, not {tuple(t.shape)}")
+    _device(t, what)
     if kind is not None and _type(t) != kind:
         raise ValueError(f"{what}: another type than the operator's ({t.dtype})")
     return t.data_ptr(), stride[0]
@@ -110,6 +118,7 @@ def _vec(t, shape, dtype: str, what: str):
         name = _dtype_named[d] = str(d)
     if t.shape != shape or name != dtype or not t.is_contiguous():
         raise ValueError(f"{what}: a contiguous {dtype} array of {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
+    _device(t, what)
     return t.data_ptr()
 
 
@@ -119,7 +128,10 @@ def _ok(status: int) -> None:
 
 
 def _room(workspace):
-    return (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    if workspace is None:
+        return None, 0
+    _device(workspace, "workspace")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 # ---- the choice of experts -------------------------------------------------------------------------------------------
@@ -195,6 +207,7 @@ class Experts:
         for t, shape, what in ((gate, (n, f, width), "gate"), (up, (n, f, width), "up"), (down, (n, d, wide), "down")):
             if tuple(t.shape) != shape or t.dtype != gate.dtype or not t.is_contiguous():
                 raise ValueError(f"{what}: a contiguous array of {shape}, not {tuple(t.shape)} {t.dtype}")
+            _device(t, what)
         e = cls(n, d, f, kind)
         e.keep = (gate, up, down)
         for p, t in enumerate(e.keep):
@@ -204,6 +217,7 @@ class Experts:
     @classmethod
     def in_table(cls, table, d_model: int, d_ff: int, kind: str) -> "Experts":
         """table: int64 / uint64 [n] of unit addresses on the device (ss_layer_view.table_dev)."""
+        _device(table, "table")
         e = cls(table.numel(), d_model, d_ff, kind)
         e.keep = table
         e.s.table = table.data_ptr()
