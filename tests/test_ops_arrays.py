@@ -57,3 +57,16 @@ CALLS = {
 def test_an_array_of_the_host_is_refused(name):
     with pytest.raises(ValueError, match=f"{name}.*device memory"):
         CALLS[name]({name: Host})
+
+
+class Spaced(Array):
+    def is_contiguous(self):
+        return False
+
+
+@pytest.mark.parametrize("table", [Array(8, dtype="torch.int32"), Array(4, dtype="torch.float64"), Array(2, 4, dtype="torch.int64"),
+                                   Spaced(4, dtype="torch.int64")])
+def test_a_table_is_an_array_of_64_bit_addresses(table):
+    with pytest.raises(ValueError, match="table"):
+        ops.Experts.in_table(table, 64, 96, "bf16")
+    assert ops.Experts.in_table(Array(4, dtype="torch.int64"), 64, 96, "bf16").s.table

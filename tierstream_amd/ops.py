@@ -217,6 +217,8 @@ class Experts:
     @classmethod
     def in_table(cls, table, d_model: int, d_ff: int, kind: str) -> "Experts":
         """table: int64 / uint64 [n] of unit addresses on the device (ss_layer_view.table_dev)."""
+        if len(table.shape) != 1 or str(table.dtype) not in ("torch.int64", "torch.uint64") or not table.is_contiguous():
+            raise ValueError(f"table: a contiguous array of 64-bit addresses, not {table.dtype} {tuple(table.shape)}")
         _device(table, "table")
         e = cls(table.numel(), d_model, d_ff, kind)
         e.keep = table
