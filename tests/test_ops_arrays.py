@@ -70,3 +70,10 @@ def test_a_table_is_an_array_of_64_bit_addresses(table):
     with pytest.raises(ValueError, match="table"):
         ops.Experts.in_table(table, 64, 96, "bf16")
     assert ops.Experts.in_table(Array(4, dtype="torch.int64"), 64, 96, "bf16").s.table
+
+
+@pytest.mark.parametrize("f,width,wide", [(96, 37, 54), (96, 17, 54), (80, 36, 36)])
+def test_stacked_4_bit_rows_are_whole_blocks(f, width, wide):
+    parts = [Array(2, f, width, dtype="torch.uint8"), Array(2, f, width, dtype="torch.uint8"), Array(2, width // 18 * 32, wide, dtype="torch.uint8")]
+    with pytest.raises(ValueError, match="blocks"):
+        ops.Experts.stacked(*parts)

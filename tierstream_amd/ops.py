@@ -202,6 +202,8 @@ class Experts:
         """gate, up [n][d_ff][d_model], down [n][d_model][d_ff] (uint8: rows of 4-bit blocks), each contiguous."""
         n, f, width = gate.shape
         kind = _type(gate)
+        if kind == Q4 and (width % _Q4_BYTES or f % _Q4_BLOCK):
+            raise ValueError(f"gate: 4-bit rows are whole blocks of {_Q4_BYTES} bytes and d_ff a multiple of {_Q4_BLOCK}, not {f} rows of {width} bytes")
         d = width // _Q4_BYTES * _Q4_BLOCK if kind == Q4 else width
         wide = f // _Q4_BLOCK * _Q4_BYTES if kind == Q4 else f
         for t, shape, what in ((gate, (n, f, width), "gate"), (up, (n, f, width), "up"), (down, (n, d, wide), "down")):
