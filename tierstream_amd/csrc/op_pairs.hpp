@@ -200,8 +200,8 @@ uint32_t most_tiles(uint32_t pairs, uint32_t n, uint32_t rows_per_tile) {
   return pairs / rows_per_tile + (n < pairs ? n : pairs);
 }
 
-// Pairs that one workgroup groups (a multiple of 1024); of more than 64 times as many, 64 share them.
-constexpr uint32_t kPlanOne = 2048;
+// Pairs that one workgroup groups (a multiple of 1024); more than kPlanMost times as many are shared by at most so many workgroups.
+constexpr uint32_t kPlanOne = 2048, kPlanMost = 64;
 
 Plan take_plan(Room& r, uint32_t n, uint32_t pairs, uint32_t top_k, uint32_t rows_per_tile) {
   Plan p;
@@ -214,9 +214,11 @@ Plan take_plan(Room& r, uint32_t n, uint32_t pairs, uint32_t top_k, uint32_t row
   p.n_tiles = r.take<uint32_t>(1);
   p.pairs = pairs;
   p.stretch = pairs > kPlanOne ? kPlanOne : pairs;
-  if (pairs > 64 * kPlanOne) p.stretch = (pairs / 64 + kPlanOne) / 1024 * 1024;
+  const bool many = pairs > kPlanMost * kPlanOne;
+  if (many) p.stretch = uint32_t(up_to((pairs + kPlanMost - 1) / kPlanMost, 1024));
   p.groups = pairs > kPlanOne ? (pairs + p.stretch - 1) / p.stretch : 1;
-  p.counts = r.take<uint32_t>(p.groups > 1 ? uint64_t(p.groups) * n : 0);
+  // (kPlanMost of them however few there are: a workspace that holds a call holds every one of fewer rows)
+  p.counts = r.take<uint32_t>(p.groups > 1 ? uint64_t(many ? kPlanMost : p.groups) * n : 0);
   p.top_k = top_k;
   p.n = n;
   return p;
