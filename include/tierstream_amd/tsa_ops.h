@@ -94,7 +94,9 @@ typedef struct tsa_experts {
 } tsa_experts;
 
 /* y_t = residual_t + sum_j weights_tj x down (act(gate x_t) * (up x_t)), the weights of expert ids_tj. An id below 0 or
- * from n_experts up adds nothing; a row may have none. ids NULL: every row through expert 0 (top_k 1). */
+ * from n_experts up adds nothing; a row may have none. ids NULL: every row through expert 0 (top_k 1).
+ * All sums are in 32 bits; act(gate x) * (up x) is rounded once to 16 (with its weight, where there is one row), in half
+ * precision behind a power of two that its row's largest value chooses, so that nothing that 32 bits hold overflows or is lost. */
 typedef struct tsa_ffn_args {
   const void* x;           /* [rows][d_model] of type */
   uint64_t x_stride;

@@ -45,6 +45,38 @@ struct F16 {
   static __device__ __forceinline__ u16 down(float v) { return __builtin_bit_cast(u16, (_Float16)v); }
 };
 
+// A product's result on its way to be the operand of the next one. bf16 has the range of 32 bits: it is rounded where it is made.
+// Half precision ends at 65504 and has fewer bits below 6e-5, so such a value stays in 32 bits until the largest of its row is
+// known, and is rounded as what a power of two leaves of it (fit_kernel).
+template <class T>
+struct Held {
+  typedef u16 type;
+  static __device__ __forceinline__ u16 of(float v) { return T::down(v); }
+};
+template <>
+struct Held<F16> {
+  typedef float type;
+  static __device__ __forceinline__ float of(float v) { return v; }
+};
+template <class T>
+using held = typename Held<T>::type;
+
+// The larger of two sizes, infinities and NaN left out.
+__device__ __forceinline__ float peak(float top, float v) {
+  const float a = fabsf(v);
+  return a < INFINITY && a > top ? a : top;
+}
+// 2^-e and 2^e with the largest value `top` x 2^-e in [2^14, 2^15): 39 powers of two below it, half precision still has all its
+// bits for 29 of them.
+struct Fit {
+  float down, up;
+  explicit __device__ __forceinline__ Fit(float top) {
+    const int x = int(__builtin_bit_cast(uint32_t, top) >> 23) - 127 - 14, e = x < -100 ? -100 : x;  // (113 at most)
+    down = __builtin_bit_cast(float, uint32_t(127 - e) << 23);
+    up = __builtin_bit_cast(float, uint32_t(127 + e) << 23);
+  }
+};
+
 // 1 / (1 + exp(-v)) with the hardware's exponential and reciprocal: a few units of the last place of 32 bits for |v| below
 // about 8, an absolute error below that beyond.
 __device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.0f + __expf(-v)); }

@@ -96,6 +96,18 @@ struct FloatRows {
   }
 };
 
+// A wave's part of a tile to rows of what is held (stride and columns multiples of 8): out is the first row, c0 the tile's first column.
+template <class T, int NI, int MJ>
+__device__ __forceinline__ void hand_out_held(void* memory, const f32x4 (&acc)[NI][MJ], held<T>* out, uint64_t stride, uint32_t rows,
+                                              uint32_t c0, uint32_t n_cols) {
+  if constexpr (std::is_same_v<T, F16>) {
+    FloatRows o{out, stride, rows, c0, n_cols};
+    hand_out<NI, MJ>(memory, acc, o);
+  } else {
+    hand_out_bits<T, NI, MJ>(memory, acc, out + c0, stride, rows, n_cols - c0);
+  }
+}
+
 // Gate and up rows of the same 16 NI columns as one operand of 32 NI: each wave gets 8 NI of both.
 template <int NI>
 __device__ __forceinline__ TileRowsSource<NI> gate_up_source(const Plan& p, const TileRows& t, uint32_t d, uint32_t f,
@@ -116,12 +128,13 @@ __device__ __forceinline__ TileRowsSource<MJ> sorted_rows(const TileRows& t, con
                             [&](uint32_t r) { return x + uint64_t(t.first + (r < t.rows ? r : t.rows - 1)) * stride; });
 }
 
-// out_t = residual_t + sum_j w_tj v_{at(t, j)}, in the order of j; kWide columns a thread (a multiple of 4: one access each).
+// out_t = residual_t + sum_j w_tj scale_{at(t, j)} v_{at(t, j)}, in the order of j; kWide columns a thread (a multiple of 4: one access each).
 // By blocks first.. of `n_blocks` of 256 threads.
 struct Combine {
   Plan p;
   uint32_t rows = 0, d = 0, n_blocks = 0;
   const float *v = nullptr, *weights = nullptr;
+  const float* scale = nullptr;  // of the sorted positions' v (null: 1)
   const u16* residual = nullptr;
   uint64_t residual_stride = 0;
   u16* out = nullptr;
@@ -157,7 +170,9 @@ __device__ __forceinline__ void combine(const Combine& a, uint32_t block) {
       }
 #pragma unroll
       for (uint32_t j = 0; j < 4; ++j) {
-        const float* from = v + uint64_t(uint32_t(at[j] < 0 ? 0 : at[j])) * d + c;
+        const uint32_t pos = uint32_t(at[j] < 0 ? 0 : at[j]);
+        const float* from = v + uint64_t(pos) * d + c;
+        if (a.scale) w[j] *= at[j] < 0 ? 1.0f : a.scale[pos];
         if constexpr (kWide == 4) {
           const f32x4 y = at[j] >= 0 ? *reinterpret_cast<const f32x4*>(from) : f32x4{0, 0, 0, 0};
 #pragma unroll
