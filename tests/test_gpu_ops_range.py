@@ -102,3 +102,18 @@ def test_a_row_without_experts_beside_large_ones(ops, act):
         y = torch.full_like(x, 7.0)
         ops.ffn(layer.e, x, y, ids=i, weights=w, act=act, workspace=room(ops.ffn_workspace(layer.e, 1, 3)), stream=stream())
         near_rows(y, ffn64(layer, x, i, w, None, act), str(ids))
+
+
+@pytest.mark.parametrize("rows", [3, 200])
+def test_a_column_beyond_32_bits_in_a_ragged_tile(ops, rows):
+    """act(gate x) (up x) of the last column is infinite in 32 bits: so is the weight's gradient, of its own sign, and not NaN."""
+    g = gen(12)
+    d, f = 64, 40
+    layer = Layer(ops, g, "stacked", 1, d, f, "bf16")
+    x, dy = mat(g, rows, d, "bf16").abs() + 0.5, mat(g, rows, d, "bf16").abs() + 0.5
+    for p in layer.keep[:2]:
+        p[0, -1] = 1e20
+    layer.keep[2][0, :, -1] = 0.5
+    dw = torch.full((rows, 1), 7.0, device="cuda")
+    ops.ffn_backward(layer.e, x, dy, None, dweights=dw, workspace=room(ops.ffn_backward_workspace(layer.e, rows)), stream=stream())
+    assert bool((dw == math.inf).all())

@@ -186,17 +186,19 @@ __global__ __launch_bounds__(kTileThreads, 2) void hidden_grad_tile_kernel(Plan 
   for (int j = 0; j < MJ; ++j) {
     float sum = 0.0f;
     f32x4 b[kHalf];
+    bool in[kHalf];  // (behind the last column stands the last one again: not part of the sum)
 #pragma unroll
     for (int i = 0; i < kHalf; ++i) {
       const uint32_t c = f0 + (wave & 1u) * 8 * NI + 16 * i + (lane >> 4) * 4;
-      b[i] = c < f ? *reinterpret_cast<const f32x4*>(back + uint64_t(pos[j]) * f + c) : f32x4{0, 0, 0, 0};
+      in[i] = c < f;
+      b[i] = in[i] ? *reinterpret_cast<const f32x4*>(back + uint64_t(pos[j]) * f + c) : f32x4{0, 0, 0, 0};
     }
 #pragma unroll
     for (int i = 0; i < kHalf; ++i)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const float g = gu[i][j][q], u = gu[i + kHalf][j][q], a = activate(act, g);
-        sum += a * u * b[i][q];
+        sum += in[i] ? a * u * b[i][q] : 0.0f;
         h[i][j][q] = w[j] * a * u;
         gu[i][j][q] = w[j] * b[i][q] * u * slope(act, g);  // dg, du in the products' places
         gu[i + kHalf][j][q] = w[j] * b[i][q] * a;
