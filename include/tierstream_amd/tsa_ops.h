@@ -115,7 +115,9 @@ SS_API ss_status tsa_ffn(const tsa_experts* e, const tsa_ffn_args* a, void* work
                          void* stream);
 
 /* The gradients of tsa_ffn for dy (the residual's gradient is dy itself). Nothing of the forward pass is kept: gate x and
- * up x are computed again, in 32 bits. The experts' w_type is args' type (4-bit weights have no backward pass). */
+ * up x are computed again, in 32 bits. The experts' w_type is args' type (4-bit weights have no backward pass).
+ * All sums are in 32 bits; of what lies between them the gradients of gate x and up x, and the weighted act(gate x) * (up x), are
+ * rounded once to 16 bits, in half precision behind a power of two that the largest value of the expert's rows chooses. */
 typedef struct tsa_ffn_grad_args {
   const void* x;           /* [rows][d_model] of type */
   uint64_t x_stride;

@@ -19,9 +19,12 @@ def ops(gpu):
     return ops
 
 
-def near_rows(got, want, what=""):
+def near_rows(got, want, what="", sums=True):
+    """sums: False where a row may be one product, so that an operand's rounding is the whole row's: 2^-11 for it and for the output."""
     assert got.shape == want.shape and bool(torch.isfinite(got).all()), f"{what}: not finite"
     off, norm = (got.double() - want).norm(dim=-1), want.norm(dim=-1)
+    if not sums:
+        off = off / 2 - 2.0 ** -25 * math.sqrt(want.shape[-1])  # (and the type's own spacing)
     worst = int((off / norm.clamp_min(1e-30)).argmax())
     assert bool((off <= BOUND[got.dtype] * norm + 1e-30).all()), f"{what}: row {worst} off by {float(off.flatten()[worst] / norm.flatten()[worst]):.3g}"
 
@@ -117,3 +120,36 @@ def test_a_column_beyond_32_bits_in_a_ragged_tile(ops, rows):
     dw = torch.full((rows, 1), 7.0, device="cuda")
     ops.ffn_backward(layer.e, x, dy, None, dweights=dw, workspace=room(ops.ffn_backward_workspace(layer.e, rows)), stream=stream())
     assert bool((dw == math.inf).all())
+
+
+# Powers of two of gate, up, down, x, dy and the range of the experts' weights; what is looked at besides the weights' gradient.
+BACK = {
+    "w h beyond 65504": (4, 13, -10, 0, -11, (0.25, 1.0), ("ddown",)),
+    "dg beyond 65504": (-7, 10, 2, -8, 12, (0.25, 1.0), ("dgate", "dx")),
+    "du beyond 65504": (7, -5, 3, -6, 10, (0.25, 1.0), ("dup",)),
+    "all below 6e-5": (-10, -17, -12, 8, 8, (0.0025, 0.01), ("dgate", "dup", "ddown")),
+    "dg below 6e-5": (10, -6, -2, -10, 0, (0.0125, 0.05), ("dx",)),
+}
+
+
+@pytest.mark.parametrize("what", BACK)
+@pytest.mark.parametrize("rows,n,k,d,f,shift", [(1, 3, 2, 256, 128, 0), (37, 4, 2, 128, 200, 0), (90, 3, 2, 131, 77, 1), (300, 2, 1, 160, 264, 0),
+                                                (3001, 2, 2, 256, 1672, 0)])
+def test_block_backward(ops, rows, n, k, d, f, shift, what):
+    gate, up, down, xs, dys, (low, high), looked = BACK[what]
+    g = gen(rows + d)
+    layer = scaled(ops, g, n, d, f, "f16", 2.0 ** gate, 2.0 ** up, 2.0 ** down)
+    pad = 8 if shift == 0 else 3
+    x, dy = (mat(g, rows, d, "f16", pad=pad, shift=shift, sigma=2.0 ** s) for s in (xs, dys))
+    ids, w = choices(g, rows, n, k, holes=False)
+    w = low + (high - low) * torch.rand(w.shape, device="cuda", generator=g)
+    want_dx, want_dw, want = ffn64(layer, x, ids, w, None, "silu", dy)
+    want = {"dx": want_dx, **dict(zip(("dgate", "dup", "ddown"), want))}
+    got = {name: torch.full(t.shape, 7.0, dtype=torch.float16, device="cuda") for name, t in want.items()}
+    dw = torch.full((rows, k), 7.0, device="cuda")
+    ops.ffn_backward(layer.e, x, dy, got["dx"], ids=ids, weights=w, dweights=dw, dgate=got["dgate"], dup=got["dup"], ddown=got["ddown"],
+                     workspace=room(ops.ffn_backward_workspace(layer.e, rows, k)), stream=stream())
+    for name in looked:
+        assert float(want[name].abs().max()) < 6e4 and float(want[name].abs().max()) > 1e-3, name
+        near_rows(got[name], want[name], name, sums=name == "dx")
+    assert float((dw.double() - want_dw).norm()) <= BOUND[torch.float32] * float(want_dw.norm())

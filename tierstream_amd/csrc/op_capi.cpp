@@ -219,7 +219,7 @@ uint64_t tsa_ffn_backward_workspace(const tsa_experts* e, uint32_t rows, uint32_
   (void)guard([&] {
     experts_of("tsa_ffn_backward_workspace", e, false);
     check_pairs("tsa_ffn_backward_workspace", rows, top_k, reinterpret_cast<const int32_t*>(16), nullptr);
-    n = ffn_backward_workspace(e->n_experts, e->d_model, e->d_ff, rows, top_k);
+    n = ffn_backward_workspace(e->n_experts, e->d_model, e->d_ff, e->w_type, rows, top_k);
   });
   return n;
 }
@@ -247,7 +247,7 @@ ss_status tsa_ffn_backward(const tsa_experts* e, const tsa_ffn_grad_args* a, voi
       check_array(w, "ddown", a->ddown, 2);
     }
     if (a->rows == 0 && !a->dgate) return;
-    check_workspace(w, workspace, workspace_bytes, ffn_backward_workspace(e->n_experts, e->d_model, e->d_ff, a->rows, a->top_k));
+    check_workspace(w, workspace, workspace_bytes, ffn_backward_workspace(e->n_experts, e->d_model, e->d_ff, e->w_type, a->rows, a->top_k));
     launched(launch_ffn_backward(m, e->d_model, e->d_ff, *a, workspace, static_cast<hipStream_t>(stream)), "tsa_ffn_backward");
   });
 }

@@ -2,21 +2,83 @@
 //
 // b = down^T dy of every pair; with gate x and up x computed again, d w = <h, b>, dg = w b up act'(gate), du = w b act(gate) and
 // w h; dx' = gate^T dg + up^T du, added over a row's pairs; d gate = dg^T x, d up = du^T x and d down = dy^T (w h) over an expert's
-// pairs. dg, du and w h are rounded once to the operands' 16 bits; b and dx' stay in 32 bits. No sum depends on an order that
-// changes.
+// pairs. dg, du and w h are rounded once to the operands' 16 bits (half precision: as what a power of two of their expert's leaves of
+// them, so that none overflows or loses bits; the sums over an expert's pairs need one for all of them); b and dx' stay in 32
+// bits. No sum depends on an order that changes.
 #include "op_pairs.hpp"
 
 namespace tsa {
 namespace op {
 namespace {
 
+// The two largest values of a workgroup of four waves from its threads', by way of 8 places in LDS: wave by wave here, read
+// behind a barrier.
+__device__ __forceinline__ void leave_peaks(float (*tops)[2], float top_g, float top_h) {
+  for (int s = 1; s < 64; s <<= 1) {
+    top_g = fmaxf(top_g, __shfl_xor(top_g, s, 64));
+    top_h = fmaxf(top_h, __shfl_xor(top_h, s, 64));
+  }
+  if ((threadIdx.x & 63u) == 0) {
+    tops[threadIdx.x >> 6][0] = top_g;
+    tops[threadIdx.x >> 6][1] = top_h;
+  }
+}
+__device__ __forceinline__ float joint_peak(const float (*tops)[2], int i) {
+  return fmaxf(fmaxf(tops[0][i], tops[1][i]), fmaxf(tops[2][i], tops[3][i]));
+}
+
+// Half precision: dg | du and w h of every pair behind the powers of two that the largest of its expert choose, whose inverses go
+// to scale, one array after the other. peaks: [tile][shares][2], as the workgroups that made the values left them.
+// kFitParts workgroups a tile of pairs. Bound by the bytes: 16384 pairs of 768 (226 MB) 43 us, 5.2 TB/s; 74 of 512 4 us, a launch.
+constexpr uint32_t kFitParts = 16;
+template <int kWide>
+__device__ __forceinline__ void fit_values(const float* from, u16* to, uint32_t n, float by) {
+  typedef float wide_t __attribute__((ext_vector_type(kWide)));
+  typedef u16 bits_t __attribute__((ext_vector_type(kWide)));
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x; i < n / kWide; i += 256) {
+    const wide_t x = reinterpret_cast<const wide_t*>(from)[i];
+    bits_t o;
+#pragma unroll
+    for (int q = 0; q < kWide; ++q) o[q] = F16::down(x[q] * by);
+    reinterpret_cast<bits_t*>(to)[i] = o;
+  }
+}
+template <int kWide>
+__global__ __launch_bounds__(256) void fit_grads_kernel(Plan p, uint32_t rows_per_tile, uint32_t f, uint32_t shares, const float* peaks,
+                                                        const float* dgu, const float* wh, u16* dgu_to, u16* wh_to, float* scale) {
+  __shared__ float tops[4][2];
+  TileRows t;
+  if (!tile_rows(p, blockIdx.x / kFitParts, rows_per_tile, t)) return;
+  const uint32_t begin = p.first[t.e], tiles = (p.first[t.e + 1] - begin + rows_per_tile - 1) / rows_per_tile;  // of the expert
+  const float* mine = peaks + uint64_t(t.tile - (t.first - begin) / rows_per_tile) * shares * 2;
+  float top_g = 0.0f, top_h = 0.0f;
+  for (uint64_t i = threadIdx.x; i < uint64_t(tiles) * shares; i += 256) {
+    top_g = fmaxf(top_g, mine[2 * i]);
+    top_h = fmaxf(top_h, mine[2 * i + 1]);
+  }
+  leave_peaks(tops, top_g, top_h);
+  __syncthreads();
+  const Fit g(joint_peak(tops, 0)), h(joint_peak(tops, 1));
+  for (uint32_t r = blockIdx.x % kFitParts; r < t.rows; r += kFitParts) {
+    const uint64_t pos = t.first + r;
+    if (threadIdx.x == 0) {
+      scale[pos] = g.up;
+      scale[p.pairs + pos] = h.up;
+    }
+    fit_values<kWide>(dgu + pos * 2 * f, dgu_to + pos * 2 * f, 2 * f, g.down);
+    fit_values<kWide>(wh + pos * f, wh_to + pos * f, f, h.down);
+  }
+}
+
 // Of every pair: dg | du as one row of 2 f values, w h, and this tile's share of d w (d_share[f tile][sorted position]).
 template <class T>
 __global__ __launch_bounds__(256) void hidden_grad_any_kernel(Plan p, const u16* x, uint64_t x_stride, const u16* dy,
                                                               uint64_t dy_stride, const float* weights, uint32_t d, uint32_t f,
-                                                              uint32_t act, u16* dgu, u16* wh, float* d_share) {
+                                                              uint32_t act, held<T>* dgu, held<T>* wh, float* d_share,
+                                                              float* peaks) {
   __shared__ TileMemory m;
-  __shared__ float share[64][2];
+  __shared__ float share[64][2], tops[4][2];
   const uint32_t tf = (f + 63) / 64;
   const uint32_t ft = blockIdx.x % tf, f0 = ft * 64;
   TileRows t;
@@ -28,6 +90,7 @@ __global__ __launch_bounds__(256) void hidden_grad_any_kernel(Plan p, const u16*
   const Operand down{reinterpret_cast<const u16*>(p.part[3 * t.e + 2]), 1, f, f, d, nullptr};  // (f, d): its columns as rows
   tile64<T, false>(down, f0, dys, 0, d, m, b);
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  float top_g = 0.0f, top_h = 0.0f;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const uint32_t r = (wave >> 1) * 32 + 16 * j + (lane & 15u);
@@ -42,15 +105,20 @@ __global__ __launch_bounds__(256) void hidden_grad_any_kernel(Plan p, const u16*
         const float a = activate(act, g[i][j][q]), back = b[i][j][q];
         if (c >= f || r >= t.rows) continue;
         sum += a * u[i][j][q] * back;
-        dgu[uint64_t(pos) * 2 * f + c] = T::down(w * back * u[i][j][q] * slope(act, g[i][j][q]));
-        dgu[uint64_t(pos) * 2 * f + f + c] = T::down(w * back * a);
-        wh[uint64_t(pos) * f + c] = T::down(w * a * u[i][j][q]);
+        const float dg = w * back * u[i][j][q] * slope(act, g[i][j][q]), du = w * back * a, h = w * a * u[i][j][q];
+        dgu[uint64_t(pos) * 2 * f + c] = Held<T>::of(dg);
+        dgu[uint64_t(pos) * 2 * f + f + c] = Held<T>::of(du);
+        wh[uint64_t(pos) * f + c] = Held<T>::of(h);
+        top_g = peak(peak(top_g, dg), du);
+        top_h = peak(top_h, h);
       }
     sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
     if (lane < 16) share[r][wave & 1u] = sum;
   }
+  if (std::is_same_v<T, F16>) leave_peaks(tops, top_g, top_h);
   __syncthreads();
+  if (std::is_same_v<T, F16> && threadIdx.x < 2) peaks[(uint64_t(t.tile) * tf + ft) * 2 + threadIdx.x] = joint_peak(tops, threadIdx.x);
   if (threadIdx.x < t.rows) d_share[uint64_t(ft) * p.pairs + t.first + threadIdx.x] = share[threadIdx.x][0] + share[threadIdx.x][1];
 }
 
@@ -73,11 +141,11 @@ __global__ __launch_bounds__(256) void input_grad_any_kernel(Plan p, const u16* 
 }
 
 // out[e][b][a] = sum over expert e's pairs of left[pair][a] right[pair][b] (0 for an expert without pairs): left through
-// the rows' map where left_map, right where right_map.
+// the rows' map where left_map, right where right_map; times scale (null: 1) of the expert's first position.
 template <class T>
 __global__ __launch_bounds__(256) void weight_grad_any_kernel(Plan p, const u16* left, uint64_t left_stride, bool left_map,
                                                               uint32_t n_left, const u16* right, uint64_t right_stride,
-                                                              bool right_map, uint32_t n_right, u16* out) {
+                                                              bool right_map, uint32_t n_right, const float* scale, u16* out) {
   __shared__ TileMemory m;
   const uint32_t ta = (n_left + 63) / 64, tb = (n_right + 63) / 64;
   const uint32_t per = ta * tb;
@@ -103,8 +171,9 @@ __global__ __launch_bounds__(256) void weight_grad_any_kernel(Plan p, const u16*
     const Rows r{right_map ? right : right + first * right_stride, right_stride, right_map ? p.row + first : nullptr, n_right, n};
     f32x4 acc[2][2] = {};
     tile64<T, false>(l, a0, r, b0, n, m, acc);
+    const float up = scale && n ? scale[first] : 1.0f;
     each64(acc, [&](uint32_t i, uint32_t j, float v) {
-      if (a0 + i < n_left && b0 + j < n_right) out[(uint64_t(e) * n_right + b0 + j) * n_left + a0 + i] = T::down(v);
+      if (a0 + i < n_left && b0 + j < n_right) out[(uint64_t(e) * n_right + b0 + j) * n_left + a0 + i] = T::down(v * up);
     });
     __syncthreads();
   }
@@ -158,11 +227,12 @@ __global__ __launch_bounds__(kTileThreads, 2) void back_tile_kernel(Plan p, cons
 template <class T, class S>
 __global__ __launch_bounds__(kTileThreads, 2) void hidden_grad_tile_kernel(Plan p, const u16* x, uint64_t x_stride,
                                                                            const float* back, const float* weights, uint32_t d,
-                                                                           uint32_t f, uint32_t act, u16* dgu, u16* wh,
-                                                                           float* d_share) {
+                                                                           uint32_t f, uint32_t act, held<T>* dgu, held<T>* wh,
+                                                                           float* d_share, float* peaks) {
   extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
   constexpr int NI = S::NI, MJ = S::MJ, kHalf = NI / 2;
-  float* share = reinterpret_cast<float*>(memory) + S::kLds / 4 - 2 * S::kB;  // (behind what hand_out uses)
+  float* share = reinterpret_cast<float*>(memory) + S::kLds / 4 - 2 * S::kB;  // (behind what hand_out uses, as tops)
+  float (*tops)[2] = reinterpret_cast<float (*)[2]>(share - 8);
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   TileRows t;
   uint32_t at;
@@ -181,6 +251,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void hidden_grad_tile_kernel(Plan 
     w[j] = weights ? weights[p.pair[pos[j]]] : 1.0f;
   }
   f32x4 h[kHalf][MJ];
+  float top_g = 0.0f, top_h = 0.0f;
   __syncthreads();  // the product's reads are done
 #pragma unroll
   for (int j = 0; j < MJ; ++j) {
@@ -202,12 +273,19 @@ __global__ __launch_bounds__(kTileThreads, 2) void hidden_grad_tile_kernel(Plan 
         h[i][j][q] = w[j] * a * u;
         gu[i][j][q] = w[j] * b[i][q] * u * slope(act, g);  // dg, du in the products' places
         gu[i + kHalf][j][q] = w[j] * b[i][q] * a;
+        if (std::is_same_v<T, F16> && in[i] && (wave >> 1) * 16 * MJ + 16 * j + (lane & 15u) < t.rows) {
+          top_g = peak(peak(top_g, gu[i][j][q]), gu[i + kHalf][j][q]);
+          top_h = peak(top_h, h[i][j][q]);
+        }
       }
     sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
     if (lane < 16) share[2 * ((wave >> 1) * 16 * MJ + 16 * j + lane) + (wave & 1u)] = sum;
   }
-  hand_out_bits<T, kHalf, MJ>(memory, h, wh + uint64_t(t.first) * f + f0, f, t.rows, f - f0);  // (behind its barrier `share` is whole)
+  if (std::is_same_v<T, F16>) leave_peaks(tops, top_g, top_h);
+  hand_out_held<T, kHalf, MJ>(memory, h, wh + uint64_t(t.first) * f, f, t.rows, f0, f);  // (behind its barrier `share` and `tops` are whole)
+  if (std::is_same_v<T, F16> && threadIdx.x < 2)
+    peaks[(uint64_t(t.tile) * ((f + 16 * NI - 1) / (16 * NI)) + at) * 2 + threadIdx.x] = joint_peak(tops, threadIdx.x);
   if (threadIdx.x < t.rows) d_share[uint64_t(at) * p.pairs + t.first + threadIdx.x] = share[2 * threadIdx.x] + share[2 * threadIdx.x + 1];
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
@@ -215,7 +293,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void hidden_grad_tile_kernel(Plan 
     for (int i = 0; i < kHalf; ++i)
 #pragma unroll
       for (int j = 0; j < MJ; ++j) h[i][j] = gu[i + kHalf * half][j];
-    hand_out_bits<T, kHalf, MJ>(memory, h, dgu + uint64_t(t.first) * 2 * f + half * f + f0, uint64_t(2) * f, t.rows, f - f0);
+    hand_out_held<T, kHalf, MJ>(memory, h, dgu + uint64_t(t.first) * 2 * f + half * f, uint64_t(2) * f, t.rows, f0, f);
   }
 }
 
@@ -246,7 +324,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void input_grad_tile_kernel(Plan p
 template <class T, class S, bool kMapLeft>
 __device__ __forceinline__ void weight_grad_tile(f32x4* memory, uint32_t block, const Plan& p, const u16* left, uint64_t left_stride,
                                                  uint32_t n_left, const u16* right, uint64_t right_stride, uint32_t n_right,
-                                                 uint32_t n_outs, u16* out, u16* out2) {
+                                                 uint32_t n_outs, const float* scale, u16* out, u16* out2) {
   constexpr int NI = S::NI, MJ = S::MJ;
   uint32_t* map = reinterpret_cast<uint32_t*>(memory) + S::kLds / 4;
   const uint32_t wave = threadIdx.x >> 6;
@@ -276,6 +354,13 @@ __device__ __forceinline__ void weight_grad_tile(f32x4* memory, uint32_t block, 
       TileColumnsSource<MJ, true> r(pairs, wave >> 1, right, right_stride, b0, n_right, map);
       tile_product<T, NI, MJ, S::NB>(l, r, pairs, lds_offset(memory), acc, refill);
     }
+    if constexpr (std::is_same_v<T, F16>) {
+      const float up = scale[first];
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < MJ; ++j) acc[i][j] *= up;
+    }
   }
   hand_out_bits<T, NI, MJ, true>(memory, acc, (which ? out2 : out) + (uint64_t(e) * n_right + b0) * n_left + a0, n_left, n_right - b0,
                            n_left - a0);
@@ -285,13 +370,13 @@ __device__ __forceinline__ void weight_grad_tile(f32x4* memory, uint32_t block, 
 template <class T, class S>
 __global__ __launch_bounds__(kTileThreads, 2) void weight_grad_tile_kernel(Plan p, uint32_t n_up, const u16* x, uint64_t x_stride,
                                                                            const u16* dy, uint64_t dy_stride, uint32_t d,
-                                                                           uint32_t f, const u16* dgu, const u16* wh, u16* dgate,
-                                                                           u16* dup, u16* ddown) {
+                                                                           uint32_t f, const u16* dgu, const u16* wh, const float* scale,
+                                                                           u16* dgate, u16* dup, u16* ddown) {
   extern __shared__ __attribute__((aligned(1024))) f32x4 memory[];
   if (blockIdx.x < n_up)
-    weight_grad_tile<T, S, true>(memory, blockIdx.x, p, x, x_stride, d, dgu, uint64_t(2) * f, f, 2, dgate, dup);
+    weight_grad_tile<T, S, true>(memory, blockIdx.x, p, x, x_stride, d, dgu, uint64_t(2) * f, f, 2, scale, dgate, dup);
   else
-    weight_grad_tile<T, S, false>(memory, blockIdx.x - n_up, p, wh, f, f, dy, dy_stride, d, 1, ddown, nullptr);
+    weight_grad_tile<T, S, false>(memory, blockIdx.x - n_up, p, wh, f, f, dy, dy_stride, d, 1, scale + p.pairs, ddown, nullptr);
 }
 
 // ---- launches ----
@@ -299,11 +384,16 @@ struct Backward {
   Plan plan;
   u16 *dgu, *wh;
   float *share, *out, *back;  // (back and out share their place: out is written behind back's last reader)
+  float *dgu_wide, *wh_wide, *scale, *peaks;  // half precision
 };
-Backward take_backward(Room& r, uint32_t n, uint32_t d, uint32_t f, uint32_t rows, uint32_t top_k) {
+Backward take_backward(Room& r, uint32_t n, uint32_t d, uint32_t f, uint32_t rows, uint32_t top_k, bool half) {
   const uint64_t pairs = uint64_t(rows) * top_k;
   Backward w;
   w.plan = take_plan(r, n, uint32_t(pairs), top_k, 64);
+  w.dgu_wide = r.take<float>(half ? pairs * 2 * f : 0);
+  w.wh_wide = r.take<float>(half ? pairs * f : 0);
+  w.scale = r.take<float>(half ? 2 * pairs : 0);
+  w.peaks = r.take<float>(half ? uint64_t(2) * most_tiles(uint32_t(pairs), n, 64) * ((f + 31) / 32) : 0);  // (the smallest tiles')
   w.dgu = r.take<u16>(pairs * 2 * f);
   w.wh = r.take<u16>(pairs * f);
   w.share = r.take<float>(pairs * ((f + 31) / 32));  // (the narrowest tile's)
@@ -311,11 +401,36 @@ Backward take_backward(Room& r, uint32_t n, uint32_t d, uint32_t f, uint32_t row
   return w;
 }
 
+// Where the hidden gradients are left, and the launch that makes operands of them.
+template <class T>
+held<T>* made_dgu(const Backward& w) {
+  if constexpr (std::is_same_v<T, F16>) return w.dgu_wide;
+  else return w.dgu;
+}
+template <class T>
+held<T>* made_wh(const Backward& w) {
+  if constexpr (std::is_same_v<T, F16>) return w.wh_wide;
+  else return w.wh;
+}
+template <class T>
+void launch_fit(const Backward& w, uint32_t tiles, uint32_t rows_per_tile, uint32_t f, uint32_t shares, hipStream_t s) {
+  if constexpr (std::is_same_v<T, F16>) {
+    const dim3 grid(tiles * kFitParts);
+    if (f % 4 == 0)
+      hipLaunchKernelGGL((fit_grads_kernel<4>), grid, dim3(256), 0, s, w.plan, rows_per_tile, f, shares, w.peaks, w.dgu_wide, w.wh_wide, w.dgu, w.wh, w.scale);
+    else
+      hipLaunchKernelGGL((fit_grads_kernel<1>), grid, dim3(256), 0, s, w.plan, rows_per_tile, f, shares, w.peaks, w.dgu_wide, w.wh_wide, w.dgu, w.wh, w.scale);
+  }
+}
+
 template <class T>
 int launch_sums(const Backward& w, const tsa_ffn_grad_args& a, uint32_t d, uint32_t shares, hipStream_t s) {
   bool wide = true;
   Combine c;
-  if (a.dx) c = combine_of(w.plan, a.rows, d, w.out, nullptr, nullptr, 0, a.dx, a.dx_stride, wide);
+  if (a.dx) {
+    c = combine_of(w.plan, a.rows, d, w.out, nullptr, nullptr, 0, a.dx, a.dx_stride, wide);
+    if (std::is_same_v<T, F16>) c.scale = w.scale;
+  }
   WeightShares g;
   g.n = shares;
   g.share = w.share;
@@ -330,7 +445,7 @@ int launch_sums(const Backward& w, const tsa_ffn_grad_args& a, uint32_t d, uint3
 template <class T, class S, class W>
 int backward_tiles(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_grad_args& a, void* ws, hipStream_t s) {
   Room room(ws);
-  const Backward w = take_backward(room, e.n, d, f, a.rows, a.top_k);
+  const Backward w = take_backward(room, e.n, d, f, a.rows, a.top_k, std::is_same_v<T, F16>);
   if (int err = launch_plan(e, a.ids, w.plan, S::kB, s)) return err;
   const auto of = [](uint32_t n, uint32_t each) { return (n + each - 1) / each; };
   const uint32_t tiles = most_tiles(w.plan.pairs, e.n, S::kB), shares = of(f, S::kA / 2);
@@ -339,7 +454,8 @@ int backward_tiles(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_gra
     hipLaunchKernelGGL((back_tile_kernel<T, S>), dim3(tiles * of(f, S::kA)), dim3(kTileThreads), S::kLds, s, w.plan, dy, a.dy_stride, d,
                        f, w.back);
     hipLaunchKernelGGL((hidden_grad_tile_kernel<T, S>), dim3(tiles * shares), dim3(kTileThreads), S::kLds, s, w.plan, x, a.x_stride,
-                       w.back, a.weights, d, f, a.act, w.dgu, w.wh, w.share);
+                       w.back, a.weights, d, f, a.act, made_dgu<T>(w), made_wh<T>(w), w.share, w.peaks);
+    launch_fit<T>(w, tiles, S::kB, f, shares, s);
   }
   if (a.dx && tiles)
     hipLaunchKernelGGL((input_grad_tile_kernel<T, S>), dim3(tiles * of(d, S::kA)), dim3(kTileThreads), S::kLds, s, w.plan, w.dgu, d, f,
@@ -349,7 +465,7 @@ int backward_tiles(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_gra
   if (a.dgate) {
     const uint32_t n_up = e.n * of(d, W::kA) * of(f, W::kB) * 2, n_down = e.n * of(f, W::kA) * of(d, W::kB);
     hipLaunchKernelGGL((weight_grad_tile_kernel<T, W>), dim3(n_up + n_down), dim3(kTileThreads), W::kLds + 4 * kMapRing, s, w.plan, n_up,
-                       x, a.x_stride, dy, a.dy_stride, d, f, w.dgu, w.wh, static_cast<u16*>(a.dgate), static_cast<u16*>(a.dup),
+                       x, a.x_stride, dy, a.dy_stride, d, f, w.dgu, w.wh, w.scale, static_cast<u16*>(a.dgate), static_cast<u16*>(a.dup),
                        static_cast<u16*>(a.ddown));
   }
   return int(hipGetLastError());
@@ -368,24 +484,28 @@ int backward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_grad_args
     return small_out ? backward_tiles<T, BigTile, SmallTile>(e, d, f, a, ws, s) : backward_tiles<T, BigTile, WideTile>(e, d, f, a, ws, s);
   }
   Room room(ws);
-  const Backward w = take_backward(room, e.n, d, f, a.rows, a.top_k);
+  const Backward w = take_backward(room, e.n, d, f, a.rows, a.top_k, std::is_same_v<T, F16>);
   if (int err = launch_plan(e, a.ids, w.plan, 64, s)) return err;
   const uint32_t tiles = most_tiles(w.plan.pairs, e.n, 64), tf = (f + 63) / 64, td = (d + 63) / 64;
   const u16 *x = static_cast<const u16*>(a.x), *dy = static_cast<const u16*>(a.dy);
-  if (tiles)
+  if (tiles) {
     hipLaunchKernelGGL((hidden_grad_any_kernel<T>), dim3(tiles * tf), dim3(256), 0, s, w.plan, x, a.x_stride, dy, a.dy_stride,
-                       a.weights, d, f, a.act, w.dgu, w.wh, w.share);
+                       a.weights, d, f, a.act, made_dgu<T>(w), made_wh<T>(w), w.share, w.peaks);
+    launch_fit<T>(w, tiles, 64, f, tf, s);
+  }
   if (a.dx && tiles)
     hipLaunchKernelGGL((input_grad_any_kernel<T>), dim3(tiles * td), dim3(256), 0, s, w.plan, w.dgu, d, f, w.out);
   if (tiles)
     if (int err = launch_sums<T>(w, a, d, tf, s)) return err;
   if (a.dgate) {
+    constexpr bool kHalf = std::is_same_v<T, F16>;
     const uint32_t g = blocks(uint64_t(e.n) * tf * td);
     for (int half = 0; half < 2; ++half)
       hipLaunchKernelGGL((weight_grad_any_kernel<T>), dim3(g), dim3(256), 0, s, w.plan, x, a.x_stride, true, d,
-                         w.dgu + half * uint64_t(f), uint64_t(2) * f, false, f, static_cast<u16*>(half ? a.dup : a.dgate));
+                         w.dgu + half * uint64_t(f), uint64_t(2) * f, false, f,
+                         kHalf ? w.scale : nullptr, static_cast<u16*>(half ? a.dup : a.dgate));
     hipLaunchKernelGGL((weight_grad_any_kernel<T>), dim3(g), dim3(256), 0, s, w.plan, w.wh, uint64_t(f), false, f, dy,
-                       a.dy_stride, true, d, static_cast<u16*>(a.ddown));
+                       a.dy_stride, true, d, kHalf ? w.scale + w.plan.pairs : nullptr, static_cast<u16*>(a.ddown));
   }
   return int(hipGetLastError());
 }
@@ -393,9 +513,9 @@ int backward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_grad_args
 }  // namespace
 }  // namespace op
 
-uint64_t ffn_backward_workspace(uint32_t n, uint32_t d, uint32_t f, uint32_t rows, uint32_t top_k) {
+uint64_t ffn_backward_workspace(uint32_t n, uint32_t d, uint32_t f, uint32_t w_type, uint32_t rows, uint32_t top_k) {
   op::Room room(nullptr);
-  op::take_backward(room, n, d, f, rows, top_k);
+  op::take_backward(room, n, d, f, rows, top_k, w_type != TSA_BF16);
   return room.bytes;
 }
 int launch_ffn_backward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_grad_args& a, void* ws, hipStream_t stream) {

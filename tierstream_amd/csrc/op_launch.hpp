@@ -51,7 +51,7 @@ int launch_linear(const tsa_linear_args& a, void* workspace, hipStream_t stream)
 uint64_t ffn_workspace(uint32_t n, uint32_t d, uint32_t f, uint32_t w_type, uint32_t rows, uint32_t top_k);
 int launch_ffn(const ExpertMap& e, uint32_t d, uint32_t f, uint32_t w_type, const tsa_ffn_args& a, void* workspace,
                hipStream_t stream);
-uint64_t ffn_backward_workspace(uint32_t n, uint32_t d, uint32_t f, uint32_t rows, uint32_t top_k);
+uint64_t ffn_backward_workspace(uint32_t n, uint32_t d, uint32_t f, uint32_t w_type, uint32_t rows, uint32_t top_k);
 int launch_ffn_backward(const ExpertMap& e, uint32_t d, uint32_t f, const tsa_ffn_grad_args& a, void* workspace,
                         hipStream_t stream);
 

@@ -46,11 +46,12 @@ __device__ __forceinline__ uint32_t expert_of(const ExpertMap& m, const int32_t*
 
 // One tile's expert and rows (rows_per_tile of the plan); false behind the last tile.
 struct TileRows {
-  uint32_t e, first, rows;
+  uint32_t tile, e, first, rows;
   const uint32_t* map;
 };
 __device__ __forceinline__ bool tile_rows(const Plan& p, uint32_t tile, uint32_t rows_per_tile, TileRows& t) {
   if (tile >= *p.n_tiles) return false;
+  t.tile = tile;
   t.e = p.tile[2 * tile];
   t.first = p.tile[2 * tile + 1];
   const uint32_t end = p.first[t.e + 1];
