@@ -14,8 +14,13 @@
  * for the same inputs. Outputs may not overlap inputs, except where a residual is the output itself. Return: SS_OK,
  * SS_E_INVALID (argument checks, done on the host before any launch), SS_E_BACKEND (a HIP error).
  *
- * Alignment: every matrix at its element's size, workspaces at 16 bytes. Rows that start 16-byte aligned (base and
- * stride) and hold a multiple of 8 values are the fastest. 4-bit weights: 4 bytes; 16 is faster.
+ * Alignment: every matrix at its element's size, workspaces at 16 bytes, the units of a table at 16 (their addresses are the
+ * device's, no call can look at them; a descriptor's unit_align is 256 unless it says otherwise, and has to be 16 at least). Rows
+ * that start 16-byte aligned (base and stride) and hold a multiple of 8 values are the fastest. 4-bit weights outside a table: 4
+ * bytes; 16 is faster.
+ *
+ * Infinities and NaN stay in the rows they stand in, and what an id, a table entry or a logit masks is not read. With 4-bit
+ * weights (whose scales are finite) an infinity in a row of x may give NaN where the formula gives an infinity.
  */
 #ifndef TIERSTREAM_AMD_TSA_OPS_H
 #define TIERSTREAM_AMD_TSA_OPS_H
@@ -88,7 +93,7 @@ typedef struct tsa_experts {
   const void* part[3];             /* expert e's part p at part[p] + e x part_stride[p] bytes */
   uint64_t part_stride[3];
   const uint64_t* table;           /* ss_layer_view.table_dev: expert e's unit (its parts back to back) at table[e];
-                                      an entry of 0 (not acquired) counts as no expert */
+                                      an entry of 0 (not acquired) counts as no expert, every other is 16-byte aligned */
   const ss_dg_device_view* view;   /* host struct, copied: gated layer `gated`, read behind its ss_dg_enqueue_wait */
   uint32_t gated, reserved;
 } tsa_experts;

@@ -297,3 +297,21 @@ def test_an_infinite_row_stays_alone(ops, rows, kind):
     ops.ffn(layer.e, x, y2, ids=ids, weights=w, workspace=ws, stream=stream())
     assert torch.equal(y[1:rows - 1], y2[1:rows - 1])
     assert not bool(torch.isfinite(y2[0]).any()) and bool(torch.isnan(y2[rows - 1]).all())
+
+
+@pytest.mark.parametrize("rows", [2, 20, 300])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_an_infinite_row_stays_alone_with_4_bit_weights(ops, rows, kind):
+    g = gen(rows)
+    x, w = mat(g, rows, 96, kind).contiguous(), q4(g, 48, 96)
+    y, y2 = torch.empty((rows, 48), device="cuda"), torch.empty((rows, 48), device="cuda")
+    layer = Layer(ops, g, "stacked", 2, 96, 64, "q4")
+    ids, weights = choices(g, rows, 2, 2, holes=False)
+    z, z2 = torch.empty_like(x), torch.empty_like(x)
+    for out, block in ((y, z), (y2, z2)):
+        ops.linear(x, w, out, workspace=room(ops.linear_workspace(x, w, out)), stream=stream())
+        ops.ffn(layer.e, x, block, ids=ids, weights=weights, workspace=room(ops.ffn_workspace(layer.e, rows, 2)), stream=stream())
+        x[0, 7], x[rows - 1, 95] = math.inf, math.nan
+    assert torch.equal(y[1:rows - 1], y2[1:rows - 1]) and torch.equal(z[1:rows - 1], z2[1:rows - 1])
+    assert not bool(torch.isfinite(y2[0]).any()) and bool(torch.isnan(y2[rows - 1]).all())
+    assert not bool(torch.isfinite(z2[0]).any()) and bool(torch.isnan(z2[rows - 1]).all())

@@ -275,7 +275,8 @@ inline Combine combine_of(const Plan& p, uint32_t rows, uint32_t d, const float*
 bool aligned16(const void* p, uint64_t stride_bytes) { return (reinterpret_cast<uintptr_t>(p) | stride_bytes) % 16 == 0; }
 
 // Whether every weight row, x row and row of h starts 16-byte aligned and holds whole groups of 8 values. The addresses of
-// a table's units are the device's: its units are 256-byte aligned, as the library lays them out.
+// a table's units are the device's: that they are 16-byte aligned is the caller's part (the library lays units out at the
+// descriptor's unit_align, 256 by default).
 bool wide_weights(const ExpertMap& e) {
   for (int p = 0; p < 3; ++p) {
     if (e.form == 0 && !aligned16(e.part[p], e.stride[p])) return false;

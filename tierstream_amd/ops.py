@@ -218,7 +218,7 @@ class Experts:
 
     @classmethod
     def in_table(cls, table, d_model: int, d_ff: int, kind: str) -> "Experts":
-        """table: int64 / uint64 [n] of unit addresses on the device (ss_layer_view.table_dev)."""
+        """table: int64 / uint64 [n] of unit addresses on the device (ss_layer_view.table_dev), each 0 or 16-byte aligned."""
         if len(table.shape) != 1 or str(table.dtype) not in ("torch.int64", "torch.uint64") or not table.is_contiguous():
             raise ValueError(f"table: a contiguous array of 64-bit addresses, not {table.dtype} {tuple(table.shape)}")
         _device(table, "table")
