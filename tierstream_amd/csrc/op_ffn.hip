@@ -88,7 +88,7 @@ __global__ __launch_bounds__(256) void down_any_kernel(Plan p, const u16* h, uin
 }
 
 // ---- few rows: the weights' bytes -------------------------------------------------------------------------------------
-// The part pointers of an expert in LDS, by thread 0 of the workgroup; false (to every thread) if there is none.
+// The part pointers of an expert, in every thread that asks; false if there is none.
 __device__ __forceinline__ bool resolve(const ExpertMap& m, uint32_t e, const char* (&p)[3]) {
   if (e == ~0u) return false;
   part_pointers(m, e, p);

@@ -79,9 +79,9 @@ struct Rows16 {
   }
 };
 
-// 4-bit halves as 16-bit floating values, offset so that it takes a byte permutation: bf16 holds 16 + q as 0x4180 + 8 q,
-// half precision 1024 + q as 0x6400 + q. The offset's part of the sum is taken off with a product of x and the constant
-// (exact: -24 and -1032 have a short form in either type): bf16 keeps 24 instead of 136 so that it cancels few bits.
+// 4-bit halves as 16-bit floating values, offset so that it takes a byte permutation: bf16 holds 16 + q as 0x4180 + 8 q, half
+// precision as 0x4C00 + 64 q. The offset's part of the sum, 24 to the value q - 8, is taken off with a product of x and -24
+// (exact in either type; 16 is the least power of two above all q, so that it cancels few bits).
 template <class T>
 struct HalfBytes;
 template <>
