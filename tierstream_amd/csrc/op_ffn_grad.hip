@@ -320,7 +320,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void input_grad_tile_kernel(Plan p
 // As weight_grad_any_kernel, out[e][b][a]: a tile of columns a of `left` and b of `right` a workgroup, the sum over the expert's
 // pairs. One of the two is read through the rows' map (kMapLeft: left). Columns from n_right on belong to out2 (the
 // gradients of gate and up are one product). 128 experts of 2048 x 768 (1.2 GB written): 454 us, 2.7 TB/s: a sum of 128 pairs is
-// 4 steps, so a tile is its first loads and its stores. Tiles of 128 x 128, three a CU: 523 for 492; an expert's on one XCD: 560.
+// 4 steps, so a tile is its first loads and its stores (the matrix cores are busy 19 % of the time). Tiles of 128 x 128, three a CU: 523 for 492; an expert's on one XCD: 560.
 template <class T, class S, bool kMapLeft>
 __device__ __forceinline__ void weight_grad_tile(f32x4* memory, uint32_t block, const Plan& p, const u16* left, uint64_t left_stride,
                                                  uint32_t n_left, const u16* right, uint64_t right_stride, uint32_t n_right,

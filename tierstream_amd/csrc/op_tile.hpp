@@ -16,9 +16,9 @@
 // column of 4 rows; pairs of pieces are permuted by the row so that the 8 rows of a half wave hit all banks. In both, the
 // permutation is made by the loads' addresses: LDS itself is filled in lane order.
 //
-// 2047 rows through 4096 x 28672 with bias, tanh gelu and residual: 520 us, 920 TFLOP/s (950 in a product of 2048 rows without
-// them; 1065 with operands of zeros, which take less power). What bounds it are the loads: without them the loop runs at 1820,
-// with one operand always in L2 at 1135. Tried without gain: 256 x 256 by eight waves (a third less from L2, but one workgroup a
+// 2047 rows through 4096 x 28672 with bias, tanh gelu and residual: 520 us, 920 TFLOP/s (970 in a product of 2048 rows without
+// them; 1065 with operands of zeros, which take less power). What bounds it are the loads: without them the loop runs at 1625,
+// with one operand always in L2 at 1075; the matrix cores are busy 44 % of the time, L2 gives 12.7 TB/s. Tried without gain: 256 x 256 by eight waves (a third less from L2, but one workgroup a
 // CU, whose epilogue stands alone: 517 us for 496), lines sent for to L2 six steps ahead, buffers of whole lines (552 for 523),
 // priorities.
 #pragma once
