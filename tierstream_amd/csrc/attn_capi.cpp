@@ -90,7 +90,7 @@ void check_cached_shape(const char* what, const tsa_cache* c, const tsa_attend_c
   REQUIRE(a != nullptr, SS_E_INVALID, std::string(what) + ": null arguments");
   check_half(what, a->type);
   REQUIRE(a->q.heads >= 1 && a->q.heads <= kMaxHeads && a->q.heads % c->kv_heads == 0, SS_E_INVALID, std::string(what) + ": q's heads a multiple of the cache's");
-  REQUIRE(a->tokens < kMaxTokens, SS_E_INVALID, std::string(what) + ": below 2^24 tokens");
+  REQUIRE(a->tokens < kMaxTokens && uint64_t(a->tokens) * a->q.heads < (1u << 26), SS_E_INVALID, std::string(what) + ": below 2^24 tokens, tokens x heads below 2^26");
   REQUIRE(a->requests <= TSA_CACHE_MAX_REQUESTS, SS_E_INVALID, std::string(what) + ": at most " + std::to_string(TSA_CACHE_MAX_REQUESTS) + " requests");
   REQUIRE(a->width >= 1 && a->width < (1u << 25), SS_E_INVALID, std::string(what) + ": a table of 1..2^25 - 1 pages a request");
 }
