@@ -1,9 +1,10 @@
 // Attention of new tokens over the pages of their requests, keys and values of 4 bits.
 //
-// A workgroup takes 16 query rows that share a kept head (a request's new tokens x the heads of its group) and a run of the
-// request's pages; its four waves take pages in turn, each with the running maximum and sum of its softmax, and join at the end. Runs of
-// a request that has several are joined by a second launch. How long runs are follows on the device from all requests' lengths (a total
-// that fills the chip, no request's length sets the time), so that the host needs to know none of them.
+// A workgroup takes 16 query rows that share a kept head (a request's new tokens x the heads of its group) and a stretch of the
+// request's pages; its four waves take pages in turn, each with the running maximum and sum of its softmax, and join at the end. All
+// requests' pages are cut into equal shares, as many as workgroups work at once, so that no request's length sets the time (cut into runs
+// of one request each, a few more runs than workgroups took twice the time); what falls into several is joined by a second
+// launch. The cuts follow on the device from the lengths, of which the host needs to know none.
 //
 // A page is one contiguous piece per head and goes straight to LDS, one page ahead. Scores are S^T = K Q^T and outputs O^T = V^T P^T
 // by v_mfma_f32_16x16x32: then a lane's column is its query row in both, its scores are what the second product takes as its other
@@ -18,8 +19,8 @@ namespace tsa {
 namespace op {
 namespace {
 
-constexpr uint32_t kWaves = 4, kRows = 16, kMinRun = kWaves;  // waves, query rows and the fewest pages of a run
-constexpr uint32_t kRuns = 1024;                              // runs x kept heads that are aimed at
+constexpr uint32_t kWaves = 4, kRows = 16, kMinShare = kWaves;  // waves, query rows and the fewest pages of a workgroup
+constexpr uint32_t kGroups = 512;                               // workgroups that are at work at once (two to a CU)
 
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i32x2 lds_i32x2_t;
@@ -27,110 +28,99 @@ typedef __attribute__((address_space(3))) const u32x4 lds_words_t;
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) const u32x2 lds_two_words_t;
 typedef __attribute__((address_space(3))) const uint32_t lds_word_t;
+typedef __attribute__((address_space(3))) u16 lds_half_t;
 
 struct CachedShape {
   uint32_t group;     // query heads of a kept one
-  uint32_t runs;      // of all requests together, about
-  uint32_t parts;     // room in the workspace, in runs
+  uint32_t shares;    // workgroups of a kept head, at most
   float c;            // scale / ln 2
 };
 
 // ---- who does what --------------------------------------------------------------------------------------------------------
+// All requests' tiles of 16 query rows, one behind the other, each with its pages (one at least), are one row of pages. It is
+// cut into equal shares, a workgroup each, wherever the cuts fall. A tile inside one share is written at once; a share's piece of any
+// other is left in the workspace: at place 0 of the share where it begins with the share, at place 1 where it begins inside.
+
+// Request i's new tokens, the tokens it ends with, its tiles and their pages.
+struct Request {
+  uint32_t first, fresh, tiles, pages;
+  int32_t end;
+  Request() = default;
+  __device__ __forceinline__ Request(const tsa_attend_cached_args& a, uint32_t i, uint32_t group) {
+    const Span s = span_of(a.first, i, a.tokens);
+    first = s.begin, fresh = s.count;
+    tiles = (fresh * group + kRows - 1) / kRows;
+    end = max(0, min(a.ends[i], int32_t(a.width * kPage)));  // (width is below 2^25)
+    pages = (uint32_t(end) + kPage - 1) / kPage;
+  }
+  __device__ __forceinline__ uint32_t places() const { return pages ? pages : 1; }
+};
+
 struct Place {
-  uint32_t request, tile, run, runs, pages_a_run;
-  uint32_t part;      // place of a run in the workspace
+  uint64_t share, all;  // pages of a share and of all
+  uint64_t at;          // first page of the tile
+  uint32_t request, tile;
 };
 struct PlaceMemory {
   uint64_t pages[kWaves];
-  uint32_t sums[3][kWaves];
+  uint32_t tiles[kWaves];
   Place found;
 };
 
-__device__ __forceinline__ uint64_t lanes_up_to(uint64_t v) {
+template <class V>
+__device__ __forceinline__ V lanes_up_to(V v) {
 #pragma unroll
   for (uint32_t s = 1; s < 64; s <<= 1) {
-    const uint64_t o = __shfl_up(v, s, 64);
+    const V o = __shfl_up(v, s, 64);
     if ((threadIdx.x & 63u) >= s) v += o;
   }
   return v;
 }
 
-// Request i's new tokens, the tokens it ends with, its tiles of 16 rows and its pages.
-struct Request {
-  uint32_t first, fresh, tiles, pages;
-  int64_t end;
-  __device__ __forceinline__ Request(const tsa_attend_cached_args& a, uint32_t i, uint32_t group) {
-    const Span s = span_of(a.first, i, a.tokens);
-    first = s.begin, fresh = s.count;
-    tiles = (fresh * group + kRows - 1) / kRows;
-    end = a.ends[i];
-    const int64_t room = int64_t(a.width) * kPage;
-    end = end < 0 ? 0 : end > room ? room : end;
-    pages = uint32_t((end + kPage - 1) / kPage);
-  }
-};
-__device__ __forceinline__ uint32_t runs_of(const Request& r, uint32_t pages_a_run) {
-  return r.pages <= pages_a_run ? 1 : (r.pages + pages_a_run - 1) / pages_a_run;
-}
-
-// What number `want` is, among all runs (kByTile: among all tiles). By the whole workgroup; false: there are fewer.
+// The tile that holds the first page of share `want` (kByTile: tile number `want`). By the whole workgroup; false: there is none.
 template <bool kByTile>
-__device__ __forceinline__ bool place_of_group(const tsa_attend_cached_args& a, const CachedShape& s, uint32_t want, PlaceMemory& m, Place& out) {
+__device__ __forceinline__ bool find_place(const tsa_attend_cached_args& a, const CachedShape& s, uint32_t want, PlaceMemory& m, Place& out) {
   const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6, per = (a.requests + 64 * kWaves - 1) / (64 * kWaves);
   const uint32_t i0 = min(t * per, a.requests), i1 = min(i0 + per, a.requests);
   uint64_t pages = 0;
+  uint32_t tiles = 0;
   for (uint32_t i = i0; i < i1; ++i) {
     const Request r(a, i, s.group);
-    pages += uint64_t(r.tiles) * r.pages;
+    pages += uint64_t(r.tiles) * r.places();
+    tiles += r.tiles;
   }
-  pages = lanes_up_to(pages);
-  if (lane == 63) m.pages[wave] = pages;
-  __syncthreads();
-  pages = 0;
-#pragma unroll
-  for (uint32_t w = 0; w < kWaves; ++w) pages += m.pages[w];
-  const uint64_t even = (pages + s.runs - 1) / s.runs;
-  const uint32_t run = even < kMinRun ? kMinRun : uint32_t(even);
-  uint32_t sum[3] = {0, 0, 0};  // tiles, runs, runs that need joining
-  for (uint32_t i = i0; i < i1; ++i) {
-    const Request r(a, i, s.group);
-    const uint32_t n = runs_of(r, run);
-    sum[0] += r.tiles, sum[1] += r.tiles * n, sum[2] += n > 1 ? r.tiles * n : 0;
-  }
-  uint32_t upto[3];
-#pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    upto[k] = uint32_t(lanes_up_to(sum[k]));
-    if (lane == 63) m.sums[k][wave] = upto[k];
+  const uint64_t pages_upto = lanes_up_to(pages);
+  const uint32_t tiles_upto = kByTile ? lanes_up_to(tiles) : 0;
+  if (lane == 63) {
+    m.pages[wave] = pages_upto;
+    m.tiles[wave] = tiles_upto;
   }
   __syncthreads();
-  uint32_t all = 0, before[3] = {0, 0, 0};
+  Place p = {};
+  uint64_t page0 = pages_upto - pages;
+  uint32_t tile0 = tiles_upto - tiles, every = 0;
 #pragma unroll
   for (uint32_t w = 0; w < kWaves; ++w) {
-    all += m.sums[kByTile ? 0 : 1][w];
-#pragma unroll
-    for (int k = 0; k < 3; ++k) before[k] += w < wave ? m.sums[k][w] : 0;
+    p.all += m.pages[w];
+    every += m.tiles[w];
+    if (w < wave) page0 += m.pages[w], tile0 += m.tiles[w];
   }
-  if (want >= all) return false;
-#pragma unroll
-  for (int k = 0; k < 3; ++k) before[k] += upto[k] - sum[k];
-  const uint32_t from = before[kByTile ? 0 : 1];
-  if (want >= from && want < from + sum[kByTile ? 0 : 1]) {
-    uint32_t at = want - from, part = before[2];
+  const uint64_t even = (p.all + s.shares - 1) / s.shares;
+  p.share = even < kMinShare ? kMinShare : even;
+  const uint64_t page = uint64_t(want) * p.share;
+  if (kByTile ? want >= every : page >= p.all) return false;
+  if (kByTile ? want >= tile0 && want < tile0 + tiles : page >= page0 && page < page0 + pages) {
     for (uint32_t i = i0; i < i1; ++i) {
       const Request r(a, i, s.group);
-      const uint32_t n = runs_of(r, run), have = kByTile ? r.tiles : r.tiles * n;
-      if (at < have) {
-        m.found.request = i;
-        m.found.tile = kByTile ? at : at / n;
-        m.found.run = kByTile ? 0 : at % n;
-        m.found.runs = n;
-        m.found.pages_a_run = run;
-        m.found.part = part + (kByTile ? at * n : at);
+      const uint64_t have = uint64_t(r.tiles) * r.places();
+      if (kByTile ? want < tile0 + r.tiles : page < page0 + have) {
+        p.request = i;
+        p.tile = kByTile ? want - tile0 : uint32_t((page - page0) / r.places());
+        p.at = page0 + uint64_t(p.tile) * r.places();
+        m.found = p;
         break;
       }
-      at -= have;
-      if (n > 1) part += r.tiles * n;
+      page0 += have, tile0 += r.tiles;
     }
   }
   __syncthreads();
@@ -140,22 +130,26 @@ __device__ __forceinline__ bool place_of_group(const tsa_attend_cached_args& a, 
 
 // ---- numbers of 4 bits ----------------------------------------------------------------------------------------------------
 // The half bytes 0, 4, 1, 5, 2, 6, 3, 7 of a word as 16-bit numbers n + 128 (bf16) or n + 16 (half precision).
+// `one` and `mask` are kept in registers: as literals each would take an instruction of its own.
 template <bool kHalf>
-__device__ __forceinline__ bits8 numbers(uint32_t x) {
-  u32x4 v;
-  if constexpr (kHalf) {
-    const uint32_t mask = 0x03C003C0u, one = 0x4C004C00u;
-    v = u32x4{((x << 6) & mask) | one, ((x << 2) & mask) | one, ((x >> 2) & mask) | one, ((x >> 6) & mask) | one};
-  } else {
-    const uint32_t mask = 0x000F000Fu, one = 0x43004300u;
-    v = u32x4{(x & mask) | one, ((x >> 4) & mask) | one, ((x >> 8) & mask) | one, ((x >> 12) & mask) | one};
+struct Numbers {
+  uint32_t mask = kHalf ? 0x03C003C0u : 0x000F000Fu, one = kHalf ? 0x4C004C00u : 0x43004300u;
+  __device__ __forceinline__ Numbers() { asm("" : "+s"(mask), "+v"(one)); }
+  __device__ __forceinline__ bits8 of(uint32_t x) const {
+    u32x4 v;
+    if constexpr (kHalf) v = u32x4{((x << 6) & mask) | one, ((x << 2) & mask) | one, ((x >> 2) & mask) | one, ((x >> 6) & mask) | one};
+    else v = u32x4{(x & mask) | one, ((x >> 4) & mask) | one, ((x >> 8) & mask) | one, ((x >> 12) & mask) | one};
+    return __builtin_bit_cast(bits8, v);
   }
-  return __builtin_bit_cast(bits8, v);
-}
+};
 // Value i of a word's eight, in that order, of word g of a block.
 __device__ __forceinline__ uint32_t value_of_word(uint32_t g, uint32_t i) { return 4 * g + ((i >> 1) & 1u) * 16 + ((i & 1u) << 1) + (i >> 2); }
 
-__device__ __forceinline__ uint32_t pack(float a, float b) { return uint32_t(Bf16::down(a)) | uint32_t(Bf16::down(b)) << 16; }
+__device__ __forceinline__ uint32_t pack(float a, float b) {
+  typedef __bf16 two __attribute__((ext_vector_type(2)));
+  typedef float two_f __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((two_f{a, b}), two));
+}
 
 // The larger of a value in the four lanes of a column.
 __device__ __forceinline__ float column_max(float v) {
@@ -211,249 +205,289 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cached_kernel(tsa_cache c, tsa
   __shared__ PlaceMemory place_s;
   static_assert(sizeof(page_s) >= kWaves * kRows * D * 4, "the waves' outputs take the pages' place");
   Place at;
-  const uint32_t kept = blockIdx.x % c.kv_heads;
-  if (!place_of_group<false>(a, s, blockIdx.x / c.kv_heads, place_s, at)) return;
-  const Request r(a, at.request, s.group);
+  const uint32_t kept = blockIdx.x % c.kv_heads, share = blockIdx.x / c.kv_heads;
+  if (!find_place<false>(a, s, share, place_s, at)) return;
+  const uint64_t from = share * at.share, upto = min(from + at.share, at.all);  // this share's pages
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
-  const uint32_t x = at.tile * kRows + (lane & 15u);
-  const bool on = x < r.fresh * s.group;
-  const uint32_t token = on ? x / s.group : 0, head = kept * s.group + (on ? x % s.group : 0);
-  const int64_t limit = on ? r.end - r.fresh + token + 1 : 0;  // keys that this row attends to
-  const int64_t whole = r.end - r.fresh + 1;                   // keys that every row attends to
-
-  // this row's queries, in the order of the keys' half bytes, and what takes their offset off
-  bits8 q[NB];
-  f32x4 off[NB];
-  const u16* qp = row_of<u16>(a.q, r.first + token, head);
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    float sum = 0.0f;
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-      q[b][i] = on ? qp[32 * b + value_of_word(g, i)] : 0;
-      sum += T::up(q[b][i]);
-    }
-    sum = column_sum(sum) * (kHalf ? -24.0f : -136.0f);
-    off[b] = f32x4{sum, sum, sum, sum};
-  }
-
-  f32x4 o[2 * NB];
-#pragma unroll
-  for (int i = 0; i < 2 * NB; ++i) o[i] = f32x4{0, 0, 0, 0};
-  float top = -INFINITY, total = 0.0f;
-  const bits8 eight = {0xC308, 0xC308, 0xC308, 0xC308, 0xC308, 0xC308, 0xC308, 0xC308};  // -136
-
-  const uint32_t begin = at.run * at.pages_a_run, end = min(begin + at.pages_a_run, r.pages);
-  const int32_t* table = a.table + uint64_t(at.request) * a.table_stride;
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_offset(page_s[wave][0]));
-  // page p's bytes to buffer `to`; what is not there (or behind the end) reads page 0 or nothing and is not looked at
-  auto fetch = [&](uint32_t page, uint32_t to) {
-    const unsigned char* from = static_cast<const unsigned char*>(c.pages) + (uint64_t(page) * c.kv_heads + kept) * Page::kBytes;
-#pragma unroll
-    for (uint32_t i = 0; i < Page::kLoads; ++i) {
-      const uint32_t byte = i * 1024 + lane * 16;
-      load_to_lds(from + (byte < Page::kBytes ? byte : Page::kBytes - 16), lds0 + to * Page::kRoom + i * 1024);
-    }
-  };
-  // this wave's pages, 64 in the lanes at a time (a load in the loop would wait for the pages behind it)
-  uint32_t ids = 0, next = ~0u, buffer = 0;
-  auto turn = [&](uint32_t p, uint32_t n) {  // page p, the wave's n-th
-    if (n % 64 == 0) {
-      const uint64_t mine = uint64_t(p) + lane * kWaves;
-      ids = mine < end ? uint32_t(table[mine]) : ~0u;
-    }
-    return uint32_t(__builtin_amdgcn_readlane(ids, n % 64));
-  };
-  next = turn(begin + wave, 0);
-  if (next < c.n_pages) fetch(next, 0);
-  for (uint32_t p = begin + wave, n = 1; p < end; p += kWaves, ++n) {
-    const uint32_t page = next;
-    next = turn(p + kWaves, n);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the other buffer's reads are done
-    if (next < c.n_pages) {
-      fetch(next, buffer ^ 1);
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(Page::kLoads) : "memory");
-    } else {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
-    const uint32_t lds = lds0 + buffer * Page::kRoom;
-    buffer ^= 1;
-    if (page >= c.n_pages) continue;
-    const int64_t key0 = int64_t(p) * kPage;
-    const bool edge = key0 + int64_t(kPage) > whole;
+  const Numbers<kHalf> keys;
+  const Numbers<false> values;
+  const bits8 eight = {0xC308, 0xC308, 0xC308, 0xC308, 0xC308, 0xC308, 0xC308, 0xC308};  // -136
+  Request r(a, at.request, s.group);
+  while (true) {  // the share's tiles
+    const uint32_t x = at.tile * kRows + (lane & 15u);
+    const bool on = x < r.fresh * s.group;
+    const uint32_t token = on ? x / s.group : 0, head = kept * s.group + (on ? x % s.group : 0);
+    const int32_t limit = on ? r.end - int32_t(r.fresh) + int32_t(token) + 1 : 0;  // keys that this row attends to
+    const int32_t whole = r.end - int32_t(r.fresh) + 1;                            // keys that every row attends to
 
-    // scores: tile j holds tokens 16 j + 4 g + 0..3 of this lane's row
-    f32x4 score[4];
+    // this row's queries, in the order of the keys' half bytes, and what takes their offset off
+    bits8 q[NB];
+    f32x4 off[NB];
+    const u16* qp = row_of<u16>(a.q, r.first + token, head);
 #pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) {
-      uint32_t words[4];
-      const uint32_t key = lds + (16 * j + (lane & 15u)) * 16 * NB + g * 4 * NB;
+    for (int b = 0; b < NB; ++b) {
+      float sum = 0.0f;
 #pragma unroll
-      for (int b = 0; b < NB; ++b) words[b] = reinterpret_cast<lds_word_t*>(key)[b];
-      const Scales<NB> scale(lds + Page::kKeyScales + (16 * j + 4 * g) * 2 * NB);
-      f32x4 sum = {0, 0, 0, 0};
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const f32x4 v = T::mfma(numbers<kHalf>(words[b]), q[b], off[b]);
-#pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) sum[k] = __builtin_fmaf(scale.at(k, b), v[k], sum[k]);
+      for (uint32_t i = 0; i < 8; ++i) {
+        q[b][i] = on ? qp[32 * b + value_of_word(g, i)] : 0;
+        sum += T::up(q[b][i]);
       }
-#pragma unroll
-      for (uint32_t k = 0; k < 4; ++k) score[j][k] = sum[k] * s.c;
+      sum = column_sum(sum) * (kHalf ? -24.0f : -136.0f);
+      off[b] = f32x4{sum, sum, sum, sum};
     }
-    if (edge) {
+
+    f32x4 o[2 * NB];
+#pragma unroll
+    for (int i = 0; i < 2 * NB; ++i) o[i] = f32x4{0, 0, 0, 0};
+    float top = -INFINITY, total = 0.0f;
+
+    const uint32_t begin = uint32_t(max(from, at.at) - at.at), end = uint32_t(min(uint64_t(r.pages), upto - at.at));
+    const int32_t* table = a.table + uint64_t(at.request) * a.table_stride;
+    // page p's bytes to buffer `to`; what is not there (or behind the end) reads page 0 or nothing and is not looked at
+    auto fetch = [&](uint32_t page, uint32_t to) {
+      const unsigned char* from = static_cast<const unsigned char*>(c.pages) + (uint64_t(page) * c.kv_heads + kept) * Page::kBytes;
+#pragma unroll
+      for (uint32_t i = 0; i < Page::kLoads; ++i) {
+        const uint32_t byte = i * 1024 + lane * 16;
+        load_to_lds(from + (byte < Page::kBytes ? byte : Page::kBytes - 16), lds0 + to * Page::kRoom + i * 1024);
+      }
+    };
+    // this wave's pages, 64 in the lanes at a time (a load in the loop would wait for the pages behind it)
+    uint32_t ids = 0, next = ~0u, buffer = 0;
+    auto turn = [&](uint32_t p, uint32_t n) {  // page p, the wave's n-th
+      if (n % 64 == 0) {
+        const uint64_t mine = uint64_t(p) + lane * kWaves;
+        ids = mine < end ? uint32_t(table[mine]) : ~0u;
+      }
+      return uint32_t(__builtin_amdgcn_readlane(ids, n % 64));
+    };
+    next = turn(begin + wave, 0);
+    if (next < c.n_pages) fetch(next, 0);
+    for (uint32_t p = begin + wave, n = 1; p < end; p += kWaves, ++n) {
+      const uint32_t page = next;
+      next = turn(p + kWaves, n);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the other buffer's reads are done
+      if (next < c.n_pages) {
+        fetch(next, buffer ^ 1);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(Page::kLoads) : "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
+      const uint32_t lds = lds0 + buffer * Page::kRoom;
+      buffer ^= 1;
+      if (page >= c.n_pages) continue;
+      const int32_t key0 = int32_t(p * kPage);
+      const bool edge = key0 + int32_t(kPage) > whole;
+      // Tokens that not every row attends to must not reach the others through 0 x NaN: behind the last key the values' scales become 0;
+      // before it one that is no number becomes 0 and its key's scale NaN, which reaches only the rows that attend to it.
+      if (edge && key0 + int32_t(lane) >= whole) {
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b) {
+          lds_half_t* const scale = reinterpret_cast<lds_half_t*>(lds + Page::kValueScales + (lane * NB + b) * 2);
+          const bool none = (*scale & 0x7C00u) == 0x7C00u;
+          if (none) *reinterpret_cast<lds_half_t*>(lds + Page::kKeyScales + (lane * NB + b) * 2) = 0x7E00;
+          if (none || key0 + int32_t(lane) >= r.end) *scale = 0;
+        }
+      }
+
+      // scores: tile j holds tokens 16 j + 4 g + 0..3 of this lane's row
+      f32x4 score[4];
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        typedef uint32_t row_words __attribute__((ext_vector_type(NB)));
+        const uint32_t key = lds + (16 * j + (lane & 15u)) * 16 * NB + g * 4 * NB;
+        row_words words;
+        if constexpr (NB == 3) {  // (4-byte aligned)
+#pragma unroll
+          for (int b = 0; b < NB; ++b) words[b] = reinterpret_cast<lds_word_t*>(key)[b];
+        } else {
+          words = *reinterpret_cast<__attribute__((address_space(3))) const row_words*>(key);
+        }
+        const Scales<NB> scale(lds + Page::kKeyScales + (16 * j + 4 * g) * 2 * NB);
+        f32x4 sum = {0, 0, 0, 0};
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const f32x4 v = T::mfma(keys.of(words[b]), q[b], off[b]);
+#pragma unroll
+          for (uint32_t k = 0; k < 4; ++k) sum[k] = __builtin_fmaf(scale.at(k, b), v[k], sum[k]);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) score[j][k] = sum[k] * s.c;
+      }
+      if (edge) {
+        asm volatile("" ::: "memory");  // (kept out of the other pages' way)
+        const int32_t left = limit - key0 - int32_t(4 * g);
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j)
+#pragma unroll
+          for (uint32_t k = 0; k < 4; ++k)
+            if (int32_t(16 * j + k) >= left) score[j][k] = -INFINITY;
+      }
+
+      // the running maximum: followed only where it is passed by 2^8 (probabilities are then up to 2^8, which 32 bits and bf16 hold)
+      float most = -INFINITY;
 #pragma unroll
       for (uint32_t j = 0; j < 4; ++j)
 #pragma unroll
-        for (uint32_t k = 0; k < 4; ++k)
-          if (key0 + 16 * j + 4 * g + k >= limit) score[j][k] = -INFINITY;
-    }
-
-    // the running maximum: followed only where it is passed by 2^8 (probabilities are then up to 2^8, which 32 bits and bf16 hold)
-    float most = -INFINITY;
+        for (uint32_t k = 0; k < 4; ++k) most = fmaxf(most, score[j][k]);
+      most = column_max(most);
+      if (__any(most > top + 8.0f)) {
+        const float up = fmaxf(most, top), keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - up);
+        top = up;
+        total *= keep;
 #pragma unroll
-    for (uint32_t j = 0; j < 4; ++j)
-#pragma unroll
-      for (uint32_t k = 0; k < 4; ++k) most = fmaxf(most, score[j][k]);
-    most = column_max(most);
-    if (__any(most > top + 8.0f)) {
-      const float up = fmaxf(most, top), keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - up);
-      top = up;
-      total *= keep;
-#pragma unroll
-      for (int i = 0; i < 2 * NB; ++i) o[i] *= keep;
-    }
-    const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-    for (uint32_t j = 0; j < 4; ++j)
-#pragma unroll
-      for (uint32_t k = 0; k < 4; ++k) {
-        score[j][k] = __builtin_amdgcn_exp2f(score[j][k] - base);
-        total += score[j][k];
+        for (int i = 0; i < 2 * NB; ++i) o[i] *= keep;
       }
+      const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j)
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+          score[j][k] = __builtin_amdgcn_exp2f(score[j][k] - base);
+          total += score[j][k];
+        }
 
-    // outputs, 32 tokens a step; a lane's eight are tiles 2 t and 2 t + 1
-    Scales<NB> scales[4];
+      // outputs, 32 tokens a step; a lane's eight are tiles 2 t and 2 t + 1
+      Scales<NB> scales[4];
 #pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) scales[j] = Scales<NB>(lds + Page::kValueScales + (16 * j + 4 * g) * 2 * NB);
-    // row i of the transposed read is lane i's token: word t of the result holds, in the order of numbers(), the lane's eight of step t
-    const uint32_t i16 = lane & 15u, e = ((i16 & 3u) << 1) | ((i16 >> 2) & 1u);
-    const uint32_t row = 32 * (i16 >> 3) + (e < 4 ? 4 * g + e : 16 + 4 * g + e - 4);
+      for (uint32_t j = 0; j < 4; ++j) scales[j] = Scales<NB>(lds + Page::kValueScales + (16 * j + 4 * g) * 2 * NB);
+      // row i of the transposed read is lane i's token: word t of the result holds, in the order of Numbers, the lane's eight of step t
+      const uint32_t i16 = lane & 15u, e = ((i16 & 3u) << 1) | ((i16 >> 2) & 1u);
+      const uint32_t row = 32 * (i16 >> 3) + (e < 4 ? 4 * g + e : 16 + 4 * g + e - 4);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      i32x2 words[2];
+      for (int b = 0; b < NB; ++b) {
+        i32x2 words[2];
 #pragma unroll
-      for (uint32_t h = 0; h < 2; ++h)
-        words[h] = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-            reinterpret_cast<lds_i32x2_t*>(lds + Page::kValues + (b * kPage + row) * 16 + 8 * h));
+        for (uint32_t h = 0; h < 2; ++h)
+          words[h] = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+              reinterpret_cast<lds_i32x2_t*>(lds + Page::kValues + (b * kPage + row) * 16 + 8 * h));
 #pragma unroll
-      for (uint32_t t = 0; t < 2; ++t) {
-        float w[8];
+        for (uint32_t t = 0; t < 2; ++t) {
+          float w[8];
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) {
-          const uint32_t j = 2 * t + i / 4, k = i % 4;
-          w[i] = score[j][k] * scales[j].at(k, b);
-          if (edge && score[j][k] == 0.0f) w[i] = 0.0f;  // (what lies behind the last key may be no number)
-        }
-        const u32x4 hi = {pack(w[0], w[1]), pack(w[2], w[3]), pack(w[4], w[5]), pack(w[6], w[7])};
-        const bits8 p = __builtin_bit_cast(bits8, hi);
-#pragma unroll
-        for (uint32_t h = 0; h < 2; ++h) {
-          o[2 * b + h] = Bf16::mfma(eight, p, o[2 * b + h]);
-          o[2 * b + h] = Bf16::mfma(numbers<false>(uint32_t(words[h][t])), p, o[2 * b + h]);
-        }
-        if constexpr (kHalf) {
-          u32x4 lo;
-#pragma unroll
-          for (uint32_t i = 0; i < 4; ++i)
-            lo[i] = pack(w[2 * i] - Bf16::up(u16(hi[i])), w[2 * i + 1] - Bf16::up(u16(hi[i] >> 16)));
-          const bits8 rest = __builtin_bit_cast(bits8, lo);
+          for (uint32_t i = 0; i < 8; ++i) {
+            const uint32_t j = 2 * t + i / 4, k = i % 4;
+            w[i] = __builtin_fmaf(score[j][k], scales[j].at(k, b), 0.0f);  // (takes the scale as it is)
+          }
+          const u32x4 hi = {pack(w[0], w[1]), pack(w[2], w[3]), pack(w[4], w[5]), pack(w[6], w[7])};
+          const bits8 p = __builtin_bit_cast(bits8, hi);
 #pragma unroll
           for (uint32_t h = 0; h < 2; ++h) {
-            o[2 * b + h] = Bf16::mfma(eight, rest, o[2 * b + h]);
-            o[2 * b + h] = Bf16::mfma(numbers<false>(uint32_t(words[h][t])), rest, o[2 * b + h]);
+            o[2 * b + h] = Bf16::mfma(eight, p, o[2 * b + h]);
+            o[2 * b + h] = Bf16::mfma(values.of(uint32_t(words[h][t])), p, o[2 * b + h]);
+          }
+          if constexpr (kHalf) {
+            u32x4 lo;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i)
+              lo[i] = pack(w[2 * i] - Bf16::up(u16(hi[i])), w[2 * i + 1] - Bf16::up(u16(hi[i] >> 16)));
+            const bits8 rest = __builtin_bit_cast(bits8, lo);
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {
+              o[2 * b + h] = Bf16::mfma(eight, rest, o[2 * b + h]);
+              o[2 * b + h] = Bf16::mfma(values.of(uint32_t(words[h][t])), rest, o[2 * b + h]);
+            }
           }
         }
       }
     }
-  }
 
-  // the waves' parts together
-  total = column_sum(total);
-  if (lane < kRows) stat_s[wave][lane] = {top, total};
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __syncthreads();  // every wave is done with its pages
-  float best = -INFINITY;
+    // the waves' parts together
+    total = column_sum(total);
+    if (lane < kRows) stat_s[wave][lane] = {top, total};
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __syncthreads();  // every wave is done with its pages
+    float best = -INFINITY;
 #pragma unroll
-  for (uint32_t w = 0; w < kWaves; ++w) best = fmaxf(best, stat_s[w][lane & 15u].x);
-  const float by = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - best);
-  float* mine = reinterpret_cast<float*>(&page_s[0][0][0]) + (wave * kRows + (lane & 15u)) * D;
+    for (uint32_t w = 0; w < kWaves; ++w) best = fmaxf(best, stat_s[w][lane & 15u].x);
+    const float by = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - best);
+    float* mine = reinterpret_cast<float*>(&page_s[0][0][0]) + (wave * kRows + (lane & 15u)) * D;
 #pragma unroll
-  for (int i = 0; i < 2 * NB; ++i)
+    for (int i = 0; i < 2 * NB; ++i)
 #pragma unroll
-    for (uint32_t k = 0; k < 4; ++k)  // column 4 g + k of the tile: byte (4 g + k) / 2 of the half block, low half bytes first
-      mine[32 * (i / 2) + 8 * (i % 2) + (4 * g + k) / 2 + 16 * (k & 1u)] = o[i][k] * by;
-  __syncthreads();
-  const float* all = reinterpret_cast<const float*>(&page_s[0][0][0]);
-  for (uint32_t i = threadIdx.x; i < kRows * D; i += 64 * kWaves) {
-    const uint32_t col = i / D, d = i % D, y = at.tile * kRows + col;
-    if (y >= r.fresh * s.group) break;
-    float m = -INFINITY, sum = 0.0f, v = 0.0f;
+      for (uint32_t k = 0; k < 4; ++k)  // column 4 g + k of the tile: byte (4 g + k) / 2 of the half block, low half bytes first
+        mine[32 * (i / 2) + 8 * (i % 2) + (4 * g + k) / 2 + 16 * (k & 1u)] = o[i][k] * by;
+    __syncthreads();
+    const float* all = reinterpret_cast<const float*>(&page_s[0][0][0]);
+    for (uint32_t i = threadIdx.x; i < kRows * D; i += 64 * kWaves) {
+      const uint32_t col = i / D, d = i % D, y = at.tile * kRows + col;
+      if (y >= r.fresh * s.group) break;
+      float m = -INFINITY, sum = 0.0f, v = 0.0f;
 #pragma unroll
-    for (uint32_t w = 0; w < kWaves; ++w) m = fmaxf(m, stat_s[w][col].x);
+      for (uint32_t w = 0; w < kWaves; ++w) m = fmaxf(m, stat_s[w][col].x);
 #pragma unroll
-    for (uint32_t w = 0; w < kWaves; ++w) {
-      const float2 st = stat_s[w][col];
-      sum += st.x == -INFINITY ? 0.0f : st.y * __builtin_amdgcn_exp2f(st.x - m);
-      v += all[w * kRows * D + i];
+      for (uint32_t w = 0; w < kWaves; ++w) {
+        const float2 st = stat_s[w][col];
+        sum += st.x == -INFINITY ? 0.0f : st.y * __builtin_amdgcn_exp2f(st.x - m);
+        v += all[w * kRows * D + i];
+      }
+      if (at.at >= from && at.at + r.places() <= upto) {
+        u16* out = const_cast<u16*>(row_of<u16>(a.out, r.first + y / s.group, kept * s.group + y % s.group));
+        out[d] = T::down(sum == 0.0f ? 0.0f : v / sum);
+      } else {
+        const uint64_t part = (2 * share + (at.at > from)) * c.kv_heads + kept;
+        parts[part * kRows * D + i] = v;
+        if (d == 0) stats[part * kRows + col] = {m, sum};
+      }
     }
-    if (at.runs == 1) {
-      u16* out = const_cast<u16*>(row_of<u16>(a.out, r.first + y / s.group, kept * s.group + y % s.group));
-      out[d] = T::down(sum == 0.0f ? 0.0f : v / sum);
-    } else {
-      const uint64_t part = uint64_t(at.part) * c.kv_heads + kept;
-      parts[part * kRows * D + i] = v;
-      if (d == 0) stats[part * kRows + col] = {m, sum};
+    at.at += r.places();
+    if (at.at >= upto) break;
+    ++at.tile;
+    while (at.tile >= r.tiles) {
+      if (++at.request >= a.requests) return;  // (lengths that change meanwhile)
+      r = Request(a, at.request, s.group);
+      at.tile = 0;
     }
+    __syncthreads();  // the outputs are read, pages take their place again
   }
 }
 
-// The runs of a tile together: threads of a row take four values and every eighth run or so.
+// Sums of exponentials with their maxima: (best, total, sum) and another's.
+__device__ __forceinline__ void add(float& best, float& total, f32x4& sum, float top, float more, f32x4 v) {
+  const float up = fmaxf(best, top), base = up == -INFINITY ? 0.0f : up;
+  const float a = __builtin_amdgcn_exp2f(best - base), b = __builtin_amdgcn_exp2f(top - base);
+  best = up;
+  total = total * a + more * b;
+  sum = sum * a + v * b;
+}
+
+// The pieces of a tile together: threads of a row take four values and every eighth piece or so.
 template <class T, int NB>
 __global__ __launch_bounds__(64 * kWaves) void join_kernel(tsa_cache c, tsa_attend_cached_args a, CachedShape s, const float* parts, const float2* stats) {
   constexpr uint32_t D = 32 * NB, kLanes = D / 4, kTurns = 64 * kWaves / kLanes;
   __shared__ PlaceMemory place_s;
   __shared__ f32x4 sum_s[kTurns][kLanes];
-  __shared__ float total_s[kTurns];
+  __shared__ float2 stat_s[kTurns];
   Place at;
   const uint32_t kept = blockIdx.x % c.kv_heads;
-  if (!place_of_group<true>(a, s, blockIdx.x / c.kv_heads, place_s, at) || at.runs == 1) return;
+  if (!find_place<true>(a, s, blockIdx.x / c.kv_heads, place_s, at)) return;
   const Request r(a, at.request, s.group);
+  const uint32_t begin = uint32_t(at.at / at.share), end = uint32_t((at.at + r.places() - 1) / at.share);  // the shares that hold it
+  if (begin == end) return;
   const uint32_t turn = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
   for (uint32_t col = blockIdx.y; col < kRows; col += gridDim.y) {
     const uint32_t y = at.tile * kRows + col;
     if (y >= r.fresh * s.group) break;
-    float best = -INFINITY;
-    for (uint32_t k = 0; k < at.runs; ++k) best = fmaxf(best, stats[((uint64_t(at.part) + k) * c.kv_heads + kept) * kRows + col].x);
     f32x4 sum = {0, 0, 0, 0};
-    float total = 0.0f;
-    if (turn < kTurns)
-      for (uint32_t k = turn; k < at.runs; k += kTurns) {
-        const uint64_t part = (uint64_t(at.part) + k) * c.kv_heads + kept;
+    float total = 0.0f, best = -INFINITY;
+    if (turn < kTurns) {
+#pragma unroll 4
+      for (uint32_t k = begin + turn; k <= end; k += kTurns) {
+        const uint64_t part = (2 * k + (at.at > k * at.share)) * c.kv_heads + kept;
         const float2 st = stats[part * kRows + col];
-        const float by = st.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.x - best);
         const f32x4 v = *reinterpret_cast<const f32x4*>(parts + (part * kRows + col) * D + 4 * lane);
-        sum += v * by;
-        total += st.y * by;
+        add(best, total, sum, st.x, st.y, v);
       }
+    }
     __syncthreads();  // the last row's sums are read
     if (turn < kTurns) {
       sum_s[turn][lane] = sum;
-      if (lane == 0) total_s[turn] = total;
+      if (lane == 0) stat_s[turn] = {best, total};
     }
     __syncthreads();
     if (threadIdx.x < kLanes) {
-      for (uint32_t k = 1; k < kTurns; ++k) sum += sum_s[k][lane], total += total_s[k];
+      for (uint32_t k = 1; k < kTurns; ++k) add(best, total, sum, stat_s[k].x, stat_s[k].y, sum_s[k][lane]);
       u16* out = const_cast<u16*>(row_of<u16>(a.out, r.first + y / s.group, kept * s.group + y % s.group));
 #pragma unroll
       for (uint32_t k = 0; k < 4; ++k) out[4 * lane + k] = T::down(total == 0.0f ? 0.0f : sum[k] / total);
@@ -465,32 +499,31 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(tsa_cache c, tsa_atte
 uint64_t tiles_at_most(const tsa_attend_cached_args& a, uint32_t group) {
   return (a.requests < a.tokens ? a.requests : a.tokens) + uint64_t(a.tokens) * group / kRows;
 }
+// Shares that the pages make: kGroups together, fewer where there are not kMinShare pages for each.
 CachedShape shape_of(const tsa_cache& c, const tsa_attend_cached_args& a) {
   CachedShape s;
   s.group = a.q.heads / c.kv_heads;
-  s.runs = (kRuns + c.kv_heads - 1) / c.kv_heads;
-  // A run that needs joining stands for half a run's pages at least; a request has no more than one for each kMinRun pages.
-  const uint64_t most = tiles_at_most(a, s.group) * ((a.width + kMinRun - 1) / kMinRun);
-  s.parts = a.width <= kMinRun ? 0 : uint32_t(most < 2 * s.runs ? most : 2 * s.runs);
+  const uint64_t shares = (kGroups + c.kv_heads - 1) / c.kv_heads, most = (tiles_at_most(a, s.group) * a.width + kMinShare - 1) / kMinShare;
+  s.shares = uint32_t(shares < most ? shares : most);
   s.c = a.scale * 1.44269504f;
   return s;
 }
 
 template <class T, int NB>
 void attend_cached(const tsa_cache& c, const tsa_attend_cached_args& a, const CachedShape& s, void* workspace, hipStream_t stream) {
-  const uint64_t tiles = tiles_at_most(a, s.group), every = tiles * ((a.width + kMinRun - 1) / kMinRun), runs = tiles + s.runs;
+  const uint32_t tiles = uint32_t(tiles_at_most(a, s.group)) * c.kv_heads;
   float* parts = static_cast<float*>(workspace);
-  float2* stats = reinterpret_cast<float2*>(parts + uint64_t(s.parts) * c.kv_heads * kRows * 32 * NB);
-  hipLaunchKernelGGL((cached_kernel<T, NB>), dim3(uint32_t((every < runs ? every : runs) * c.kv_heads)), dim3(64 * kWaves), 0, stream, c, a, s, parts, stats);
-  // (a workgroup a row where there are few)
-  if (s.parts) hipLaunchKernelGGL((join_kernel<T, NB>), dim3(uint32_t(tiles * c.kv_heads), tiles * c.kv_heads < 512 ? kRows : 1), dim3(64 * kWaves), 0, stream, c, a, s, parts, stats);
+  float2* stats = reinterpret_cast<float2*>(parts + uint64_t(2) * s.shares * c.kv_heads * kRows * 32 * NB);
+  hipLaunchKernelGGL((cached_kernel<T, NB>), dim3(s.shares * c.kv_heads), dim3(64 * kWaves), 0, stream, c, a, s, parts, stats);
+  // (a workgroup a row where there are few; one share holds every tile whole)
+  if (s.shares > 1) hipLaunchKernelGGL((join_kernel<T, NB>), dim3(tiles, tiles < 512 ? kRows : 1), dim3(64 * kWaves), 0, stream, c, a, s, parts, stats);
 }
 
 }  // namespace
 }  // namespace op
 
 uint64_t attend_cached_workspace(const tsa_cache& c, const tsa_attend_cached_args& a) {
-  return uint64_t(op::shape_of(c, a).parts) * c.kv_heads * op::kRows * (4 * c.head_dim + 8);
+  return uint64_t(2) * op::shape_of(c, a).shares * c.kv_heads * op::kRows * (4 * c.head_dim + 8);
 }
 
 int launch_attend_cached(const tsa_cache& c, const tsa_attend_cached_args& a, void* workspace, hipStream_t stream) {
