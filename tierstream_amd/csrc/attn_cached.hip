@@ -20,7 +20,9 @@ namespace op {
 namespace {
 
 constexpr uint32_t kWaves = 4, kRows = 16, kMinShare = kWaves;  // waves, query rows and the fewest pages of a workgroup
-constexpr uint32_t kGroups = 512;                               // workgroups that are at work at once (two to a CU)
+// Workgroups of a CU that the registers leave room for, and of the chip.
+constexpr uint32_t per_cu(uint32_t head_dim) { return head_dim <= 64 ? 4 : 3; }
+constexpr uint32_t groups(uint32_t head_dim) { return 256 * per_cu(head_dim); }
 
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i32x2 lds_i32x2_t;
@@ -57,13 +59,12 @@ struct Request {
 };
 
 struct Place {
-  uint64_t share, all;  // pages of a share and of all
-  uint64_t at;          // first page of the tile
+  uint32_t share, all;  // pages of a share and of all
+  uint32_t at;          // first page of the tile
   uint32_t request, tile;
 };
 struct PlaceMemory {
-  uint64_t pages[kWaves];
-  uint32_t tiles[kWaves];
+  uint32_t pages[kWaves], tiles[kWaves];
   Place found;
 };
 
@@ -82,14 +83,13 @@ template <bool kByTile>
 __device__ __forceinline__ bool find_place(const tsa_attend_cached_args& a, const CachedShape& s, uint32_t want, PlaceMemory& m, Place& out) {
   const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6, per = (a.requests + 64 * kWaves - 1) / (64 * kWaves);
   const uint32_t i0 = min(t * per, a.requests), i1 = min(i0 + per, a.requests);
-  uint64_t pages = 0;
-  uint32_t tiles = 0;
+  uint32_t pages = 0, tiles = 0;
   for (uint32_t i = i0; i < i1; ++i) {
     const Request r(a, i, s.group);
-    pages += uint64_t(r.tiles) * r.places();
+    pages += r.tiles * r.places();
     tiles += r.tiles;
   }
-  const uint64_t pages_upto = lanes_up_to(pages);
+  const uint32_t pages_upto = lanes_up_to(pages);
   const uint32_t tiles_upto = kByTile ? lanes_up_to(tiles) : 0;
   if (lane == 63) {
     m.pages[wave] = pages_upto;
@@ -97,26 +97,25 @@ __device__ __forceinline__ bool find_place(const tsa_attend_cached_args& a, cons
   }
   __syncthreads();
   Place p = {};
-  uint64_t page0 = pages_upto - pages;
-  uint32_t tile0 = tiles_upto - tiles, every = 0;
+  uint32_t page0 = pages_upto - pages, tile0 = tiles_upto - tiles, every = 0;
 #pragma unroll
   for (uint32_t w = 0; w < kWaves; ++w) {
     p.all += m.pages[w];
     every += m.tiles[w];
     if (w < wave) page0 += m.pages[w], tile0 += m.tiles[w];
   }
-  const uint64_t even = (p.all + s.shares - 1) / s.shares;
+  const uint32_t even = p.all / s.shares + (p.all % s.shares != 0);
   p.share = even < kMinShare ? kMinShare : even;
-  const uint64_t page = uint64_t(want) * p.share;
+  const uint64_t page = uint64_t(want) * p.share;  // (past all of them, perhaps by far)
   if (kByTile ? want >= every : page >= p.all) return false;
   if (kByTile ? want >= tile0 && want < tile0 + tiles : page >= page0 && page < page0 + pages) {
     for (uint32_t i = i0; i < i1; ++i) {
       const Request r(a, i, s.group);
-      const uint64_t have = uint64_t(r.tiles) * r.places();
+      const uint32_t have = r.tiles * r.places();
       if (kByTile ? want < tile0 + r.tiles : page < page0 + have) {
         p.request = i;
         p.tile = kByTile ? want - tile0 : uint32_t((page - page0) / r.places());
-        p.at = page0 + uint64_t(p.tile) * r.places();
+        p.at = page0 + p.tile * r.places();
         m.found = p;
         break;
       }
@@ -162,11 +161,28 @@ __device__ __forceinline__ float column_sum(float v) {
 }
 
 // ---- the pages --------------------------------------------------------------------------------------------------------------
+// A page of a head in memory, and in LDS, where the scales have room for whole loads.
 template <int NB>
-struct PageBytes {
-  static constexpr uint32_t kBytes = 72 * 32 * NB, kLoads = (kBytes + 1023) / 1024, kRoom = kLoads * 1024;
-  static constexpr uint32_t kKeyScales = 1024 * NB, kValueScales = 1152 * NB, kValues = 1280 * NB;
+struct Page {
+  static constexpr uint32_t kBytes = 2304 * NB, kKeyScalesAt = 1024 * NB, kValueScalesAt = 1152 * NB, kValuesAt = 1280 * NB;
+  static constexpr uint32_t kScaleLoads = (NB + 1) / 2, kLoads = NB + kScaleLoads;  // of the keys' half, and of the values'
+  static constexpr uint32_t kKeyScales = 1024 * NB, kValueScales = kKeyScales + 256 * kScaleLoads, kValues = kValueScales + 256 * kScaleLoads,
+                            kRoom = kValues + 1024 * NB;
 };
+
+// 64 lanes x 4 bytes to LDS at `at` (the same in every lane) in lane order.
+__device__ __forceinline__ void load_words_to_lds(const void* g, uint32_t at) {
+  asm volatile(
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dword %0, off"
+      :
+      : "v"(g), "s"(at)
+      : "memory", "m0");
+}
+__device__ __forceinline__ void reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void loads_left() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
 // The scales of four tokens, from LDS.
 template <int NB>
@@ -196,20 +212,20 @@ struct Scales {
 };
 
 template <class T, int NB>
-__global__ __launch_bounds__(64 * kWaves, 2) void cached_kernel(tsa_cache c, tsa_attend_cached_args a, CachedShape s, float* parts, float2* stats) {
-  typedef PageBytes<NB> Page;
+__global__ __launch_bounds__(64 * kWaves, per_cu(32 * NB)) void cached_kernel(tsa_cache c, tsa_attend_cached_args a, CachedShape s, float* parts, float2* stats) {
+  typedef Page<NB> P;
   constexpr bool kHalf = std::is_same_v<T, F16>;
   constexpr uint32_t D = 32 * NB;
-  __shared__ __attribute__((aligned(16))) unsigned char page_s[kWaves][2][Page::kRoom];
+  __shared__ __attribute__((aligned(16))) unsigned char page_s[kWaves][P::kRoom];
   __shared__ float2 stat_s[kWaves][kRows];
   __shared__ PlaceMemory place_s;
-  static_assert(sizeof(page_s) >= kWaves * kRows * D * 4, "the waves' outputs take the pages' place");
+  static_assert(P::kRoom >= kRows * D * 4, "a wave's outputs take its page's place");
   Place at;
   const uint32_t kept = blockIdx.x % c.kv_heads, share = blockIdx.x / c.kv_heads;
   if (!find_place<false>(a, s, share, place_s, at)) return;
-  const uint64_t from = share * at.share, upto = min(from + at.share, at.all);  // this share's pages
+  const uint32_t from = share * at.share, upto = min(from + at.share, at.all);  // this share's pages
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
-  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_offset(page_s[wave][0]));
+  const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_offset(page_s[wave]));
   const Numbers<kHalf> keys;
   const Numbers<false> values;
   const bits8 eight = {0xC308, 0xC308, 0xC308, 0xC308, 0xC308, 0xC308, 0xC308, 0xC308};  // -136
@@ -242,51 +258,53 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cached_kernel(tsa_cache c, tsa
     for (int i = 0; i < 2 * NB; ++i) o[i] = f32x4{0, 0, 0, 0};
     float top = -INFINITY, total = 0.0f;
 
-    const uint32_t begin = uint32_t(max(from, at.at) - at.at), end = uint32_t(min(uint64_t(r.pages), upto - at.at));
+    const uint32_t begin = max(from, at.at) - at.at, end = min(r.pages, upto - at.at);
     const int32_t* table = a.table + uint64_t(at.request) * a.table_stride;
-    // page p's bytes to buffer `to`; what is not there (or behind the end) reads page 0 or nothing and is not looked at
-    auto fetch = [&](uint32_t page, uint32_t to) {
-      const unsigned char* from = static_cast<const unsigned char*>(c.pages) + (uint64_t(page) * c.kv_heads + kept) * Page::kBytes;
+    // Half a page to LDS, keys or values. While the keys of one are multiplied its values are on their way, and while these are the next
+    // page's keys: one buffer is enough for that, and three or four workgroups fit a CU.
+    auto fetch = [&](uint32_t page, bool value) {
+      const unsigned char* at = static_cast<const unsigned char*>(c.pages) + (uint64_t(page) * c.kv_heads + kept) * P::kBytes;
+      const unsigned char* scales = at + (value ? P::kValueScalesAt : P::kKeyScalesAt);
 #pragma unroll
-      for (uint32_t i = 0; i < Page::kLoads; ++i) {
-        const uint32_t byte = i * 1024 + lane * 16;
-        load_to_lds(from + (byte < Page::kBytes ? byte : Page::kBytes - 16), lds0 + to * Page::kRoom + i * 1024);
-      }
+      for (uint32_t i = 0; i < uint32_t(NB); ++i) load_to_lds(at + (value ? P::kValuesAt : 0) + i * 1024 + lane * 16, lds + (value ? P::kValues : 0) + i * 1024);
+#pragma unroll
+      for (uint32_t i = 0; i < P::kScaleLoads; ++i)  // (what a last half load is too much stays in its room)
+        load_words_to_lds(scales + min(i * 256 + lane * 4, 128u * NB - 4), lds + (value ? P::kValueScales : P::kKeyScales) + i * 256);
     };
-    // this wave's pages, 64 in the lanes at a time (a load in the loop would wait for the pages behind it)
-    uint32_t ids = 0, next = ~0u, buffer = 0;
-    auto turn = [&](uint32_t p, uint32_t n) {  // page p, the wave's n-th
-      if (n % 64 == 0) {
-        const uint64_t mine = uint64_t(p) + lane * kWaves;
-        ids = mine < end ? uint32_t(table[mine]) : ~0u;
+    // this wave's pages, 64 in the lanes at a time (a load in the loop would wait for the pages behind it), absent ones left out
+    uint32_t ids = 0, p = begin + wave, turn = 0;
+    auto page_here = [&]() {
+      for (; p < end; p += kWaves, ++turn) {
+        if (turn % 64 == 0) {
+          const uint64_t mine = uint64_t(p) + lane * kWaves;
+          ids = mine < end ? uint32_t(table[mine]) : ~0u;
+        }
+        const uint32_t page = uint32_t(__builtin_amdgcn_readlane(ids, turn % 64));
+        if (page < c.n_pages) return page;
       }
-      return uint32_t(__builtin_amdgcn_readlane(ids, n % 64));
+      return ~0u;
     };
-    next = turn(begin + wave, 0);
-    if (next < c.n_pages) fetch(next, 0);
-    for (uint32_t p = begin + wave, n = 1; p < end; p += kWaves, ++n) {
-      const uint32_t page = next;
-      next = turn(p + kWaves, n);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the other buffer's reads are done
-      if (next < c.n_pages) {
-        fetch(next, buffer ^ 1);
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(Page::kLoads) : "memory");
-      } else {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      }
-      const uint32_t lds = lds0 + buffer * Page::kRoom;
-      buffer ^= 1;
-      if (page >= c.n_pages) continue;
+    uint32_t page = page_here();
+    if (p < end) {
+      fetch(page, false);
+      fetch(page, true);
+    }
+    while (p < end) {
       const int32_t key0 = int32_t(p * kPage);
       const bool edge = key0 + int32_t(kPage) > whole;
+      p += kWaves, ++turn;
+      page = page_here();  // the next one
+      const bool more = p < end;
+      loads_left<P::kLoads>();
       // Tokens that not every row attends to must not reach the others through 0 x NaN: behind the last key the values' scales become 0;
       // before it one that is no number becomes 0 and its key's scale NaN, which reaches only the rows that attend to it.
+      if (edge) loads_left<0>();
       if (edge && key0 + int32_t(lane) >= whole) {
 #pragma unroll
         for (uint32_t b = 0; b < NB; ++b) {
-          lds_half_t* const scale = reinterpret_cast<lds_half_t*>(lds + Page::kValueScales + (lane * NB + b) * 2);
+          lds_half_t* const scale = reinterpret_cast<lds_half_t*>(lds + P::kValueScales + (lane * NB + b) * 2);
           const bool none = (*scale & 0x7C00u) == 0x7C00u;
-          if (none) *reinterpret_cast<lds_half_t*>(lds + Page::kKeyScales + (lane * NB + b) * 2) = 0x7E00;
+          if (none) *reinterpret_cast<lds_half_t*>(lds + P::kKeyScales + (lane * NB + b) * 2) = 0x7E00;
           if (none || key0 + int32_t(lane) >= r.end) *scale = 0;
         }
       }
@@ -304,7 +322,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cached_kernel(tsa_cache c, tsa
         } else {
           words = *reinterpret_cast<__attribute__((address_space(3))) const row_words*>(key);
         }
-        const Scales<NB> scale(lds + Page::kKeyScales + (16 * j + 4 * g) * 2 * NB);
+        const Scales<NB> scale(lds + P::kKeyScales + (16 * j + 4 * g) * 2 * NB);
         f32x4 sum = {0, 0, 0, 0};
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -324,6 +342,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cached_kernel(tsa_cache c, tsa
           for (uint32_t k = 0; k < 4; ++k)
             if (int32_t(16 * j + k) >= left) score[j][k] = -INFINITY;
       }
+
+      reads_done();
+      if (more) fetch(page, false);
 
       // the running maximum: followed only where it is passed by 2^8 (probabilities are then up to 2^8, which 32 bits and bf16 hold)
       float most = -INFINITY;
@@ -349,33 +370,31 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cached_kernel(tsa_cache c, tsa
         }
 
       // outputs, 32 tokens a step; a lane's eight are tiles 2 t and 2 t + 1
-      Scales<NB> scales[4];
-#pragma unroll
-      for (uint32_t j = 0; j < 4; ++j) scales[j] = Scales<NB>(lds + Page::kValueScales + (16 * j + 4 * g) * 2 * NB);
-      // row i of the transposed read is lane i's token: word t of the result holds, in the order of Numbers, the lane's eight of step t
+      if (more) loads_left<P::kLoads>();
+      else loads_left<0>();
+      // row i of the transposed read is lane i's token, of both halves of a block: a word of the result holds, in the order of Numbers, the
+      // lane's eight tokens of one column
       const uint32_t i16 = lane & 15u, e = ((i16 & 3u) << 1) | ((i16 >> 2) & 1u);
-      const uint32_t row = 32 * (i16 >> 3) + (e < 4 ? 4 * g + e : 16 + 4 * g + e - 4);
+      const uint32_t row = (e < 4 ? 4 * g + e : 16 + 4 * g + e - 4) * 16 + 8 * (i16 >> 3);
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        i32x2 words[2];
+      for (uint32_t t = 0; t < 2; ++t) {
+        Scales<NB> scales[2];
 #pragma unroll
-        for (uint32_t h = 0; h < 2; ++h)
-          words[h] = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-              reinterpret_cast<lds_i32x2_t*>(lds + Page::kValues + (b * kPage + row) * 16 + 8 * h));
+        for (uint32_t j = 0; j < 2; ++j) scales[j] = Scales<NB>(lds + P::kValueScales + (32 * t + 16 * j + 4 * g) * 2 * NB);
 #pragma unroll
-        for (uint32_t t = 0; t < 2; ++t) {
+        for (int b = 0; b < NB; ++b) {
+          const i32x2 words = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+              reinterpret_cast<lds_i32x2_t*>(lds + P::kValues + b * 1024 + t * 512 + row));
           float w[8];
 #pragma unroll
-          for (uint32_t i = 0; i < 8; ++i) {
-            const uint32_t j = 2 * t + i / 4, k = i % 4;
-            w[i] = __builtin_fmaf(score[j][k], scales[j].at(k, b), 0.0f);  // (takes the scale as it is)
-          }
+          for (uint32_t i = 0; i < 8; ++i)
+            w[i] = __builtin_fmaf(score[2 * t + i / 4][i % 4], scales[i / 4].at(i % 4, b), 0.0f);  // (takes the scale as it is)
           const u32x4 hi = {pack(w[0], w[1]), pack(w[2], w[3]), pack(w[4], w[5]), pack(w[6], w[7])};
-          const bits8 p = __builtin_bit_cast(bits8, hi);
+          const bits8 p16 = __builtin_bit_cast(bits8, hi);
 #pragma unroll
           for (uint32_t h = 0; h < 2; ++h) {
-            o[2 * b + h] = Bf16::mfma(eight, p, o[2 * b + h]);
-            o[2 * b + h] = Bf16::mfma(values.of(uint32_t(words[h][t])), p, o[2 * b + h]);
+            o[2 * b + h] = Bf16::mfma(eight, p16, o[2 * b + h]);
+            o[2 * b + h] = Bf16::mfma(values.of(uint32_t(words[h])), p16, o[2 * b + h]);
           }
           if constexpr (kHalf) {
             u32x4 lo;
@@ -386,11 +405,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cached_kernel(tsa_cache c, tsa
 #pragma unroll
             for (uint32_t h = 0; h < 2; ++h) {
               o[2 * b + h] = Bf16::mfma(eight, rest, o[2 * b + h]);
-              o[2 * b + h] = Bf16::mfma(values.of(uint32_t(words[h][t])), rest, o[2 * b + h]);
+              o[2 * b + h] = Bf16::mfma(values.of(uint32_t(words[h])), rest, o[2 * b + h]);
             }
           }
         }
       }
+      reads_done();
+      if (more) fetch(page, true);
     }
 
     // the waves' parts together
@@ -402,14 +423,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cached_kernel(tsa_cache c, tsa
 #pragma unroll
     for (uint32_t w = 0; w < kWaves; ++w) best = fmaxf(best, stat_s[w][lane & 15u].x);
     const float by = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - best);
-    float* mine = reinterpret_cast<float*>(&page_s[0][0][0]) + (wave * kRows + (lane & 15u)) * D;
+    float* mine = reinterpret_cast<float*>(page_s[wave]) + (lane & 15u) * D;
 #pragma unroll
     for (int i = 0; i < 2 * NB; ++i)
 #pragma unroll
       for (uint32_t k = 0; k < 4; ++k)  // column 4 g + k of the tile: byte (4 g + k) / 2 of the half block, low half bytes first
         mine[32 * (i / 2) + 8 * (i % 2) + (4 * g + k) / 2 + 16 * (k & 1u)] = o[i][k] * by;
     __syncthreads();
-    const float* all = reinterpret_cast<const float*>(&page_s[0][0][0]);
     for (uint32_t i = threadIdx.x; i < kRows * D; i += 64 * kWaves) {
       const uint32_t col = i / D, d = i % D, y = at.tile * kRows + col;
       if (y >= r.fresh * s.group) break;
@@ -420,7 +440,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cached_kernel(tsa_cache c, tsa
       for (uint32_t w = 0; w < kWaves; ++w) {
         const float2 st = stat_s[w][col];
         sum += st.x == -INFINITY ? 0.0f : st.y * __builtin_amdgcn_exp2f(st.x - m);
-        v += all[w * kRows * D + i];
+        v += reinterpret_cast<const float*>(page_s[w])[i];
       }
       if (at.at >= from && at.at + r.places() <= upto) {
         u16* out = const_cast<u16*>(row_of<u16>(a.out, r.first + y / s.group, kept * s.group + y % s.group));
@@ -463,7 +483,7 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(tsa_cache c, tsa_atte
   const uint32_t kept = blockIdx.x % c.kv_heads;
   if (!find_place<true>(a, s, blockIdx.x / c.kv_heads, place_s, at)) return;
   const Request r(a, at.request, s.group);
-  const uint32_t begin = uint32_t(at.at / at.share), end = uint32_t((at.at + r.places() - 1) / at.share);  // the shares that hold it
+  const uint32_t begin = at.at / at.share, end = (at.at + r.places() - 1) / at.share;  // the shares that hold it
   if (begin == end) return;
   const uint32_t turn = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
   for (uint32_t col = blockIdx.y; col < kRows; col += gridDim.y) {
@@ -499,11 +519,11 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(tsa_cache c, tsa_atte
 uint64_t tiles_at_most(const tsa_attend_cached_args& a, uint32_t group) {
   return (a.requests < a.tokens ? a.requests : a.tokens) + uint64_t(a.tokens) * group / kRows;
 }
-// Shares that the pages make: kGroups together, fewer where there are not kMinShare pages for each.
+// Shares that the pages make: groups() together, fewer where there are not kMinShare pages for each.
 CachedShape shape_of(const tsa_cache& c, const tsa_attend_cached_args& a) {
   CachedShape s;
   s.group = a.q.heads / c.kv_heads;
-  const uint64_t shares = (kGroups + c.kv_heads - 1) / c.kv_heads, most = (tiles_at_most(a, s.group) * a.width + kMinShare - 1) / kMinShare;
+  const uint64_t shares = (groups(c.head_dim) + c.kv_heads - 1) / c.kv_heads, most = (tiles_at_most(a, s.group) * a.width + kMinShare - 1) / kMinShare;
   s.shares = uint32_t(shares < most ? shares : most);
   s.c = a.scale * 1.44269504f;
   return s;
@@ -516,7 +536,8 @@ void attend_cached(const tsa_cache& c, const tsa_attend_cached_args& a, const Ca
   float2* stats = reinterpret_cast<float2*>(parts + uint64_t(2) * s.shares * c.kv_heads * kRows * 32 * NB);
   hipLaunchKernelGGL((cached_kernel<T, NB>), dim3(s.shares * c.kv_heads), dim3(64 * kWaves), 0, stream, c, a, s, parts, stats);
   // (a workgroup a row where there are few; one share holds every tile whole)
-  if (s.shares > 1) hipLaunchKernelGGL((join_kernel<T, NB>), dim3(tiles, tiles < 512 ? kRows : 1), dim3(64 * kWaves), 0, stream, c, a, s, parts, stats);
+  const uint32_t rows = tiles * kRows <= 1024 ? kRows : tiles < 1024 ? 1024 / tiles : 1;
+  if (s.shares > 1) hipLaunchKernelGGL((join_kernel<T, NB>), dim3(tiles, rows), dim3(64 * kWaves), 0, stream, c, a, s, parts, stats);
 }
 
 }  // namespace

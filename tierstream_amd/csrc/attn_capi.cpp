@@ -93,6 +93,8 @@ void check_cached_shape(const char* what, const tsa_cache* c, const tsa_attend_c
   REQUIRE(a->tokens < kMaxTokens && uint64_t(a->tokens) * a->q.heads < (1u << 26), SS_E_INVALID, std::string(what) + ": below 2^24 tokens, tokens x heads below 2^26");
   REQUIRE(a->requests <= TSA_CACHE_MAX_REQUESTS, SS_E_INVALID, std::string(what) + ": at most " + std::to_string(TSA_CACHE_MAX_REQUESTS) + " requests");
   REQUIRE(a->width >= 1 && a->width < (1u << 25), SS_E_INVALID, std::string(what) + ": a table of 1..2^25 - 1 pages a request");
+  const uint64_t tiles = (a->requests < a->tokens ? a->requests : a->tokens) + uint64_t(a->tokens) * (a->q.heads / c->kv_heads) / 16;
+  REQUIRE(tiles * a->width < (uint64_t(1) << 31), SS_E_INVALID, std::string(what) + ": the tables of all tiles of 16 query rows below 2^31 pages");
 }
 
 }  // namespace
