@@ -170,16 +170,6 @@ struct Page {
                             kRoom = kValues + 1024 * NB;
 };
 
-// 64 lanes x 4 bytes to LDS at `at` (the same in every lane) in lane order.
-__device__ __forceinline__ void load_words_to_lds(const void* g, uint32_t at) {
-  asm volatile(
-      "s_mov_b32 m0, %1\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dword %0, off"
-      :
-      : "v"(g), "s"(at)
-      : "memory", "m0");
-}
 __device__ __forceinline__ void reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void loads_left() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }

@@ -63,6 +63,9 @@ void check_attend_shape(const char* what, const tsa_attend_args* a) {
   REQUIRE(a->tokens < kMaxTokens && a->k_tokens < kMaxTokens && a->sequences < kMaxTokens, SS_E_INVALID, std::string(what) + ": below 2^24 tokens and sequences");
   REQUIRE(a->q.heads >= 1 && a->q.heads <= kMaxHeads && a->k.heads >= 1 && a->q.heads % a->k.heads == 0 && a->v.heads == a->k.heads, SS_E_INVALID,
           std::string(what) + ": q's heads a multiple of k's and v's");
+  REQUIRE(uint64_t(a->tokens) * a->q.heads < (uint64_t(1) << 30) && uint64_t(a->k_tokens) * a->k.heads < (uint64_t(1) << 30) &&
+              uint64_t(a->sequences) * a->q.heads < (1u << 23),
+          SS_E_INVALID, std::string(what) + ": tokens x heads below 2^30, sequences x heads below 2^23");
   REQUIRE(a->causal <= 1 && std::isfinite(a->scale), SS_E_INVALID, std::string(what) + ": causal 0 or 1, a finite scale");
 }
 

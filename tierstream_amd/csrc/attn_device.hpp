@@ -41,10 +41,15 @@ __device__ __forceinline__ const T* row_of(const tsa_heads& h, uint64_t token, u
   return static_cast<const T*>(h.p) + token * h.token_stride + head * h.head_stride;
 }
 
-__device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) v += __shfl_xor(v, s, 64);
-  return v;
+// 64 lanes x 4 bytes to LDS at `at` (the same in every lane) in lane order.
+__device__ __forceinline__ void load_words_to_lds(const void* g, uint32_t at) {
+  asm volatile(
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dword %0, off"
+      :
+      : "v"(g), "s"(at)
+      : "memory", "m0");
 }
 
 }  // namespace op

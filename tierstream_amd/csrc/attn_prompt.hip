@@ -1,122 +1,152 @@
-// Attention over packed sequences and its gradients, a wave a row: the running maximum and sum of its softmax, a key at a time.
-#include "attn_device.hpp"
+// Attention over packed sequences: O^T = V^T P^T with S^T = K Q^T, 128 queries of a head a workgroup (32 a wave), keys and values in tiles
+// of 64 through LDS, the next one on its way while one is multiplied. A lane's column is its query in scores and outputs alike: the
+// softmax runs in the lane's own registers, and its probabilities are the second product's operand as they stand.
+#include "attn_tile.hpp"
 
 namespace tsa {
 namespace op {
 namespace {
 
-template <class T>
-struct Row {
-  float v[2];
-  __device__ __forceinline__ Row(const tsa_heads& h, uint64_t t, uint32_t head, uint32_t dim) {
-    const u16* p = row_of<u16>(h, t, head);
-    for (int k = 0; k < 2; ++k) v[k] = threadIdx.x + 64 * k < dim ? T::up(p[threadIdx.x + 64 * k]) : 0.0f;
+template <class T, int kD, bool kAligned>
+__global__ __launch_bounds__(64 * kTileWaves, 2) void attend_kernel(tsa_attend_args a, float c) {
+  typedef TileShapes<kD> S;
+  constexpr float kUp = std::is_same_v<T, F16> ? 7.0f : 0.0f;  // half precision: probabilities up to 2^15, so that small ones keep their bits
+  __shared__ __attribute__((aligned(16))) unsigned char tile_s[2][2][S::kBytes];  // keys and values, two of each
+  __shared__ OwnTileMemory own_s;
+  __shared__ __attribute__((aligned(16))) float mark_s[kTile];
+  OwnTile own;
+  const uint32_t head = head_of_group(blockIdx.x % a.q.heads, a.q.heads), kept = head / (a.q.heads / a.k.heads);
+  if (!find_own_tile<true>(a.first, a.sequences, a.tokens, blockIdx.x / a.q.heads, own_s, own)) return;
+  const Span qs = span_of(a.first, own.sequence, a.tokens), ks = span_of(a.k_first ? a.k_first : a.first, own.sequence, a.k_tokens);
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  const uint32_t row0 = own.row0 + wave * kOwn, row = row0 + (lane & 31u);
+  const bool on = row < qs.count;
+  // keys that a row attends to, and those that every row and any row of this wave, and any of the workgroup does
+  const int32_t ahead = a.causal ? int32_t(ks.count) - int32_t(qs.count) + 1 : 0;
+  auto keys_of = [&](uint32_t r) {
+    const int32_t n = a.causal ? int32_t(r) + ahead : int32_t(ks.count);
+    return n < 0 ? 0u : min(uint32_t(n), ks.count);
+  };
+  const uint32_t limit = on ? keys_of(row) : 0, all_rows = keys_of(own.row0), whole = keys_of(row0), any = row0 < qs.count ? keys_of(min(row0 + kOwn, qs.count) - 1) : 0;
+  const uint32_t end = keys_of(min(own.row0 + kTileOwn, qs.count) - 1);
+
+  // a negative scale turns the queries' signs, a scale of 0 takes them away
+  const OwnRows<kD, kAligned> raw(a.q, uint64_t(qs.begin) + row, head, a.head_dim, on);
+  bits8 q[kD / 16];
+#pragma unroll
+  for (uint32_t k = 0; k < kD / 16; ++k) q[k] = c == 0.0f ? bits8{0, 0, 0, 0, 0, 0, 0, 0} : raw.v[k] ^ u16(c < 0.0f ? 0x8000 : 0);
+  c = c == 0.0f ? 1.0f : fabsf(c);
+
+  const TileReads<kD> reads;
+  const TileLoads<kD, kAligned> keys(a.k, ks.begin, kept, a.head_dim), values(a.v, ks.begin, kept, a.head_dim);
+  const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_offset(tile_s));
+  f32x16 o[kD / 32];
+#pragma unroll
+  for (int t = 0; t < kD / 32; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+  float top = -INFINITY, total = 0.0f;
+  if (end) {
+    keys.fetch(0, ks.count, lds);
+    values.fetch(0, ks.count, lds + S::kBytes);
   }
-  __device__ __forceinline__ float dot(const Row& o) const { return lanes_sum(v[0] * o.v[0] + v[1] * o.v[1]); }
-};
-template <class T>
-__device__ __forceinline__ void put(const tsa_heads& h, uint64_t t, uint32_t head, uint32_t dim, const float (&v)[2], float by) {
-  u16* p = const_cast<u16*>(row_of<u16>(h, t, head));
-  for (int k = 0; k < 2; ++k)
-    if (threadIdx.x + 64 * k < dim) p[threadIdx.x + 64 * k] = T::down(v[k] * by);
-}
-
-template <class T>
-__global__ __launch_bounds__(64) void attend_kernel(tsa_attend_args a) {
-  const uint32_t r = blockIdx.x, h = blockIdx.y, kept = h / (a.q.heads / a.k.heads);
-  const uint32_t i = sequence_of(a.first, a.sequences, r);
-  if (i >= a.sequences) return;
-  const Span q = span_of(a.first, i, a.tokens), k = span_of(a.k_first ? a.k_first : a.first, i, a.k_tokens);
-  if (r < q.begin || r >= q.begin + q.count) return;
-  const int64_t keys = a.causal ? int64_t(k.count) - q.count + (r - q.begin) + 1 : k.count;
-  const Row<T> x(a.q, r, h, a.head_dim);
-  float o[2] = {0, 0}, top = -INFINITY, sum = 0;
-  for (int64_t j = 0; j < keys; ++j) {
-    const float score = x.dot(Row<T>(a.k, k.begin + j, kept, a.head_dim)) * a.scale;
-    const Row<T> v(a.v, k.begin + j, kept, a.head_dim);
-    const float next = fmaxf(top, score), keep = top == -INFINITY ? 0.0f : expf(top - next), w = score == -INFINITY ? 0.0f : expf(score - next);
-    sum = sum * keep + w;
-    for (int e = 0; e < 2; ++e) o[e] = o[e] * keep + w * v.v[e];
-    top = next;
-  }
-  put<T>(a.out, r, h, a.head_dim, o, sum == 0 ? 0.0f : 1.0f / sum);
-  if (a.lse && threadIdx.x == 0) a.lse[uint64_t(h) * a.tokens + r] = sum == 0 ? -INFINITY : top + logf(sum);
-}
-
-// p and ds of row r and key j.
-template <class T>
-__device__ __forceinline__ float2 pair_of(const tsa_attend_grad_args& g, const Row<T>& q, const Row<T>& k, const Row<T>& v, const Row<T>& out,
-                                          const Row<T>& dout, float lse) {
-  const float score = q.dot(k) * g.f.scale, p = lse == -INFINITY ? 0.0f : expf(score - lse);
-  return {p, p * (dout.dot(v) - dout.dot(out)) * g.f.scale};
-}
-
-template <class T>
-__global__ __launch_bounds__(64) void queries_kernel(tsa_attend_grad_args g) {
-  const tsa_attend_args& a = g.f;
-  const uint32_t r = blockIdx.x, h = blockIdx.y, kept = h / (a.q.heads / a.k.heads);
-  const uint32_t i = sequence_of(a.first, a.sequences, r);
-  if (i >= a.sequences) return;
-  const Span q = span_of(a.first, i, a.tokens), k = span_of(a.k_first ? a.k_first : a.first, i, a.k_tokens);
-  if (r < q.begin || r >= q.begin + q.count) return;
-  const int64_t keys = a.causal ? int64_t(k.count) - q.count + (r - q.begin) + 1 : k.count;
-  const Row<T> x(a.q, r, h, a.head_dim), out(a.out, r, h, a.head_dim), dout(g.dout, r, h, a.head_dim);
-  const float lse = a.lse[uint64_t(h) * a.tokens + r];
-  float o[2] = {0, 0};
-  for (int64_t j = 0; j < keys; ++j) {
-    const Row<T> key(a.k, k.begin + j, kept, a.head_dim), v(a.v, k.begin + j, kept, a.head_dim);
-    const float2 w = pair_of(g, x, key, v, out, dout, lse);
-    for (int e = 0; e < 2; ++e) o[e] += w.y * key.v[e];
-  }
-  put<T>(g.dq, r, h, a.head_dim, o, 1.0f);
-}
-
-template <class T>
-__global__ __launch_bounds__(64) void keys_kernel(tsa_attend_grad_args g) {
-  const tsa_attend_args& a = g.f;
-  const uint32_t r = blockIdx.x, kept = blockIdx.y, group = a.q.heads / a.k.heads;
-  const int32_t* k_first = a.k_first ? a.k_first : a.first;
-  const uint32_t i = sequence_of(k_first, a.sequences, r);
-  if (i >= a.sequences) return;
-  const Span q = span_of(a.first, i, a.tokens), k = span_of(k_first, i, a.k_tokens);
-  if (r < k.begin || r >= k.begin + k.count) return;
-  const Row<T> key(a.k, r, kept, a.head_dim), v(a.v, r, kept, a.head_dim);
-  float dk[2] = {0, 0}, dv[2] = {0, 0};
-  const int64_t from = a.causal ? int64_t(r - k.begin) - (int64_t(k.count) - q.count) : 0;  // the first query that sees it
-  for (uint32_t h = kept * group; h < (kept + 1) * group; ++h)
-    for (int64_t t = from < 0 ? 0 : from; t < q.count; ++t) {
-      const uint64_t row = q.begin + t;
-      const Row<T> x(a.q, row, h, a.head_dim), out(a.out, row, h, a.head_dim), dout(g.dout, row, h, a.head_dim);
-      const float2 w = pair_of(g, x, key, v, out, dout, a.lse[uint64_t(h) * a.tokens + row]);
-      for (int e = 0; e < 2; ++e) dk[e] += w.y * x.v[e], dv[e] += w.x * dout.v[e];
+  for (uint32_t key0 = 0, buffer = 0; key0 < end; key0 += kTile, buffer ^= 1) {
+    tile_ready();
+    const uint32_t k_at = lds + buffer * 2 * S::kBytes, v_at = k_at + S::kBytes, other = lds + (buffer ^ 1) * 2 * S::kBytes;
+    if (key0 + kTile < end) {
+      keys.fetch(key0 + kTile, ks.count, other);
+      values.fetch(key0 + kTile, ks.count, other + S::kBytes);
     }
-  put<T>(g.dk, r, kept, a.head_dim, dk, 1.0f);
-  put<T>(g.dv, r, kept, a.head_dim, dv, 1.0f);
+    if (a.causal && key0 + kTile > all_rows) {
+      mark_rows(clean_tile<T, kD>(v_at), mark_s);
+      clean_done();
+    }
+    if (key0 >= any) continue;
+
+    f32x16 s[2];
+#pragma unroll
+    for (uint32_t r = 0; r < 2; ++r) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[r][i] = 0.0f;
+#pragma unroll
+      for (uint32_t k = 0; k < kD / 16; ++k) s[r] = mfma32<T>(reads.rows(k_at, r, k), q[k], s[r]);
+    }
+    if (key0 + kTile > whole) {
+      if (a.causal) {
+#pragma unroll
+        for (uint32_t r = 0; r < 2; ++r)
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i) {
+            const f32x4 mark = marks_of(mark_s, r, i);
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) s[r][4 * i + k] += mark[k];
+          }
+      }
+      const int32_t left = int32_t(limit) - int32_t(key0 + 4 * h);
+#pragma unroll
+      for (uint32_t r = 0; r < 2; ++r)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (int32_t(32 * r + 8 * (i / 4) + i % 4) >= left) s[r][i] = -INFINITY;
+    }
+
+    // the running maximum: followed where it is passed by 2^8
+    float most = -INFINITY;
+#pragma unroll
+    for (uint32_t r = 0; r < 2; ++r)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) most = fmaxf(most, s[r][i]);
+    most = fmaxf(most, __shfl_xor(most, 32, 64)) * c;
+    if (__any(most > top + 8.0f)) {
+      const float up = fmaxf(most, top), keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - up);
+      top = up;
+      total *= keep;
+#pragma unroll
+      for (int t = 0; t < kD / 32; ++t) o[t] *= keep;
+    }
+    const float base = top == -INFINITY ? 0.0f : kUp - top;
+#pragma unroll
+    for (uint32_t r = 0; r < 2; ++r)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[r][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][i], c, base));
+        total += s[r][i];
+      }
+#pragma unroll
+    for (uint32_t u = 0; u < 4; ++u) {
+      const bits8 p = pack8<T>(s[u / 2], u % 2);
+#pragma unroll
+      for (uint32_t t = 0; t < kD / 32; ++t) o[t] = mfma32<T>(reads.columns(v_at, t, u), p, o[t]);
+    }
+  }
+  if (!on) return;
+  total += __shfl_xor(total, 32, 64);
+  put_columns<T, kD, kAligned>(a.out, uint64_t(qs.begin) + row, head, a.head_dim, o, total == 0.0f ? 0.0f : 1.0f / total);
+  if (a.lse && h == 0)
+    a.lse[uint64_t(head) * a.tokens + qs.begin + row] = total == 0.0f ? -INFINITY : (top - kUp + __builtin_amdgcn_logf(total)) * 0.69314718f;
 }
 
 }  // namespace
 }  // namespace op
 
 int launch_attend(const tsa_attend_args& a, hipStream_t stream) {
-  const dim3 grid(a.tokens, a.q.heads);
-  if (a.type == TSA_BF16) hipLaunchKernelGGL(op::attend_kernel<op::Bf16>, grid, dim3(64), 0, stream, a);
-  else hipLaunchKernelGGL(op::attend_kernel<op::F16>, grid, dim3(64), 0, stream, a);
-  return int(hipGetLastError());
-}
-
-uint64_t attend_backward_workspace(const tsa_attend_args&) { return 0; }
-
-int launch_attend_backward(const tsa_attend_grad_args& g, void*, hipStream_t stream) {
-  const dim3 queries(g.f.tokens, g.f.q.heads), keys(g.f.k_tokens, g.f.k.heads);
-  const bool bf = g.f.type == TSA_BF16;
-  if (g.dq.p && g.f.tokens) {
-    if (bf) hipLaunchKernelGGL(op::queries_kernel<op::Bf16>, queries, dim3(64), 0, stream, g);
-    else hipLaunchKernelGGL(op::queries_kernel<op::F16>, queries, dim3(64), 0, stream, g);
+  using namespace op;
+  const dim3 grid(uint32_t(own_tiles_at_most(a.sequences, a.tokens) * a.q.heads)), block(64 * kTileWaves);
+  const float c = a.scale * 1.44269504f;
+  const bool aligned = vector_heads(a.q) && vector_heads(a.out) && (a.k_tokens == 0 || (vector_heads(a.k) && vector_heads(a.v)));
+#define CALL(T, D)                                                                                      \
+  do {                                                                                                  \
+    if (aligned) hipLaunchKernelGGL((attend_kernel<T, D, true>), grid, block, 0, stream, a, c);         \
+    else hipLaunchKernelGGL((attend_kernel<T, D, false>), grid, block, 0, stream, a, c);                \
+  } while (0)
+  if (a.type == TSA_BF16) {
+    if (a.head_dim <= 64) CALL(Bf16, 64);
+    else CALL(Bf16, 128);
+  } else {
+    if (a.head_dim <= 64) CALL(F16, 64);
+    else CALL(F16, 128);
   }
-  if (g.dk.p && g.f.k_tokens) {
-    if (bf) hipLaunchKernelGGL(op::keys_kernel<op::Bf16>, keys, dim3(64), 0, stream, g);
-    else hipLaunchKernelGGL(op::keys_kernel<op::F16>, keys, dim3(64), 0, stream, g);
-  }
+#undef CALL
   return int(hipGetLastError());
 }
 
