@@ -36,6 +36,7 @@ struct CachedShape {
   uint32_t group;     // query heads of a kept one
   uint32_t shares;    // workgroups of a kept head, at most
   float c;            // scale / ln 2
+  bool aligned;       // q and out in pieces of 8
 };
 
 // ---- who does what --------------------------------------------------------------------------------------------------------
@@ -141,9 +142,6 @@ struct Numbers {
     return __builtin_bit_cast(bits8, v);
   }
 };
-// Value i of a word's eight, in that order, of word g of a block.
-__device__ __forceinline__ uint32_t value_of_word(uint32_t g, uint32_t i) { return 4 * g + ((i >> 1) & 1u) * 16 + ((i & 1u) << 1) + (i >> 2); }
-
 __device__ __forceinline__ uint32_t pack(float a, float b) {
   typedef __bf16 two __attribute__((ext_vector_type(2)));
   typedef float two_f __attribute__((ext_vector_type(2)));
@@ -207,6 +205,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(32 * NB)) void cached_kernel(ts
   constexpr bool kHalf = std::is_same_v<T, F16>;
   constexpr uint32_t D = 32 * NB;
   __shared__ __attribute__((aligned(16))) unsigned char page_s[kWaves][P::kRoom];
+  __shared__ __attribute__((aligned(16))) u16 query_s[kRows][D + 4];  // (rows apart by banks)
   __shared__ float2 stat_s[kWaves][kRows];
   __shared__ PlaceMemory place_s;
   static_assert(P::kRoom >= kRows * D * 4, "a wave's outputs take its page's place");
@@ -223,22 +222,37 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(32 * NB)) void cached_kernel(ts
   while (true) {  // the share's tiles
     const uint32_t x = at.tile * kRows + (lane & 15u);
     const bool on = x < r.fresh * s.group;
-    const uint32_t token = on ? x / s.group : 0, head = kept * s.group + (on ? x % s.group : 0);
+    const uint32_t token = on ? x / s.group : 0;
     const int32_t limit = on ? r.end - int32_t(r.fresh) + int32_t(token) + 1 : 0;  // keys that this row attends to
     const int32_t whole = r.end - int32_t(r.fresh) + 1;                            // keys that every row attends to
 
-    // this row's queries, in the order of the keys' half bytes, and what takes their offset off
+    // The queries, once for all waves (each by itself, value by value, took 9 us). Pieces of 8 where they start 16-byte aligned.
+    for (uint32_t i = threadIdx.x; i < kRows * D / 8; i += 64 * kWaves) {
+      const uint32_t y = at.tile * kRows + i / (D / 8), d = i % (D / 8) * 8;
+      bits8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (y < r.fresh * s.group) {
+        const u16* p = row_of<u16>(a.q, r.first + y / s.group, kept * s.group + y % s.group) + d;
+        if (s.aligned) {
+          v = *reinterpret_cast<const bits8*>(p);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = p[k];
+        }
+      }
+      *reinterpret_cast<uint2*>(&query_s[i / (D / 8)][d]) = uint2{__builtin_bit_cast(u32x4, v)[0], __builtin_bit_cast(u32x4, v)[1]};
+      *reinterpret_cast<uint2*>(&query_s[i / (D / 8)][d + 4]) = uint2{__builtin_bit_cast(u32x4, v)[2], __builtin_bit_cast(u32x4, v)[3]};
+    }
+    __syncthreads();
+    // this row's, in the order of the keys' half bytes, and what takes their offset off
     bits8 q[NB];
     f32x4 off[NB];
-    const u16* qp = row_of<u16>(a.q, r.first + token, head);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
+      const bits4 lo = *reinterpret_cast<const bits4*>(&query_s[lane & 15u][32 * b + 4 * g]), hi = *reinterpret_cast<const bits4*>(&query_s[lane & 15u][32 * b + 16 + 4 * g]);
+      q[b] = bits8{lo[0], lo[2], hi[0], hi[2], lo[1], lo[3], hi[1], hi[3]};
       float sum = 0.0f;
 #pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) {
-        q[b][i] = on ? qp[32 * b + value_of_word(g, i)] : 0;
-        sum += T::up(q[b][i]);
-      }
+      for (uint32_t i = 0; i < 8; ++i) sum += T::up(q[b][i]);
       sum = column_sum(sum) * (kHalf ? -24.0f : -136.0f);
       off[b] = f32x4{sum, sum, sum, sum};
     }
@@ -409,10 +423,17 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(32 * NB)) void cached_kernel(ts
     if (lane < kRows) stat_s[wave][lane] = {top, total};
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __syncthreads();  // every wave is done with its pages
-    float best = -INFINITY;
+    float best = -INFINITY, sum = 0.0f;
 #pragma unroll
     for (uint32_t w = 0; w < kWaves; ++w) best = fmaxf(best, stat_s[w][lane & 15u].x);
-    const float by = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - best);
+    const float base = best == -INFINITY ? 0.0f : best;
+#pragma unroll
+    for (uint32_t w = 0; w < kWaves; ++w) {
+      const float2 st = stat_s[w][lane & 15u];
+      sum += st.y * __builtin_amdgcn_exp2f(st.x - base);
+    }
+    const bool whole_tile = at.at >= from && at.at + r.places() <= upto;
+    const float by = __builtin_amdgcn_exp2f(top - base) * (!whole_tile ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum);
     float* mine = reinterpret_cast<float*>(page_s[wave]) + (lane & 15u) * D;
 #pragma unroll
     for (int i = 0; i < 2 * NB; ++i)
@@ -420,25 +441,25 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(32 * NB)) void cached_kernel(ts
       for (uint32_t k = 0; k < 4; ++k)  // column 4 g + k of the tile: byte (4 g + k) / 2 of the half block, low half bytes first
         mine[32 * (i / 2) + 8 * (i % 2) + (4 * g + k) / 2 + 16 * (k & 1u)] = o[i][k] * by;
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < kRows * D; i += 64 * kWaves) {
-      const uint32_t col = i / D, d = i % D, y = at.tile * kRows + col;
+    const uint32_t part = (2 * share + (at.at > from)) * c.kv_heads + kept;
+    if (!whole_tile && threadIdx.x < kRows) stats[part * kRows + threadIdx.x] = {best, sum};
+    for (uint32_t i = threadIdx.x; i < kRows * D / 4; i += 64 * kWaves) {
+      const uint32_t y = at.tile * kRows + i / (D / 4), d = i % (D / 4) * 4;
       if (y >= r.fresh * s.group) break;
-      float m = -INFINITY, sum = 0.0f, v = 0.0f;
+      f32x4 v = {0, 0, 0, 0};
 #pragma unroll
-      for (uint32_t w = 0; w < kWaves; ++w) m = fmaxf(m, stat_s[w][col].x);
-#pragma unroll
-      for (uint32_t w = 0; w < kWaves; ++w) {
-        const float2 st = stat_s[w][col];
-        sum += st.x == -INFINITY ? 0.0f : st.y * __builtin_amdgcn_exp2f(st.x - m);
-        v += reinterpret_cast<const float*>(page_s[w])[i];
+      for (uint32_t w = 0; w < kWaves; ++w) v += reinterpret_cast<const f32x4*>(page_s[w])[i];
+      if (!whole_tile) {
+        reinterpret_cast<f32x4*>(parts)[uint64_t(part) * (kRows * D / 4) + i] = v;
+        continue;
       }
-      if (at.at >= from && at.at + r.places() <= upto) {
-        u16* out = const_cast<u16*>(row_of<u16>(a.out, r.first + y / s.group, kept * s.group + y % s.group));
-        out[d] = T::down(sum == 0.0f ? 0.0f : v / sum);
+      u16* out = const_cast<u16*>(row_of<u16>(a.out, r.first + y / s.group, kept * s.group + y % s.group)) + d;
+      const bits4 w = {T::down(v[0]), T::down(v[1]), T::down(v[2]), T::down(v[3])};
+      if (s.aligned) {
+        *reinterpret_cast<bits4*>(out) = w;
       } else {
-        const uint64_t part = (2 * share + (at.at > from)) * c.kv_heads + kept;
-        parts[part * kRows * D + i] = v;
-        if (d == 0) stats[part * kRows + col] = {m, sum};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) out[k] = w[k];
       }
     }
     at.at += r.places();
@@ -516,6 +537,7 @@ CachedShape shape_of(const tsa_cache& c, const tsa_attend_cached_args& a) {
   const uint64_t shares = (groups(c.head_dim) + c.kv_heads - 1) / c.kv_heads, most = (tiles_at_most(a, s.group) * a.width + kMinShare - 1) / kMinShare;
   s.shares = uint32_t(shares < most ? shares : most);
   s.c = a.scale * 1.44269504f;
+  s.aligned = vector_heads(a.q) && vector_heads(a.out);
   return s;
 }
 

@@ -3,38 +3,124 @@
 //   dk = scale ds^T Q, dv = p^T dout    a workgroup has 128 keys of a kept head and runs over the queries of its group's heads,
 // each in tiles of 64 through LDS as in the forward pass: the wave's own rows are the columns of every product, and p and ds, as they
 // come out of the first products, the operand of the second. Scores are computed twice, and nothing is added up across
-// workgroups: the same bits every time, without atomics or partial sums in memory. lse and dout . out go to the workspace first, a pair a row.
+// workgroups: the same bits every time, without atomics or partial sums in memory. lse and sum p dp go to the
+// workspace first, a pair a row.
 #include "attn_tile.hpp"
 
 namespace tsa {
 namespace op {
 namespace {
 
-// (lse / ln 2, dout . out) of each row; a row without keys has an lse of infinity, which makes its probabilities 0.
-template <class T, bool kAligned>
-__global__ __launch_bounds__(256) void rows_kernel(tsa_attend_grad_args g, float2* rows) {
+template <int N>
+__device__ __forceinline__ void clear(f32x16 (&v)[N]) {
+#pragma unroll
+  for (int t = 0; t < N; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[t][i] = 0.0f;
+}
+
+// The queries of a workgroup, and what of the keys they attend to.
+struct Queries {
+  Span qs, ks;
+  uint32_t head, kept;
+  uint32_t row;        // this lane's
+  bool on;
+  uint32_t limit, all_rows, whole, any, end;  // keys that this row; every row of the workgroup; every, and any, row of this wave; any row attends to
+};
+// By the whole workgroup; false: there are no more.
+template <bool kFromEnd>
+__device__ __forceinline__ bool find_queries(const tsa_attend_args& a, OwnTileMemory& m, Queries& o) {
+  OwnTile own;
+  o.head = head_of_group(blockIdx.x % a.q.heads, a.q.heads), o.kept = o.head / (a.q.heads / a.k.heads);
+  if (!find_own_tile<kFromEnd>(a.first, a.sequences, a.tokens, blockIdx.x / a.q.heads, m, own)) return false;
+  o.qs = span_of(a.first, own.sequence, a.tokens), o.ks = span_of(a.k_first ? a.k_first : a.first, own.sequence, a.k_tokens);
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row0 = own.row0 + wave * kOwn;
+  o.row = row0 + (threadIdx.x & 31u), o.on = o.row < o.qs.count;
+  const int32_t ahead = int32_t(o.ks.count) - int32_t(o.qs.count) + 1;
+  auto keys_of = [&](uint32_t r) {
+    const int32_t n = a.causal ? int32_t(r) + ahead : int32_t(o.ks.count);
+    return n < 0 ? 0u : min(uint32_t(n), o.ks.count);
+  };
+  o.limit = o.on ? keys_of(o.row) : 0, o.all_rows = keys_of(own.row0), o.whole = keys_of(row0);
+  o.any = row0 < o.qs.count ? keys_of(min(row0 + kOwn, o.qs.count) - 1) : 0;
+  o.end = keys_of(min(own.row0 + kTileOwn, o.qs.count) - 1);
+  return true;
+}
+
+// What is taken off the gradients of a row's probabilities, sum_j p_j dp_j. It is dout . out, but out is rounded to 16 bits, which over a
+// few keys is as large an error in the gradients as their own rounding (over 10 keys they are off by 1.7 times what rounding the results
+// costs, 1.4 without it; over 1000 it is lost in it): rows of workgroups that attend to no more keys than this add up p dp itself.
+constexpr uint32_t kExactKeys = 512;
+
+// (lse / ln 2, sum_j p_j dp_j) of each row; a row without keys has an lse of infinity, which makes its probabilities 0.
+template <class T, int kD, bool kAligned>
+__global__ __launch_bounds__(64 * kTileWaves, 2) void rows_kernel(tsa_attend_grad_args g, float2* rows, float c) {
+  typedef TileShapes<kD> S;
+  __shared__ __attribute__((aligned(16))) unsigned char tile_s[2][S::kBytes];  // keys and values
+  __shared__ OwnTileMemory own_s;
   const tsa_attend_args& a = g.f;
-  const uint32_t head = blockIdx.x % a.q.heads, t = blockIdx.x / a.q.heads * 16 + threadIdx.x / 16, value = (threadIdx.x & 15u) * 8;
-  if (t >= a.tokens) return;
-  float sum = 0.0f;
-  if (value < a.head_dim) {
-    const u16 *x = row_of<u16>(a.out, t, head) + value, *y = row_of<u16>(g.dout, t, head) + value;
-    if constexpr (kAligned) {
-      const bits8 u = *reinterpret_cast<const bits8*>(x), v = *reinterpret_cast<const bits8*>(y);
+  Queries o;
+  if (!find_queries<false>(a, own_s, o)) return;  // (those with few keys first: they take longer)
+  const uint32_t lane = threadIdx.x & 63u, h = lane >> 5;
+  if (o.end > kExactKeys) {
+    const uint32_t row0 = o.row - (lane & 31u) - (threadIdx.x >> 6) * kOwn, value = (lane & 15u) * 8;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += T::up(u[i]) * T::up(v[i]);
-    } else {
+    for (uint32_t j = 0; j < kTileOwn / (4 * kTileWaves); ++j) {
+      const uint32_t i = j * 4 * kTileWaves + threadIdx.x / 16;
+      const bool on = row0 + i < o.qs.count;
+      const uint64_t t = uint64_t(o.qs.begin) + (on ? row0 + i : row0);
+      float sum = 0.0f;
+      if (value < a.head_dim) {
+        const u16 *x = row_of<u16>(a.out, t, o.head) + value, *y = row_of<u16>(g.dout, t, o.head) + value;
+        if constexpr (kAligned) {
+          const bits8 u = *reinterpret_cast<const bits8*>(x), v = *reinterpret_cast<const bits8*>(y);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += T::up(x[i]) * T::up(y[i]);
+          for (int k = 0; k < 8; ++k) sum += T::up(u[k]) * T::up(v[k]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) sum += T::up(x[k]) * T::up(y[k]);
+        }
+      }
+#pragma unroll
+      for (int s = 1; s < 16; s <<= 1) sum += __shfl_xor(sum, s, 64);
+      if (on && value == 0) {
+        const uint64_t at = uint64_t(o.head) * a.tokens + t;
+        const float lse = a.lse[at];
+        rows[at] = {lse == -INFINITY ? INFINITY : lse * 1.44269504f, sum};
+      }
+    }
+    return;
+  }
+  const uint64_t at = uint64_t(o.head) * a.tokens + o.qs.begin + o.row;
+  const OwnRows<kD, kAligned> q(a.q, uint64_t(o.qs.begin) + o.row, o.head, a.head_dim, o.on), dout(g.dout, uint64_t(o.qs.begin) + o.row, o.head, a.head_dim, o.on);
+  float lse = o.on ? a.lse[at] : -INFINITY, sum = 0.0f;
+  lse = lse == -INFINITY ? INFINITY : lse * 1.44269504f;
+  const TileReads<kD> reads;
+  const TileLoads<kD, kAligned> keys(a.k, o.ks.begin, o.kept, a.head_dim), values(a.v, o.ks.begin, o.kept, a.head_dim);
+  const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_offset(tile_s));
+  for (uint32_t key0 = 0; key0 < o.end; key0 += kTile) {
+    if (key0) tile_ready();  // the last tile's reads are done
+    keys.fetch(key0, o.ks.count, lds);
+    values.fetch(key0, o.ks.count, lds + S::kBytes);
+    tile_ready();
+    if (key0 >= o.any) continue;
+    const int32_t left = int32_t(o.limit) - int32_t(key0 + 4 * h);
+#pragma unroll
+    for (uint32_t r = 0; r < 2; ++r) {
+      f32x16 one[2];
+      clear(one);
+#pragma unroll
+      for (uint32_t k = 0; k < kD / 16; ++k) {
+        one[0] = mfma32<T>(reads.rows(lds, r, k), q.v[k], one[0]);
+        one[1] = mfma32<T>(reads.rows(lds + S::kBytes, r, k), dout.v[k], one[1]);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (int32_t(32 * r + 8 * (i / 4) + i % 4) < left) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(one[0][i], c, -lse)) * one[1][i];
     }
   }
-#pragma unroll
-  for (int s = 1; s < 16; s <<= 1) sum += __shfl_xor(sum, s, 64);
-  if (value == 0) {
-    const uint64_t at = uint64_t(head) * a.tokens + t;
-    const float lse = a.lse[at];
-    rows[at] = {lse == -INFINITY ? INFINITY : lse * 1.44269504f, sum};
-  }
+  sum += __shfl_xor(sum, 32, 64);
+  if (o.on && h == 0) rows[at] = {lse, sum};
 }
 
 // Gradients of scores on their way to 16 bits. bf16 has the range of 32 bits. Half precision has not: a column's are multiplied by
@@ -67,14 +153,6 @@ struct Raised<F16> {
   __device__ __forceinline__ float down() const { return by == 0.0f ? 0.0f : 1.0f / by; }
 };
 
-template <int N>
-__device__ __forceinline__ void clear(f32x16 (&v)[N]) {
-#pragma unroll
-  for (int t = 0; t < N; ++t)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[t][i] = 0.0f;
-}
-
 template <class T, int kD, bool kAligned>
 __global__ __launch_bounds__(64 * kTileWaves, 2) void queries_kernel(tsa_attend_grad_args g, const float2* rows, float c) {
   typedef TileShapes<kD> S;
@@ -82,46 +160,34 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void queries_kernel(tsa_attend_
   __shared__ __attribute__((aligned(16))) float mark_s[kTile];
   __shared__ OwnTileMemory own_s;
   const tsa_attend_args& a = g.f;
-  OwnTile own;
-  const uint32_t head = head_of_group(blockIdx.x % a.q.heads, a.q.heads), kept = head / (a.q.heads / a.k.heads);
-  if (!find_own_tile<true>(a.first, a.sequences, a.tokens, blockIdx.x / a.q.heads, own_s, own)) return;
-  const Span qs = span_of(a.first, own.sequence, a.tokens), ks = span_of(a.k_first ? a.k_first : a.first, own.sequence, a.k_tokens);
-  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
-  const uint32_t row0 = own.row0 + wave * kOwn, row = row0 + (lane & 31u);
-  const bool on = row < qs.count;
-  const int32_t ahead = a.causal ? int32_t(ks.count) - int32_t(qs.count) + 1 : 0;
-  auto keys_of = [&](uint32_t r) {  // keys that a query attends to
-    const int32_t n = a.causal ? int32_t(r) + ahead : int32_t(ks.count);
-    return n < 0 ? 0u : min(uint32_t(n), ks.count);
-  };
-  const uint32_t limit = on ? keys_of(row) : 0, all_rows = keys_of(own.row0), whole = keys_of(row0), any = row0 < qs.count ? keys_of(min(row0 + kOwn, qs.count) - 1) : 0;
-  const uint32_t end = keys_of(min(own.row0 + kTileOwn, qs.count) - 1);
-
-  const OwnRows<kD, kAligned> q(a.q, uint64_t(qs.begin) + row, head, a.head_dim, on), dout(g.dout, uint64_t(qs.begin) + row, head, a.head_dim, on);
-  const float2 mine = on ? rows[uint64_t(head) * a.tokens + qs.begin + row] : float2{INFINITY, 0.0f};
+  Queries o;
+  if (!find_queries<true>(a, own_s, o)) return;
+  const uint32_t h = (threadIdx.x & 63u) >> 5;
+  const OwnRows<kD, kAligned> q(a.q, uint64_t(o.qs.begin) + o.row, o.head, a.head_dim, o.on), dout(g.dout, uint64_t(o.qs.begin) + o.row, o.head, a.head_dim, o.on);
+  const float2 mine = o.on ? rows[uint64_t(o.head) * a.tokens + o.qs.begin + o.row] : float2{INFINITY, 0.0f};
   const TileReads<kD> reads;
-  const TileLoads<kD, kAligned> keys(a.k, ks.begin, kept, a.head_dim), values(a.v, ks.begin, kept, a.head_dim);
+  const TileLoads<kD, kAligned> keys(a.k, o.ks.begin, o.kept, a.head_dim), values(a.v, o.ks.begin, o.kept, a.head_dim);
   const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_offset(tile_s));
   f32x16 dq[kD / 32];
   clear(dq);
   Raised<T> raised;
 
-  if (end) {
-    keys.fetch(0, ks.count, lds);
-    values.fetch(0, ks.count, lds + S::kBytes);
+  if (o.end) {
+    keys.fetch(0, o.ks.count, lds);
+    values.fetch(0, o.ks.count, lds + S::kBytes);
   }
-  for (uint32_t key0 = 0, buffer = 0; key0 < end; key0 += kTile, buffer ^= 1) {
+  for (uint32_t key0 = 0, buffer = 0; key0 < o.end; key0 += kTile, buffer ^= 1) {
     tile_ready();
     const uint32_t k_at = lds + buffer * 2 * S::kBytes, v_at = k_at + S::kBytes, other = lds + (buffer ^ 1) * 2 * S::kBytes;
-    if (key0 + kTile < end) {
-      keys.fetch(key0 + kTile, ks.count, other);
-      values.fetch(key0 + kTile, ks.count, other + S::kBytes);
+    if (key0 + kTile < o.end) {
+      keys.fetch(key0 + kTile, o.ks.count, other);
+      values.fetch(key0 + kTile, o.ks.count, other + S::kBytes);
     }
-    if (a.causal && key0 + kTile > all_rows) {
+    if (a.causal && key0 + kTile > o.all_rows) {
       mark_rows(clean_tile<T, kD>(k_at), mark_s);
       clean_done();
     }
-    if (key0 >= any) continue;
+    if (key0 >= o.any) continue;
 #pragma unroll
     for (uint32_t r = 0; r < 2; ++r) {
       f32x16 one[2];  // scores, then their gradients; gradients of probabilities
@@ -134,7 +200,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void queries_kernel(tsa_attend_
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         one[0][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(one[0][i], c, -mine.x)) * (one[1][i] - mine.y);
-      if (key0 + kTile > whole) {
+      if (key0 + kTile > o.whole) {
         if (a.causal) {
 #pragma unroll
           for (uint32_t i = 0; i < 4; ++i) {
@@ -143,7 +209,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void queries_kernel(tsa_attend_
             for (uint32_t k = 0; k < 4; ++k) one[0][4 * i + k] += mark[k];
           }
         }
-        const int32_t left = int32_t(limit) - int32_t(key0 + 4 * h);
+        const int32_t left = int32_t(o.limit) - int32_t(key0 + 4 * h);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (int32_t(32 * r + 8 * (i / 4) + i % 4) >= left) one[0][i] = 0.0f;
@@ -158,13 +224,31 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void queries_kernel(tsa_attend_
       }
     }
   }
-  if (on) put_columns<T, kD, kAligned>(g.dq, uint64_t(qs.begin) + row, head, a.head_dim, dq, a.scale * raised.down());
+  if (o.on) put_columns<T, kD, kAligned>(g.dq, uint64_t(o.qs.begin) + o.row, o.head, a.head_dim, dq, a.scale * raised.down());
 }
 
-template <class T, int kD, bool kAligned>
-__global__ __launch_bounds__(64 * kTileWaves, kD == 64 ? 2 : 1) void keys_kernel(tsa_attend_grad_args g, const float2* rows, float c) {
+// Half precision: probabilities of up to 2^14, so that small ones keep their bits.
+template <class T>
+constexpr float probability_up() {
+  return std::is_same_v<T, F16> ? 14.0f : 0.0f;
+}
+// A result of the second kind to 32 bits in memory.
+template <int kD>
+__device__ __forceinline__ void put_part(float* p, const f32x16 (&v)[kD / 32], float by) {
+#pragma unroll
+  for (uint32_t t = 0; t < kD / 32; ++t)
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+      *reinterpret_cast<f32x4*>(p + 32 * t + 8 * i + 4 * ((threadIdx.x & 63u) >> 5)) =
+          f32x4{v[t][4 * i] * by, v[t][4 * i + 1] * by, v[t][4 * i + 2] * by, v[t][4 * i + 3] * by};
+}
+
+// Both gradients of keys and values, or one. With 128 values both together need 430 registers, one wave a SIMD: they took 840 us in three
+// packed sequences of 8192 together, one after the other with the scores computed again 660.
+template <class T, int kD, bool kAligned, bool kKeys, bool kValues>
+__global__ __launch_bounds__(64 * kTileWaves, 2) void keys_kernel(tsa_attend_grad_args g, const float2* rows, float c, uint32_t pieces, float* parts) {
   typedef TileShapes<kD> S;
-  constexpr float kUp = std::is_same_v<T, F16> ? 14.0f : 0.0f;  // half precision: probabilities up to 2^14
+  constexpr float kUp = probability_up<T>();
   __shared__ __attribute__((aligned(16))) unsigned char tile_s[2][2][S::kBytes];  // queries and the outputs' gradients, two of each
   __shared__ __attribute__((aligned(16))) float2 row_s[2][kTile];
   __shared__ __attribute__((aligned(16))) float mark_s[kTile];
@@ -173,7 +257,8 @@ __global__ __launch_bounds__(64 * kTileWaves, kD == 64 ? 2 : 1) void keys_kernel
   const int32_t* k_first = a.k_first ? a.k_first : a.first;
   OwnTile own;
   const uint32_t kept = head_of_group(blockIdx.x % a.k.heads, a.k.heads), group = a.q.heads / a.k.heads;
-  if (!find_own_tile<false>(k_first, a.sequences, a.k_tokens, blockIdx.x / a.k.heads, own_s, own)) return;
+  const uint32_t piece = blockIdx.x / a.k.heads % pieces;
+  if (!find_own_tile<false>(k_first, a.sequences, a.k_tokens, blockIdx.x / a.k.heads / pieces, own_s, own)) return;
   const Span qs = span_of(a.first, own.sequence, a.tokens), ks = span_of(k_first, own.sequence, a.k_tokens);
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const uint32_t row0 = own.row0 + wave * kOwn, row = row0 + (lane & 31u);
@@ -184,17 +269,20 @@ __global__ __launch_bounds__(64 * kTileWaves, kD == 64 ? 2 : 1) void keys_kernel
     return n < 0 ? 0u : uint32_t(n);
   };
   const uint32_t from = from_of(row), any = from_of(row0), whole = from_of(row0 + kOwn - 1), all_rows = from_of(own.row0 + kTileOwn - 1);
-  const uint32_t begin = from_of(own.row0) / kTile * kTile, tiles = begin < qs.count ? (qs.count - begin + kTile - 1) / kTile : 0, steps = tiles * group;
+  const uint32_t begin = from_of(own.row0) / kTile * kTile, tiles = begin < qs.count ? (qs.count - begin + kTile - 1) / kTile : 0;
+  // this piece's steps: a query tile of a head each
+  const uint32_t step0 = uint32_t(uint64_t(tiles) * group * piece / pieces), steps = uint32_t(uint64_t(tiles) * group * (piece + 1) / pieces) - step0;
 
   const OwnRows<kD, kAligned> k(a.k, uint64_t(ks.begin) + row, kept, a.head_dim, on), v(a.v, uint64_t(ks.begin) + row, kept, a.head_dim, on);
   const TileReads<kD> reads;
   const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_offset(tile_s)), row_lds = __builtin_amdgcn_readfirstlane(lds_offset(row_s));
-  f32x16 dk[kD / 32], dv[kD / 32];
+  f32x16 dk[kKeys ? kD / 32 : 1], dv[kValues ? kD / 32 : 1];
   clear(dk);
   clear(dv);
   Raised<T> raised;
 
-  uint32_t head = kept * group, q0 = begin;  // of the step whose loads go next
+  uint32_t head = kept * group + (steps ? step0 / tiles : 0), q0 = begin + (steps ? step0 % tiles : 0) * kTile;  // of the step whose loads go next
+  const uint32_t first_q = q0;
   auto fetch = [&](uint32_t buffer) {
     const TileLoads<kD, kAligned> queries(a.q, qs.begin, head, a.head_dim), douts(g.dout, qs.begin, head, a.head_dim);
     queries.fetch(q0, qs.count, lds + buffer * 2 * S::kBytes);
@@ -208,7 +296,7 @@ __global__ __launch_bounds__(64 * kTileWaves, kD == 64 ? 2 : 1) void keys_kernel
     if (q0 >= qs.count) q0 = begin, ++head;
   };
   if (steps) fetch(0);
-  for (uint32_t step = 0, buffer = 0, row_at = begin; step < steps; ++step, buffer ^= 1) {
+  for (uint32_t step = 0, buffer = 0, row_at = first_q; step < steps; ++step, buffer ^= 1) {
     tile_ready();
     const uint32_t q_at = lds + buffer * 2 * S::kBytes, d_at = q_at + S::kBytes, at = row_at;
     if (step + 1 < steps) fetch(buffer ^ 1);
@@ -226,7 +314,7 @@ __global__ __launch_bounds__(64 * kTileWaves, kD == 64 ? 2 : 1) void keys_kernel
 #pragma unroll
       for (uint32_t i = 0; i < kD / 16; ++i) {
         one[0] = mfma32<T>(reads.rows(q_at, r, i), k.v[i], one[0]);
-        one[1] = mfma32<T>(reads.rows(d_at, r, i), v.v[i], one[1]);
+        if constexpr (kKeys) one[1] = mfma32<T>(reads.rows(d_at, r, i), v.v[i], one[1]);
       }
 #pragma unroll
       for (uint32_t i = 0; i < 4; ++i) {
@@ -256,59 +344,108 @@ __global__ __launch_bounds__(64 * kTileWaves, kD == 64 ? 2 : 1) void keys_kernel
           if (x < lo || x >= hi) one[0][i] = one[1][i] = 0.0f;
         }
       }
-      raised.raise(one[1], dk);
-      if constexpr (std::is_same_v<T, F16>) one[1] *= raised.by;
+      if constexpr (kKeys) {
+        raised.raise(one[1], dk);
+        if constexpr (std::is_same_v<T, F16>) one[1] *= raised.by;
+      }
 #pragma unroll
       for (uint32_t u = 0; u < 2; ++u) {
         const bits8 p = pack8<T>(one[0], u), ds = pack8<T>(one[1], u);
 #pragma unroll
         for (uint32_t t = 0; t < kD / 32; ++t) {
-          dv[t] = mfma32<T>(reads.columns(d_at, t, 2 * r + u), p, dv[t]);
-          dk[t] = mfma32<T>(reads.columns(q_at, t, 2 * r + u), ds, dk[t]);
+          if constexpr (kValues) dv[t] = mfma32<T>(reads.columns(d_at, t, 2 * r + u), p, dv[t]);
+          if constexpr (kKeys) dk[t] = mfma32<T>(reads.columns(q_at, t, 2 * r + u), ds, dk[t]);
         }
       }
     }
   }
   if (!on) return;
+  if (pieces > 1) {
+    float* const part = parts + ((uint64_t(piece) * a.k_tokens + ks.begin + row) * a.k.heads + kept) * 2 * kD;
+    if constexpr (kKeys) put_part<kD>(part, dk, raised.down());
+    if constexpr (kValues) put_part<kD>(part + kD, dv, 1.0f);
+    return;
+  }
   const float back = __builtin_amdgcn_exp2f(-kUp);
-  put_columns<T, kD, kAligned>(g.dk, uint64_t(ks.begin) + row, kept, a.head_dim, dk, a.scale * back * raised.down());
-  put_columns<T, kD, kAligned>(g.dv, uint64_t(ks.begin) + row, kept, a.head_dim, dv, back);
+  if constexpr (kKeys) put_columns<T, kD, kAligned>(g.dk, uint64_t(ks.begin) + row, kept, a.head_dim, dk, a.scale * back * raised.down());
+  if constexpr (kValues) put_columns<T, kD, kAligned>(g.dv, uint64_t(ks.begin) + row, kept, a.head_dim, dv, back);
 }
 
-template <class T, bool kAligned>
-void rows_of(const tsa_attend_grad_args& g, float2* rows, hipStream_t stream) {
-  const uint64_t n = uint64_t(g.f.tokens + 15) / 16 * g.f.q.heads;
-  hipLaunchKernelGGL((rows_kernel<T, kAligned>), dim3(uint32_t(n)), dim3(256), 0, stream, g, rows);
-}
+// The pieces' sums, rounded: four values a thread.
 template <class T, int kD, bool kAligned>
-void gradients(const tsa_attend_grad_args& g, float2* rows, hipStream_t stream) {
+__global__ __launch_bounds__(256) void join_kernel(tsa_attend_grad_args g, uint32_t pieces, const float* parts) {
+  const tsa_attend_args& a = g.f;
+  const uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x;
+  constexpr uint32_t kRow = 2 * kD / 4;
+  const uint32_t in = uint32_t(i % kRow), d = in * 4 % kD;
+  const uint64_t head_row = i / kRow, row = head_row / a.k.heads;
+  if (row >= a.k_tokens || d >= a.head_dim) return;
+  const int32_t* k_first = a.k_first ? a.k_first : a.first;
+  const uint32_t n = sequence_of(k_first, a.sequences, uint32_t(row));
+  if (n >= a.sequences) return;
+  const Span ks = span_of(k_first, n, a.k_tokens);
+  if (row < ks.begin || row >= uint64_t(ks.begin) + ks.count) return;
+  f32x4 sum = {0, 0, 0, 0};
+  for (uint32_t p = 0; p < pieces; ++p) sum += reinterpret_cast<const f32x4*>(parts)[p * (uint64_t(a.k_tokens) * a.k.heads * kRow) + i];
+  const bool value = in * 4 >= kD;
+  sum *= (value ? 1.0f : a.scale) * __builtin_amdgcn_exp2f(-probability_up<T>());
+  put4<T, kAligned>(const_cast<u16*>(row_of<u16>(value ? g.dv : g.dk, row, uint32_t(head_row % a.k.heads))) + d, sum[0], sum[1], sum[2], sum[3]);
+}
+
+// Pieces that a workgroup's queries are cut into: where there are few tiles of keys these would leave the chip idle, or wait for the
+// longest (the first keys of the longest sequence have all queries, the last ones a tile). Each piece's sums go to memory in 32 bits. In three
+// packed sequences of 8192 together, 520 tiles: 1080 us uncut, 704 in three pieces (with 44 to join them), 820 in seven.
+constexpr uint32_t kUnits = 2048, kMaxPieces = 8;
+uint32_t pieces_of(const tsa_attend_args& a) {
+  const uint64_t tiles = (uint64_t(a.k_tokens) / kTileOwn + 1) * a.k.heads, n = kUnits / tiles;
+  return n < 1 ? 1 : n > kMaxPieces ? kMaxPieces : uint32_t(n);
+}
+
+template <class T, int kD, bool kAligned>
+void gradients(const tsa_attend_grad_args& g, float2* rows, float* parts, hipStream_t stream) {
   const tsa_attend_args& a = g.f;
   const float c = a.scale * 1.44269504f;
-  if (a.tokens) rows_of<T, kAligned>(g, rows, stream);
-  if (a.tokens && g.dq.p)
-    hipLaunchKernelGGL((queries_kernel<T, kD, kAligned>), dim3(uint32_t(own_tiles_at_most(a.sequences, a.tokens) * a.q.heads)), dim3(64 * kTileWaves), 0,
-                       stream, g, rows, c);
-  if (a.k_tokens && g.dk.p)
-    hipLaunchKernelGGL((keys_kernel<T, kD, kAligned>), dim3(uint32_t(own_tiles_at_most(a.sequences, a.k_tokens) * a.k.heads)), dim3(64 * kTileWaves), 0,
-                       stream, g, rows, c);
+  const dim3 queries(uint32_t(own_tiles_at_most(a.sequences, a.tokens) * a.q.heads)), block(64 * kTileWaves);
+  if (a.tokens) hipLaunchKernelGGL((rows_kernel<T, kD, kAligned>), queries, block, 0, stream, g, rows, c);
+  if (a.tokens && g.dq.p) hipLaunchKernelGGL((queries_kernel<T, kD, kAligned>), queries, block, 0, stream, g, rows, c);
+  if (a.k_tokens && g.dk.p) {
+    const uint32_t pieces = pieces_of(a);
+    const dim3 keys(uint32_t(own_tiles_at_most(a.sequences, a.k_tokens) * a.k.heads * pieces));
+    if constexpr (kD == 64) {
+      hipLaunchKernelGGL((keys_kernel<T, kD, kAligned, true, true>), keys, block, 0, stream, g, rows, c, pieces, parts);
+    } else {
+      hipLaunchKernelGGL((keys_kernel<T, kD, kAligned, true, false>), keys, block, 0, stream, g, rows, c, pieces, parts);
+      hipLaunchKernelGGL((keys_kernel<T, kD, kAligned, false, true>), keys, block, 0, stream, g, rows, c, pieces, parts);
+    }
+    if (pieces > 1) {
+      const uint64_t n = uint64_t(a.k_tokens) * a.k.heads * (2 * kD / 4);
+      hipLaunchKernelGGL((join_kernel<T, kD, kAligned>), dim3(uint32_t((n + 255) / 256)), dim3(256), 0, stream, g, pieces, parts);
+    }
+  }
 }
 
 }  // namespace
 }  // namespace op
 
-uint64_t attend_backward_workspace(const tsa_attend_args& f) { return uint64_t(f.tokens) * f.q.heads * sizeof(float2); }
+// The rows' pairs, then the pieces (their rows together are at most kMaxPieces times the keys, and at most what kUnits tiles hold: so
+// that more rows never need less).
+uint64_t attend_backward_workspace(const tsa_attend_args& f) {
+  const uint64_t many = uint64_t(op::kMaxPieces) * f.k_tokens * f.k.heads, most = uint64_t(op::kUnits) * op::kTileOwn;
+  return up_to(uint64_t(f.tokens) * f.q.heads * sizeof(float2), 16) + (many < most ? many : most) * 2 * (f.head_dim <= 64 ? 64 : 128) * sizeof(float);
+}
 
 int launch_attend_backward(const tsa_attend_grad_args& g, void* workspace, hipStream_t stream) {
   using namespace op;
   const tsa_attend_args& a = g.f;
   float2* rows = static_cast<float2*>(workspace);
+  float* parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + up_to(uint64_t(a.tokens) * a.q.heads * sizeof(float2), 16));
   bool aligned = true;
   if (a.tokens) aligned = vector_heads(a.q) && vector_heads(a.out) && vector_heads(g.dout) && (!g.dq.p || vector_heads(g.dq));
   if (a.k_tokens) aligned = aligned && vector_heads(a.k) && vector_heads(a.v) && (!g.dk.p || (vector_heads(g.dk) && vector_heads(g.dv)));
 #define CALL(T, D)                                                     \
   do {                                                                 \
-    if (aligned) gradients<T, D, true>(g, rows, stream);               \
-    else gradients<T, D, false>(g, rows, stream);                      \
+    if (aligned) gradients<T, D, true>(g, rows, parts, stream);               \
+    else gradients<T, D, false>(g, rows, parts, stream);                      \
   } while (0)
   if (a.type == TSA_BF16) {
     if (a.head_dim <= 64) CALL(Bf16, 64);
