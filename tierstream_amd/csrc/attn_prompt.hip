@@ -63,13 +63,14 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_kernel(tsa_attend_a
     }
     if (key0 >= any) continue;
 
+    const auto k_rows = reads.rows(k_at);
     f32x16 s[2];
 #pragma unroll
     for (uint32_t r = 0; r < 2; ++r) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[r][i] = 0.0f;
 #pragma unroll
-      for (uint32_t k = 0; k < kD / 16; ++k) s[r] = mfma32<T>(reads.rows(k_at, r, k), q[k], s[r]);
+      for (uint32_t k = 0; k < kD / 16; ++k) s[r] = mfma32<T>(k_rows(r, k), q[k], s[r]);
     }
     if (key0 + kTile > whole) {
       if (a.causal) {
@@ -112,11 +113,12 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_kernel(tsa_attend_a
         s[r][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][i], c, base));
         total += s[r][i];
       }
+    const auto v_columns = reads.columns(v_at);
 #pragma unroll
     for (uint32_t u = 0; u < 4; ++u) {
       const bits8 p = pack8<T>(s[u / 2], u % 2);
 #pragma unroll
-      for (uint32_t t = 0; t < kD / 32; ++t) o[t] = mfma32<T>(reads.columns(v_at, t, u), p, o[t]);
+      for (uint32_t t = 0; t < kD / 32; ++t) o[t] = mfma32<T>(v_columns(t, u), p, o[t]);
     }
   }
   if (!on) return;
@@ -133,7 +135,7 @@ int launch_attend(const tsa_attend_args& a, hipStream_t stream) {
   using namespace op;
   const dim3 grid(uint32_t(own_tiles_at_most(a.sequences, a.tokens) * a.q.heads)), block(64 * kTileWaves);
   const float c = a.scale * 1.44269504f;
-  const bool aligned = vector_heads(a.q) && vector_heads(a.out) && (a.k_tokens == 0 || (vector_heads(a.k) && vector_heads(a.v)));
+  const bool aligned = vector_heads(a.q) && vector_heads(a.out) && (a.k_tokens == 0 || (tile_heads(a.k) && tile_heads(a.v)));
 #define CALL(T, D)                                                                                      \
   do {                                                                                                  \
     if (aligned) hipLaunchKernelGGL((attend_kernel<T, D, true>), grid, block, 0, stream, a, c);         \

@@ -105,14 +105,15 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void rows_kernel(tsa_attend_gra
     tile_ready();
     if (key0 >= o.any) continue;
     const int32_t left = int32_t(o.limit) - int32_t(key0 + 4 * h);
+    const auto k_rows = reads.rows(lds), v_rows = reads.rows(lds + S::kBytes);
 #pragma unroll
     for (uint32_t r = 0; r < 2; ++r) {
       f32x16 one[2];
       clear(one);
 #pragma unroll
       for (uint32_t k = 0; k < kD / 16; ++k) {
-        one[0] = mfma32<T>(reads.rows(lds, r, k), q.v[k], one[0]);
-        one[1] = mfma32<T>(reads.rows(lds + S::kBytes, r, k), dout.v[k], one[1]);
+        one[0] = mfma32<T>(k_rows(r, k), q.v[k], one[0]);
+        one[1] = mfma32<T>(v_rows(r, k), dout.v[k], one[1]);
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i)
@@ -188,14 +189,16 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void queries_kernel(tsa_attend_
       clean_done();
     }
     if (key0 >= o.any) continue;
+    const auto k_rows = reads.rows(k_at), v_rows = reads.rows(v_at);
+    const auto k_columns = reads.columns(k_at);
 #pragma unroll
     for (uint32_t r = 0; r < 2; ++r) {
       f32x16 one[2];  // scores, then their gradients; gradients of probabilities
       clear(one);
 #pragma unroll
       for (uint32_t k = 0; k < kD / 16; ++k) {
-        one[0] = mfma32<T>(reads.rows(k_at, r, k), q.v[k], one[0]);
-        one[1] = mfma32<T>(reads.rows(v_at, r, k), dout.v[k], one[1]);
+        one[0] = mfma32<T>(k_rows(r, k), q.v[k], one[0]);
+        one[1] = mfma32<T>(v_rows(r, k), dout.v[k], one[1]);
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i)
@@ -220,7 +223,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void queries_kernel(tsa_attend_
       for (uint32_t u = 0; u < 2; ++u) {
         const bits8 ds = pack8<T>(one[0], u);
 #pragma unroll
-        for (uint32_t t = 0; t < kD / 32; ++t) dq[t] = mfma32<T>(reads.columns(k_at, t, 2 * r + u), ds, dq[t]);
+        for (uint32_t t = 0; t < kD / 32; ++t) dq[t] = mfma32<T>(k_columns(t, 2 * r + u), ds, dq[t]);
       }
     }
   }
@@ -307,14 +310,16 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void keys_kernel(tsa_attend_gra
       clean_done();
     }
     if (at + kTile <= any) continue;
+    const auto q_rows = reads.rows(q_at), d_rows = reads.rows(d_at);
+    const auto q_columns = reads.columns(q_at), d_columns = reads.columns(d_at);
 #pragma unroll
     for (uint32_t r = 0; r < 2; ++r) {
       f32x16 one[2];  // scores, then probabilities; their gradients, then the scores'
       clear(one);
 #pragma unroll
       for (uint32_t i = 0; i < kD / 16; ++i) {
-        one[0] = mfma32<T>(reads.rows(q_at, r, i), k.v[i], one[0]);
-        if constexpr (kKeys) one[1] = mfma32<T>(reads.rows(d_at, r, i), v.v[i], one[1]);
+        one[0] = mfma32<T>(q_rows(r, i), k.v[i], one[0]);
+        if constexpr (kKeys) one[1] = mfma32<T>(d_rows(r, i), v.v[i], one[1]);
       }
 #pragma unroll
       for (uint32_t i = 0; i < 4; ++i) {
@@ -353,8 +358,8 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void keys_kernel(tsa_attend_gra
         const bits8 p = pack8<T>(one[0], u), ds = pack8<T>(one[1], u);
 #pragma unroll
         for (uint32_t t = 0; t < kD / 32; ++t) {
-          if constexpr (kValues) dv[t] = mfma32<T>(reads.columns(d_at, t, 2 * r + u), p, dv[t]);
-          if constexpr (kKeys) dk[t] = mfma32<T>(reads.columns(q_at, t, 2 * r + u), ds, dk[t]);
+          if constexpr (kValues) dv[t] = mfma32<T>(d_columns(t, 2 * r + u), p, dv[t]);
+          if constexpr (kKeys) dk[t] = mfma32<T>(q_columns(t, 2 * r + u), ds, dk[t]);
         }
       }
     }
@@ -440,8 +445,8 @@ int launch_attend_backward(const tsa_attend_grad_args& g, void* workspace, hipSt
   float2* rows = static_cast<float2*>(workspace);
   float* parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + up_to(uint64_t(a.tokens) * a.q.heads * sizeof(float2), 16));
   bool aligned = true;
-  if (a.tokens) aligned = vector_heads(a.q) && vector_heads(a.out) && vector_heads(g.dout) && (!g.dq.p || vector_heads(g.dq));
-  if (a.k_tokens) aligned = aligned && vector_heads(a.k) && vector_heads(a.v) && (!g.dk.p || (vector_heads(g.dk) && vector_heads(g.dv)));
+  if (a.tokens) aligned = tile_heads(a.q) && vector_heads(a.out) && tile_heads(g.dout) && (!g.dq.p || vector_heads(g.dq));
+  if (a.k_tokens) aligned = aligned && tile_heads(a.k) && tile_heads(a.v) && (!g.dk.p || (vector_heads(g.dk) && vector_heads(g.dv)));
 #define CALL(T, D)                                                     \
   do {                                                                 \
     if (aligned) gradients<T, D, true>(g, rows, parts, stream);               \

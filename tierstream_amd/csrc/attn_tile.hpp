@@ -54,43 +54,71 @@ struct TileShapes {
   }
 };
 
-// Loads of one head's tiles. kAligned: pieces start 16-byte aligned; otherwise value by value.
+// 64 lanes x 16 bytes from base + offset to LDS at `at` (base and at the same in every lane) in lane order.
+__device__ __forceinline__ void load_from_to_lds(const void* base, uint32_t offset, uint32_t at) {
+  asm volatile(
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %0, %1"
+      :
+      : "v"(offset), "s"(base), "s"(at)
+      : "memory", "m0");
+}
+
+// Loads of one head's tiles. kAligned: pieces start 16-byte aligned, and a tile's rows lie within 2^31 bytes; otherwise value by value.
 template <int kD, bool kAligned>
 struct TileLoads {
   typedef TileShapes<kD> S;
-  const u16* p;       // this lane's piece of the head's first tile's first row of its own
+  const u16* p;       // the head's first row
   uint64_t stride;
   uint32_t row, at, dim;
+  uint32_t offset[kAligned ? S::kLoads : 1];  // this lane's pieces from a tile's first row, in bytes
   __device__ __forceinline__ TileLoads(const tsa_heads& h, uint64_t first, uint32_t head, uint32_t head_dim) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     row = wave * S::kLoads * S::kRowsALoad + lane / S::kPieces;
-    // (the permutation repeats every 16 rows: the first load's is the others' too, or their rows' own)
     p = row_of<u16>(h, first, head);
     stride = h.token_stride;
     at = __builtin_amdgcn_readfirstlane(wave) * S::kLoads * 1024;
     dim = head_dim;
+    if constexpr (kAligned) {
+#pragma unroll
+      for (uint32_t j = 0; j < S::kLoads; ++j) offset[j] = uint32_t((row + j * S::kRowsALoad) * stride * 2) + 2 * value_of(j);
+    }
+  }
+  __device__ __forceinline__ uint32_t value_of(uint32_t j) const {
+    return 8 * (((threadIdx.x & 63u) % S::kPieces) ^ S::turn(row + j * S::kRowsALoad));
   }
   // Rows row0.. of `rows` to the buffer at lds; rows behind the last are zeros.
   __device__ __forceinline__ void fetch(uint32_t row0, uint32_t rows, uint32_t lds) const {
-    const uint32_t lane = threadIdx.x & 63u;
+    if constexpr (kAligned) {
+      const u16* const base = p + row0 * stride;
+      if (row0 + kTile <= rows && dim == kD) {
 #pragma unroll
-    for (uint32_t j = 0; j < S::kLoads; ++j) {
-      const uint32_t r = row + j * S::kRowsALoad, value = 8 * ((lane % S::kPieces) ^ S::turn(r));
-      const bool in = row0 + r < rows && value < dim;
-      const u16* g = p + uint64_t(row0 + r) * stride + value;
-      if constexpr (kAligned) {
-        load_to_lds(in ? static_cast<const void*>(g) : &kZeroPiece, lds + at + j * 1024);
+        for (uint32_t j = 0; j < S::kLoads; ++j) load_from_to_lds(base, offset[j], lds + at + j * 1024);
       } else {
+#pragma unroll
+        for (uint32_t j = 0; j < S::kLoads; ++j) {
+          const bool in = row0 + row + j * S::kRowsALoad < rows && value_of(j) < dim;
+          load_to_lds(in ? static_cast<const void*>(base + offset[j] / 2) : &kZeroPiece, lds + at + j * 1024);
+        }
+      }
+    } else {
+#pragma unroll
+      for (uint32_t j = 0; j < S::kLoads; ++j) {
+        const uint32_t r = row0 + row + j * S::kRowsALoad;
         bits8 v = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (in) {
+        if (r < rows && value_of(j) < dim) {
+          const u16* g = p + r * stride + value_of(j);
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] = g[i];
         }
-        *reinterpret_cast<lds_eight_put_t*>(lds + at + j * 1024 + lane * 16) = v;
+        *reinterpret_cast<lds_eight_put_t*>(lds + at + j * 1024 + (threadIdx.x & 63u) * 16) = v;
       }
     }
   }
 };
+// Whether heads are read in whole pieces, offsets inside a tile in 32 bits.
+inline bool tile_heads(const tsa_heads& h) { return vector_heads(h) && h.token_stride < (uint64_t(1) << 24); }
 
 // This wave's own rows as the second operand: column l % 32, values 16 k + 8 (l / 32)..; zeros where there is none.
 template <int kD, bool kAligned>
@@ -132,15 +160,40 @@ struct TileReads {
         columns_at[t][s] = r * S::kRowBytes + (piece ^ S::turn(r)) * 16 + (l & 1u) * 8;
       }
   }
-  // Rows 32 r.. at values 16 k..
-  __device__ __forceinline__ bits8 rows(uint32_t lds, uint32_t r, uint32_t k) const {
-    return *reinterpret_cast<lds_eight_t*>(lds + rows_at[k] + r * 32 * S::kRowBytes);
+  // The places in the buffer at lds, added up once a tile (the compiler would add the buffer's to each read's).
+  struct Rows {
+    uint32_t at[kD / 16];
+    __device__ __forceinline__ bits8 operator()(uint32_t r, uint32_t k) const {  // rows 32 r.. at values 16 k..
+      return *reinterpret_cast<lds_eight_t*>(at[k] + r * 32 * S::kRowBytes);
+    }
+  };
+  struct Columns {
+    uint32_t at[kD / 32][2];
+    __device__ __forceinline__ bits8 operator()(uint32_t t, uint32_t u) const {  // columns 32 t.. of rows 16 u..
+      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_four_t*>(at[t][0] + u * 16 * S::kRowBytes));
+      const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_four_t*>(at[t][1] + u * 16 * S::kRowBytes));
+      return __builtin_bit_cast(bits8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  };
+  __device__ __forceinline__ Rows rows(uint32_t lds) const {
+    Rows r;
+#pragma unroll
+    for (uint32_t k = 0; k < kD / 16; ++k) {
+      r.at[k] = lds + rows_at[k];
+      asm("" : "+v"(r.at[k]));
+    }
+    return r;
   }
-  // Columns 32 t.. of rows 16 u..
-  __device__ __forceinline__ bits8 columns(uint32_t lds, uint32_t t, uint32_t u) const {
-    const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_four_t*>(lds + columns_at[t][0] + u * 16 * S::kRowBytes));
-    const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_four_t*>(lds + columns_at[t][1] + u * 16 * S::kRowBytes));
-    return __builtin_bit_cast(bits8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  __device__ __forceinline__ Columns columns(uint32_t lds) const {
+    Columns c;
+#pragma unroll
+    for (uint32_t t = 0; t < kD / 32; ++t)
+#pragma unroll
+      for (uint32_t s = 0; s < 2; ++s) {
+        c.at[t][s] = lds + columns_at[t][s];
+        asm("" : "+v"(c.at[t][s]));
+      }
+    return c;
   }
 };
 
