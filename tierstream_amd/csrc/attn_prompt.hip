@@ -41,10 +41,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_kernel(tsa_attend_a
   const TileLoads<kD, kAligned> keys(a.k, ks.begin, kept, a.head_dim), values(a.v, ks.begin, kept, a.head_dim);
   const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_offset(tile_s));
   f32x16 o[kD / 32];
-#pragma unroll
-  for (int t = 0; t < kD / 32; ++t)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+  clear(o);
   float top = -INFINITY, total = 0.0f;
   if (end) {
     keys.fetch(0, ks.count, lds);
@@ -65,13 +62,12 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_kernel(tsa_attend_a
 
     const auto k_rows = reads.rows(k_at);
     f32x16 s[2];
+    clear(s);
 #pragma unroll
-    for (uint32_t r = 0; r < 2; ++r) {
+    for (uint32_t k = 0; k < kD / 16; ++k)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[r][i] = 0.0f;
-#pragma unroll
-      for (uint32_t k = 0; k < kD / 16; ++k) s[r] = mfma32<T>(k_rows(r, k), q[k], s[r]);
-    }
+      for (uint32_t r = 0; r < 2; ++r) s[r] = mfma32<T>(k_rows(r, k), q[k], s[r]);
+    products_behind_reads<kD / 8, 4>();
     if (key0 + kTile > whole) {
       if (a.causal) {
 #pragma unroll
@@ -91,6 +87,11 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_kernel(tsa_attend_a
           if (int32_t(32 * r + 8 * (i / 4) + i % 4) >= left) s[r][i] = -INFINITY;
     }
 
+    const auto v_columns = reads.columns(v_at);
+    bits8 v0[kD / 32];
+#pragma unroll
+    for (uint32_t t = 0; t < kD / 32; ++t) v0[t] = v_columns(t, 0);
+    __builtin_amdgcn_sched_barrier(0);
     // the running maximum: followed where it is passed by 2^8
     float most = -INFINITY;
 #pragma unroll
@@ -113,12 +114,11 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_kernel(tsa_attend_a
         s[r][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][i], c, base));
         total += s[r][i];
       }
-    const auto v_columns = reads.columns(v_at);
 #pragma unroll
     for (uint32_t u = 0; u < 4; ++u) {
       const bits8 p = pack8<T>(s[u / 2], u % 2);
 #pragma unroll
-      for (uint32_t t = 0; t < kD / 32; ++t) o[t] = mfma32<T>(v_columns(t, u), p, o[t]);
+      for (uint32_t t = 0; t < kD / 32; ++t) o[t] = mfma32<T>(u ? v_columns(t, u) : v0[t], p, o[t]);
     }
   }
   if (!on) return;

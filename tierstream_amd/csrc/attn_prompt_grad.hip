@@ -11,14 +11,6 @@ namespace tsa {
 namespace op {
 namespace {
 
-template <int N>
-__device__ __forceinline__ void clear(f32x16 (&v)[N]) {
-#pragma unroll
-  for (int t = 0; t < N; ++t)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[t][i] = 0.0f;
-}
-
 // The queries of a workgroup, and what of the keys they attend to.
 struct Queries {
   Span qs, ks;
@@ -115,6 +107,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void rows_kernel(tsa_attend_gra
         one[0] = mfma32<T>(k_rows(r, k), q.v[k], one[0]);
         one[1] = mfma32<T>(v_rows(r, k), dout.v[k], one[1]);
       }
+      products_behind_reads<kD / 8, 4>();
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         if (int32_t(32 * r + 8 * (i / 4) + i % 4) < left) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(one[0][i], c, -lse)) * one[1][i];
@@ -200,6 +193,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void queries_kernel(tsa_attend_
         one[0] = mfma32<T>(k_rows(r, k), q.v[k], one[0]);
         one[1] = mfma32<T>(v_rows(r, k), dout.v[k], one[1]);
       }
+      products_behind_reads<kD / 8, 4>();
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         one[0][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(one[0][i], c, -mine.x)) * (one[1][i] - mine.y);
@@ -321,6 +315,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void keys_kernel(tsa_attend_gra
         one[0] = mfma32<T>(q_rows(r, i), k.v[i], one[0]);
         if constexpr (kKeys) one[1] = mfma32<T>(d_rows(r, i), v.v[i], one[1]);
       }
+      if constexpr (kKeys) products_behind_reads<kD / 8, 4>();
 #pragma unroll
       for (uint32_t i = 0; i < 4; ++i) {
         const f32x4* pair = reinterpret_cast<const f32x4*>(&row_s[buffer][32 * r + 8 * i + 4 * h]);

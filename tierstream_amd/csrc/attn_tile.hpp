@@ -197,6 +197,27 @@ struct TileReads {
   }
 };
 
+template <int N>
+__device__ __forceinline__ void clear(f32x16 (&v)[N]) {
+#pragma unroll
+  for (int t = 0; t < N; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[t][i] = 0.0f;
+}
+
+// The order of kProducts matrix instructions and the 16-byte reads from LDS that feed one each: kAhead reads stand before the
+// first, so that each has the time of kAhead products (left to itself the compiler reads one ahead, and every product waits).
+template <int kProducts, int kAhead>
+__device__ __forceinline__ void products_behind_reads() {
+  __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+  for (int i = 0; i < kProducts - kAhead; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+}
+
 // Own loads landed, own reads done, and all waves here.
 __device__ __forceinline__ void tile_ready() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
