@@ -43,6 +43,9 @@ def test_struct_sizes_are_the_headers(tmp_path):
         lines += [f"_Static_assert(offsetof({name}, {f[0]}) == {getattr(cls, f[0]).offset}, \"{name}.{f[0]}\");" for f in cls._fields_]
     src = tmp_path / "sizes.c"
     src.write_text("#include <stddef.h>\n#include \"tierstream_amd/tsa_attn.h\"\n" + "\n".join(lines) + "\nint main(void) { return 0; }\n")
+    packed = {attn._ROTATE: attn.TsaRotateArgs, attn._PLAN: attn.TsaCachePlanArgs, attn._ROWS: attn.TsaCacheRowsArgs, attn._CACHED: attn.TsaAttendCachedArgs,
+              attn._ATTEND: attn.TsaAttendArgs, attn._GRAD: attn.TsaAttendGradArgs}
+    assert all(p.size == C.sizeof(cls) for p, cls in packed.items())
     r = subprocess.run(["gcc", f"-I{ROOT / 'include'}", "-c", str(src), "-o", str(tmp_path / "sizes.o")], capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
 

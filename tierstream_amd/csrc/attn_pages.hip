@@ -7,30 +7,33 @@ namespace op {
 namespace {
 
 // ---- pages and slots ----
-constexpr uint32_t kPlanThreads = 1024, kPlanPer = TSA_CACHE_MAX_REQUESTS / kPlanThreads;
-constexpr uint32_t kPlanRows = 8192;  // rows that the planning workgroup writes itself: a second launch costs more below
+__device__ __forceinline__ uint32_t pages_of(uint32_t tokens) { return tokens / kPage + (tokens % kPage != 0); }
 
-__device__ __forceinline__ uint32_t pages_of(int64_t tokens) { return uint32_t((tokens + kPage - 1) / kPage); }
-
-// Inclusive sums of 64-bit counts over the workgroup's threads; `all`: the whole sum.
-__device__ __forceinline__ int64_t scan(int64_t v, int64_t* waves, int64_t& all) {
+// Three 64-bit counts of each thread: their sums over the threads before it, and over all.
+template <uint32_t kThreads>
+__device__ __forceinline__ void scan(const int64_t (&v)[3], int64_t (&before)[3], int64_t (&all)[3], int64_t (&waves)[3][kThreads / 64]) {
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
 #pragma unroll
-  for (uint32_t s = 1; s < 64; s <<= 1) {
-    const int64_t o = __shfl_up(v, s, 64);
-    if (lane >= s) v += o;
-  }
-  __syncthreads();  // the last scan's sums are read
-  if (lane == 63) waves[wave] = v;
-  __syncthreads();
-  all = 0;
-  int64_t before = 0;
+  for (int k = 0; k < 3; ++k) {
+    int64_t upto = v[k];
 #pragma unroll
-  for (uint32_t w = 0; w < kPlanThreads / 64; ++w) {
-    if (w == wave) before = all;
-    all += waves[w];
+    for (uint32_t s = 1; s < 64; s <<= 1) {
+      const int64_t o = __shfl_up(upto, s, 64);
+      if (lane >= s) upto += o;
+    }
+    before[k] = upto - v[k];
+    if (lane == 63) waves[k][wave] = upto;
   }
-  return before + v;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    all[k] = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kThreads / 64; ++w) {
+      if (w < wave) before[k] += waves[k][w];
+      all[k] += waves[k][w];
+    }
+  }
 }
 
 // The last i with first[i] <= x, of first[0] = 0 <= ... <= first[n], x < first[n].
@@ -45,13 +48,139 @@ __device__ __forceinline__ uint32_t owner_of(const I* first, uint32_t n, I x) {
   return lo;
 }
 
-// Row r's position and slot, from the requests' rows (first) and ends.
-__device__ __forceinline__ void write_slot(const tsa_cache_plan_args& a, const int32_t* first, int64_t rows, const int32_t* ends, uint32_t r) {
+// A plan's sums over the requests before each: its rows, the pages it takes and the pages it gives back; and its length before.
+template <uint32_t kMost>
+struct PlanSums {
+  int32_t first[kMost + 1], taken[kMost + 1], given[kMost + 1], length[kMost];
+};
+
+// The whole plan by one workgroup, or (more than kPlanMany rows) its pages and rows by several and what replaces the inputs by another launch
+// behind them: lengths may become ends in place. Each workgroup adds up all requests itself. Pages given back and pages taken in
+// one plan pass each other by: the k-th page taken is the k-th last given, or lies that far down in the stack, so that nothing waits for
+// what another thread writes. 32 requests 3 us, a launch and three memory latencies (9 with 1024 threads and a barrier between giving and
+// taking); 2047 requests with 65536 rows and some 10,000 pages given back 12 and 5 (26 together).
+template <uint32_t kThreads, uint32_t kPer>
+__global__ __launch_bounds__(kThreads) void plan_kernel(tsa_cache_plan_args a, bool work, bool finish) {
+  constexpr uint32_t kMost = kThreads * kPer;
+  __shared__ int64_t waves[3][kThreads / 64];
+  __shared__ PlanSums<kMost> sum_s;
+  __shared__ uint32_t bad_s;
+  const uint32_t t = threadIdx.x;
+  if (t == 0) bad_s = 0;
+  const int64_t n_free = a.n_free[0];
+  // memory in whole lines and all at once (one request after the other a thread waited for each: 9 us for 2047), then by way of LDS
+  int32_t line[2][kPer];
+#pragma unroll
+  for (uint32_t k = 0; k < kPer; ++k) {
+    const uint32_t i = k * kThreads + t;
+    line[0][k] = i < a.requests ? a.lengths[i] : 0;
+    line[1][k] = i < a.requests ? a.fresh[i] : 0;
+  }
+#pragma unroll
+  for (uint32_t k = 0; k < kPer; ++k) {
+    sum_s.length[k * kThreads + t] = line[0][k];
+    sum_s.first[k * kThreads + t] = line[1][k];
+  }
+  __syncthreads();
+  int32_t length[kPer], fresh[kPer];
+  int64_t add = 0, need = 0, gone = 0;
+  uint32_t bad = 0;
+#pragma unroll
+  for (uint32_t k = 0; k < kPer; ++k) {  // thread t has requests kPer t..
+    const uint32_t i = t * kPer + k;
+    length[k] = sum_s.length[i];
+    fresh[k] = sum_s.first[i];
+  }
+#pragma unroll
+  for (uint32_t k = 0; k < kPer; ++k) {
+    if (length[k] < 0) {
+      bad |= 8;
+      continue;
+    }
+    const uint32_t end = uint32_t(length[k]) + (fresh[k] < 0 ? 0u : uint32_t(fresh[k])), have = pages_of(uint32_t(length[k]));
+    if (pages_of(end) > a.width || end > uint32_t(INT32_MAX)) bad |= 4;
+    if (fresh[k] < 0) gone += have;
+    else add += fresh[k], need += pages_of(end) - have;
+  }
+  int64_t before[3], all[3];
+  scan<kThreads>({add, need, gone}, before, all, waves);
+  const int64_t adds = all[0], needs = all[1], gones = all[2];
+  if (n_free < 0 || n_free > a.pages || n_free + gones > a.pages) bad |= 8;
+  if (needs > n_free + gones) bad |= 1;
+  if (adds > a.rows) bad |= 2;
+  if (bad) atomicOr(&bad_s, bad);
+  __syncthreads();
+  const bool ok = bad_s == 0;
+  int64_t at_add = before[0], at_need = before[1], at_gone = before[2];
+#pragma unroll
+  for (uint32_t k = 0; k < kPer; ++k) {
+    const uint32_t i = t * kPer + k;
+    if (i >= a.requests) break;
+    const bool over = fresh[k] < 0;
+    sum_s.first[i] = ok ? int32_t(at_add) : 0;
+    sum_s.taken[i] = int32_t(at_need);
+    sum_s.given[i] = int32_t(at_gone);
+    if (!ok) continue;
+    if (over) at_gone += pages_of(uint32_t(length[k]));
+    else at_add += fresh[k], at_need += pages_of(uint32_t(length[k]) + uint32_t(fresh[k])) - pages_of(uint32_t(length[k]));
+  }
+  const uint32_t rows = ok ? uint32_t(adds) : 0;
+  if (t == 0) {
+    sum_s.first[a.requests] = int32_t(rows);
+    if (finish) {
+      a.first[a.requests] = int32_t(rows);
+      a.left[0] = int32_t(ok ? n_free + gones - needs : n_free);
+      a.status[0] = int32_t(bad_s);
+    }
+  }
+  __syncthreads();
+  if (finish) {
+#pragma unroll
+    for (uint32_t k = 0; k < kPer; ++k) {
+      const uint32_t i = k * kThreads + t;
+      if (i >= a.requests) break;
+      a.ends[i] = !ok ? line[0][k] : line[1][k] < 0 ? 0 : line[0][k] + line[1][k];
+      a.first[i] = sum_s.first[i];
+    }
+  }
+  if (!work) return;
+  const uint32_t step = gridDim.x * kThreads, from = blockIdx.x * kThreads + t;
+  // page j of those given back, and the k-th page taken
+  auto given = [&](uint32_t j) {
+    const uint32_t i = owner_of(sum_s.given, a.requests, int32_t(j));
+    return a.table[i * a.table_stride + (j - uint32_t(sum_s.given[i]))];
+  };
+  auto taken = [&](uint32_t k) { return k < gones ? given(uint32_t(gones) - 1 - k) : a.free[n_free - 1 - (int64_t(k) - gones)]; };
+  if (ok) {
+    for (uint32_t j = from; j < uint32_t(gones); j += step) a.free[n_free + j] = given(j);
+    for (uint32_t k = from; k < uint32_t(needs); k += step) {
+      const uint32_t i = owner_of(sum_s.taken, a.requests, int32_t(k));
+      a.table[i * a.table_stride + pages_of(uint32_t(sum_s.length[i])) + (k - uint32_t(sum_s.taken[i]))] = taken(k);
+    }
+  }
+  for (uint32_t r = from; r < a.rows; r += step) {
+    int32_t position = -1, slot = -1;
+    if (r < rows) {
+      const uint32_t i = owner_of(sum_s.first, a.requests, int32_t(r)), have = pages_of(uint32_t(sum_s.length[i]));
+      position = sum_s.length[i] + int32_t(r - uint32_t(sum_s.first[i]));
+      const uint32_t p = uint32_t(position) / kPage;
+      const int32_t page = p < have ? a.table[i * a.table_stride + p] : taken(uint32_t(sum_s.taken[i]) + p - have);
+      if (page >= 0 && page < (1 << 25)) slot = page * int32_t(kPage) + position % int32_t(kPage);
+    }
+    a.positions[r] = position;
+    a.slots[r] = slot;
+  }
+}
+
+__global__ __launch_bounds__(256) void slots_kernel(tsa_cache_plan_args a) {
+  const uint32_t r = blockIdx.x * 256 + threadIdx.x;
+  if (r >= a.rows) return;
+  const int64_t rows = a.requests ? a.first[a.requests] : 0;
   int64_t position = -1;
   int32_t slot = -1;
   if (int64_t(r) < rows) {
-    const uint32_t i = owner_of(first, a.requests, int32_t(r));
-    position = int64_t(ends[i]) - first[i + 1] + r;
+    const uint32_t i = owner_of(a.first, a.requests, int32_t(r));
+    position = int64_t(a.ends[i]) - a.first[i + 1] + r;
     if (position < 0) {
       position = -1;
     } else if (position / kPage < a.width) {
@@ -61,91 +190,6 @@ __device__ __forceinline__ void write_slot(const tsa_cache_plan_args& a, const i
   }
   a.positions[r] = int32_t(position);
   a.slots[r] = slot;
-}
-
-__global__ __launch_bounds__(kPlanThreads) void plan_kernel(tsa_cache_plan_args a, uint32_t write_rows) {
-  __shared__ int64_t waves[kPlanThreads / 64];
-  __shared__ int32_t first_s[TSA_CACHE_MAX_REQUESTS + 1], end_s[TSA_CACHE_MAX_REQUESTS];
-  __shared__ int32_t taken_s[TSA_CACHE_MAX_REQUESTS + 1], given_s[TSA_CACHE_MAX_REQUESTS + 1];
-  __shared__ uint32_t bad_s;
-  const uint32_t t = threadIdx.x;
-  if (t == 0) bad_s = 0;
-  int32_t length[kPlanPer], fresh[kPlanPer];
-  int64_t add = 0, need = 0, gone = 0;
-  uint32_t bad = 0;
-#pragma unroll
-  for (uint32_t k = 0; k < kPlanPer; ++k) {  // thread t has requests 4 t..
-    const uint32_t i = t * kPlanPer + k;
-    length[k] = i < a.requests ? a.lengths[i] : 0;
-    fresh[k] = i < a.requests ? a.fresh[i] : 0;
-    if (length[k] < 0) {
-      bad |= 8;
-      continue;
-    }
-    const int64_t end = int64_t(length[k]) + fresh[k];
-    if (fresh[k] < 0) {
-      gone += pages_of(length[k]);
-      if (pages_of(length[k]) > a.width) bad |= 4;
-    } else {
-      add += fresh[k];
-      if (pages_of(end) > a.width || end > INT32_MAX) bad |= 4;
-      else need += pages_of(end) - pages_of(length[k]);
-    }
-  }
-  int64_t adds, needs, gones;
-  const int64_t add0 = scan(add, waves, adds) - add, need0 = scan(need, waves, needs) - need, gone0 = scan(gone, waves, gones) - gone;
-  const int64_t n_free = a.n_free[0];
-  if (n_free < 0 || n_free > a.pages || n_free + gones > a.pages) bad |= 8;
-  if (needs > n_free + gones) bad |= 1;
-  if (adds > a.rows) bad |= 2;
-  if (bad) atomicOr(&bad_s, bad);
-  __syncthreads();
-  const bool ok = bad_s == 0;
-  const int32_t count = int32_t(ok ? n_free + gones : n_free);
-  int64_t at_add = add0, at_need = need0, at_gone = gone0;
-#pragma unroll
-  for (uint32_t k = 0; k < kPlanPer; ++k) {
-    const uint32_t i = t * kPlanPer + k;
-    if (i >= a.requests) break;
-    const bool over = fresh[k] < 0;
-    const int32_t end = !ok ? length[k] : over ? 0 : length[k] + fresh[k];
-    first_s[i] = ok ? int32_t(at_add) : 0;
-    end_s[i] = end;
-    taken_s[i] = int32_t(at_need);
-    given_s[i] = int32_t(at_gone);
-    a.ends[i] = end;
-    a.first[i] = first_s[i];
-    if (!ok) continue;
-    if (over) at_gone += pages_of(length[k]);
-    else at_add += fresh[k], at_need += pages_of(end) - pages_of(length[k]);
-  }
-  const int32_t rows = ok ? int32_t(adds) : 0;
-  if (t == 0) {
-    first_s[a.requests] = rows;
-    a.first[a.requests] = rows;
-    a.left[0] = ok ? int32_t(count - needs) : count;
-    a.status[0] = int32_t(bad_s);
-  }
-  __syncthreads();
-  if (ok) {
-    for (uint32_t j = t; j < uint32_t(gones); j += kPlanThreads) {
-      const uint32_t i = owner_of(given_s, a.requests, int32_t(j));
-      a.free[n_free + j] = a.table[i * a.table_stride + (j - given_s[i])];
-    }
-    __syncthreads();  // the stack is whole before pages are taken
-    for (uint32_t j = t; j < uint32_t(needs); j += kPlanThreads) {
-      const uint32_t i = owner_of(taken_s, a.requests, int32_t(j));
-      const uint32_t next = i + 1 < a.requests ? taken_s[i + 1] : uint32_t(needs);
-      a.table[i * a.table_stride + (pages_of(end_s[i]) - (next - j))] = a.free[count - 1 - int32_t(j)];
-    }
-    __syncthreads();
-  }
-  for (uint32_t r = t; r < write_rows; r += kPlanThreads) write_slot(a, first_s, rows, end_s, r);
-}
-
-__global__ __launch_bounds__(256) void slots_kernel(tsa_cache_plan_args a) {
-  const uint32_t r = blockIdx.x * 256 + threadIdx.x;
-  if (r < a.rows) write_slot(a, a.first, a.requests ? a.first[a.requests] : 0, a.ends, r);
 }
 
 // ---- keys and values to their slots and back ----
@@ -174,17 +218,15 @@ struct RowPiece {  // piece j of block b of head h of k (0) or v (1) of token t
   bool on;
 };
 __device__ __forceinline__ RowPiece row_piece(const tsa_cache& c, uint32_t tokens) {
-  const uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x;
-  const uint32_t nb = c.head_dim / 32, row = 2 * c.kv_heads * nb;
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x, nb = c.head_dim / 32, row = 2 * c.kv_heads * nb;  // (pieces are below 2^31)
   RowPiece p;
-  const uint64_t block = i >> 2;
-  p.j = uint32_t(i) & 3u;
-  p.t = uint32_t(block / row);
-  uint32_t in = uint32_t(block % row);
-  p.b = in % nb;
-  in /= nb;
-  p.h = in % c.kv_heads;
-  p.which = in / c.kv_heads;
+  p.j = i & 3u;
+  p.t = (i >> 2) / row;
+  uint32_t in = (i >> 2) - p.t * row;
+  p.b = nb == 4 ? in & 3u : in % nb;
+  in = nb == 4 ? in >> 2 : in / nb;
+  p.which = in >= c.kv_heads;
+  p.h = p.which ? in - c.kv_heads : in;
   p.on = p.t < tokens;
   return p;
 }
@@ -194,37 +236,45 @@ __device__ __forceinline__ BlockPlace place_of(const tsa_cache& c, uint32_t slot
 
 template <class T>
 __global__ __launch_bounds__(256) void store_kernel(tsa_cache c, tsa_cache_rows_args a, bool vector) {
+  constexpr uint32_t kInfinity = std::is_same_v<T, Bf16> ? 0x7F80 : 0x7C00;
   const RowPiece p = row_piece(c, a.tokens);
   const uint32_t slot = p.on ? uint32_t(a.slots[p.t]) : ~0u;
   if (slot >= c.n_pages * kPage) return;  // (a block's four lanes go together)
   const tsa_heads& h = p.which ? a.v : a.k;
   const bits8 raw = load8(h, uint64_t(p.t) * h.token_stride + uint64_t(p.h) * h.head_stride + p.b * 32 + p.j * 8, vector);
-  float x[8], top = 0.0f;
-  bool finite = true;
-  float big = 0.0f;  // the value of the largest size, the first of equal ones
+  // the largest size, by its bits; then the first value that has it
+  const bits8 size = raw & u16(0x7FFF);
+  uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    x[i] = T::up(raw[i]);
-    finite = finite && fabsf(x[i]) < INFINITY;
-    if (fabsf(x[i]) > top) top = fabsf(x[i]), big = x[i];
-  }
+  for (int i = 0; i < 8; ++i) top = size[i] > top ? size[i] : top;
 #pragma unroll
   for (int s = 1; s < 4; s <<= 1) {
-    const float other = __shfl_xor(big, s, 64);
-    finite = finite & (__shfl_xor(int(finite), s, 64) != 0);
-    const bool lower = (p.j & s) != 0;  // the other lane's values stand before this one's
-    if (fabsf(other) > fabsf(big) || (lower && fabsf(other) == fabsf(big))) big = other;
+    const uint32_t o = __shfl_xor(top, s, 64);
+    top = o > top ? o : top;
   }
+  uint32_t mine = 0;
+  bool there = false;
+#pragma unroll
+  for (int i = 7; i >= 0; --i)
+    if (size[i] == top) mine = raw[i], there = true;
+  const uint32_t lane = threadIdx.x & 63u, quad = lane & 60u;
+  const uint32_t has = uint32_t(__ballot(there) >> quad) & 15u, minus = uint32_t(__ballot(there && (mine & 0x8000u)) >> quad) & 15u;
+  const bool finite = top < kInfinity, negative = (minus & has & (0u - has)) != 0;
   // (-big / 8 is exact; a scale beyond half precision is an infinity and 0 times it is NaN, as it should be)
-  const u16 scale = finite ? F16::down(big * -0.125f) : u16(0x7E00);
-  const float step = F16::up(scale);
+  const float big = T::up(u16(top));
+  const u16 scale = finite ? F16::down(negative ? big * 0.125f : big * -0.125f) : u16(0x7E00);
+  const float step = F16::up(scale), each = finite && big != 0.0f && step != 0.0f ? 1.0f / step : 0.0f;
   uint32_t lo = 0, hi = 0;  // 8 half bytes, one a byte
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    // The quotient of a 16-bit value and a half-precision step is no nearer than 2^-15 of itself to a border between two steps
-    // unless it is on it, so that its rounding to 32 bits takes none over.
-    float q = step == 0.0f || !finite ? 0.0f : rintf(x[i] / step);
-    q = fminf(fmaxf(q, -8.0f), 7.0f);
+    // The nearest whole step, ties to even. The quotient of a 16-bit value and a half-precision step lies on a border between two
+    // steps or 2^-15 of itself away from it: taken through the reciprocal it is off by 2^-23, which moves it over none, but may move it off one
+    // that it lies on. What is left of it is exact, and is half a step on a border alone.
+    const float x = T::up(raw[i]);
+    float q = each == 0.0f ? 0.0f : rintf(x * each);
+    const float left = 2.0f * __builtin_fmaf(-q, step, x);
+    if (fabsf(left) == fabsf(step) && (int(q) & 1)) q += (left < 0.0f) == (step < 0.0f) ? 1.0f : -1.0f;
+    q = __builtin_amdgcn_fmed3f(q, -8.0f, 7.0f);
     const uint32_t n = uint32_t(int(q) + 8);
     if (i < 4) lo |= n << (8 * i);
     else hi |= n << (8 * (i - 4));
@@ -277,10 +327,28 @@ uint32_t row_grid(const tsa_cache& c, uint32_t tokens) {
 }  // namespace
 }  // namespace op
 
+namespace op {
+namespace {
+constexpr uint32_t kPlanMany = 8192;  // rows that one workgroup writes faster than a second launch begins
+
+template <uint32_t kThreads, uint32_t kPer>
+void plan(const tsa_cache_plan_args& a, hipStream_t stream) {
+  if (a.rows <= kPlanMany) {
+    hipLaunchKernelGGL((plan_kernel<kThreads, kPer>), dim3(1), dim3(kThreads), 0, stream, a, true, true);
+    return;
+  }
+  const uint32_t groups = (a.rows + 2 * kThreads - 1) / (2 * kThreads);
+  hipLaunchKernelGGL((plan_kernel<kThreads, kPer>), dim3(groups < 256 ? groups : 256), dim3(kThreads), 0, stream, a, true, false);
+  hipLaunchKernelGGL((plan_kernel<kThreads, kPer>), dim3(1), dim3(kThreads), 0, stream, a, false, true);
+}
+}  // namespace
+}  // namespace op
+
 int launch_cache_plan(const tsa_cache_plan_args& a, hipStream_t stream) {
-  const bool one = a.rows <= op::kPlanRows;
-  hipLaunchKernelGGL(op::plan_kernel, dim3(1), dim3(op::kPlanThreads), 0, stream, a, one ? a.rows : 0u);
-  if (!one) hipLaunchKernelGGL(op::slots_kernel, dim3((a.rows + 255) / 256), dim3(256), 0, stream, a);
+  // the fewest threads that hold the requests, and do not take many turns over the rows
+  if (a.requests <= 64 && (a.rows <= 256 || a.rows > op::kPlanMany)) op::plan<64, 1>(a, stream);
+  else if (a.requests <= 256 && (a.rows <= 1024 || a.rows > op::kPlanMany)) op::plan<256, 1>(a, stream);
+  else op::plan<512, TSA_CACHE_MAX_REQUESTS / 512>(a, stream);
   return int(hipGetLastError());
 }
 
