@@ -411,7 +411,8 @@ def cached64(q, pages, dim, table, ends, counts, scale, n_pages):
 CACHED = [  # ends, fresh, kept, group, dim
     ([1], [1], 1, 1, 32), ([64], [1], 2, 4, 128), ([65], [1], 8, 4, 128), ([63, 1, 128, 700], [1] * 4, 4, 8, 128), ([2100], [1], 1, 16, 64),
     ([5, 300], [5, 2], 2, 5, 96), ([200, 0, 77], [3, 0, 8], 2, 1, 64), ([1000, 130], [1, 0], 3, 3, 128), ([4099], [4], 2, 4, 128), ([90], [40], 1, 6, 128),
-    ([3], [5], 2, 2, 64), ([129, 64, 65, 63, 1, 2, 192, 500, 3], [1] * 9, 2, 2, 32), ([300], [17], 1, 33, 64)]
+    ([3], [5], 2, 2, 64), ([129, 64, 65, 63, 1, 2, 192, 500, 3], [1] * 9, 2, 2, 32), ([300], [17], 1, 33, 64),
+    ([9000, 17000], [1, 2], 8, 4, 128), ([20001], [1], 8, 2, 64), ([700] * 12, [2] * 12, 16, 1, 96)]  # (more pages than take both parts of a probability)
 
 
 @pytest.mark.parametrize("kind", ["bf16", "f16"])
@@ -514,7 +515,8 @@ def attend64(q, k, v, counts, k_counts, causal, scale, dout=None):
 ATTEND = [  # queries, keys (None: as many), kept, group, dim
     ([1], None, 1, 1, 64), ([64], None, 2, 2, 128), ([65], None, 1, 4, 128), ([1, 2, 3, 127, 128, 129], None, 2, 1, 64), ([300], None, 1, 2, 72),
     ([33, 0, 200], None, 2, 3, 8), ([10, 70], [300, 5], 2, 2, 128), ([40], [40 + 512], 1, 4, 64), ([5, 64], [0, 64], 1, 1, 32), ([257, 31], None, 4, 1, 104),
-    ([513], None, 1, 1, 128), ([1, 1, 1, 1], [1, 64, 65, 1000], 2, 4, 128), ([5] * 70, None, 1, 2, 64)]
+    ([513], None, 1, 1, 128), ([1, 1, 1, 1], [1, 64, 65, 1000], 2, 4, 128), ([5] * 70, None, 1, 2, 64),
+    ([300, 77], None, 2, 4, 128), ([1, 600], [70, 650], 4, 2, 64), ([190, 3, 130], [260, 64, 100], 1, 8, 72)]  # (more rows than take both parts)
 
 
 def attend_case(kind, counts, k_counts, kept, group, dim, layout, pad=3):

@@ -20,6 +20,10 @@ namespace op {
 namespace {
 
 constexpr uint32_t kWaves = 4, kRows = 16, kMinShare = kWaves;  // waves, query rows and the fewest pages of a workgroup
+// Probabilities times scales go to the matrix instruction as two bf16 numbers each, rounded to 16 bits, in half precision; in bf16 too up to so
+// many pages (of all heads): few outputs may be off by more than their own rounding otherwise, and such calls are all latency (one token
+// behind 4096: 10.4 us either way). Beyond, as one number: its error is like the output's own, and the second takes a fifth of the time.
+constexpr uint64_t kSplitPages = 2048;
 // Workgroups of a CU that the registers leave room for, and of the chip.
 constexpr uint32_t per_cu(uint32_t head_dim) { return head_dim <= 64 ? 4 : 3; }
 constexpr uint32_t groups(uint32_t head_dim) { return 256 * per_cu(head_dim); }
@@ -199,7 +203,7 @@ struct Scales {
   }
 };
 
-template <class T, int NB>
+template <class T, int NB, bool kSplit>
 __global__ __launch_bounds__(64 * kWaves, per_cu(32 * NB)) void cached_kernel(tsa_cache c, tsa_attend_cached_args a, CachedShape s, float* parts, float2* stats) {
   typedef Page<NB> P;
   constexpr bool kHalf = std::is_same_v<T, F16>;
@@ -400,7 +404,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(32 * NB)) void cached_kernel(ts
             o[2 * b + h] = Bf16::mfma(eight, p16, o[2 * b + h]);
             o[2 * b + h] = Bf16::mfma(values.of(uint32_t(words[h])), p16, o[2 * b + h]);
           }
-          if constexpr (kHalf) {
+          if constexpr (kSplit) {
             u32x4 lo;
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i)
@@ -546,7 +550,10 @@ void attend_cached(const tsa_cache& c, const tsa_attend_cached_args& a, const Ca
   const uint32_t tiles = uint32_t(tiles_at_most(a, s.group)) * c.kv_heads;
   float* parts = static_cast<float*>(workspace);
   float2* stats = reinterpret_cast<float2*>(parts + uint64_t(2) * s.shares * c.kv_heads * kRows * 32 * NB);
-  hipLaunchKernelGGL((cached_kernel<T, NB>), dim3(s.shares * c.kv_heads), dim3(64 * kWaves), 0, stream, c, a, s, parts, stats);
+  const dim3 grid(s.shares * c.kv_heads), block(64 * kWaves);
+  constexpr bool kHalf = std::is_same_v<T, F16>;
+  if (kHalf || uint64_t(tiles) * a.width <= kSplitPages) hipLaunchKernelGGL((cached_kernel<T, NB, true>), grid, block, 0, stream, c, a, s, parts, stats);
+  else hipLaunchKernelGGL((cached_kernel<T, NB, kHalf>), grid, block, 0, stream, c, a, s, parts, stats);
   // (a workgroup a row where there are few; one share holds every tile whole)
   const uint32_t rows = tiles * kRows <= 1024 ? kRows : tiles < 1024 ? 1024 / tiles : 1;
   if (s.shares > 1) hipLaunchKernelGGL((join_kernel<T, NB>), dim3(tiles, rows), dim3(64 * kWaves), 0, stream, c, a, s, parts, stats);

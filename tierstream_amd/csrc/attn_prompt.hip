@@ -7,7 +7,7 @@ namespace tsa {
 namespace op {
 namespace {
 
-template <class T, int kD, bool kAligned>
+template <class T, int kD, bool kAligned, bool kSplit>
 __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_kernel(tsa_attend_args a, float c) {
   typedef TileShapes<kD> S;
   constexpr float kUp = std::is_same_v<T, F16> ? 7.0f : 0.0f;  // half precision: probabilities up to 2^15, so that small ones keep their bits
@@ -116,9 +116,9 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_kernel(tsa_attend_a
       }
 #pragma unroll
     for (uint32_t u = 0; u < 4; ++u) {
-      const bits8 p = pack8<T>(s[u / 2], u % 2);
+      const Second<T, kSplit> p(s[u / 2], u % 2);
 #pragma unroll
-      for (uint32_t t = 0; t < kD / 32; ++t) o[t] = mfma32<T>(u ? v_columns(t, u) : v0[t], p, o[t]);
+      for (uint32_t t = 0; t < kD / 32; ++t) p.add(u ? v_columns(t, u) : v0[t], o[t]);
     }
   }
   if (!on) return;
@@ -136,10 +136,11 @@ int launch_attend(const tsa_attend_args& a, hipStream_t stream) {
   const dim3 grid(uint32_t(own_tiles_at_most(a.sequences, a.tokens) * a.q.heads)), block(64 * kTileWaves);
   const float c = a.scale * 1.44269504f;
   const bool aligned = vector_heads(a.q) && vector_heads(a.out) && (a.k_tokens == 0 || (tile_heads(a.k) && tile_heads(a.v)));
-#define CALL(T, D)                                                                                      \
-  do {                                                                                                  \
-    if (aligned) hipLaunchKernelGGL((attend_kernel<T, D, true>), grid, block, 0, stream, a, c);         \
-    else hipLaunchKernelGGL((attend_kernel<T, D, false>), grid, block, 0, stream, a, c);                \
+#define CALL(T, D)                                                                                       \
+  do {                                                                                                   \
+    if (!aligned) hipLaunchKernelGGL((attend_kernel<T, D, false, true>), grid, block, 0, stream, a, c);  \
+    else if (split_rows(a)) hipLaunchKernelGGL((attend_kernel<T, D, true, true>), grid, block, 0, stream, a, c); \
+    else hipLaunchKernelGGL((attend_kernel<T, D, true, false>), grid, block, 0, stream, a, c);           \
   } while (0)
   if (a.type == TSA_BF16) {
     if (a.head_dim <= 64) CALL(Bf16, 64);

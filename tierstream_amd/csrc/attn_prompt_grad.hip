@@ -147,7 +147,7 @@ struct Raised<F16> {
   __device__ __forceinline__ float down() const { return by == 0.0f ? 0.0f : 1.0f / by; }
 };
 
-template <class T, int kD, bool kAligned>
+template <class T, int kD, bool kAligned, bool kSplit>
 __global__ __launch_bounds__(64 * kTileWaves, 2) void queries_kernel(tsa_attend_grad_args g, const float2* rows, float c) {
   typedef TileShapes<kD> S;
   __shared__ __attribute__((aligned(16))) unsigned char tile_s[2][2][S::kBytes];  // keys and values, two of each
@@ -215,9 +215,9 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void queries_kernel(tsa_attend_
       if constexpr (std::is_same_v<T, F16>) one[0] *= raised.by;
 #pragma unroll
       for (uint32_t u = 0; u < 2; ++u) {
-        const bits8 ds = pack8<T>(one[0], u);
+        const Second<T, kSplit> ds(one[0], u);
 #pragma unroll
-        for (uint32_t t = 0; t < kD / 32; ++t) dq[t] = mfma32<T>(k_columns(t, 2 * r + u), ds, dq[t]);
+        for (uint32_t t = 0; t < kD / 32; ++t) ds.add(k_columns(t, 2 * r + u), dq[t]);
       }
     }
   }
@@ -242,7 +242,7 @@ __device__ __forceinline__ void put_part(float* p, const f32x16 (&v)[kD / 32], f
 
 // Both gradients of keys and values, or one. With 128 values both together need 430 registers, one wave a SIMD: they took 840 us in three
 // packed sequences of 8192 together, one after the other with the scores computed again 660.
-template <class T, int kD, bool kAligned, bool kKeys, bool kValues>
+template <class T, int kD, bool kAligned, bool kSplit, bool kKeys, bool kValues>
 __global__ __launch_bounds__(64 * kTileWaves, 2) void keys_kernel(tsa_attend_grad_args g, const float2* rows, float c, uint32_t pieces, float* parts) {
   typedef TileShapes<kD> S;
   constexpr float kUp = probability_up<T>();
@@ -350,11 +350,11 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void keys_kernel(tsa_attend_gra
       }
 #pragma unroll
       for (uint32_t u = 0; u < 2; ++u) {
-        const bits8 p = pack8<T>(one[0], u), ds = pack8<T>(one[1], u);
+        const Second<T, kSplit> p(one[0], u), ds(one[1], u);
 #pragma unroll
         for (uint32_t t = 0; t < kD / 32; ++t) {
-          if constexpr (kValues) dv[t] = mfma32<T>(d_columns(t, 2 * r + u), p, dv[t]);
-          if constexpr (kKeys) dk[t] = mfma32<T>(q_columns(t, 2 * r + u), ds, dk[t]);
+          if constexpr (kValues) p.add(d_columns(t, 2 * r + u), dv[t]);
+          if constexpr (kKeys) ds.add(q_columns(t, 2 * r + u), dk[t]);
         }
       }
     }
@@ -401,21 +401,21 @@ uint32_t pieces_of(const tsa_attend_args& a) {
   return n < 1 ? 1 : n > kMaxPieces ? kMaxPieces : uint32_t(n);
 }
 
-template <class T, int kD, bool kAligned>
+template <class T, int kD, bool kAligned, bool kSplit>
 void gradients(const tsa_attend_grad_args& g, float2* rows, float* parts, hipStream_t stream) {
   const tsa_attend_args& a = g.f;
   const float c = a.scale * 1.44269504f;
   const dim3 queries(uint32_t(own_tiles_at_most(a.sequences, a.tokens) * a.q.heads)), block(64 * kTileWaves);
   if (a.tokens) hipLaunchKernelGGL((rows_kernel<T, kD, kAligned>), queries, block, 0, stream, g, rows, c);
-  if (a.tokens && g.dq.p) hipLaunchKernelGGL((queries_kernel<T, kD, kAligned>), queries, block, 0, stream, g, rows, c);
+  if (a.tokens && g.dq.p) hipLaunchKernelGGL((queries_kernel<T, kD, kAligned, kSplit>), queries, block, 0, stream, g, rows, c);
   if (a.k_tokens && g.dk.p) {
     const uint32_t pieces = pieces_of(a);
     const dim3 keys(uint32_t(own_tiles_at_most(a.sequences, a.k_tokens) * a.k.heads * pieces));
     if constexpr (kD == 64) {
-      hipLaunchKernelGGL((keys_kernel<T, kD, kAligned, true, true>), keys, block, 0, stream, g, rows, c, pieces, parts);
+      hipLaunchKernelGGL((keys_kernel<T, kD, kAligned, kSplit, true, true>), keys, block, 0, stream, g, rows, c, pieces, parts);
     } else {
-      hipLaunchKernelGGL((keys_kernel<T, kD, kAligned, true, false>), keys, block, 0, stream, g, rows, c, pieces, parts);
-      hipLaunchKernelGGL((keys_kernel<T, kD, kAligned, false, true>), keys, block, 0, stream, g, rows, c, pieces, parts);
+      hipLaunchKernelGGL((keys_kernel<T, kD, kAligned, kSplit, true, false>), keys, block, 0, stream, g, rows, c, pieces, parts);
+      hipLaunchKernelGGL((keys_kernel<T, kD, kAligned, kSplit, false, true>), keys, block, 0, stream, g, rows, c, pieces, parts);
     }
     if (pieces > 1) {
       const uint64_t n = uint64_t(a.k_tokens) * a.k.heads * (2 * kD / 4);
@@ -442,10 +442,11 @@ int launch_attend_backward(const tsa_attend_grad_args& g, void* workspace, hipSt
   bool aligned = true;
   if (a.tokens) aligned = tile_heads(a.q) && vector_heads(a.out) && tile_heads(g.dout) && (!g.dq.p || vector_heads(g.dq));
   if (a.k_tokens) aligned = aligned && tile_heads(a.k) && tile_heads(a.v) && (!g.dk.p || (vector_heads(g.dk) && vector_heads(g.dv)));
-#define CALL(T, D)                                                     \
-  do {                                                                 \
-    if (aligned) gradients<T, D, true>(g, rows, parts, stream);               \
-    else gradients<T, D, false>(g, rows, parts, stream);                      \
+#define CALL(T, D)                                                             \
+  do {                                                                         \
+    if (!aligned) gradients<T, D, false, true>(g, rows, parts, stream);        \
+    else if (split_rows(a)) gradients<T, D, true, true>(g, rows, parts, stream); \
+    else gradients<T, D, true, false>(g, rows, parts, stream);                 \
   } while (0)
   if (a.type == TSA_BF16) {
     if (a.head_dim <= 64) CALL(Bf16, 64);

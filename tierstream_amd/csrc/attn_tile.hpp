@@ -45,6 +45,29 @@ __device__ __forceinline__ bits8 pack8(const f32x16& v, int u) {
                                          pack2<T>(v[8 * u + 6], v[8 * u + 7])});
 }
 
+// Rows 16 u.. of a result as the second operand of the next product: rounded to 16 bits, and (kSplit) what that leaves of them.
+template <class T, bool kSplit>
+struct Second {
+  bits8 part[kSplit ? 2 : 1];
+  __device__ __forceinline__ Second(const f32x16& v, int u) {
+    part[0] = pack8<T>(v, u);
+    if constexpr (kSplit) {
+      f32x16 rest;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) rest[i] = v[8 * u + i] - T::up(part[0][i]);
+      part[1] = pack8<T>(rest, 0);
+    }
+  }
+  __device__ __forceinline__ void add(bits8 a, f32x16& sum) const {
+    sum = mfma32<T>(a, part[0], sum);
+    if constexpr (kSplit) sum = mfma32<T>(a, part[1], sum);
+  }
+};
+// Up to so many rows (of all heads) the products of probabilities and of the scores' gradients take both parts: their error is then a few
+// elements' and may exceed the results' own rounding by far, and the calls are all latency (301 rows of 4 heads: 8.9 us for 8.4, the gradients 33 either way).
+constexpr uint64_t kSplitRows = 2048;
+inline bool split_rows(const tsa_attend_args& a) { return uint64_t(a.tokens) * a.q.heads <= kSplitRows; }
+
 template <int kD>
 struct TileShapes {
   static constexpr uint32_t kRowBytes = 2 * kD, kPieces = kD / 8, kBytes = kTile * kRowBytes, kRowsALoad = 64 / kPieces,
