@@ -7,6 +7,7 @@ about sqrt(n) 2^-24 of the terms, 2e-6 at the longest used here. A rounding to b
 the mean square, one to half precision by 1.5e-4. An output behind one rounded operand (probabilities, or the scores'
 gradients) carries sqrt(2) of that, a gradient that also takes in the rounded output sqrt(3). The bounds are about twice those: 4e-3
 (bf16), 5e-4 (f16), 1e-5 (f32, and a log sum of exponentials made of hardware's exponentials and logarithms)."""
+import gc
 import math
 
 import pytest
@@ -22,7 +23,9 @@ PAGE = 64
 @pytest.fixture(scope="module")
 def attn(gpu):
     from tierstream_amd import attn
-    return attn
+    yield attn
+    gc.collect()              # graphs and tensors go now, not in the middle of another module's token,
+    torch.cuda.synchronize()  # and the null stream is idle: streams of a device-gated context wait for what it still has
 
 
 def gen(seed):

@@ -1,5 +1,6 @@
 """The routed layers of tierstream_amd.moe with attention before them: the gradient step against autograd of the same formulas in 64
 bits, and decode through the 4-bit cache, a token a captured graph, against those formulas over what the cache holds."""
+import gc
 import math
 
 import pytest
@@ -12,7 +13,9 @@ pytestmark = pytest.mark.gpu
 @pytest.fixture(scope="module")
 def moe(gpu):
     from tierstream_amd import moe
-    return moe
+    yield moe
+    gc.collect()              # graphs and tensors go now, not in the middle of another module's token,
+    torch.cuda.synchronize()  # and the null stream is idle: streams of a device-gated context wait for what it still has
 
 
 def turned(x, positions, turns):
