@@ -136,8 +136,8 @@ SS_API ss_status tsa_cache_load(const tsa_cache* c, const tsa_cache_rows_args* a
  * the rows first[i]..first[i + 1]; they are the last ones of its length ends[i] (stored before the call), and each attends to
  * the tokens up to itself. Query head h reads kept head h / (heads / kv_heads). A row without keys is 0; rows behind the last request
  * are left as they were. A token on a page out of range counts as absent. For one or a few tokens a request; it
- * holds for any number. Probabilities are rounded once, with the value's scale, in bf16 to 8 bits and in half precision to 16;
- * all sums are in 32 bits. */
+ * holds for any number. Probabilities times their values' scales are rounded to half precision, in ranges of their own (a scale below 2^-15
+ * of the largest of its block of the request keeps fewer bits); all sums are in 32 bits. */
 typedef struct tsa_attend_cached_args {
   tsa_heads q, out;        /* heads a multiple of kv_heads */
   const int32_t* table;    /* [requests][width] */

@@ -489,6 +489,53 @@ def test_attend_cached_scales_of_values(attn, value):
     near(out, want, slack=2.0 ** -25 * math.sqrt(out.numel()))
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_attend_cached_scales_of_values_far_apart(attn, kind):
+    """Largest scales that grow from page to page, small ones beside them, and blocks of very different ones; scores that pick few tokens."""
+    g = gen(16)
+    for sigma in (0.2, 6.0):
+        pages = random_pages(g, 40, 2, 64, (sigma, 0.1))
+        scales = pages[..., 36 * 64:40 * 64].view(torch.float16).view(40, 2, PAGE, 2)
+        by = torch.exp2(-torch.randint(0, 13, scales.shape, device="cuda", generator=g).float())
+        by *= torch.exp2(torch.arange(40, device="cuda")[:, None, None, None] / 5)
+        by[..., 1] *= 2.0 ** -8
+        scales *= by.half()
+        table = torch.arange(40, device="cuda", dtype=torch.int32)[None]
+        q, out = rows(g, 2, 6, 64, kind), torch.empty((2, 6, 64), dtype=KINDS[kind], device="cuda")
+        cache = attn.Cache(pages, 2, 64)
+        attn.attend_cached(cache, q, out, table, i32([2500]), i32([0, 2]), workspace=room(attn.attend_cached_workspace(cache, q, table)), stream=stream())
+        want = cached64(q, pages, 64, table, [2500], [2], 0.125, 40)
+        for b in range(2):  # (each by itself: the second is 2^8 smaller)
+            near(out[..., 32 * b:32 * b + 32], want[..., 32 * b:32 * b + 32])
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, -0.0, 1e-38])
+def test_attend_cached_scale_of_any_sign(attn, scale):
+    g = gen(17)
+    pages = random_pages(g, 8, 2, 96)
+    table = i32([[3, 1, 0, 7, 2], [4, 5, 6, -1, -1]])
+    q, out = rows(g, 5, 4, 96, "f16"), torch.empty((5, 4, 96), dtype=torch.float16, device="cuda")
+    cache, ends, fresh = attn.Cache(pages, 2, 96), [290, 129], [2, 3]
+    attn.attend_cached(cache, q, out, table, i32(ends), first_of(fresh), scale=scale, workspace=room(attn.attend_cached_workspace(cache, q, table)), stream=stream())
+    near(out, cached64(q, pages, 96, table, ends, fresh, scale, 8))
+
+
+@pytest.mark.parametrize("requests", [257, 700, 1025])
+def test_attend_cached_of_many_requests(attn, requests):
+    """Most of a page or two, some without new tokens, one long and in pieces, wherever it stands."""
+    g = gen(requests)
+    pages = random_pages(g, 70, 1, 32)
+    ends = torch.randint(1, 100, (requests,), device="cuda", generator=g).tolist()
+    fresh = [int(i % 7 != 3) for i in range(requests)]
+    for long in (0, requests // 2 + 1, requests - 1):
+        ends[long], fresh[long] = 60 * PAGE + 5, 3
+    table = torch.randint(0, 70, (requests, 61), device="cuda", generator=g, dtype=torch.int32)
+    q = rows(g, sum(fresh), 8, 32, "f16")
+    out, cache = torch.empty_like(q), attn.Cache(pages, 1, 32)
+    attn.attend_cached(cache, q, out, table, i32(ends), first_of(fresh), workspace=room(attn.attend_cached_workspace(cache, q, table)), stream=stream())
+    near(out, cached64(q, pages, 32, table, ends, fresh, 32 ** -0.5, 70))
+
+
 # ---- attention over packed sequences -----------------------------------------------------------------------------------------
 def attend64(q, k, v, counts, k_counts, causal, scale, dout=None):
     group = q.shape[1] // k.shape[1]
