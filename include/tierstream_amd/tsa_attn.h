@@ -19,7 +19,13 @@
  * range and a length below 0 count as none, lengths and sequences end at the arrays they index.
  *
  * Alignment: every array at its element's size, pages and workspaces at 16 bytes. Heads that start 16-byte aligned (base and strides)
- * with a head_dim that is a multiple of 8 are the fastest. Infinities and NaN stay in the rows that attend to them.
+ * with a head_dim that is a multiple of 8 are the fastest. Infinities and NaN stay in the rows that attend to them (a row near whose
+ * last key there is one is NaN as a whole). Arrays and stream belong to the current device. A workspace belongs to one stream, or to
+ * graphs that do not run at once; nothing in it is kept from call to call.
+ *
+ * Sizes: tokens and sequences below 2^24, pages and a table's width below 2^25, heads up to 1024; tsa_cache_store and _load: tokens x
+ * kv_heads x head_dim below 2^33; tsa_attend_cached: tokens x heads below 2^26, and (requests with tokens + tokens x heads / kv_heads /
+ * 16) x width below 2^31; tsa_attend and its gradients: tokens x heads below 2^30, sequences x heads below 2^23.
  */
 #ifndef TIERSTREAM_AMD_TSA_ATTN_H
 #define TIERSTREAM_AMD_TSA_ATTN_H
@@ -158,8 +164,9 @@ SS_API ss_status tsa_attend_cached(const tsa_cache* c, const tsa_attend_cached_a
 
 /* out_t = sum_j p_tj v_j, p_t the softmax of scale q_t . k_j over the keys of t's sequence: with n queries and m keys, all of them,
  * or (causal) those up to j = i + m - n for the sequence's query i. A row without keys is 0 (its lse -infinity); rows behind the
- * last sequence are left as they were. Query head h reads key head h / (heads / kv_heads). Probabilities are rounded once to type (in half
- * precision times 2^15), all sums are in 32 bits. */
+ * last sequence are left as they were. Query head h reads key head h / (heads / kv_heads). Probabilities are rounded to type (in half
+ * precision times 2^15), and where tokens x heads is at most 2048, or rows do not start 16-byte aligned, what that leaves of them is
+ * multiplied too; all sums are in 32 bits. */
 typedef struct tsa_attend_args {
   tsa_heads q, k, v, out;
   const int32_t* first;    /* [sequences + 1]: a sequence's first query row; ascending from 0. NULL: one sequence of all rows */
@@ -176,7 +183,9 @@ SS_API ss_status tsa_attend(const tsa_attend_args* a, void* stream);
 
 /* The gradients for dout, from the forward call's inputs, out and lse. dq, or dk and dv together, may be absent (p NULL). Keys that
  * no query attends to get 0; rows behind the last sequence are left as they were. Probabilities and the scores' gradients are rounded
- * once to type (in half precision behind a power of two that the largest of a row so far chooses); all sums are in 32 bits. */
+ * as tsa_attend's probabilities are (the latter in half precision behind a power of two that the largest of a row so far chooses); all sums
+ * are in 32 bits. A row's sum_j p_j dout . v_j is added up where its tile of 128 queries attends to at most 512 keys, and taken as dout . out
+ * beyond. */
 typedef struct tsa_attend_grad_args {
   tsa_attend_args f;
   tsa_heads dout, dq, dk, dv;

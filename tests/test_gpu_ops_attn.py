@@ -865,3 +865,138 @@ def test_nothing_of_no_token(attn):
     dk, dv = torch.ones_like(q), torch.ones_like(q)
     attn.attend_backward(e, q, q, e, e, torch.empty((2, 0), device="cuda"), e, dk, dv, workspace=room(attn.attend_backward_workspace(e, q)), stream=stream())
     assert bool((dk == 0).all()) and bool((dv == 0).all())  # keys without a query
+
+
+# ---- what the documents allow beyond that ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("first", [[0, 2, 1, 9], [-4, 1, 3, 1 << 30], [3, 0, 0, 3], [5, 5, 5, 5]])
+def test_attend_cached_takes_requests_as_they_are(attn, first):
+    """first that is not ascending, or goes beyond the rows: nothing out of range is read or written."""
+    g = gen(31)
+    pages = random_pages(g, 12, 1, 64)
+    table = torch.arange(12, device="cuda", dtype=torch.int32).view(3, 4)
+    whole = torch.full((9, 4, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    q, out = rows(g, 3, 4, 64, "bf16"), whole[3:6]
+    cache = attn.Cache(pages, 1, 64)
+    size = attn.attend_cached_workspace(cache, q, table)
+    ws = torch.full((size + 1024,), 99, dtype=torch.uint8, device="cuda")
+    attn.attend_cached(cache, q, out, table, i32([250, 200, 256]), i32(first), workspace=ws[:size], stream=stream())
+    assert bool(torch.isfinite(out.float()).all()) and bool((whole[:3] == 7).all()) and bool((whole[6:] == 7).all()) and bool((ws[size:] == 99).all())
+
+
+def test_a_cache_beyond_4_gib(attn):
+    """Slots and pages whose bytes pass 32 bits."""
+    g, kept, dim, n = gen(32), 8, 128, 70000
+    pages = torch.empty((n, kept, 72 * dim), dtype=torch.uint8, device="cuda")
+    assert pages.numel() > 1 << 32
+    cache = attn.Cache(pages, kept, dim)
+    used = [n - 1, 3, n - 2, 58254]  # (2^32 bytes lie in the last one)
+    slots = torch.cat([torch.arange(p * PAGE, (p + 1) * PAGE) for p in used])[:230].to(torch.int32).cuda()
+    k, v = rows(g, 230, kept, dim, "bf16"), rows(g, 230, kept, dim, "bf16")
+    attn.store(cache, k, v, slots, stream=stream())
+    a, b = torch.empty_like(k), torch.empty_like(v)
+    attn.load(cache, slots, a, b, stream=stream())
+    assert torch.equal(a, kept64(k).to(torch.bfloat16)) and torch.equal(b, kept64(v).to(torch.bfloat16))
+    q, out, table = rows(g, 2, 16, dim, "bf16"), torch.empty((2, 16, dim), dtype=torch.bfloat16, device="cuda"), i32([used])
+    attn.attend_cached(cache, q, out, table, i32([230]), i32([0, 2]), workspace=room(attn.attend_cached_workspace(cache, q, table)), stream=stream())
+    few = pages[torch.tensor(used, device="cuda")]
+    near(out, cached64(q, few, dim, i32([[0, 1, 2, 3]]), [230], [2], dim ** -0.5, 4))
+
+
+def test_rows_far_apart(attn):
+    """Strides whose bytes pass 32 bits: tokens 2^30 + 4 values apart, in every operator that takes rows."""
+    g, apart, t, dim = gen(33), (1 << 30) + 4, 3, 64
+    flat = torch.empty(2 * apart + 4096, dtype=torch.bfloat16, device="cuda")
+    far = lambda at, heads: flat[at:].as_strided((t, heads, dim), (apart, dim, 1))  # noqa: E731
+    q, k, v, out = far(0, 4), far(256, 2), far(384, 2), far(512, 4)
+    dout, dq, dk, dv = far(768, 4), far(1024, 4), far(1280, 2), far(1408, 2)
+    for x in (q, k, v, dout):
+        x.copy_(torch.randn(x.shape, device="cuda", generator=g))
+    r, positions = attn.Rotary(64), i32([0, 5, 900])
+    turned = rotated64(q, positions, r, False)
+    attn.rotate(r, positions, q, stream=stream())
+    near(q, turned)
+    lse = torch.empty((4, t), device="cuda")
+    attn.attend(q, k, v, out, lse=lse, stream=stream())
+    attn.attend_backward(q, k, v, out, dout, lse, dq, dk, dv, workspace=room(attn.attend_backward_workspace(q, k)), stream=stream())
+    want = attend64(q, k, v, [t], [t], True, dim ** -0.5, dout)
+    small = BOUND[torch.bfloat16] / 4 * float(dout.double().norm()) * float(v.double().norm(dim=-1).max()) * dim ** -0.5 * 0.05  # (row 0 attends to one key)
+    near(out, want[0], "out")
+    for name, got, exact in (("dq", dq, want[2]), ("dk", dk, want[3]), ("dv", dv, want[4])):
+        near(got, exact, name, slack=0.0 if name == "dv" else small)
+    cache = attn.Cache(torch.zeros((1, 2, 72 * dim), dtype=torch.uint8, device="cuda"), 2, dim)
+    attn.store(cache, k, v, i32([4, 0, 63]), stream=stream())
+    attn.load(cache, i32([4, 0, 63]), dk, dv, stream=stream())
+    assert torch.equal(dk, kept64(k).to(torch.bfloat16)) and torch.equal(dv, kept64(v).to(torch.bfloat16))
+    attn.attend_cached(cache, q[:1], out[:1], i32([[0]]), i32([1]), i32([0, 1]), workspace=room(attn.attend_cached_workspace(cache, q[:1], i32([[0]]))), stream=stream())
+    near(out[:1], kept64(v)[1:2].repeat_interleave(2, 1))
+
+
+@pytest.mark.parametrize("n", [257, 600])
+def test_attend_many_short_sequences(attn, n):
+    g, dim = gen(n), 64
+    counts = torch.randint(0, 4, (n,), device="cuda", generator=g).tolist()
+    counts[n // 2] = 140
+    q, k, v, dout, _, first, _ = attend_case("f16", counts, None, 1, 2, dim, "packed", pad=0)
+    out, lse = torch.empty_like(q), torch.empty((2, len(q)), device="cuda")
+    attn.attend(q, k, v, out, lse=lse, first=first, stream=stream())
+    want = attend64(q, k, v, counts, counts, True, dim ** -0.5, dout)
+    near(out, want[0])
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    attn.attend_backward(q, k, v, out, dout, lse, dq, dk, dv, first=first, workspace=room(attn.attend_backward_workspace(q, k)), stream=stream())
+    for name, got, exact in (("dq", dq, want[2]), ("dk", dk, want[3]), ("dv", dv, want[4])):
+        near(got, exact, name)
+
+
+def test_a_slot_that_is_given_twice_holds_a_mixture_alone(attn):
+    """Of values that were given to it, and nothing beside it changes."""
+    g = gen(34)
+    pages = torch.zeros((2, 2, 72 * 32), dtype=torch.uint8, device="cuda")
+    cache, k = attn.Cache(pages, 2, 32), rows(g, 130, 2, 32, "f16")
+    slots = torch.full((130,), 70, dtype=torch.int32, device="cuda")
+    slots[5] = 3
+    attn.store(cache, k, k, slots, stream=stream())
+    every = torch.arange(128, device="cuda", dtype=torch.int32)
+    a, b = torch.empty((128, 2, 32), dtype=torch.float16, device="cuda"), torch.empty((128, 2, 32), dtype=torch.float16, device="cuda")
+    attn.load(cache, every, a, b, stream=stream())
+    other = torch.ones(128, dtype=torch.bool, device="cuda")
+    other[3] = other[70] = False
+    assert bool((a[other] == 0).all()) and bool((b[other] == 0).all())
+    assert torch.equal(a[3], kept64(k[5:6]).half()[0]) and bool((a[70].abs() <= k.abs().max()).all())
+
+
+def test_replays_of_one_operator_each(attn):
+    """Captured alone and replayed, with other inputs each time."""
+    g = gen(35)
+    r, cache = attn.Rotary(64), attn.Cache(random_pages(g, 6, 2, 64), 2, 64)
+    positions, k = torch.zeros(70, dtype=torch.int32, device="cuda"), rows(g, 70, 2, 64, "bf16")
+    turned, back, back_v = torch.empty_like(k), torch.empty_like(k), torch.empty_like(k)
+    at = torch.zeros(70, dtype=torch.int32, device="cuda")
+    table, ends, first = i32([[5, 0, 3], [1, 2, 4]]), i32([0, 0]), i32([0, 40, 70])
+    q, out = rows(g, 2, 4, 64, "bf16"), torch.empty((2, 4, 64), dtype=torch.bfloat16, device="cuda")
+    ws = room(attn.attend_cached_workspace(cache, q, table))
+    where = torch.empty(70, dtype=torch.int32, device="cuda")
+
+    def change(i):
+        positions.copy_(torch.randint(0, 5000, (70,), device="cuda", generator=g))
+        ends.copy_(i32([100 + 13 * i, 64 + 31 * i]))
+        k.copy_(torch.randn(k.shape, device="cuda", generator=g))
+
+    def calls():
+        attn.rotate(r, positions, k, q_out=turned, stream=stream())
+        attn.slots(table, ends, first, where, at, stream=stream())
+        attn.store(cache, turned, k, at, stream=stream())
+        attn.load(cache, at, back, back_v, stream=stream())
+        attn.attend_cached(cache, q, out, table, ends, i32_one, workspace=ws, stream=stream())
+
+    i32_one = i32([0, 1, 2])
+    change(0)
+    state = {"i": 0}
+
+    def check(_):
+        near(turned, rotated64(k, positions, r, False))
+        assert torch.equal(back, kept64(turned).to(torch.bfloat16)) and torch.equal(back_v, kept64(k).to(torch.bfloat16))
+        near(out, cached64(q, cache.pages, 64, table, ends.tolist(), [1, 1], 0.125, 6))
+        state["i"] += 1
+        change(state["i"])
+
+    replays(calls, check)

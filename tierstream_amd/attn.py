@@ -1,5 +1,5 @@
 """The attention operators of include/tierstream_amd/tsa_attn.h, on array objects as tierstream_amd.ops takes them (data_ptr(), shape,
-stride() and dtype as torch's tensors have), all in device memory and on the same device. Queries, keys and values are [tokens][heads][head_dim] with contiguous
+stride(), dtype and device as torch's tensors have), all in the memory of the current device, to which the stream belongs too. Queries, keys and values are [tokens][heads][head_dim] with contiguous
 values and any strides of tokens and heads, so that slices of one product's output go as they are. Streams are hipStream_t
 handles; outputs and workspaces are the caller's. Errors are raised as SsError, arrays that do not fit together as ValueError.
 
