@@ -118,6 +118,23 @@ def test_decode_attends_to_what_its_cache_holds(moe, tmp_path):
         d.close()
 
 
+def test_work_left_on_the_null_stream(moe, tmp_path):
+    """A token begins behind what its caller left there, however long that takes."""
+    s = moe.Shape(layers=2, experts=8, top_k=2, d_model=128, d_ff=128, vocab=64, heads=4, kv_heads=2, head_dim=32)
+    d = moe.Decoder(moe.Model(s, seed=6), moe.Model(s, seed=6).write(tmp_path / "experts.bin"), context=64)
+    try:
+        want = [d.token(3 * t % s.vocab) for t in range(8)]
+        d.forget()
+        x = torch.randn((2048, 2048), device="cuda")
+        for t in range(8):
+            for _ in range(20):
+                x = torch.tanh(x @ x)
+            assert d.token(3 * t % s.vocab) == want[t]
+        assert bool(torch.isfinite(x).all()) and d.ctx.verify_failures() == 0
+    finally:
+        d.close()
+
+
 def test_command_runs_with_attention(moe, capsys):
     moe.main(["--layers", "2", "--experts", "8", "--d-model", "128", "--d-ff", "128", "--vocab", "64", "--steps", "3", "--tokens", "16", "--heads", "4"])
     assert "failed checks 0" in capsys.readouterr().out.splitlines()[-1]

@@ -193,7 +193,9 @@ __global__ __launch_bounds__(256) void slots_kernel(tsa_cache_plan_args a) {
 }
 
 // ---- keys and values to their slots and back ----
-// Four lanes a block of 32 values, 8 each. kVector: rows whose pieces of 8 values start 16-byte aligned.
+// Four lanes a block of 32 values, 8 each: whole blocks are read in whole lines, and the largest of a block is two moves inside four lanes.
+// 8191 tokens of 8 heads of 128: a store 18.2 us (2.3 TB/s read and written), a load 14.9 (2.8); what bounds them are the instructions of the
+// rounding and the short rows of a page, 64 bytes of keys and 16 of values at a time. 32 tokens: 3.7 and 2.9, a launch. kVector: rows whose pieces of 8 values start 16-byte aligned.
 __device__ __forceinline__ bits8 load8(const tsa_heads& h, uint64_t at, bool vector) {
   const u16* p = static_cast<const u16*>(h.p) + at;
   if (vector) return *reinterpret_cast<const bits8*>(p);

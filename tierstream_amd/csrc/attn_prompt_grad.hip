@@ -2,9 +2,12 @@
 //   dq = scale ds K    a workgroup has 128 queries of a head and runs over the keys,
 //   dk = scale ds^T Q, dv = p^T dout    a workgroup has 128 keys of a kept head and runs over the queries of its group's heads,
 // each in tiles of 64 through LDS as in the forward pass: the wave's own rows are the columns of every product, and p and ds, as they
-// come out of the first products, the operand of the second. Scores are computed twice, and nothing is added up across
-// workgroups: the same bits every time, without atomics or partial sums in memory. lse and sum p dp go to the
-// workspace first, a pair a row.
+// come out of the first products, the operand of the second. Scores are computed again in each pass. Sums over a workgroup's rows stay in
+// its registers; where there are few tiles of keys their queries are cut into pieces, whose sums go to memory in 32 bits and are added
+// up in order by a last launch: no atomics, the same bits every time. lse and sum p dp go to the workspace first, a pair a row.
+// Measured: 8192 tokens in three sequences, 32 heads on 8 of 128, causal, after a forward pass of 250 us: the pairs 45, dq 324, dk 364, dv
+// 269, the joining launch 45. The matrix units are busy 44 to 52 % of the cycles; what they wait for is what stands between the first
+// products and the second, as in the forward pass. 301 tokens of 4 heads of 64: 7.5, 10.8, 10.0 (dk and dv at once) and 4.7, latency.
 #include "attn_tile.hpp"
 
 namespace tsa {

@@ -1,7 +1,10 @@
 // Rotary positions: pairs (a, b) of a head's values become (a cos - b sin, a sin + b cos) of position x frequency. Read once and
 // written once; what bounds it is memory. The angle of a pair is the same for every head of a token, so a workgroup takes whole
 // tokens: a thread each makes the sine and cosine of one pair (in 64 bits down to an eighth of a turn, where short power series
-// give 32), they go to LDS, and every head reads them from there. No table of all positions is read.
+// give 32), they go to LDS, and every head reads them from there. No table of all positions is read. Pieces of 8 values a lane, a piece of
+// each half where the halves are pairs.
+// Measured: 8191 tokens of 36 heads of 128, 64 of them turned, 33.7 us (302 MB with the gradient's in 67: 4.5 TB/s, a large copy reaches
+// 4.9); one token of 40 heads 2.9, a launch and two memory latencies.
 #include "op_device.hpp"
 // (behind the HIP runtime's own header)
 #include "attn_launch.hpp"

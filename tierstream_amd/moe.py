@@ -270,6 +270,9 @@ class Decoder:
 
     def token(self, token: int) -> int:
         """The likeliest token behind `token`."""
+        # What a caller left on the null stream ends first: the library's streams wait for it, and where it shares the graph's hardware queue
+        # their wait would stand behind the token's own waits, which wait for them.
+        torch.cuda.default_stream().synchronize()
         with torch.cuda.stream(self.stream):
             self.x[0].copy_(self.embedding[token:token + 1])
             self.ctx.begin()
