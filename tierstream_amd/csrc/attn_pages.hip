@@ -194,8 +194,9 @@ __global__ __launch_bounds__(256) void slots_kernel(tsa_cache_plan_args a) {
 
 // ---- keys and values to their slots and back ----
 // Four lanes a block of 32 values, 8 each: whole blocks are read in whole lines, and the largest of a block is two moves inside four lanes.
-// 8191 tokens of 8 heads of 128: a store 18.2 us (2.3 TB/s read and written), a load 14.9 (2.8); what bounds them are the instructions of the
-// rounding and the short rows of a page, 64 bytes of keys and 16 of values at a time. 32 tokens: 3.7 and 2.9, a launch. kVector: rows whose pieces of 8 values start 16-byte aligned.
+// 8191 tokens of 8 heads of 128: a store 14.8 us (2.9 TB/s read and written), a load 11.0 (3.9); what bounds the store are the instructions of
+// the rounding, some 20 a value. 32 tokens: 3.7 and 3.1, a launch. Keys and values of a block by one thread were 0.2 and 0.7 us faster on many
+// tokens and 0.7 and 0.2 slower on few. kVector: rows whose pieces of 8 values start 16-byte aligned.
 __device__ __forceinline__ bits8 load8(const tsa_heads& h, uint64_t at, bool vector) {
   const u16* p = static_cast<const u16*>(h.p) + at;
   if (vector) return *reinterpret_cast<const bits8*>(p);
@@ -215,35 +216,38 @@ struct BlockPlace {
     return reinterpret_cast<u16*>(page + nb * (value ? 1152 : 1024)) + row * nb + b;
   }
 };
-struct RowPiece {  // piece j of block b of head h of k (0) or v (1) of token t
-  uint32_t t, which, h, b, j;
+struct RowPiece {  // piece j of block b of head h of token t, of k and of v
+  uint32_t t, h, b, j;
   bool on;
 };
+// A workgroup takes a head of as many tokens as there are threads for: tokens behind each other lie behind each other in a page, and
+// its lines are written whole by one XCD (two tokens of all heads a workgroup: 17.8 us and 14.2).
 __device__ __forceinline__ RowPiece row_piece(const tsa_cache& c, uint32_t tokens) {
-  const uint32_t i = blockIdx.x * 256 + threadIdx.x, nb = c.head_dim / 32, row = 2 * c.kv_heads * nb;  // (pieces are below 2^31)
+  const uint32_t nb = c.head_dim / 32, many = 64 / nb, block = threadIdx.x >> 2;
   RowPiece p;
-  p.j = i & 3u;
-  p.t = (i >> 2) / row;
-  uint32_t in = (i >> 2) - p.t * row;
-  p.b = nb == 4 ? in & 3u : in % nb;
-  in = nb == 4 ? in >> 2 : in / nb;
-  p.which = in >= c.kv_heads;
-  p.h = p.which ? in - c.kv_heads : in;
-  p.on = p.t < tokens;
+  p.j = threadIdx.x & 3u;
+  const uint32_t t = nb == 4 ? block / 4 : block / nb;
+  p.b = block - t * nb;
+  p.t = blockIdx.x * many + t;
+  p.h = blockIdx.y;
+  p.on = t < many && p.t < tokens;
   return p;
 }
 __device__ __forceinline__ BlockPlace place_of(const tsa_cache& c, uint32_t slot, const RowPiece& p) {
   return {static_cast<unsigned char*>(c.pages) + (uint64_t(slot / kPage) * c.kv_heads + p.h) * (72 * c.head_dim), slot % kPage, c.head_dim / 32, p.b};
 }
+__device__ __forceinline__ uint64_t place_in(const tsa_heads& h, const RowPiece& p) {
+  return uint64_t(p.t) * h.token_stride + uint64_t(p.h) * h.head_stride + p.b * 32 + p.j * 8;
+}
 
+// A block by its four lanes: the scale, and (in lanes 0 and 1) this lane's 8 bytes.
+struct Packed {
+  uint32_t lo, hi;
+  u16 scale;
+};
 template <class T>
-__global__ __launch_bounds__(256) void store_kernel(tsa_cache c, tsa_cache_rows_args a, bool vector) {
+__device__ __forceinline__ Packed pack_block(bits8 raw) {
   constexpr uint32_t kInfinity = std::is_same_v<T, Bf16> ? 0x7F80 : 0x7C00;
-  const RowPiece p = row_piece(c, a.tokens);
-  const uint32_t slot = p.on ? uint32_t(a.slots[p.t]) : ~0u;
-  if (slot >= c.n_pages * kPage) return;  // (a block's four lanes go together)
-  const tsa_heads& h = p.which ? a.v : a.k;
-  const bits8 raw = load8(h, uint64_t(p.t) * h.token_stride + uint64_t(p.h) * h.head_stride + p.b * 32 + p.j * 8, vector);
   // the largest size, by its bits; then the first value that has it
   const bits8 size = raw & u16(0x7FFF);
   uint32_t top = 0;
@@ -284,14 +288,28 @@ __global__ __launch_bounds__(256) void store_kernel(tsa_cache c, tsa_cache_rows_
   // values 16.. of the block go to the high halves of bytes 0..
   lo |= __shfl_xor(lo, 2, 64) << 4;
   hi |= __shfl_xor(hi, 2, 64) << 4;
+  return {lo, hi, scale};
+}
+
+// What a thread reads is on its way before its slot is known.
+template <class T>
+__global__ __launch_bounds__(256) void store_kernel(tsa_cache c, tsa_cache_rows_args a, bool vector) {
+  const RowPiece p = row_piece(c, a.tokens);
+  if (!p.on) return;
+  const bool value = blockIdx.z;
+  const uint32_t slot = uint32_t(a.slots[p.t]);
+  const tsa_heads& h = value ? a.v : a.k;
+  const bits8 raw = load8(h, place_in(h, p), vector);
+  if (slot >= c.n_pages * kPage) return;  // (a block's four lanes go together)
   const BlockPlace at = place_of(c, slot, p);
-  if (p.j == 3) *at.scale(p.which) = scale;
+  const Packed w = pack_block<T>(raw);
+  if (p.j == 3) *at.scale(value) = w.scale;
   if (p.j >= 2) return;
-  if (p.which) {
-    *reinterpret_cast<uint2*>(at.value_bytes() + 8 * p.j) = uint2{lo, hi};
+  if (value) {
+    *reinterpret_cast<uint2*>(at.value_bytes() + 8 * p.j) = uint2{w.lo, w.hi};
   } else {
-    *reinterpret_cast<uint32_t*>(at.key_word(2 * p.j)) = lo;
-    *reinterpret_cast<uint32_t*>(at.key_word(2 * p.j + 1)) = hi;
+    *reinterpret_cast<uint32_t*>(at.key_word(2 * p.j)) = w.lo;
+    *reinterpret_cast<uint32_t*>(at.key_word(2 * p.j + 1)) = w.hi;
   }
 }
 
@@ -300,20 +318,21 @@ __global__ __launch_bounds__(256) void load_kernel(tsa_cache c, tsa_cache_rows_a
   const RowPiece p = row_piece(c, a.tokens);
   const uint32_t slot = p.on ? uint32_t(a.slots[p.t]) : ~0u;
   if (slot >= c.n_pages * kPage) return;
+  const bool value = blockIdx.z;
   const BlockPlace at = place_of(c, slot, p);
   uint2 w;
   const uint32_t half = p.j & 1u;
-  if (p.which) w = *reinterpret_cast<const uint2*>(at.value_bytes() + 8 * half);
+  if (value) w = *reinterpret_cast<const uint2*>(at.value_bytes() + 8 * half);
   else w = uint2{*reinterpret_cast<const uint32_t*>(at.key_word(2 * half)), *reinterpret_cast<const uint32_t*>(at.key_word(2 * half + 1))};
-  const float step = F16::up(*at.scale(p.which));
+  const float step = F16::up(*at.scale(value));
   bits8 out;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const uint32_t n = ((i < 4 ? w.x : w.y) >> (8 * (i & 3) + (p.j >= 2 ? 4 : 0))) & 15u;
     out[i] = T::down(float(int(n) - 8) * step);
   }
-  const tsa_heads& h = p.which ? a.v : a.k;
-  u16* to = static_cast<u16*>(h.p) + uint64_t(p.t) * h.token_stride + uint64_t(p.h) * h.head_stride + p.b * 32 + p.j * 8;
+  const tsa_heads& h = value ? a.v : a.k;
+  u16* to = static_cast<u16*>(h.p) + place_in(h, p);
   if (vector) {
     *reinterpret_cast<bits8*>(to) = out;
   } else {
@@ -322,8 +341,9 @@ __global__ __launch_bounds__(256) void load_kernel(tsa_cache c, tsa_cache_rows_a
   }
 }
 
-uint32_t row_grid(const tsa_cache& c, uint32_t tokens) {
-  return uint32_t((uint64_t(tokens) * 2 * c.kv_heads * (c.head_dim / 32) * 4 + 255) / 256);
+dim3 row_grid(const tsa_cache& c, uint32_t tokens) {
+  const uint32_t many = 64 / (c.head_dim / 32);
+  return dim3((tokens + many - 1) / many, c.kv_heads, 2);
 }
 
 }  // namespace
@@ -361,7 +381,7 @@ int launch_cache_slots(const tsa_cache_plan_args& a, hipStream_t stream) {
 
 int launch_cache_store(const tsa_cache& c, const tsa_cache_rows_args& a, hipStream_t stream) {
   const bool vector = op::vector_heads(a.k) && op::vector_heads(a.v);
-  const dim3 grid(op::row_grid(c, a.tokens));
+  const dim3 grid = op::row_grid(c, a.tokens);
   if (a.type == TSA_BF16) hipLaunchKernelGGL(op::store_kernel<op::Bf16>, grid, dim3(256), 0, stream, c, a, vector);
   else hipLaunchKernelGGL(op::store_kernel<op::F16>, grid, dim3(256), 0, stream, c, a, vector);
   return int(hipGetLastError());
@@ -369,7 +389,7 @@ int launch_cache_store(const tsa_cache& c, const tsa_cache_rows_args& a, hipStre
 
 int launch_cache_load(const tsa_cache& c, const tsa_cache_rows_args& a, hipStream_t stream) {
   const bool vector = op::vector_heads(a.k) && op::vector_heads(a.v);
-  const dim3 grid(op::row_grid(c, a.tokens));
+  const dim3 grid = op::row_grid(c, a.tokens);
   if (a.type == TSA_BF16) hipLaunchKernelGGL(op::load_kernel<op::Bf16>, grid, dim3(256), 0, stream, c, a, vector);
   else hipLaunchKernelGGL(op::load_kernel<op::F16>, grid, dim3(256), 0, stream, c, a, vector);
   return int(hipGetLastError());
