@@ -3,7 +3,7 @@
 // softmax runs in the lane's own registers, and its probabilities are the second product's operand as they stand. Four waves of 32
 // queries share each tile, and two workgroups a CU fill each other's waits; the longest rows begin first.
 // Measured: 8191 tokens of 32 heads on 8 of 128, causal, 535 us: 1030 TFLOP/s (a library's large product reaches 1400); the matrix units
-// are busy 57 % of the cycles, and wait for the exponentials between the two products. 301 tokens of 4 heads: 8.8 us, latency.
+// are busy 57 % of the cycles, at 1.6 GHz. The next tile's scores made in the shadow of this one's exponentials took 4 % longer. 301 tokens of 4 heads: 8.8 us, latency.
 #include "attn_tile.hpp"
 
 namespace tsa {
