@@ -5,9 +5,9 @@
 // come out of the first products, the operand of the second. Scores are computed again in each pass. Sums over a workgroup's rows stay in
 // its registers; where there are few tiles of keys their queries are cut into pieces, whose sums go to memory in 32 bits and are added
 // up in order by a last launch: no atomics, the same bits every time. lse and sum p dp go to the workspace first, a pair a row.
-// Measured: 8192 tokens in three sequences, 32 heads on 8 of 128, causal, after a forward pass of 250 us: the pairs 45, dq 324, dk 364, dv
-// 269, the joining launch 45. The matrix units are busy 44 to 52 % of the cycles; what they wait for is what stands between the first
-// products and the second, as in the forward pass. 301 tokens of 4 heads of 64: 7.5, 10.8, 10.0 (dk and dv at once) and 4.7, latency.
+// Measured: 8192 tokens in three sequences, 32 heads on 8 of 128, causal, after a forward pass of 250 us: the pairs 45, the gradients 907
+// (ten products for the formula's seven, forward pass included: 840 TFLOP/s; alone dq takes 324, dk 364, dv 269), the joining launch 37. The matrix units
+// are busy 44 to 52 % of the cycles, at 1.8 GHz. 301 tokens of 4 heads of 64: 7.7, 11.0 and 4.6, latency.
 #include "attn_tile.hpp"
 
 namespace tsa {
@@ -24,10 +24,10 @@ struct Queries {
 };
 // By the whole workgroup; false: there are no more.
 template <bool kFromEnd>
-__device__ __forceinline__ bool find_queries(const tsa_attend_args& a, OwnTileMemory& m, Queries& o) {
+__device__ __forceinline__ bool find_queries(const tsa_attend_args& a, uint32_t group, OwnTileMemory& m, Queries& o) {
   OwnTile own;
-  o.head = head_of_group(blockIdx.x % a.q.heads, a.q.heads), o.kept = o.head / (a.q.heads / a.k.heads);
-  if (!find_own_tile<kFromEnd>(a.first, a.sequences, a.tokens, blockIdx.x / a.q.heads, m, own)) return false;
+  o.head = head_of_group(group % a.q.heads, a.q.heads), o.kept = o.head / (a.q.heads / a.k.heads);
+  if (!find_own_tile<kFromEnd>(a.first, a.sequences, a.tokens, group / a.q.heads, m, own)) return false;
   o.qs = span_of(a.first, own.sequence, a.tokens), o.ks = span_of(a.k_first ? a.k_first : a.first, own.sequence, a.k_tokens);
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row0 = own.row0 + wave * kOwn;
   o.row = row0 + (threadIdx.x & 31u), o.on = o.row < o.qs.count;
@@ -55,7 +55,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void rows_kernel(tsa_attend_gra
   __shared__ OwnTileMemory own_s;
   const tsa_attend_args& a = g.f;
   Queries o;
-  if (!find_queries<false>(a, own_s, o)) return;  // (those with few keys first: they take longer)
+  if (!find_queries<false>(a, blockIdx.x, own_s, o)) return;  // (those with few keys first: they take longer)
   const uint32_t lane = threadIdx.x & 63u, h = lane >> 5;
   if (o.end > kExactKeys) {
     const uint32_t row0 = o.row - (lane & 31u) - (threadIdx.x >> 6) * kOwn, value = (lane & 15u) * 8;
@@ -150,21 +150,26 @@ struct Raised<F16> {
   __device__ __forceinline__ float down() const { return by == 0.0f ? 0.0f : 1.0f / by; }
 };
 
+template <int kD>
+struct GradMemory {
+  __attribute__((aligned(16))) unsigned char tile[2][2][TileShapes<kD>::kBytes];  // what a workgroup runs over, two tiles of each of two arrays
+  __attribute__((aligned(16))) float2 row[2][kTile];
+  __attribute__((aligned(16))) float mark[kTile];
+  OwnTileMemory own;
+};
+
 template <class T, int kD, bool kAligned, bool kSplit>
-__global__ __launch_bounds__(64 * kTileWaves, 2) void queries_kernel(tsa_attend_grad_args g, const float2* rows, float c) {
+__device__ __forceinline__ void queries_part(const tsa_attend_grad_args& g, const float2* rows, float c, uint32_t group, GradMemory<kD>& m) {
   typedef TileShapes<kD> S;
-  __shared__ __attribute__((aligned(16))) unsigned char tile_s[2][2][S::kBytes];  // keys and values, two of each
-  __shared__ __attribute__((aligned(16))) float mark_s[kTile];
-  __shared__ OwnTileMemory own_s;
   const tsa_attend_args& a = g.f;
   Queries o;
-  if (!find_queries<true>(a, own_s, o)) return;
+  if (!find_queries<true>(a, group, m.own, o)) return;
   const uint32_t h = (threadIdx.x & 63u) >> 5;
   const OwnRows<kD, kAligned> q(a.q, uint64_t(o.qs.begin) + o.row, o.head, a.head_dim, o.on), dout(g.dout, uint64_t(o.qs.begin) + o.row, o.head, a.head_dim, o.on);
   const float2 mine = o.on ? rows[uint64_t(o.head) * a.tokens + o.qs.begin + o.row] : float2{INFINITY, 0.0f};
   const TileReads<kD> reads;
   const TileLoads<kD, kAligned> keys(a.k, o.ks.begin, o.kept, a.head_dim), values(a.v, o.ks.begin, o.kept, a.head_dim);
-  const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_offset(tile_s));
+  const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_offset(m.tile));
   f32x16 dq[kD / 32];
   clear(dq);
   Raised<T> raised;
@@ -181,7 +186,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void queries_kernel(tsa_attend_
       values.fetch(key0 + kTile, o.ks.count, other + S::kBytes);
     }
     if (a.causal && key0 + kTile > o.all_rows) {
-      mark_rows(clean_tile<T, kD>(k_at), mark_s);
+      mark_rows(clean_tile<T, kD>(k_at), m.mark);
       clean_done();
     }
     if (key0 >= o.any) continue;
@@ -204,7 +209,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void queries_kernel(tsa_attend_
         if (a.causal) {
 #pragma unroll
           for (uint32_t i = 0; i < 4; ++i) {
-            const f32x4 mark = marks_of(mark_s, r, i);
+            const f32x4 mark = marks_of(m.mark, r, i);
 #pragma unroll
             for (uint32_t k = 0; k < 4; ++k) one[0][4 * i + k] += mark[k];
           }
@@ -246,19 +251,15 @@ __device__ __forceinline__ void put_part(float* p, const f32x16 (&v)[kD / 32], f
 // Both gradients of keys and values, or one. With 128 values both together need 430 registers, one wave a SIMD: they took 840 us in three
 // packed sequences of 8192 together, one after the other with the scores computed again 660.
 template <class T, int kD, bool kAligned, bool kSplit, bool kKeys, bool kValues>
-__global__ __launch_bounds__(64 * kTileWaves, 2) void keys_kernel(tsa_attend_grad_args g, const float2* rows, float c, uint32_t pieces, float* parts) {
+__device__ __forceinline__ void keys_part(const tsa_attend_grad_args& g, const float2* rows, float c, uint32_t pieces, float* parts, uint32_t index, GradMemory<kD>& m) {
   typedef TileShapes<kD> S;
   constexpr float kUp = probability_up<T>();
-  __shared__ __attribute__((aligned(16))) unsigned char tile_s[2][2][S::kBytes];  // queries and the outputs' gradients, two of each
-  __shared__ __attribute__((aligned(16))) float2 row_s[2][kTile];
-  __shared__ __attribute__((aligned(16))) float mark_s[kTile];
-  __shared__ OwnTileMemory own_s;
   const tsa_attend_args& a = g.f;
   const int32_t* k_first = a.k_first ? a.k_first : a.first;
   OwnTile own;
-  const uint32_t kept = head_of_group(blockIdx.x % a.k.heads, a.k.heads), group = a.q.heads / a.k.heads;
-  const uint32_t piece = blockIdx.x / a.k.heads % pieces;
-  if (!find_own_tile<false>(k_first, a.sequences, a.k_tokens, blockIdx.x / a.k.heads / pieces, own_s, own)) return;
+  const uint32_t kept = head_of_group(index % a.k.heads, a.k.heads), group = a.q.heads / a.k.heads;
+  const uint32_t piece = index / a.k.heads % pieces;
+  if (!find_own_tile<false>(k_first, a.sequences, a.k_tokens, index / a.k.heads / pieces, m.own, own)) return;
   const Span qs = span_of(a.first, own.sequence, a.tokens), ks = span_of(k_first, own.sequence, a.k_tokens);
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const uint32_t row0 = own.row0 + wave * kOwn, row = row0 + (lane & 31u);
@@ -275,7 +276,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void keys_kernel(tsa_attend_gra
 
   const OwnRows<kD, kAligned> k(a.k, uint64_t(ks.begin) + row, kept, a.head_dim, on), v(a.v, uint64_t(ks.begin) + row, kept, a.head_dim, on);
   const TileReads<kD> reads;
-  const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_offset(tile_s)), row_lds = __builtin_amdgcn_readfirstlane(lds_offset(row_s));
+  const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_offset(m.tile)), row_lds = __builtin_amdgcn_readfirstlane(lds_offset(m.row));
   f32x16 dk[kKeys ? kD / 32 : 1], dv[kValues ? kD / 32 : 1];
   clear(dk);
   clear(dv);
@@ -303,7 +304,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void keys_kernel(tsa_attend_gra
     row_at = at + kTile >= qs.count ? begin : at + kTile;
     if (a.causal && at < all_rows) {
       const bool first = clean_tile<T, kD>(q_at), second = clean_tile<T, kD>(d_at);
-      mark_rows(first || second, mark_s);
+      mark_rows(first || second, m.mark);
       clean_done();
     }
     if (at + kTile <= any) continue;
@@ -321,7 +322,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void keys_kernel(tsa_attend_gra
       if constexpr (kKeys) products_behind_reads<kD / 8, 4>();
 #pragma unroll
       for (uint32_t i = 0; i < 4; ++i) {
-        const f32x4* pair = reinterpret_cast<const f32x4*>(&row_s[buffer][32 * r + 8 * i + 4 * h]);
+        const f32x4* pair = reinterpret_cast<const f32x4*>(&m.row[buffer][32 * r + 8 * i + 4 * h]);
         const f32x4 x = pair[0], y = pair[1];
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
@@ -335,7 +336,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void keys_kernel(tsa_attend_gra
         if (a.causal && at < all_rows) {
 #pragma unroll
           for (uint32_t i = 0; i < 4; ++i) {
-            const f32x4 mark = marks_of(mark_s, r, i);
+            const f32x4 mark = marks_of(m.mark, r, i);
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j) one[0][4 * i + j] += mark[j], one[1][4 * i + j] += mark[j];
           }
@@ -374,6 +375,22 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void keys_kernel(tsa_attend_gra
   if constexpr (kValues) put_columns<T, kD, kAligned>(g.dv, uint64_t(ks.begin) + row, kept, a.head_dim, dv, back);
 }
 
+// All gradients in one launch, whose parts fill what others leave idle (one launch each took 50 us more of 1000, and 9 of 21 where all is
+// latency). The keys', with up to 64 values at once with the values', first: theirs are the longest workgroups.
+struct GradGrid {
+  uint32_t queries, keys;  // workgroups
+};
+template <class T, int kD, bool kAligned, bool kSplit>
+__global__ __launch_bounds__(64 * kTileWaves, 2) void gradients_kernel(tsa_attend_grad_args g, const float2* rows, float c, uint32_t pieces, float* parts, GradGrid n) {
+  __shared__ GradMemory<kD> m;
+  if (blockIdx.y + 1 == gridDim.y) {
+    if (blockIdx.x < n.queries) queries_part<T, kD, kAligned, kSplit>(g, rows, c, blockIdx.x, m);
+  } else if (blockIdx.x < n.keys) {
+    if (blockIdx.y == 0) keys_part<T, kD, kAligned, kSplit, true, kD == 64>(g, rows, c, pieces, parts, blockIdx.x, m);
+    else if constexpr (kD != 64) keys_part<T, kD, kAligned, kSplit, false, true>(g, rows, c, pieces, parts, blockIdx.x, m);
+  }
+}
+
 // The pieces' sums, rounded: four values a thread.
 template <class T, int kD, bool kAligned>
 __global__ __launch_bounds__(256) void join_kernel(tsa_attend_grad_args g, uint32_t pieces, const float* parts) {
@@ -395,31 +412,26 @@ __global__ __launch_bounds__(256) void join_kernel(tsa_attend_grad_args g, uint3
   put4<T, kAligned>(const_cast<u16*>(row_of<u16>(value ? g.dv : g.dk, row, uint32_t(head_row % a.k.heads))) + d, sum[0], sum[1], sum[2], sum[3]);
 }
 
-// Pieces that a workgroup's queries are cut into: where there are few tiles of keys these would leave the chip idle, or wait for the
-// longest (the first keys of the longest sequence have all queries, the last ones a tile). Each piece's sums go to memory in 32 bits. In three
-// packed sequences of 8192 together, 520 tiles: 1080 us uncut, 704 in three pieces (with 44 to join them), 820 in seven.
-constexpr uint32_t kUnits = 2048, kMaxPieces = 8;
+// Pieces that a workgroup's queries are cut into, as many as make twice the workgroups that run at once: with fewer the chip would idle, or
+// wait for the longest (the first keys of the longest sequence have all queries, the last ones a tile). Each piece's sums go to memory in 32
+// bits. In three packed sequences of 8192 together, 520 tiles: uncut 957 us, in two pieces 907 and 37 to join them, in three 945 and 49.
+constexpr uint32_t kEnough = 1024, kMaxPieces = 8;
 uint32_t pieces_of(const tsa_attend_args& a) {
-  const uint64_t tiles = (uint64_t(a.k_tokens) / kTileOwn + 1) * a.k.heads, n = kUnits / tiles;
-  return n < 1 ? 1 : n > kMaxPieces ? kMaxPieces : uint32_t(n);
+  const uint64_t tiles = (uint64_t(a.k_tokens) / kTileOwn + 1) * a.k.heads, n = (kEnough + tiles - 1) / tiles;
+  return n > kMaxPieces ? kMaxPieces : uint32_t(n);
 }
 
 template <class T, int kD, bool kAligned, bool kSplit>
 void gradients(const tsa_attend_grad_args& g, float2* rows, float* parts, hipStream_t stream) {
   const tsa_attend_args& a = g.f;
   const float c = a.scale * 1.44269504f;
-  const dim3 queries(uint32_t(own_tiles_at_most(a.sequences, a.tokens) * a.q.heads)), block(64 * kTileWaves);
-  if (a.tokens) hipLaunchKernelGGL((rows_kernel<T, kD, kAligned>), queries, block, 0, stream, g, rows, c);
-  if (a.tokens && g.dq.p) hipLaunchKernelGGL((queries_kernel<T, kD, kAligned, kSplit>), queries, block, 0, stream, g, rows, c);
-  if (a.k_tokens && g.dk.p) {
-    const uint32_t pieces = pieces_of(a);
-    const dim3 keys(uint32_t(own_tiles_at_most(a.sequences, a.k_tokens) * a.k.heads * pieces));
-    if constexpr (kD == 64) {
-      hipLaunchKernelGGL((keys_kernel<T, kD, kAligned, kSplit, true, true>), keys, block, 0, stream, g, rows, c, pieces, parts);
-    } else {
-      hipLaunchKernelGGL((keys_kernel<T, kD, kAligned, kSplit, true, false>), keys, block, 0, stream, g, rows, c, pieces, parts);
-      hipLaunchKernelGGL((keys_kernel<T, kD, kAligned, kSplit, false, true>), keys, block, 0, stream, g, rows, c, pieces, parts);
-    }
+  const uint32_t queries = a.tokens ? uint32_t(own_tiles_at_most(a.sequences, a.tokens) * a.q.heads) : 0, pieces = pieces_of(a);
+  const bool keys = a.k_tokens && g.dk.p;
+  const GradGrid n = {g.dq.p ? queries : 0, keys ? uint32_t(own_tiles_at_most(a.sequences, a.k_tokens) * a.k.heads * pieces) : 0};
+  if (queries) hipLaunchKernelGGL((rows_kernel<T, kD, kAligned>), dim3(queries), dim3(64 * kTileWaves), 0, stream, g, rows, c);
+  const dim3 grid(n.queries > n.keys ? n.queries : n.keys, !keys ? 1 : kD == 64 ? 2 : 3);
+  hipLaunchKernelGGL((gradients_kernel<T, kD, kAligned, kSplit>), grid, dim3(64 * kTileWaves), 0, stream, g, rows, c, pieces, parts, n);
+  if (keys) {
     if (pieces > 1) {
       const uint64_t n = uint64_t(a.k_tokens) * a.k.heads * (2 * kD / 4);
       hipLaunchKernelGGL((join_kernel<T, kD, kAligned>), dim3(uint32_t((n + 255) / 256)), dim3(256), 0, stream, g, pieces, parts);
@@ -430,10 +442,10 @@ void gradients(const tsa_attend_grad_args& g, float2* rows, float* parts, hipStr
 }  // namespace
 }  // namespace op
 
-// The rows' pairs, then the pieces (their rows together are at most kMaxPieces times the keys, and at most what kUnits tiles hold: so
-// that more rows never need less).
+// The rows' pairs, then the pieces (their rows together are at most kMaxPieces times the keys, and what twice kEnough tiles hold: so that
+// more rows never need less).
 uint64_t attend_backward_workspace(const tsa_attend_args& f) {
-  const uint64_t many = uint64_t(op::kMaxPieces) * f.k_tokens * f.k.heads, most = uint64_t(op::kUnits) * op::kTileOwn;
+  const uint64_t many = uint64_t(op::kMaxPieces) * f.k_tokens * f.k.heads, most = uint64_t(2 * op::kEnough) * op::kTileOwn;
   return up_to(uint64_t(f.tokens) * f.q.heads * sizeof(float2), 16) + (many < most ? many : most) * 2 * (f.head_dim <= 64 ? 64 : 128) * sizeof(float);
 }
 

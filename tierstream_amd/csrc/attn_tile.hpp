@@ -111,18 +111,19 @@ struct TileLoads {
   __device__ __forceinline__ uint32_t value_of(uint32_t j) const {
     return 8 * (((threadIdx.x & 63u) % S::kPieces) ^ S::turn(row + j * S::kRowsALoad));
   }
-  // Rows row0.. of `rows` to the buffer at lds; rows behind the last are zeros.
-  __device__ __forceinline__ void fetch(uint32_t row0, uint32_t rows, uint32_t lds) const {
+  // Rows row0.. of `rows` to a buffer in LDS; rows behind the last are zeros.
+  __device__ __forceinline__ void fetch(uint32_t row0, uint32_t rows, uint32_t buffer) const {
+    const uint32_t lds = __builtin_amdgcn_readfirstlane(buffer + at);
     if constexpr (kAligned) {
       const u16* const base = p + row0 * stride;
       if (row0 + kTile <= rows && dim == kD) {
 #pragma unroll
-        for (uint32_t j = 0; j < S::kLoads; ++j) load_from_to_lds(base, offset[j], lds + at + j * 1024);
+        for (uint32_t j = 0; j < S::kLoads; ++j) load_from_to_lds(base, offset[j], lds + j * 1024);
       } else {
 #pragma unroll
         for (uint32_t j = 0; j < S::kLoads; ++j) {
           const bool in = row0 + row + j * S::kRowsALoad < rows && value_of(j) < dim;
-          load_to_lds(in ? static_cast<const void*>(base + offset[j] / 2) : &kZeroPiece, lds + at + j * 1024);
+          load_to_lds(in ? static_cast<const void*>(base + offset[j] / 2) : &kZeroPiece, lds + j * 1024);
         }
       }
     } else {
@@ -135,7 +136,7 @@ struct TileLoads {
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] = g[i];
         }
-        *reinterpret_cast<lds_eight_put_t*>(lds + at + j * 1024 + (threadIdx.x & 63u) * 16) = v;
+        *reinterpret_cast<lds_eight_put_t*>(lds + j * 1024 + (threadIdx.x & 63u) * 16) = v;
       }
     }
   }
@@ -326,7 +327,7 @@ __device__ __forceinline__ bool find_own_tile(const int32_t* first, uint32_t n, 
     }
   }
   __syncthreads();
-  out = m.found;
+  out = {uint32_t(__builtin_amdgcn_readfirstlane(m.found.sequence)), uint32_t(__builtin_amdgcn_readfirstlane(m.found.row0))};  // (the same in every lane)
   return true;
 }
 // Tiles of `rows` rows in n sequences, at most.
