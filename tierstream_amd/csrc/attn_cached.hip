@@ -312,8 +312,8 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(32 * NB)) void cached_kernel(ts
     }
     const uint32_t begin = max(from, at.at) - at.at, end = min(r.pages, upto - at.at);
     const int32_t* table = a.table + uint64_t(at.request) * a.table_stride;
-    // Half a page to LDS, keys or values. While the keys of one are multiplied its values are on their way, and while these are the next
-    // page's keys: one buffer is enough for that, and three or four workgroups fit a CU.
+    // Half a page to LDS, keys with all scales or values. While the keys of one are multiplied its values are on their way, and while these are
+    // the next page's keys: one buffer is enough for that (the values' scales, read to the end, have two), and three or four workgroups fit a CU.
     auto page_at = [&](uint32_t page) { return static_cast<const unsigned char*>(c.pages) + (uint64_t(page) * c.kv_heads + kept) * P::kBytes; };
     auto fetch_keys = [&](uint32_t page, uint32_t scales) {
       const unsigned char* at = page_at(page);
