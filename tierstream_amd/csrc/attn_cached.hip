@@ -29,7 +29,7 @@ namespace tsa {
 namespace op {
 namespace {
 
-constexpr uint32_t kWaves = 4, kRows = 16, kMinShare = kWaves;  // waves, query rows and the fewest pages of a workgroup
+constexpr uint32_t kWaves = 4, kRows = 16;  // waves and query rows of a workgroup
 // Workgroups of a CU that the registers leave room for, and of the chip.
 constexpr uint32_t per_cu(uint32_t head_dim) { return head_dim <= 64 ? 4 : 3; }
 constexpr uint32_t groups(uint32_t head_dim) { return 256 * per_cu(head_dim); }
@@ -52,12 +52,12 @@ struct CachedShape {
 };
 
 // ---- who does what --------------------------------------------------------------------------------------------------------
-// All requests' tiles of 16 query rows, one behind the other, each with its pages (one at least), are one row of pages. It is
-// cut into equal shares, a workgroup each, wherever the cuts fall. A tile inside one share is written at once; a share's piece of any
+// All requests' tiles of 16 query rows, one behind the other, each with the rounds that its pages make for four waves (one at least), are one row
+// of rounds. It is cut into equal shares, a workgroup each, wherever the cuts fall (cut by pages, a wave more had the last one alone). A tile inside one share is written at once; a share's piece of any
 // other is left in the workspace: at place 0 of the share where it begins with the share, at place 1 where it begins inside. For each
 // tile that begins in it a share also leaves where its pieces are.
 
-// Request i's new tokens, the tokens it ends with, its tiles and their pages.
+// Request i's new tokens, the tokens it ends with, its tiles and their pages, of which the waves take one each a round.
 struct Request {
   uint32_t first, fresh, tiles, pages;
   int32_t end;
@@ -69,12 +69,12 @@ struct Request {
     end = max(0, min(a.ends[i], int32_t(a.width * kPage)));  // (width is below 2^25)
     pages = (uint32_t(end) + kPage - 1) / kPage;
   }
-  __device__ __forceinline__ uint32_t places() const { return pages ? pages : 1; }
+  __device__ __forceinline__ uint32_t rounds() const { return pages ? (pages + kWaves - 1) / kWaves : 1; }
 };
 
 struct Place {
-  uint32_t share, all;  // pages of a share and of all
-  uint32_t at;          // first page of the tile
+  uint32_t share, all;  // rounds of a share and of all
+  uint32_t at;          // first round of the tile
   uint32_t request, tile;
   Request r;
 };
@@ -82,7 +82,7 @@ struct PlaceMemory {
   uint32_t pages[kWaves];
   Place found;
 };
-// Where a tile's pieces are: its pages of all, and the pages of a share. end 0: it is whole.
+// Where a tile's pieces are: its rounds of all, and the rounds of a share. end 0: it is whole.
 struct Pieces {
   uint32_t at, end, share;
 };
@@ -100,7 +100,7 @@ __device__ __forceinline__ V lanes_up_to(V v) {
   return v;
 }
 
-// The tile that holds the first page of share `want`. By the whole workgroup; false: there is none.
+// The tile that holds the first round of share `want`. By the whole workgroup; false: there is none.
 __device__ __forceinline__ bool find_place(const tsa_attend_cached_args& a, const CachedShape& s, uint32_t want, PlaceMemory& m, Place& out) {
   const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6, per = (a.requests + 64 * kWaves - 1) / (64 * kWaves);
   const uint32_t i0 = min(t * per, a.requests), i1 = min(i0 + per, a.requests);
@@ -108,7 +108,7 @@ __device__ __forceinline__ bool find_place(const tsa_attend_cached_args& a, cons
   Request r;  // (the last one stays: with up to 256 requests none is read twice)
   for (uint32_t i = i0; i < i1; ++i) {
     r = Request(a, i, s.group);
-    pages += r.tiles * r.places();
+    pages += r.tiles * r.rounds();
   }
   const uint32_t upto = lanes_up_to(pages);
   if (lane == 63) m.pages[wave] = upto;
@@ -121,17 +121,17 @@ __device__ __forceinline__ bool find_place(const tsa_attend_cached_args& a, cons
     if (w < wave) page0 += m.pages[w];
   }
   const uint32_t even = p.all / s.shares + (p.all % s.shares != 0);
-  p.share = even < kMinShare ? kMinShare : even;
+  p.share = even;
   const uint64_t page = uint64_t(want) * p.share;  // (past all of them, perhaps by far)
   if (page >= p.all) return false;
   if (page >= page0 && page < page0 + pages) {
     for (uint32_t i = i0; i < i1; ++i) {
       if (i1 - i0 > 1) r = Request(a, i, s.group);
-      const uint32_t have = r.tiles * r.places();
+      const uint32_t have = r.tiles * r.rounds();
       if (page < page0 + have) {
         p.request = i;
-        p.tile = uint32_t(page - page0) / r.places();
-        p.at = page0 + p.tile * r.places();
+        p.tile = uint32_t(page - page0) / r.rounds();
+        p.at = page0 + p.tile * r.rounds();
         p.r = r;
         m.found = p;
         break;
@@ -196,6 +196,20 @@ struct Page {
                             kValues = kValueScales + 2 * kScaleRoom, kRoom = kValues + 1024 * NB;
 };
 
+// kMany loads of 64 x 16 (64 x 4) bytes to LDS, behind each other there as in memory: the instruction's offset counts for both.
+template <uint32_t kMany>
+__device__ __forceinline__ void pieces_to_lds(const void* g, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(at) : "memory", "m0");
+  if constexpr (kMany > 1) asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off offset:1024" ::"v"(g), "s"(at) : "memory", "m0");
+  if constexpr (kMany > 2) asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off offset:2048" ::"v"(g), "s"(at) : "memory", "m0");
+  if constexpr (kMany > 3) asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off offset:3*1024" ::"v"(g), "s"(at) : "memory", "m0");
+}
+template <uint32_t kMany>
+__device__ __forceinline__ void words_to_lds(const void* g, uint32_t at) {
+  static_assert(kMany <= 2);
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(g), "s"(at) : "memory", "m0");
+  if constexpr (kMany > 1) asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off offset:256" ::"v"(g), "s"(at) : "memory", "m0");
+}
 __device__ __forceinline__ void reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void loads_left() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
@@ -280,7 +294,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(32 * NB)) void cached_kernel(ts
   Place at;
   const uint32_t kept = blockIdx.x % c.kv_heads, share = blockIdx.x / c.kv_heads;
   if (!find_place(a, s, share, place_s, at)) return;
-  const uint32_t from = share * at.share, upto = min(from + at.share, at.all);  // this share's pages
+  const uint32_t from = share * at.share, upto = min(from + at.share, at.all);  // this share's rounds
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
   const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_offset(page_s[wave]));
   typedef std::conditional_t<kHalf, NumbersHalf, Numbers16> KeyNumbers;
@@ -300,8 +314,10 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(32 * NB)) void cached_kernel(ts
     constexpr uint32_t kPieces = kRows * D / 8;
     static_assert(kPieces <= 64 * kWaves, "a piece a thread");
     bits8 piece = {0, 0, 0, 0, 0, 0, 0, 0};
-    const uint32_t piece_row = threadIdx.x / (D / 8), piece_at = threadIdx.x % (D / 8) * 8;
-    if (const uint32_t y = at.tile * kRows + piece_row; threadIdx.x < kPieces && y < r.fresh * s.group) {
+    uint32_t t = threadIdx.x;
+    asm volatile("" : "+v"(t));  // (what follows from it is made again for each tile: kept over the pages' loop, it took the last registers)
+    const uint32_t piece_row = t / (D / 8), piece_at = t % (D / 8) * 8;
+    if (const uint32_t y = at.tile * kRows + piece_row; t < kPieces && y < r.fresh * s.group) {
       const u16* p = row_of<u16>(a.q, r.first + y / s.group, kept * s.group + y % s.group) + piece_at;
       if (s.aligned) {
         piece = *reinterpret_cast<const bits8*>(p);
@@ -310,27 +326,27 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(32 * NB)) void cached_kernel(ts
         for (int k = 0; k < 8; ++k) piece[k] = p[k];
       }
     }
-    const uint32_t begin = max(from, at.at) - at.at, end = min(r.pages, upto - at.at);
+    const uint32_t begin = (max(from, at.at) - at.at) * kWaves, end = min(r.pages, (upto - at.at) * kWaves);
     const int32_t* table = a.table + uint64_t(at.request) * a.table_stride;
     // Half a page to LDS, keys with all scales or values. While the keys of one are multiplied its values are on their way, and while these are
     // the next page's keys: one buffer is enough for that (the values' scales, read to the end, have two), and three or four workgroups fit a CU.
     auto page_at = [&](uint32_t page) { return static_cast<const unsigned char*>(c.pages) + (uint64_t(page) * c.kv_heads + kept) * P::kBytes; };
     auto fetch_keys = [&](uint32_t page, uint32_t scales) {
-      const unsigned char* at = page_at(page);
+      const unsigned char *at = page_at(page), *words = at + P::kKeyScalesAt + lane * 4;
+      pieces_to_lds<NB>(at + lane * 16, lds);
+      if constexpr (NB % 2 == 0) {
+        words_to_lds<NB / 2>(words, lds + P::kKeyScales);
+        words_to_lds<NB / 2>(words + (P::kValueScalesAt - P::kKeyScalesAt), scales);
+      } else {
 #pragma unroll
-      for (uint32_t i = 0; i < uint32_t(NB); ++i) load_to_lds(at + i * 1024 + lane * 16, lds + i * 1024);
-#pragma unroll
-      for (uint32_t i = 0; i < P::kScaleLoads; ++i) {  // (what a last half load is too much stays in its room)
-        const uint32_t from = min(i * 256 + lane * 4, 128u * NB - 4);
-        load_words_to_lds(at + P::kKeyScalesAt + from, lds + P::kKeyScales + i * 256);
-        load_words_to_lds(at + P::kValueScalesAt + from, scales + i * 256);
+        for (uint32_t i = 0; i < P::kScaleLoads; ++i) {  // (what the last half load is too much stays in its room)
+          const uint32_t from = min(i * 256 + lane * 4, 128u * NB - 4);
+          load_words_to_lds(at + P::kKeyScalesAt + from, lds + P::kKeyScales + i * 256);
+          load_words_to_lds(at + P::kValueScalesAt + from, scales + i * 256);
+        }
       }
     };
-    auto fetch_values = [&](uint32_t page) {
-      const unsigned char* at = page_at(page) + P::kValuesAt;
-#pragma unroll
-      for (uint32_t i = 0; i < uint32_t(NB); ++i) load_to_lds(at + i * 1024 + lane * 16, lds + P::kValues + i * 1024);
-    };
+    auto fetch_values = [&](uint32_t page) { pieces_to_lds<NB>(page_at(page) + P::kValuesAt + lane * 16, lds + P::kValues); };
     // this wave's pages, 64 in the lanes at a time (a load in the loop would wait for the pages behind it), absent ones left out
     uint32_t ids = 0, p = begin + wave, turn = 0;
     auto page_here = [&]() {
@@ -346,7 +362,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(32 * NB)) void cached_kernel(ts
     };
     uint32_t page = page_here();
     uint32_t value_scales = lds + P::kValueScales, next_scales = value_scales + P::kScaleRoom;
-    if (threadIdx.x < kPieces) {
+    if (t < kPieces) {
       const u32x4 w = __builtin_bit_cast(u32x4, piece) ^ s.flip;
       *reinterpret_cast<uint2*>(&query_s[piece_row][piece_at]) = uint2{w[0], w[1]};
       *reinterpret_cast<uint2*>(&query_s[piece_row][piece_at + 4]) = uint2{w[2], w[3]};
@@ -531,33 +547,36 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(32 * NB)) void cached_kernel(ts
     }
 
     // the waves' parts together
+    t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    const uint32_t row = t & 15u, quarter = (t >> 4) & 3u;
     total = column_sum(total);
-    if (lane < kRows) stat_s[wave][lane] = {top, total};
+    if ((t & 63u) < kRows) stat_s[wave][row] = {top, total};
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __syncthreads();  // every wave is done with its pages
     float best = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (uint32_t w = 0; w < kWaves; ++w) best = fmaxf(best, stat_s[w][lane & 15u].x);
+    for (uint32_t w = 0; w < kWaves; ++w) best = fmaxf(best, stat_s[w][row].x);
     const float base = best == -INFINITY ? 0.0f : best;
 #pragma unroll
     for (uint32_t w = 0; w < kWaves; ++w) {
-      const float2 st = stat_s[w][lane & 15u];
+      const float2 st = stat_s[w][row];
       sum += st.y * __builtin_amdgcn_exp2f(st.x - base);
     }
-    const bool whole_tile = at.at >= from && at.at + r.places() <= upto;
+    const bool whole_tile = at.at >= from && at.at + r.rounds() <= upto;
     const float by = __builtin_amdgcn_exp2f(top - base) * (!whole_tile ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum);
-    float* mine = reinterpret_cast<float*>(page_s[wave]) + (lane & 15u) * kOutRow;
+    float* mine = reinterpret_cast<float*>(page_s[wave]) + row * kOutRow;
 #pragma unroll
     for (int i = 0; i < 2 * NB; ++i)
 #pragma unroll
       for (uint32_t k = 0; k < 4; ++k)  // column 4 g + k of the tile: byte (4 g + k) / 2 of the half block, low half bytes first
-        mine[32 * (i / 2) + 8 * (i % 2) + (4 * g + k) / 2 + 16 * (k & 1u)] = o[i][k] * (by * range.up(i / 2));
+        mine[32 * (i / 2) + 8 * (i % 2) + (4 * quarter + k) / 2 + 16 * (k & 1u)] = o[i][k] * (by * range.up(i / 2));
     __syncthreads();
     const uint32_t part = (2 * share + (at.at > from)) * c.kv_heads + kept;
-    if (threadIdx.x == 0 && at.at >= from)
-      pieces[uint64_t(tile_place(at.request, r.first, s.group) + at.tile) * c.kv_heads + kept] = {at.at, whole_tile ? 0 : at.at + r.places(), at.share};
-    if (!whole_tile && threadIdx.x < kRows) stats[part * kRows + threadIdx.x] = {best, sum};
-    for (uint32_t i = threadIdx.x; i < kRows * D / 4; i += 64 * kWaves) {
+    if (t == 0 && at.at >= from)
+      pieces[uint64_t(tile_place(at.request, r.first, s.group) + at.tile) * c.kv_heads + kept] = {at.at, whole_tile ? 0 : at.at + r.rounds(), at.share};
+    if (!whole_tile && t < kRows) stats[part * kRows + t] = {best, sum};
+    for (uint32_t i = t; i < kRows * D / 4; i += 64 * kWaves) {
       const uint32_t y = at.tile * kRows + i / (D / 4), d = i % (D / 4) * 4;
       if (y >= r.fresh * s.group) break;
       f32x4 v = {0, 0, 0, 0};
@@ -576,7 +595,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(32 * NB)) void cached_kernel(ts
         for (int k = 0; k < 4; ++k) out[k] = w[k];
       }
     }
-    at.at += r.places();
+    at.at += r.rounds();
     if (at.at >= upto) break;
     ++at.tile;
     while (at.tile >= r.tiles) {
@@ -677,11 +696,11 @@ uint64_t tiles_at_most(const tsa_attend_cached_args& a, uint32_t group) {
   return (a.requests < a.tokens ? a.requests : a.tokens) + uint64_t(a.tokens) * group / kRows;
 }
 uint64_t tile_places(const tsa_attend_cached_args& a, uint32_t group) { return a.requests + uint64_t(a.tokens) * group / kRows; }
-// Shares that the pages make: groups() together, fewer where there are not kMinShare pages for each.
+// Shares that the rounds make: groups() together, fewer where there are not as many rounds.
 CachedShape shape_of(const tsa_cache& c, const tsa_attend_cached_args& a) {
   CachedShape s;
   s.group = a.q.heads / c.kv_heads;
-  const uint64_t shares = (groups(c.head_dim) + c.kv_heads - 1) / c.kv_heads, most = (tiles_at_most(a, s.group) * a.width + kMinShare - 1) / kMinShare;
+  const uint64_t shares = (groups(c.head_dim) + c.kv_heads - 1) / c.kv_heads, most = tiles_at_most(a, s.group) * ((a.width + kWaves - 1) / kWaves);
   s.shares = uint32_t(shares < most ? shares : most);
   s.c = std::max(std::fabs(a.scale) * 1.44269504f, std::numeric_limits<float>::min());
   s.flip = std::signbit(a.scale) ? 0x80008000u : 0;
