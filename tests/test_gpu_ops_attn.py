@@ -520,7 +520,7 @@ def test_attend_cached_scale_of_any_sign(attn, scale):
     near(out, cached64(q, pages, 96, table, ends, fresh, scale, 8))
 
 
-@pytest.mark.parametrize("requests", [257, 700, 1025])
+@pytest.mark.parametrize("requests", [257, 700, 1025, 4096])
 def test_attend_cached_of_many_requests(attn, requests):
     """Most of a page or two, some without new tokens, one long and in pieces, wherever it stands."""
     g = gen(requests)
