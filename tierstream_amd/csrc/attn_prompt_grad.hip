@@ -7,7 +7,7 @@
 // up in order by a last launch: no atomics, the same bits every time. lse and sum p dp go to the workspace first, a pair a row.
 // Measured: 8192 tokens in three sequences, 32 heads on 8 of 128, causal, after a forward pass of 250 us: the pairs 45, the gradients 907
 // (ten products for the formula's seven, forward pass included: 840 TFLOP/s; alone dq takes 324, dk 364, dv 269), the joining launch 37. The matrix units
-// are busy 44 to 52 % of the cycles, at 1.8 GHz. 301 tokens of 4 heads of 64: 7.7, 11.0 and 4.6, latency.
+// are busy 44 to 52 % of the cycles, at 1.8 GHz. 301 tokens of 4 heads of 64: 7.2, 11.0 and 4.6, latency.
 #include "attn_tile.hpp"
 
 namespace tsa {
@@ -51,7 +51,10 @@ constexpr uint32_t kExactKeys = 512;
 template <class T, int kD, bool kAligned>
 __global__ __launch_bounds__(64 * kTileWaves, 2) void rows_kernel(tsa_attend_grad_args g, float2* rows, float c) {
   typedef TileShapes<kD> S;
-  __shared__ __attribute__((aligned(16))) unsigned char tile_s[2][S::kBytes];  // keys and values
+  // (two tiles of 128 values leave room for two workgroups a CU instead of three: rows of many keys took 56 us for 45; of 64 values they do not, and
+  // rows of 100 keys took 7.2 for 7.7)
+  constexpr uint32_t kBuffers = kD == 64 ? 2 : 1;
+  __shared__ __attribute__((aligned(16))) unsigned char tile_s[kBuffers][2][S::kBytes];  // keys and values
   __shared__ OwnTileMemory own_s;
   const tsa_attend_args& a = g.f;
   Queries o;
@@ -93,14 +96,22 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void rows_kernel(tsa_attend_gra
   const TileReads<kD> reads;
   const TileLoads<kD, kAligned> keys(a.k, o.ks.begin, o.kept, a.head_dim), values(a.v, o.ks.begin, o.kept, a.head_dim);
   const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_offset(tile_s));
-  for (uint32_t key0 = 0; key0 < o.end; key0 += kTile) {
-    if (key0) tile_ready();  // the last tile's reads are done
-    keys.fetch(key0, o.ks.count, lds);
-    values.fetch(key0, o.ks.count, lds + S::kBytes);
+  auto fetch = [&](uint32_t key0, uint32_t at) {
+    keys.fetch(key0, o.ks.count, at);
+    values.fetch(key0, o.ks.count, at + S::kBytes);
+  };
+  auto other_of = [&](uint32_t tiles) { return kBuffers == 2 ? 2 * lds + 2 * S::kBytes - tiles : lds; };
+  if (kBuffers == 2 && o.end) fetch(0, lds);
+  for (uint32_t key0 = 0, tiles = lds; key0 < o.end; key0 += kTile, tiles = other_of(tiles)) {
+    if (kBuffers == 1) {
+      if (key0) tile_ready();  // the last tile's reads are done
+      fetch(key0, lds);
+    }
     tile_ready();
+    if (kBuffers == 2 && key0 + kTile < o.end) fetch(key0 + kTile, other_of(tiles));
     if (key0 >= o.any) continue;
     const int32_t left = int32_t(o.limit) - int32_t(key0 + 4 * h);
-    const auto k_rows = reads.rows(lds), v_rows = reads.rows(lds + S::kBytes);
+    const auto k_rows = reads.rows(tiles), v_rows = reads.rows(tiles + S::kBytes);
 #pragma unroll
     for (uint32_t r = 0; r < 2; ++r) {
       f32x16 one[2];
