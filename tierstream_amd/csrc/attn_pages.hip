@@ -54,13 +54,14 @@ struct PlanSums {
   int32_t first[kMost + 1], taken[kMost + 1], given[kMost + 1], length[kMost];
 };
 
-// The whole plan by one workgroup, or (more than kPlanMany rows) its pages and rows by several and what replaces the inputs by another launch
-// behind them: lengths may become ends in place. Each workgroup adds up all requests itself. Pages given back and pages taken in
+// A plan's pages and rows by several workgroups, each of which adds up all requests itself; the first also writes what the host may have put
+// in an input's place (ends over lengths). Where it has, one workgroup does all, or with more than kPlanMany rows a launch behind them does this. Pages given back and pages taken in
 // one plan pass each other by: the k-th page taken is the k-th last given, or lies that far down in the stack, so that nothing waits for
 // what another thread writes. 32 requests 3 us, a launch and three memory latencies (9 with 1024 threads and a barrier between giving and
-// taking); 2047 requests with 65536 rows and some 10,000 pages given back 12 and 5 (26 together).
+// taking); 2047 requests with 65536 rows and some 10,000 pages given back 12.6, and 5.8 for the launch behind (26 together by one workgroup).
 template <uint32_t kThreads, uint32_t kPer>
 __global__ __launch_bounds__(kThreads) void plan_kernel(tsa_cache_plan_args a, bool work, bool finish) {
+  finish = finish && blockIdx.x == 0;
   constexpr uint32_t kMost = kThreads * kPer;
   __shared__ int64_t waves[3][kThreads / 64];
   __shared__ PlanSums<kMost> sum_s;
@@ -355,13 +356,11 @@ constexpr uint32_t kPlanMany = 8192;  // rows that one workgroup writes faster t
 
 template <uint32_t kThreads, uint32_t kPer>
 void plan(const tsa_cache_plan_args& a, hipStream_t stream) {
-  if (a.rows <= kPlanMany) {
-    hipLaunchKernelGGL((plan_kernel<kThreads, kPer>), dim3(1), dim3(kThreads), 0, stream, a, true, true);
-    return;
-  }
-  const uint32_t groups = (a.rows + 2 * kThreads - 1) / (2 * kThreads);
-  hipLaunchKernelGGL((plan_kernel<kThreads, kPer>), dim3(groups < 256 ? groups : 256), dim3(kThreads), 0, stream, a, true, false);
-  hipLaunchKernelGGL((plan_kernel<kThreads, kPer>), dim3(1), dim3(kThreads), 0, stream, a, false, true);
+  const bool in_place = (a.requests && a.ends == a.lengths) || a.left == a.n_free;
+  const uint32_t many = a.rows / (2 * kThreads) + 1, groups = in_place && a.rows <= kPlanMany ? 1 : many < 256 ? many : 256;
+  const bool behind = in_place && groups > 1;
+  hipLaunchKernelGGL((plan_kernel<kThreads, kPer>), dim3(groups), dim3(kThreads), 0, stream, a, true, !behind);
+  if (behind) hipLaunchKernelGGL((plan_kernel<kThreads, kPer>), dim3(1), dim3(kThreads), 0, stream, a, false, true);
 }
 }  // namespace
 }  // namespace op
