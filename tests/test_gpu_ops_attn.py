@@ -415,7 +415,7 @@ CACHED = [  # ends, fresh, kept, group, dim
     ([1], [1], 1, 1, 32), ([64], [1], 2, 4, 128), ([65], [1], 8, 4, 128), ([63, 1, 128, 700], [1] * 4, 4, 8, 128), ([2100], [1], 1, 16, 64),
     ([5, 300], [5, 2], 2, 5, 96), ([200, 0, 77], [3, 0, 8], 2, 1, 64), ([1000, 130], [1, 0], 3, 3, 128), ([4099], [4], 2, 4, 128), ([90], [40], 1, 6, 128),
     ([3], [5], 2, 2, 64), ([129, 64, 65, 63, 1, 2, 192, 500, 3], [1] * 9, 2, 2, 32), ([300], [17], 1, 33, 64),
-    ([9000, 17000], [1, 2], 8, 4, 128), ([20001], [1], 8, 2, 64), ([700] * 12, [2] * 12, 16, 1, 96)]  # (more pages than take both parts of a probability)
+    ([9000, 17000], [1, 2], 8, 4, 128), ([20001], [1], 8, 2, 64), ([700] * 12, [2] * 12, 16, 1, 96)]  # (thousands of pages)
 
 
 @pytest.mark.parametrize("kind", ["bf16", "f16"])
