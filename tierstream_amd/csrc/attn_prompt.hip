@@ -57,7 +57,8 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_kernel(tsa_attend_a
       keys.fetch(key0 + kTile, ks.count, other);
       values.fetch(key0 + kTile, ks.count, other + S::kBytes);
     }
-    if (a.causal && key0 + kTile > all_rows) {
+    const bool cut = a.causal && key0 + kTile > all_rows;
+    if (cut) {
       mark_rows(clean_tile<T, kD>(v_at), mark_s);
       clean_done();
     }
@@ -71,17 +72,17 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_kernel(tsa_attend_a
 #pragma unroll
       for (uint32_t r = 0; r < 2; ++r) s[r] = mfma32<T>(k_rows(r, k), q[k], s[r]);
     products_behind_reads<kD / 8, 4>();
+    if (cut) {  // (for the waves too that attend to all of the tile)
+#pragma unroll
+      for (uint32_t r = 0; r < 2; ++r)
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+          const f32x4 mark = marks_of(mark_s, r, i);
+#pragma unroll
+          for (uint32_t k = 0; k < 4; ++k) s[r][4 * i + k] += mark[k];
+        }
+    }
     if (key0 + kTile > whole) {
-      if (a.causal) {
-#pragma unroll
-        for (uint32_t r = 0; r < 2; ++r)
-#pragma unroll
-          for (uint32_t i = 0; i < 4; ++i) {
-            const f32x4 mark = marks_of(mark_s, r, i);
-#pragma unroll
-            for (uint32_t k = 0; k < 4; ++k) s[r][4 * i + k] += mark[k];
-          }
-      }
       const int32_t left = int32_t(limit) - int32_t(key0 + 4 * h);
 #pragma unroll
       for (uint32_t r = 0; r < 2; ++r)
