@@ -24,13 +24,13 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_kernel(tsa_attend_a
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const uint32_t row0 = own.row0 + wave * kOwn, row = row0 + (lane & 31u);
   const bool on = row < qs.count;
-  // keys that a row attends to, and those that every row and any row of this wave, and any of the workgroup does
+  // keys that a row attends to, those that every row of the workgroup does, any row of this wave, and any of the workgroup
   const int32_t ahead = a.causal ? int32_t(ks.count) - int32_t(qs.count) + 1 : 0;
   auto keys_of = [&](uint32_t r) {
     const int32_t n = a.causal ? int32_t(r) + ahead : int32_t(ks.count);
     return n < 0 ? 0u : min(uint32_t(n), ks.count);
   };
-  const uint32_t limit = on ? keys_of(row) : 0, all_rows = keys_of(own.row0), whole = keys_of(row0), any = row0 < qs.count ? keys_of(min(row0 + kOwn, qs.count) - 1) : 0;
+  const uint32_t limit = on ? keys_of(row) : 0, all_rows = keys_of(own.row0), any = row0 < qs.count ? keys_of(min(row0 + kOwn, qs.count) - 1) : 0;
   const uint32_t end = keys_of(min(own.row0 + kTileOwn, qs.count) - 1);
 
   // a negative scale turns the queries' signs, a scale of 0 takes them away
@@ -57,8 +57,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_kernel(tsa_attend_a
       keys.fetch(key0 + kTile, ks.count, other);
       values.fetch(key0 + kTile, ks.count, other + S::kBytes);
     }
-    const bool cut = a.causal && key0 + kTile > all_rows;
-    if (cut) {
+    if (a.causal && key0 + kTile > all_rows) {
       mark_rows(clean_tile<T, kD>(v_at), mark_s);
       clean_done();
     }
@@ -72,17 +71,17 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_kernel(tsa_attend_a
 #pragma unroll
       for (uint32_t r = 0; r < 2; ++r) s[r] = mfma32<T>(k_rows(r, k), q[k], s[r]);
     products_behind_reads<kD / 8, 4>();
-    if (cut) {  // (for the waves too that attend to all of the tile)
+    if (key0 + kTile > all_rows) {  // (by every wave that reads a cleaned tile, whether or not the mask cuts its own rows)
+      if (a.causal) {
 #pragma unroll
-      for (uint32_t r = 0; r < 2; ++r)
+        for (uint32_t r = 0; r < 2; ++r)
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-          const f32x4 mark = marks_of(mark_s, r, i);
+          for (uint32_t i = 0; i < 4; ++i) {
+            const f32x4 mark = marks_of(mark_s, r, i);
 #pragma unroll
-          for (uint32_t k = 0; k < 4; ++k) s[r][4 * i + k] += mark[k];
-        }
-    }
-    if (key0 + kTile > whole) {
+            for (uint32_t k = 0; k < 4; ++k) s[r][4 * i + k] += mark[k];
+          }
+      }
       const int32_t left = int32_t(limit) - int32_t(key0 + 4 * h);
 #pragma unroll
       for (uint32_t r = 0; r < 2; ++r)
