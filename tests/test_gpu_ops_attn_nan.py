@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_ops_attn import attend_case, stream
+from test_gpu_ops_attn import attend_case, room, stream
 
 pytestmark = pytest.mark.gpu
 
@@ -82,3 +82,52 @@ def test_a_key_or_a_query_that_is_no_number(attn, kind, counts, k_counts, dim):
                 assert torch.equal(out[~bad], plain[~bad]) and torch.equal(lse.T[~bad], one.T[~bad]), f"query {j}: elsewhere"
             else:
                 assert torch.equal(out[:, :2], plain[:, :2]) and bool(torch.isfinite(out[~bad].float()).all()), f"key {j}: elsewhere"
+
+
+def gradients(attn, q, k, v, dout, where):
+    out, lse = torch.empty_like(q), torch.empty((q.shape[1], len(q)), device="cuda")
+    attn.attend(q, k, v, out, lse=lse, **where)
+    grads = [torch.full_like(x, 7.0) for x in (q, k, v)]
+    attn.attend_backward(q, k, v, out, dout, lse, *grads, workspace=room(attn.attend_backward_workspace(q, k)), **where)
+    return out, lse, grads
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("counts,k_counts,dim", CASES)
+@pytest.mark.parametrize("layout", ["packed", "odd"])
+def test_queries_gradients_with_a_key_of_no_score(attn, kind, counts, k_counts, dim, layout):
+    """A key's value of -infinity where queries are positive: its probability is 0 and outputs are numbers, but dq = sum ds k has 0 x infinity
+    in that value for every row that attends to it. Rows that do not are as with a 0 there."""
+    q, k, v, dout, k_counts, first, k_first = attend_case(kind, counts, k_counts, 2, 2, dim, layout, pad=0)
+    ok, where = attended(counts, k_counts), dict(first=first, k_first=k_first, stream=stream())
+    for j in places(len(k)):
+        d = (5 * j) % dim
+        had, was = q[:, :, d].clone(), k[j, 1, d].clone()
+        q[:, :, d] = 1
+        k[j, 1, d] = 0
+        _, _, plain = gradients(attn, q, k, v, dout, where)
+        k[j, 1, d] = -math.inf
+        out, _, got = gradients(attn, q, k, v, dout, where)
+        q[:, :, d], k[j, 1, d] = had, was
+        sees = ok[:, j]
+        assert bool(torch.isfinite(out.float()).all())
+        assert bool(got[0][sees][:, 2:, d].isnan().all()), f"key {j}: lost"
+        assert torch.equal(got[0][~sees], plain[0][~sees]) and torch.equal(got[0][:, :2], plain[0][:, :2]), f"key {j}: elsewhere"
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("counts,k_counts,dim", CASES)
+def test_gradients_with_a_value_that_is_no_number(attn, kind, counts, k_counts, dim):
+    """In V: dq of every row that attends to it, and dk of every key that such a row attends to."""
+    q, k, v, dout, k_counts, first, k_first = attend_case(kind, counts, k_counts, 2, 2, dim, "packed", pad=0)
+    ok, where = attended(counts, k_counts), dict(first=first, k_first=k_first, stream=stream())
+    for j in places(len(v)):
+        was = v[j, 1, 1].clone()
+        v[j, 1, 1] = math.nan
+        _, _, (dq, dk, _) = gradients(attn, q, k, v, dout, where)
+        v[j, 1, 1] = was
+        sees = ok[:, j]
+        met = ok[sees].any(0)
+        assert not bool(torch.isfinite(dq[sees][:, 2:].float()).any()) and not bool(torch.isfinite(dk[met][:, 1].float()).any()), f"key {j}: lost"
+        assert bool(torch.isfinite(dq[~sees].float()).all()) and bool(torch.isfinite(dk[~met].float()).all()), f"key {j}: elsewhere"
+        assert bool(torch.isfinite(dq[:, :2].float()).all()) and bool(torch.isfinite(dk[:, 0].float()).all()), f"key {j}: elsewhere"

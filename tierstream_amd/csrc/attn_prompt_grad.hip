@@ -20,7 +20,7 @@ struct Queries {
   uint32_t head, kept;
   uint32_t row;        // this lane's
   bool on;
-  uint32_t limit, all_rows, whole, any, end;  // keys that this row; every row of the workgroup; every, and any, row of this wave; any row attends to
+  uint32_t limit, all_rows, any, end;  // keys that this row; every row of the workgroup; any row of this wave; any row attends to
 };
 // By the whole workgroup; false: there are no more.
 template <bool kFromEnd>
@@ -36,7 +36,7 @@ __device__ __forceinline__ bool find_queries(const tsa_attend_args& a, uint32_t 
     const int32_t n = a.causal ? int32_t(r) + ahead : int32_t(o.ks.count);
     return n < 0 ? 0u : min(uint32_t(n), o.ks.count);
   };
-  o.limit = o.on ? keys_of(o.row) : 0, o.all_rows = keys_of(own.row0), o.whole = keys_of(row0);
+  o.limit = o.on ? keys_of(o.row) : 0, o.all_rows = keys_of(own.row0);
   o.any = row0 < o.qs.count ? keys_of(min(row0 + kOwn, o.qs.count) - 1) : 0;
   o.end = keys_of(min(own.row0 + kTileOwn, o.qs.count) - 1);
   return true;
@@ -216,7 +216,7 @@ __device__ __forceinline__ void queries_part(const tsa_attend_grad_args& g, cons
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         one[0][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(one[0][i], c, -mine.x)) * (one[1][i] - mine.y);
-      if (key0 + kTile > o.whole) {
+      if (key0 + kTile > o.all_rows) {  // (by every wave that reads a cleaned tile, whether or not the mask cuts its own rows)
         if (a.causal) {
 #pragma unroll
           for (uint32_t i = 0; i < 4; ++i) {
