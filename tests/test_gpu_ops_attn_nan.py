@@ -117,6 +117,32 @@ def test_queries_gradients_with_a_key_of_no_score(attn, kind, counts, k_counts, 
 
 @pytest.mark.parametrize("kind", ["bf16", "f16"])
 @pytest.mark.parametrize("counts,k_counts,dim", CASES)
+@pytest.mark.parametrize("layout", ["packed", "odd"])
+def test_keys_gradients_with_a_row_that_is_no_number(attn, kind, counts, k_counts, dim, layout):
+    """One value of dout, or of a query: the gradients of every key that its row attends to, of its own query, and of no other."""
+    q, k, v, dout, k_counts, first, k_first = attend_case(kind, counts, k_counts, 2, 2, dim, layout, pad=0)
+    ok, where = attended(counts, k_counts), dict(first=first, k_first=k_first, stream=stream())
+    for x in (dout, q):
+        for i, row in enumerate(places(len(q))):
+            d, was = (3 * row) % dim, x[row, 2, (3 * row) % dim].clone()
+            x[row, 2, d] = 0
+            _, _, plain = gradients(attn, q, k, v, dout, where)
+            x[row, 2, d] = (math.nan, math.inf, -math.inf)[i % 3] if x is dout else math.nan
+            _, _, (dq, dk, dv) = gradients(attn, q, k, v, dout, where)
+            x[row, 2, d] = was
+            seen, own = ok[row], torch.zeros((len(q), 4), dtype=torch.bool, device="cuda")
+            own[row, 2] = bool(seen.any())
+            what = f"{'dout' if x is dout else 'query'} {row}"
+            assert not bool(torch.isfinite(dv[seen][:, 1, d if x is dout else slice(None)].float()).any()), f"{what}: lost in dv"
+            assert not bool(torch.isfinite(dk[seen][:, 1].float()).any()), f"{what}: lost in dk"
+            assert not bool(torch.isfinite(dq[own].float()).any()), f"{what}: lost in dq"
+            for got, want in ((dk, plain[1]), (dv, plain[2])):
+                assert torch.equal(got[~seen], want[~seen]) and torch.equal(got[:, 0], want[:, 0]), f"{what}: elsewhere"
+            assert torch.equal(dq[~own], plain[0][~own]), f"{what}: elsewhere in dq"
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("counts,k_counts,dim", CASES)
 def test_gradients_with_a_value_that_is_no_number(attn, kind, counts, k_counts, dim):
     """In V: dq of every row that attends to it, and dk of every key that such a row attends to."""
     q, k, v, dout, k_counts, first, k_first = attend_case(kind, counts, k_counts, 2, 2, dim, "packed", pad=0)

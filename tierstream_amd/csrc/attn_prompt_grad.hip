@@ -280,7 +280,7 @@ __device__ __forceinline__ void keys_part(const tsa_attend_grad_args& g, const f
     const int32_t n = a.causal ? int32_t(key) - int32_t(ks.count) + int32_t(qs.count) : 0;
     return n < 0 ? 0u : uint32_t(n);
   };
-  const uint32_t from = from_of(row), any = from_of(row0), whole = from_of(row0 + kOwn - 1), all_rows = from_of(own.row0 + kTileOwn - 1);
+  const uint32_t from = from_of(row), any = from_of(row0), all_rows = from_of(own.row0 + kTileOwn - 1);
   const uint32_t begin = from_of(own.row0) / kTile * kTile, tiles = begin < qs.count ? (qs.count - begin + kTile - 1) / kTile : 0;
   // this piece's steps: a query tile of a head each
   const uint32_t step0 = uint32_t(uint64_t(tiles) * group * piece / pieces), steps = uint32_t(uint64_t(tiles) * group * (piece + 1) / pieces) - step0;
@@ -343,7 +343,7 @@ __device__ __forceinline__ void keys_part(const tsa_attend_grad_args& g, const f
           one[1][4 * i + j] = p * (one[1][4 * i + j] - mean);
         }
       }
-      if (at < whole || at + kTile > qs.count) {
+      if (at < all_rows || at + kTile > qs.count) {  // (by every wave that reads a cleaned tile, whether or not the mask cuts its own keys)
         if (a.causal && at < all_rows) {
 #pragma unroll
           for (uint32_t i = 0; i < 4; ++i) {
