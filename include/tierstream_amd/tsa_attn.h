@@ -122,7 +122,8 @@ SS_API ss_status tsa_cache_plan(const tsa_cache_plan_args* a, void* stream);
 
 /* The same positions and slots for requests whose pages are there: the rows first[i]..first[i + 1] are the tokens of request i that
  * end with its length ends[i] (its whole context where first counts whole lengths). Reads table, ends, first, requests, width and
- * rows of the struct, writes positions and slots. A row that has no page (-1 in the table, before the first token) gets slot -1. */
+ * rows of the struct, writes positions and slots. A row that has no page (-1 in the table, before the first token) gets slot -1, one before
+ * first[0] or behind the last one -1 in both. */
 SS_API ss_status tsa_cache_slots(const tsa_cache_plan_args* a, void* stream);
 
 /* Token t's keys and values to slot slots[t]. A block's scale is its value of the largest size (of equal ones the first) over -8,

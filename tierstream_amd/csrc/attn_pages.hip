@@ -179,7 +179,7 @@ __global__ __launch_bounds__(256) void slots_kernel(tsa_cache_plan_args a) {
   const int64_t rows = a.requests ? a.first[a.requests] : 0;
   int64_t position = -1;
   int32_t slot = -1;
-  if (int64_t(r) < rows) {
+  if (int64_t(r) < rows && int64_t(r) >= a.first[0]) {
     const uint32_t i = owner_of(a.first, a.requests, int32_t(r));
     position = int64_t(a.ends[i]) - a.first[i + 1] + r;
     if (position < 0) {
