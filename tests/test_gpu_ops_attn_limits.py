@@ -27,3 +27,20 @@ def test_rows_before_the_first_request_have_no_slot(attn):
     assert slots.tolist() == [-1] * 3 + [162, 163, 256, 257, 258] + [-1] * 2
     attn.slots(i32([[1, 2]]), i32([70]), i32([12, 20]), positions, slots, stream=stream())  # (all of them)
     assert positions.tolist() == [-1] * 10 and slots.tolist() == [-1] * 10
+
+
+def test_requests_that_overlap_beyond_all_counts(attn):
+    """4096 requests that each say to have all of 16384 tokens, or none: 2048 x 16384 tiles x 255 rounds, more than 32 bits count."""
+    tokens, requests, width, dim = 16384, 4096, 1020, 32
+    cache = attn.Cache(torch.zeros((4, 1, 72 * dim), dtype=torch.uint8, device="cuda"), 1, dim)
+    table = torch.arange(requests * width, device="cuda", dtype=torch.int32).view(requests, width) % 4
+    whole = torch.full((tokens + 2, 16, dim), 7.0, dtype=torch.float16, device="cuda")
+    q, out = torch.ones((tokens, 16, dim), dtype=torch.float16, device="cuda"), whole[1:-1]
+    size = attn.attend_cached_workspace(cache, q, table)
+    ws = torch.full((size + 1024,), 99, dtype=torch.uint8, device="cuda")
+    ends = torch.full((requests,), width * 64, dtype=torch.int32, device="cuda")
+    attn.attend_cached(cache, q, out, table, ends, i32([0, tokens] * (requests // 2) + [0]), workspace=ws[:size], stream=stream())
+    torch.cuda.synchronize()
+    assert bool((whole[0] == 7).all()) and bool((whole[-1] == 7).all()) and bool((ws[size:] == 99).all())
+    attn.attend_cached(cache, q[:2], out[:2], table[:2], ends[:2], i32([0, 1, 2]), workspace=ws[:size], stream=stream())
+    assert bool((out[:2] == 0).all())  # (pages of zeros)

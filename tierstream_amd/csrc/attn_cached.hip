@@ -90,17 +90,18 @@ struct Pieces {
 // fresh * group / 16 tiles, and one more at most.
 __device__ __forceinline__ uint32_t tile_place(uint32_t request, uint32_t first, uint32_t group) { return request + uint32_t(uint64_t(first) * group / kRows); }
 
-template <class V>
-__device__ __forceinline__ V lanes_up_to(V v) {
+__device__ __forceinline__ uint32_t lanes_up_to(uint32_t v) {
 #pragma unroll
   for (uint32_t s = 1; s < 64; s <<= 1) {
-    const V o = __shfl_up(v, s, 64);
-    if ((threadIdx.x & 63u) >= s) v += o;
+    const uint32_t o = __shfl_up(v, s, 64);
+    if ((threadIdx.x & 63u) >= s) v = add_sat(v, o);
   }
   return v;
 }
 
-// The tile that holds the first round of share `want`. By the whole workgroup; false: there is none.
+// The tile that holds the first round of share `want`. By the whole workgroup; false: there is none. Of requests that follow each
+// other all rounds are below 2^31; spans that overlap (first not ascending) may have more than 32 bits count, which the sums keep to: then
+// there is none either.
 __device__ __forceinline__ bool find_place(const tsa_attend_cached_args& a, const CachedShape& s, uint32_t want, PlaceMemory& m, Place& out) {
   const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6, per = (a.requests + 64 * kWaves - 1) / (64 * kWaves);
   const uint32_t i0 = min(t * per, a.requests), i1 = min(i0 + per, a.requests);
@@ -108,7 +109,7 @@ __device__ __forceinline__ bool find_place(const tsa_attend_cached_args& a, cons
   Request r;  // (the last one stays: with up to 256 requests none is read twice)
   for (uint32_t i = i0; i < i1; ++i) {
     r = Request(a, i, s.group);
-    pages += r.tiles * r.rounds();
+    pages = add_sat(pages, r.tiles * r.rounds());  // (a request's own are below 2^31)
   }
   const uint32_t upto = lanes_up_to(pages);
   if (lane == 63) m.pages[wave] = upto;
@@ -117,9 +118,10 @@ __device__ __forceinline__ bool find_place(const tsa_attend_cached_args& a, cons
   uint32_t page0 = upto - pages;
 #pragma unroll
   for (uint32_t w = 0; w < kWaves; ++w) {
-    p.all += m.pages[w];
+    p.all = add_sat(p.all, m.pages[w]);
     if (w < wave) page0 += m.pages[w];
   }
+  if (p.all >> 31) return false;
   const uint32_t even = p.all / s.shares + (p.all % s.shares != 0);
   p.share = even;
   const uint64_t page = uint64_t(want) * p.share;  // (past all of them, perhaps by far)

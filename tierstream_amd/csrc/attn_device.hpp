@@ -13,6 +13,9 @@ inline bool vector_heads(const tsa_heads& h) {
   return reinterpret_cast<uintptr_t>(h.p) % 16 == 0 && h.token_stride % 8 == 0 && h.head_stride % 8 == 0;
 }
 
+// Sums that stay at the largest number where they would pass it.
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
+
 // A sequence's rows inside its array, whatever `first` holds.
 struct Span {
   uint32_t begin, count;
