@@ -44,3 +44,26 @@ def test_requests_that_overlap_beyond_all_counts(attn):
     assert bool((whole[0] == 7).all()) and bool((whole[-1] == 7).all()) and bool((ws[size:] == 99).all())
     attn.attend_cached(cache, q[:2], out[:2], table[:2], ends[:2], i32([0, 1, 2]), workspace=ws[:size], stream=stream())
     assert bool((out[:2] == 0).all())  # (pages of zeros)
+
+
+def test_sequences_that_overlap_beyond_all_counts(attn):
+    """65536 sequences that each say to have all of 2^24 - 1 rows, or none: 32768 x 131072 tiles are 2^32. None is taken up; then two that
+    follow each other are."""
+    many, few, n = (1 << 24) - 1, 16, 1 << 16
+    wide, small = torch.ones((many, 1, 8), dtype=torch.bfloat16, device="cuda"), torch.ones((few, 1, 8), dtype=torch.bfloat16, device="cuda")
+    far, near = i32([0, many] * (n // 2) + [0]), i32([0] * n + [few])
+    out, lse = torch.full_like(wide, 7.0), torch.full((1, many), 7.0, device="cuda")
+    ws = torch.empty(attn.attend_backward_workspace(wide, small), dtype=torch.uint8, device="cuda")
+    attn.attend(wide, small, small, out, lse=lse, first=far, k_first=near, stream=stream())
+    assert bool((out == 7).all()) and bool((lse == 7).all())
+    dq = torch.full_like(wide, 7.0)
+    attn.attend_backward(wide, small, small, out, wide, lse, dq, first=far, k_first=near, workspace=ws, stream=stream())
+    assert bool((dq == 7).all())
+    out[:20], lse[:, :20] = 7.0, 7.0
+    attn.attend(wide, small, small, out, lse=lse, first=i32([0, 9, 20]), k_first=i32([0, 9, 16]), causal=False, stream=stream())
+    assert bool((out[:20] == 1).all()) and bool((out[20:] == 7).all())
+    del out, lse, dq
+    ws = torch.empty(attn.attend_backward_workspace(small, wide), dtype=torch.uint8, device="cuda")
+    dk, dv, out, lse = torch.full_like(wide, 7.0), torch.full_like(wide, 7.0), torch.ones_like(small), torch.zeros((1, few), device="cuda")
+    attn.attend_backward(small, wide, wide, out, small, lse, None, dk, dv, first=near, k_first=far, workspace=ws, stream=stream())
+    assert bool((dk == 7).all()) and bool((dv == 7).all())

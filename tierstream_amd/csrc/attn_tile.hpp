@@ -292,28 +292,29 @@ struct OwnTileMemory {
   uint32_t sums[kTileWaves];
   OwnTile found;
 };
-// Number `want`, from the end or from the first. By the whole workgroup; false: there are fewer.
+// Number `want`, from the end or from the first. By the whole workgroup; false: there are fewer. Of sequences that follow each other all
+// tiles are below 2^25; spans that overlap (first not ascending) may have more than 32 bits count, which the sums keep to: then there is none.
 template <bool kFromEnd>
 __device__ __forceinline__ bool find_own_tile(const int32_t* first, uint32_t n, uint32_t rows, uint32_t want, OwnTileMemory& m, OwnTile& out) {
   const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6, per = (n + 64 * kTileWaves - 1) / (64 * kTileWaves);
   const uint32_t i0 = min(t * per, n), i1 = min(i0 + per, n);
   uint32_t sum = 0;
-  for (uint32_t i = i0; i < i1; ++i) sum += (span_of(first, i, rows).count + kTileOwn - 1) / kTileOwn;
+  for (uint32_t i = i0; i < i1; ++i) sum = add_sat(sum, (span_of(first, i, rows).count + kTileOwn - 1) / kTileOwn);
   uint32_t upto = sum;
 #pragma unroll
   for (uint32_t s = 1; s < 64; s <<= 1) {
     const uint32_t o = __shfl_up(upto, s, 64);
-    if (lane >= s) upto += o;
+    if (lane >= s) upto = add_sat(upto, o);
   }
   if (lane == 63) m.sums[wave] = upto;
   __syncthreads();
   uint32_t all = 0, before = upto - sum;
 #pragma unroll
   for (uint32_t w = 0; w < kTileWaves; ++w) {
-    all += m.sums[w];
+    all = add_sat(all, m.sums[w]);
     if (w < wave) before += m.sums[w];
   }
-  if (want >= all) return false;
+  if (want >= all || all >> 31) return false;
   if (kFromEnd) want = all - 1 - want;
   if (want >= before && want < before + sum) {
     uint32_t at = want - before;
