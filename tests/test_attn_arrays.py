@@ -1,0 +1,14 @@
+"""Arrays that tierstream_amd.attn refuses as ValueError beside those of test_attn_refusals.py: no GPU is needed."""
+import pytest
+
+from test_attn_refusals import Fake, i32
+from tierstream_amd import attn
+
+
+@pytest.mark.parametrize("k_first", [None, i32(0)])
+def test_a_list_of_sequences_has_an_end(k_first):
+    q, k = Fake(4, 4, 128), Fake(4, 4, 128)
+    with pytest.raises(ValueError, match="first"):
+        attn.attend(q, k, k, q, first=i32(0), k_first=k_first)
+    with pytest.raises(ValueError, match="first"):
+        attn.attend_backward(q, k, k, q, q, Fake(4, 4, dtype="torch.float32"), q, first=i32(0), k_first=k_first)

@@ -286,6 +286,8 @@ def _attend_fields(what, q, k, v, out, lse, first, k_first, causal, scale) -> tu
     x, dtype, device = _heads(q, "q"), q.dtype, q.device
     (tokens, heads, dim), (k_tokens, kept, _) = q.shape, _three(k, "k")
     shape, n = (k_tokens, kept, dim), 1 if first is None else first.shape[0] - 1
+    if n < 0:
+        raise ValueError("first: [sequences + 1], not []")
     fields = (*x, *_heads(k, "k", shape, dtype), *_heads(v, "v", shape, dtype), *_heads(out, "out", q.shape, dtype),
               0 if first is None else _ints(first, n + 1, "first"), 0 if k_first is None else _ints(k_first, n + 1, "k_first"),
               0 if lse is None else _vec(lse, (heads, tokens), "torch.float32", "lse"), tokens, k_tokens, n, dim, _type(q), causal,
