@@ -166,8 +166,8 @@ SS_API ss_status tsa_attend_cached(const tsa_cache* c, const tsa_attend_cached_a
 /* out_t = sum_j p_tj v_j, p_t the softmax of scale q_t . k_j over the keys of t's sequence: with n queries and m keys, all of them,
  * or (causal) those up to j = i + m - n for the sequence's query i. A row without keys is 0 (its lse -infinity); rows behind the
  * last sequence are left as they were. Query head h reads key head h / (heads / kv_heads). Probabilities are rounded to type (in half
- * precision times 2^15), and where tokens x heads is at most 2048, or rows do not start 16-byte aligned, what that leaves of them is
- * multiplied too; all sums are in 32 bits. */
+ * precision times 2^15), and in sequences of at most 2^17 pairs of a query and a key what that leaves of them is multiplied too; all sums
+ * are in 32 bits. */
 typedef struct tsa_attend_args {
   tsa_heads q, k, v, out;
   const int32_t* first;    /* [sequences + 1]: a sequence's first query row; ascending from 0. NULL: one sequence of all rows */

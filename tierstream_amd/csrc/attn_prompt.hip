@@ -10,17 +10,19 @@ namespace tsa {
 namespace op {
 namespace {
 
+template <int kD>
+struct PromptMemory {
+  __attribute__((aligned(16))) unsigned char tile[2][2][TileShapes<kD>::kBytes];  // keys and values, two of each
+  __attribute__((aligned(16))) float mark[kTile];
+  OwnTileMemory own;
+};
+
+// A workgroup's queries.
 template <class T, int kD, bool kAligned, bool kSplit>
-__global__ __launch_bounds__(64 * kTileWaves, 2) void attend_kernel(tsa_attend_args a, float c) {
+__device__ __forceinline__ void attend_tile(const tsa_attend_args& a, float c, uint32_t head, OwnTile own, Span qs, Span ks, PromptMemory<kD>& m) {
   typedef TileShapes<kD> S;
   constexpr float kUp = std::is_same_v<T, F16> ? 7.0f : 0.0f;  // half precision: probabilities up to 2^15, so that small ones keep their bits
-  __shared__ __attribute__((aligned(16))) unsigned char tile_s[2][2][S::kBytes];  // keys and values, two of each
-  __shared__ OwnTileMemory own_s;
-  __shared__ __attribute__((aligned(16))) float mark_s[kTile];
-  OwnTile own;
-  const uint32_t head = head_of_group(blockIdx.x % a.q.heads, a.q.heads), kept = head / (a.q.heads / a.k.heads);
-  if (!find_own_tile<true>(a.first, a.sequences, a.tokens, blockIdx.x / a.q.heads, own_s, own)) return;
-  const Span qs = span_of(a.first, own.sequence, a.tokens), ks = span_of(a.k_first ? a.k_first : a.first, own.sequence, a.k_tokens);
+  const uint32_t kept = head / (a.q.heads / a.k.heads);
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const uint32_t row0 = own.row0 + wave * kOwn, row = row0 + (lane & 31u);
   const bool on = row < qs.count;
@@ -42,7 +44,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_kernel(tsa_attend_a
 
   const TileReads<kD> reads;
   const TileLoads<kD, kAligned> keys(a.k, ks.begin, kept, a.head_dim), values(a.v, ks.begin, kept, a.head_dim);
-  const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_offset(tile_s));
+  const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_offset(m.tile));
   f32x16 o[kD / 32];
   clear(o);
   float top = -INFINITY, total = 0.0f;
@@ -58,7 +60,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_kernel(tsa_attend_a
       values.fetch(key0 + kTile, ks.count, other + S::kBytes);
     }
     if (a.causal && key0 + kTile > all_rows) {
-      mark_rows(clean_tile<T, kD>(v_at), mark_s);
+      mark_rows(clean_tile<T, kD>(v_at), m.mark);
       clean_done();
     }
     if (key0 >= any) continue;
@@ -77,7 +79,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_kernel(tsa_attend_a
         for (uint32_t r = 0; r < 2; ++r)
 #pragma unroll
           for (uint32_t i = 0; i < 4; ++i) {
-            const f32x4 mark = marks_of(mark_s, r, i);
+            const f32x4 mark = marks_of(m.mark, r, i);
 #pragma unroll
             for (uint32_t k = 0; k < 4; ++k) s[r][4 * i + k] += mark[k];
           }
@@ -131,6 +133,17 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_kernel(tsa_attend_a
     a.lse[uint64_t(head) * a.tokens + qs.begin + row] = total == 0.0f ? -INFINITY : (top - kUp + __builtin_amdgcn_logf(total)) * 0.69314718f;
 }
 
+template <class T, int kD, bool kAligned>
+__global__ __launch_bounds__(64 * kTileWaves, 2) void attend_kernel(tsa_attend_args a, float c) {
+  __shared__ PromptMemory<kD> m;
+  OwnTile own;
+  if (!find_own_tile<true>(a.first, a.sequences, a.tokens, blockIdx.x / a.q.heads, m.own, own)) return;
+  const uint32_t head = head_of_group(blockIdx.x % a.q.heads, a.q.heads);
+  const Span qs = span_of(a.first, own.sequence, a.tokens), ks = span_of(a.k_first ? a.k_first : a.first, own.sequence, a.k_tokens);
+  if (both_parts(qs.count, ks.count)) attend_tile<T, kD, kAligned, true>(a, c, head, own, qs, ks, m);
+  else attend_tile<T, kD, kAligned, false>(a, c, head, own, qs, ks, m);
+}
+
 }  // namespace
 }  // namespace op
 
@@ -139,11 +152,10 @@ int launch_attend(const tsa_attend_args& a, hipStream_t stream) {
   const dim3 grid(uint32_t(own_tiles_at_most(a.sequences, a.tokens) * a.q.heads)), block(64 * kTileWaves);
   const float c = a.scale * 1.44269504f;
   const bool aligned = vector_heads(a.q) && vector_heads(a.out) && (a.k_tokens == 0 || (tile_heads(a.k) && tile_heads(a.v)));
-#define CALL(T, D)                                                                                       \
-  do {                                                                                                   \
-    if (!aligned) hipLaunchKernelGGL((attend_kernel<T, D, false, true>), grid, block, 0, stream, a, c);  \
-    else if (split_rows(a)) hipLaunchKernelGGL((attend_kernel<T, D, true, true>), grid, block, 0, stream, a, c); \
-    else hipLaunchKernelGGL((attend_kernel<T, D, true, false>), grid, block, 0, stream, a, c);           \
+#define CALL(T, D)                                                                                      \
+  do {                                                                                                  \
+    if (aligned) hipLaunchKernelGGL((attend_kernel<T, D, true>), grid, block, 0, stream, a, c);         \
+    else hipLaunchKernelGGL((attend_kernel<T, D, false>), grid, block, 0, stream, a, c);                \
   } while (0)
   if (a.type == TSA_BF16) {
     if (a.head_dim <= 64) CALL(Bf16, 64);

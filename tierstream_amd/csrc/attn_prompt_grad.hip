@@ -42,6 +42,20 @@ __device__ __forceinline__ bool find_queries(const tsa_attend_args& a, uint32_t 
   return true;
 }
 
+// The keys of a workgroup, and the piece of their queries that it has.
+struct Keys {
+  Span qs, ks;
+  OwnTile own;
+  uint32_t kept, piece;
+};
+__device__ __forceinline__ bool find_keys(const tsa_attend_args& a, uint32_t index, uint32_t pieces, OwnTileMemory& m, Keys& o) {
+  const int32_t* k_first = a.k_first ? a.k_first : a.first;
+  o.kept = head_of_group(index % a.k.heads, a.k.heads), o.piece = index / a.k.heads % pieces;
+  if (!find_own_tile<false>(k_first, a.sequences, a.k_tokens, index / a.k.heads / pieces, m, o.own)) return false;
+  o.qs = span_of(a.first, o.own.sequence, a.tokens), o.ks = span_of(k_first, o.own.sequence, a.k_tokens);
+  return true;
+}
+
 // What is taken off the gradients of a row's probabilities, sum_j p_j dp_j. It is dout . out, but out is rounded to 16 bits, which over a
 // few keys is as large an error in the gradients as their own rounding (over 10 keys they are off by 1.7 times what rounding the results
 // costs, 1.4 without it; over 1000 it is lost in it): rows of workgroups that attend to no more keys than this add up p dp itself.
@@ -170,11 +184,9 @@ struct GradMemory {
 };
 
 template <class T, int kD, bool kAligned, bool kSplit>
-__device__ __forceinline__ void queries_part(const tsa_attend_grad_args& g, const float2* rows, float c, uint32_t group, GradMemory<kD>& m) {
+__device__ __forceinline__ void queries_part(const tsa_attend_grad_args& g, const float2* rows, float c, const Queries& o, GradMemory<kD>& m) {
   typedef TileShapes<kD> S;
   const tsa_attend_args& a = g.f;
-  Queries o;
-  if (!find_queries<true>(a, group, m.own, o)) return;
   const uint32_t h = (threadIdx.x & 63u) >> 5;
   const OwnRows<kD, kAligned> q(a.q, uint64_t(o.qs.begin) + o.row, o.head, a.head_dim, o.on), dout(g.dout, uint64_t(o.qs.begin) + o.row, o.head, a.head_dim, o.on);
   const float2 mine = o.on ? rows[uint64_t(o.head) * a.tokens + o.qs.begin + o.row] : float2{INFINITY, 0.0f};
@@ -262,16 +274,13 @@ __device__ __forceinline__ void put_part(float* p, const f32x16 (&v)[kD / 32], f
 // Both gradients of keys and values, or one. With 128 values both together need 430 registers, one wave a SIMD: they took 840 us in three
 // packed sequences of 8192 together, one after the other with the scores computed again 660.
 template <class T, int kD, bool kAligned, bool kSplit, bool kKeys, bool kValues>
-__device__ __forceinline__ void keys_part(const tsa_attend_grad_args& g, const float2* rows, float c, uint32_t pieces, float* parts, uint32_t index, GradMemory<kD>& m) {
+__device__ __forceinline__ void keys_part(const tsa_attend_grad_args& g, const float2* rows, float c, const Keys& o, uint32_t pieces, float* parts, GradMemory<kD>& m) {
   typedef TileShapes<kD> S;
   constexpr float kUp = probability_up<T>();
   const tsa_attend_args& a = g.f;
-  const int32_t* k_first = a.k_first ? a.k_first : a.first;
-  OwnTile own;
-  const uint32_t kept = head_of_group(index % a.k.heads, a.k.heads), group = a.q.heads / a.k.heads;
-  const uint32_t piece = index / a.k.heads % pieces;
-  if (!find_own_tile<false>(k_first, a.sequences, a.k_tokens, index / a.k.heads / pieces, m.own, own)) return;
-  const Span qs = span_of(a.first, own.sequence, a.tokens), ks = span_of(k_first, own.sequence, a.k_tokens);
+  const Span qs = o.qs, ks = o.ks;
+  const OwnTile own = o.own;
+  const uint32_t kept = o.kept, piece = o.piece, group = a.q.heads / a.k.heads;
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const uint32_t row0 = own.row0 + wave * kOwn, row = row0 + (lane & 31u);
   const bool on = row < ks.count;
@@ -325,12 +334,24 @@ __device__ __forceinline__ void keys_part(const tsa_attend_grad_args& g, const f
     for (uint32_t r = 0; r < 2; ++r) {
       f32x16 one[2];  // scores, then probabilities; their gradients, then the scores'
       clear(one);
+      if constexpr (kKeys) {
+        // reads kept four products ahead, in this order (with both kinds of sums behind them the compiler gave products_behind_reads up: 625 us
+        // for 611, keys of three sequences of 2730, 32 heads on 8 of 128; 600 with one kind)
+        constexpr uint32_t kProducts = kD / 8, kAhead = 4;
+        bits8 ahead[kAhead];
+        auto read = [&](uint32_t i) { ahead[i % kAhead] = i % 2 ? d_rows(r, i / 2) : q_rows(r, i / 2); };
 #pragma unroll
-      for (uint32_t i = 0; i < kD / 16; ++i) {
-        one[0] = mfma32<T>(q_rows(r, i), k.v[i], one[0]);
-        if constexpr (kKeys) one[1] = mfma32<T>(d_rows(r, i), v.v[i], one[1]);
+        for (uint32_t i = 0; i < kAhead; ++i) read(i);
+#pragma unroll
+        for (uint32_t i = 0; i < kProducts; ++i) {
+          __builtin_amdgcn_sched_barrier(0);
+          one[i % 2] = mfma32<T>(ahead[i % kAhead], i % 2 ? v.v[i / 2] : k.v[i / 2], one[i % 2]);
+          if (i + kAhead < kProducts) read(i + kAhead);
+        }
+      } else {
+#pragma unroll
+        for (uint32_t i = 0; i < kD / 16; ++i) one[0] = mfma32<T>(q_rows(r, i), k.v[i], one[0]);
       }
-      if constexpr (kKeys) products_behind_reads<kD / 8, 4>();
 #pragma unroll
       for (uint32_t i = 0; i < 4; ++i) {
         const f32x4* pair = reinterpret_cast<const f32x4*>(&m.row[buffer][32 * r + 8 * i + 4 * h]);
@@ -391,14 +412,24 @@ __device__ __forceinline__ void keys_part(const tsa_attend_grad_args& g, const f
 struct GradGrid {
   uint32_t queries, keys;  // workgroups
 };
-template <class T, int kD, bool kAligned, bool kSplit>
+template <class T, int kD, bool kAligned, bool kKeys, bool kValues>
+__device__ __forceinline__ void keys_of_group(const tsa_attend_grad_args& g, const float2* rows, float c, uint32_t pieces, float* parts, GradMemory<kD>& m) {
+  Keys o;
+  if (!find_keys(g.f, blockIdx.x, pieces, m.own, o)) return;
+  if (both_parts(o.qs.count, o.ks.count)) keys_part<T, kD, kAligned, true, kKeys, kValues>(g, rows, c, o, pieces, parts, m);
+  else keys_part<T, kD, kAligned, false, kKeys, kValues>(g, rows, c, o, pieces, parts, m);
+}
+template <class T, int kD, bool kAligned>
 __global__ __launch_bounds__(64 * kTileWaves, 2) void gradients_kernel(tsa_attend_grad_args g, const float2* rows, float c, uint32_t pieces, float* parts, GradGrid n) {
   __shared__ GradMemory<kD> m;
   if (blockIdx.y + 1 == gridDim.y) {
-    if (blockIdx.x < n.queries) queries_part<T, kD, kAligned, kSplit>(g, rows, c, blockIdx.x, m);
+    Queries o;
+    if (blockIdx.x >= n.queries || !find_queries<true>(g.f, blockIdx.x, m.own, o)) return;
+    if (both_parts(o.qs.count, o.ks.count)) queries_part<T, kD, kAligned, true>(g, rows, c, o, m);
+    else queries_part<T, kD, kAligned, false>(g, rows, c, o, m);
   } else if (blockIdx.x < n.keys) {
-    if (blockIdx.y == 0) keys_part<T, kD, kAligned, kSplit, true, kD == 64>(g, rows, c, pieces, parts, blockIdx.x, m);
-    else if constexpr (kD != 64) keys_part<T, kD, kAligned, kSplit, false, true>(g, rows, c, pieces, parts, blockIdx.x, m);
+    if (blockIdx.y == 0) keys_of_group<T, kD, kAligned, true, kD == 64>(g, rows, c, pieces, parts, m);
+    else if constexpr (kD != 64) keys_of_group<T, kD, kAligned, false, true>(g, rows, c, pieces, parts, m);
   }
 }
 
@@ -432,7 +463,7 @@ uint32_t pieces_of(const tsa_attend_args& a) {
   return n > kMaxPieces ? kMaxPieces : uint32_t(n);
 }
 
-template <class T, int kD, bool kAligned, bool kSplit>
+template <class T, int kD, bool kAligned>
 void gradients(const tsa_attend_grad_args& g, float2* rows, float* parts, hipStream_t stream) {
   const tsa_attend_args& a = g.f;
   const float c = a.scale * 1.44269504f;
@@ -441,7 +472,7 @@ void gradients(const tsa_attend_grad_args& g, float2* rows, float* parts, hipStr
   const GradGrid n = {g.dq.p ? queries : 0, keys ? uint32_t(own_tiles_at_most(a.sequences, a.k_tokens) * a.k.heads * pieces) : 0};
   if (queries) hipLaunchKernelGGL((rows_kernel<T, kD, kAligned>), dim3(queries), dim3(64 * kTileWaves), 0, stream, g, rows, c);
   const dim3 grid(n.queries > n.keys ? n.queries : n.keys, !keys ? 1 : kD == 64 ? 2 : 3);
-  hipLaunchKernelGGL((gradients_kernel<T, kD, kAligned, kSplit>), grid, dim3(64 * kTileWaves), 0, stream, g, rows, c, pieces, parts, n);
+  hipLaunchKernelGGL((gradients_kernel<T, kD, kAligned>), grid, dim3(64 * kTileWaves), 0, stream, g, rows, c, pieces, parts, n);
   if (keys) {
     if (pieces > 1) {
       const uint64_t n = uint64_t(a.k_tokens) * a.k.heads * (2 * kD / 4);
@@ -468,11 +499,10 @@ int launch_attend_backward(const tsa_attend_grad_args& g, void* workspace, hipSt
   bool aligned = true;
   if (a.tokens) aligned = tile_heads(a.q) && vector_heads(a.out) && tile_heads(g.dout) && (!g.dq.p || vector_heads(g.dq));
   if (a.k_tokens) aligned = aligned && tile_heads(a.k) && tile_heads(a.v) && (!g.dk.p || (vector_heads(g.dk) && vector_heads(g.dv)));
-#define CALL(T, D)                                                             \
-  do {                                                                         \
-    if (!aligned) gradients<T, D, false, true>(g, rows, parts, stream);        \
-    else if (split_rows(a)) gradients<T, D, true, true>(g, rows, parts, stream); \
-    else gradients<T, D, true, false>(g, rows, parts, stream);                 \
+#define CALL(T, D)                                                  \
+  do {                                                              \
+    if (aligned) gradients<T, D, true>(g, rows, parts, stream);     \
+    else gradients<T, D, false>(g, rows, parts, stream);            \
   } while (0)
   if (a.type == TSA_BF16) {
     if (a.head_dim <= 64) CALL(Bf16, 64);

@@ -63,10 +63,13 @@ struct Second {
     if constexpr (kSplit) sum = mfma32<T>(a, part[1], sum);
   }
 };
-// Up to so many rows (of all heads) the products of probabilities and of the scores' gradients take both parts: their error is then a few
-// elements' and may exceed the results' own rounding by far, and the calls are all latency (301 rows of 4 heads: 8.8 us for 8.4, the gradients 11 either way).
-constexpr uint64_t kSplitRows = 2048;
-inline bool split_rows(const tsa_attend_args& a) { return uint64_t(a.tokens) * a.q.heads <= kSplitRows; }
+// Sequences of so many pairs of a query and a key take both parts, in the forward pass and in the gradients: a sequence's results do not depend
+// on what else is in the call (keys' gradients but for the order of sums in 32 bits) or how it lies in memory. The error against 64 bits is then that of rounding the results (bf16 0.0016, with
+// one part 0.0020 to 0.0024). It costs nothing where a call is latency (301 rows of 4 heads: 10.4 us, gradients 27.3, either way), and where short
+// sequences fill the chip some of the products' time: 32 of 256 rows, 32 heads of 128, 70 us for 64 and 319 for 305; 16 of 512, which is
+// beyond, 93 for 80 and 388 for 358.
+constexpr uint32_t kSplitPairs = 1u << 17;
+__device__ __forceinline__ bool both_parts(uint32_t queries, uint32_t keys) { return uint64_t(queries) * keys <= kSplitPairs; }
 
 template <int kD>
 struct TileShapes {
