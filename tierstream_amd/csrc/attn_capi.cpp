@@ -113,8 +113,8 @@ ss_status tsa_rotary_init(const tsa_rotary_params* p, tsa_rotary* out) {
     REQUIRE(p != nullptr && out != nullptr, SS_E_INVALID, std::string(w) + ": null arguments");
     REQUIRE(p->rotated >= 2 && p->rotated % 2 == 0 && p->rotated <= 2 * TSA_ROTARY_MAX_PAIRS, SS_E_INVALID, std::string(w) + ": an even number of rotated values, 2..256");
     REQUIRE(p->interleaved <= 1, SS_E_INVALID, std::string(w) + ": interleaved 0 or 1");
-    REQUIRE(std::isfinite(p->base) && p->base > 0 && std::isfinite(p->factor) && p->factor > 0 && std::isfinite(p->amplitude), SS_E_INVALID,
-            std::string(w) + ": a positive base and factor, a finite amplitude");
+    REQUIRE(std::isfinite(p->base) && p->base > 0 && std::isfinite(p->factor) && p->factor > 0 && std::isfinite(float(p->amplitude)), SS_E_INVALID,
+            std::string(w) + ": a positive base and factor, an amplitude that 32 bits hold");
     REQUIRE(std::isfinite(p->trained) && p->trained >= 0 && std::isfinite(p->low) && std::isfinite(p->high), SS_E_INVALID, std::string(w) + ": a trained length of 0 or more, finite limits");
     REQUIRE(p->factor == 1 || p->trained == 0 || p->high > p->low, SS_E_INVALID, std::string(w) + ": high above low");
     tsa_rotary r = {};
@@ -128,6 +128,7 @@ ss_status tsa_rotary_init(const tsa_rotary_params* p, tsa_rotary* out) {
         const double keep = p->trained == 0 || !(inside > 0) ? 0.0 : inside < 1 ? inside : 1.0;
         turns *= keep + (1 - keep) / p->factor;
       }
+      REQUIRE(std::isfinite(turns * INT32_MAX), SS_E_INVALID, std::string(w) + ": a base and factor whose angles are numbers");
       r.turns[i] = turns;
     }
     *out = r;
