@@ -2,7 +2,7 @@
 import pytest
 
 import tierstream_amd as tsa
-from test_attn_refusals import Fake, i32
+from test_attn_refusals import Fake, cache, i32
 from tierstream_amd import attn
 
 
@@ -21,3 +21,15 @@ def test_angles_and_amplitudes_are_numbers(bad):
     with pytest.raises(tsa.SsError, match="tsa_rotary_init"):
         attn.Rotary(128, **bad)
     attn.Rotary(128, base=1e-300, amplitude=3e38)
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e300, float("inf"), float("nan")])
+def test_a_scale_beyond_32_bits_is_refused(scale):
+    """As a status of the library's, like any other value that it refuses."""
+    q, k = Fake(4, 4, 128), Fake(4, 4, 128)
+    with pytest.raises(tsa.SsError, match="finite scale"):
+        attn.attend(q, k, k, q, scale=scale)
+    with pytest.raises(tsa.SsError, match="finite scale"):
+        attn.attend_backward(q, k, k, q, q, Fake(4, 4, dtype="torch.float32"), q, scale=scale)
+    with pytest.raises(tsa.SsError, match="finite scale"):
+        attn.attend_cached(cache(), Fake(4, 8, 128), Fake(4, 8, 128), i32(4, 8), i32(4), i32(5), scale=scale)
