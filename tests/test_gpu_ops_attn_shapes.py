@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_ops_attn import KINDS, PAGE, attend64, first_of, gen, i32, near, random_pages, rotated64, rows, stream
+from test_gpu_ops_attn import KINDS, PAGE, attend64, cached64, first_of, gen, i32, near, random_pages, rotated64, room, rows, stream
 
 pytestmark = pytest.mark.gpu
 
@@ -104,3 +104,18 @@ def test_turned_in_place(attn, kind, interleaved, tokens, heads, kept, dim, rota
         inside = torch.zeros(len(flat), dtype=torch.bool, device="cuda")
         inside[shift:].as_strided((tokens, heads + kept, dim), (width, dim, 1))[live] = True
         assert torch.equal(flat[~inside], before[~inside])
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("ends,fresh,kept,group,dim", [([1500, 700], [1000, 300], 1, 4, 64), ([600, 64, 900], [600, 1, 33], 2, 3, 128), ([2000], [250], 2, 8, 96)])
+def test_chunks_of_a_prompt_over_the_cache(attn, kind, ends, fresh, kept, group, dim):
+    """Hundreds of new tokens a request, from the first one on or behind a long context: tiles of 16 rows that begin and end inside tokens."""
+    g, tokens = gen(sum(ends)), sum(fresh)
+    need = [(e + PAGE - 1) // PAGE for e in ends]
+    pages, table = random_pages(g, sum(need), kept, dim), torch.full((len(ends), max(need)), -1, dtype=torch.int32, device="cuda")
+    order = torch.randperm(sum(need), device="cuda", generator=g).to(torch.int32)
+    for i, n in enumerate(need):
+        table[i, :n] = order[sum(need[:i]):sum(need[:i]) + n]
+    q, out, cache = rows(g, tokens, kept * group, dim, kind), rows(g, tokens, kept * group, dim, kind, fill=7.0), attn.Cache(pages, kept, dim)
+    attn.attend_cached(cache, q, out, table, i32(ends), first_of(fresh), workspace=room(attn.attend_cached_workspace(cache, q, table)), stream=stream())
+    near(out, cached64(q, pages, dim, table, ends, fresh, dim ** -0.5, len(pages)))
