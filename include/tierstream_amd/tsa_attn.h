@@ -19,8 +19,9 @@
  * range and a length below 0 count as none, lengths and sequences end at the arrays they index.
  *
  * Alignment: every array at its element's size, pages and workspaces at 16 bytes. Heads that start 16-byte aligned (base and strides)
- * with a head_dim that is a multiple of 8 are the fastest. Infinities and NaN stay in the rows that attend to them (a row near whose
- * last key there is one is NaN as a whole). Arrays and stream belong to the current device. A workspace belongs to one stream, or to
+ * with a head_dim that is a multiple of 8 are the fastest. Infinities and NaN reach the rows that attend to them and no others; a row may
+ * be NaN as a whole, its lse too, for one in a tile of 64 keys that the mask cuts for any of 128 rows, or at a new token of its request (the
+ * cache), and so may a key's gradients. Arrays and stream belong to the current device. A workspace belongs to one stream, or to
  * graphs that do not run at once; nothing in it is kept from call to call.
  *
  * Sizes: tokens and sequences below 2^24, pages and a table's width below 2^25, heads up to 1024; tsa_cache_store and _load: tokens x
@@ -144,7 +145,7 @@ SS_API ss_status tsa_cache_load(const tsa_cache* c, const tsa_cache_rows_args* a
  * the tokens up to itself. Query head h reads kept head h / (heads / kv_heads). A row without keys is 0; rows behind the last request
  * are left as they were. A token on a page out of range counts as absent. For one or a few tokens a request; it
  * holds for any number. Probabilities times their values' scales are rounded to half precision, in ranges of their own (a scale below 2^-15
- * of the largest of its block of the request keeps fewer bits); all sums are in 32 bits. */
+ * of the largest of its block of the request keeps fewer bits; with TSA_BF16 probabilities are before that, too); all sums are in 32 bits. */
 typedef struct tsa_attend_cached_args {
   tsa_heads q, out;        /* heads a multiple of kv_heads */
   const int32_t* table;    /* [requests][width] */

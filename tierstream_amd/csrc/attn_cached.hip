@@ -17,7 +17,7 @@
 // bits, and so does a probability below 2^-17 of its row's largest. Values are read transposed, by ds_read_b64_tr_b4.
 //
 // Measured, 128 values a head: 64 requests of 1023..8191 tokens, 180 MB of pages, 46 us and 4.5 for the joining launch (3.9 TB/s; the
-// loads alone take 36); four of up to 131071, three new tokens each, 371 MB, 77 and 5.6 (4.8 TB/s; 70); one of 4097 tokens, 9 and 4. What bounds
+// loads alone take 36); four of up to 131071, three new tokens each, 371 MB, 75 to 81 and 6 (4.6 to 4.9 TB/s; 70); one of 4097 tokens, 9 and 4. What bounds
 // it: the rate of the loads, and for short shares the way to the first page (lengths, then the table and queries, then the page) and the joining
 // of the waves, 10 us or so together. The registers leave three workgroups a CU at 96 and 128 values a head: one spilled value costs 3 us.
 #include <cmath>

@@ -173,6 +173,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(tsa_cache_plan_args a, b
   }
 }
 
+// 2047 requests and 65536 rows 4.0 us, one row 1.4: a launch.
 __global__ __launch_bounds__(256) void slots_kernel(tsa_cache_plan_args a) {
   const uint32_t r = blockIdx.x * 256 + threadIdx.x;
   if (r >= a.rows) return;

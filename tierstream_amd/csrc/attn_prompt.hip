@@ -2,8 +2,8 @@
 // of 64 through LDS, the next one on its way while one is multiplied. A lane's column is its query in scores and outputs alike: the
 // softmax runs in the lane's own registers, and its probabilities are the second product's operand as they stand. Four waves of 32
 // queries share each tile, and two workgroups a CU fill each other's waits; the longest rows begin first.
-// Measured: 8191 tokens of 32 heads on 8 of 128, causal, 535 us: 1030 TFLOP/s (a library's large product reaches 1400); the matrix units
-// are busy 57 % of the cycles, at 1.6 GHz. The next tile's scores made in the shadow of this one's exponentials took 4 % longer. 301 tokens of 4 heads: 8.8 us, latency.
+// Measured: 8191 tokens of 32 heads on 8 of 128, causal, 511 to 540 us: 1020 to 1080 TFLOP/s (a library's large product reaches 1400); the matrix units
+// are busy 57 % of the cycles, at 1.6 GHz. The next tile's scores made in the shadow of this one's exponentials took 4 % longer. 301 tokens of 4 heads: 9.1 us, latency.
 #include "attn_tile.hpp"
 
 namespace tsa {

@@ -5,9 +5,9 @@
 // come out of the first products, the operand of the second. Scores are computed again in each pass. Sums over a workgroup's rows stay in
 // its registers; where there are few tiles of keys their queries are cut into pieces, whose sums go to memory in 32 bits and are added
 // up in order by a last launch: no atomics, the same bits every time. lse and sum p dp go to the workspace first, a pair a row.
-// Measured: 8192 tokens in three sequences, 32 heads on 8 of 128, causal, after a forward pass of 250 us: the pairs 45, the gradients 907
+// Measured: 8192 tokens in three sequences, 32 heads on 8 of 128, causal, after a forward pass of 239 to 250 us: the pairs 45, the gradients 861 to 907
 // (ten products for the formula's seven, forward pass included: 840 TFLOP/s; alone dq takes 324, dk 364, dv 269), the joining launch 37. The matrix units
-// are busy 44 to 52 % of the cycles, at 1.8 GHz. 301 tokens of 4 heads of 64: 7.2, 11.0 and 4.6, latency.
+// are busy 44 to 52 % of the cycles, at 1.8 GHz. 301 tokens of 4 heads of 64: 6.7, 11.7 and 4.6, latency.
 #include "attn_tile.hpp"
 
 namespace tsa {

@@ -192,7 +192,8 @@ class Model:
 class Decoder:
     """Tokens one at a time, the experts of `model` read from a device-gated context over its written source. The model may be
     trained on: the decoder keeps the weights it was made with, as the source does (a step gives the model new tensors, and
-    the captured graph goes on reading these). With attention, a token attends to those behind it since forget(), up to `context`."""
+    the captured graph goes on reading these). With attention, a token attends to those behind it since forget(), up to `context` of them
+    (in whole pages)."""
 
     def __init__(self, model: Model, desc_json: str, context: int = 1024):
         s, shape = model.s, wl.dg_shape(model.workload())
